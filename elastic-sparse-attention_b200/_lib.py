@@ -30,13 +30,19 @@ EXPORTED = ("esa_version", "esa_last_error", "esa_device_errors", "esa_forward_w
             "esa_probe_gather", "esa_copy_rows",
             # decoder-layer harness (include/esa_layer.h)
             "esa_rmsnorm_forward", "esa_rmsnorm_backward_workspace_size", "esa_rmsnorm_backward",
-            "esa_rope_apply", "esa_swiglu_forward", "esa_swiglu_backward")
+            "esa_rope_apply", "esa_swiglu_forward", "esa_swiglu_backward",
+            "esa_embedding_forward", "esa_embedding_backward_workspace_size",
+            "esa_embedding_backward", "esa_qk_norm_rope_forward",
+            "esa_qk_norm_rope_backward_workspace_size", "esa_qk_norm_rope_backward",
+            "esa_quantize_rows", "esa_dequantize_rows", "esa_rmsnorm_pack_forward",
+            "esa_rmsnorm_unpack_forward", "esa_swiglu_pack_forward", "esa_swiglu_unpack_backward")
 
 # ESA_DEVERR_* bits of the per-device error word
 DEVERR_KV_RANGE = 1
 DEVERR_TIMEOUT = 2
 DEVERR_QUERY_RANGE = 4
 DEVERR_PLAN = 8
+DEVERR_TOKEN_RANGE = 16
 
 
 class EsaTensor(ctypes.Structure):
@@ -140,6 +146,33 @@ def load() -> ctypes.CDLL:
         lib.esa_swiglu_forward.restype = ctypes.c_int
         lib.esa_swiglu_backward.argtypes = [i32, i64, i32, P, P, P, P, P]
         lib.esa_swiglu_backward.restype = ctypes.c_int
+        S, T = ctypes.c_size_t, EsaTensor
+        lib.esa_embedding_forward.argtypes = [i32, i32, i64, i64, i32, P, P, F, P, P]
+        lib.esa_embedding_forward.restype = ctypes.c_int
+        lib.esa_embedding_backward_workspace_size.argtypes = [i64, i64, i32]
+        lib.esa_embedding_backward_workspace_size.restype = S
+        lib.esa_embedding_backward.argtypes = [i32, i32, i64, i64, i32, P, P, F, i64, P, P, S, P]
+        lib.esa_embedding_backward.restype = ctypes.c_int
+        lib.esa_qk_norm_rope_forward.argtypes = [i32, i32, i64, i32, T, i32, T, i32, P, P, F, P,
+                                                 i64, P, T, T, P]
+        lib.esa_qk_norm_rope_forward.restype = ctypes.c_int
+        lib.esa_qk_norm_rope_backward_workspace_size.argtypes = [i32, i64, i32, i32, i32]
+        lib.esa_qk_norm_rope_backward_workspace_size.restype = S
+        lib.esa_qk_norm_rope_backward.argtypes = [i32, i32, i64, i32, T, i32, T, i32, P, P, F, P,
+                                                  i64, P, T, T, T, T, P, P, P, S, P]
+        lib.esa_qk_norm_rope_backward.restype = ctypes.c_int
+        lib.esa_quantize_rows.argtypes = [i32, i32, i64, i32, P, P, P, P]
+        lib.esa_quantize_rows.restype = ctypes.c_int
+        lib.esa_dequantize_rows.argtypes = [i32, i32, i64, i32, P, P, P, P]
+        lib.esa_dequantize_rows.restype = ctypes.c_int
+        lib.esa_rmsnorm_pack_forward.argtypes = [i32, i32, i64, i32, P, P, P, P, F, P, P, P, P, P]
+        lib.esa_rmsnorm_pack_forward.restype = ctypes.c_int
+        lib.esa_rmsnorm_unpack_forward.argtypes = [i32, i32, i64, i32, P, P, P, F, P, P, P, P]
+        lib.esa_rmsnorm_unpack_forward.restype = ctypes.c_int
+        lib.esa_swiglu_pack_forward.argtypes = [i32, i32, i64, i32, P, P, P, P, P]
+        lib.esa_swiglu_pack_forward.restype = ctypes.c_int
+        lib.esa_swiglu_unpack_backward.argtypes = [i32, i32, i64, i32, P, P, P, P, P, P]
+        lib.esa_swiglu_unpack_backward.restype = ctypes.c_int
         _lib = lib
     return _lib
 

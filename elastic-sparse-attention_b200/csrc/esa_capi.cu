@@ -21,6 +21,7 @@
 #include "esa_layer.h"
 #include "esa_decode.cuh"
 #include "esa_gather.cuh"
+#include "esa_host.h"
 #include "esa_keymma.cuh"
 #include "esa_layer.cuh"
 #include "esa_pattern.cuh"
@@ -31,8 +32,11 @@
 #include "esa_window_bwd.cuh"
 
 namespace {
-
 thread_local std::string g_last_error;
+}  // namespace
+
+namespace esa {
+namespace host {
 
 int fail(int code, const char* fmt, ...) {
   char buf[512];
@@ -49,6 +53,33 @@ int check_launch(const char* what) {
   if (e != cudaSuccess) return fail(ESA_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
   return ESA_OK;
 }
+
+int check_tensor(const char* name, const esa_tensor_t& t, int esize) {
+  if (!t.data) return fail(ESA_ERR_INVALID, "%s: null data pointer", name);
+  if (reinterpret_cast<uintptr_t>(t.data) % 16)
+    return fail(ESA_ERR_INVALID, "%s: data pointer must be 16-byte aligned", name);
+  if ((t.stride_b * esize) % 16 || (t.stride_h * esize) % 16 || (t.stride_s * esize) % 16)
+    return fail(ESA_ERR_INVALID,
+                "%s: strides (%lld, %lld, %lld) elements must be multiples of 16 bytes",
+                name, (long long)t.stride_b, (long long)t.stride_h, (long long)t.stride_s);
+  return ESA_OK;
+}
+
+int check_rows_op(const char* what, int32_t dtype, int64_t n_rows, int32_t dim) {
+  if (dtype != ESA_DTYPE_F32 && dtype != ESA_DTYPE_BF16 && dtype != ESA_DTYPE_F16)
+    return fail(ESA_ERR_INVALID, "%s: unknown dtype %d", what, dtype);
+  if (n_rows < 0 || dim < 1) return fail(ESA_ERR_INVALID, "%s: bad shape", what);
+  const int es = elem_size(dtype);
+  if ((dim * es) % 16) return fail(ESA_ERR_INVALID, "%s: dim * element size must be a multiple of 16 bytes", what);
+  return ESA_OK;
+}
+
+}  // namespace host
+}  // namespace esa
+
+namespace {
+
+using namespace esa::host;
 
 constexpr int64_t kMaxPosition = int64_t(1) << 24;  // float32 index math is exact below 2^24
 constexpr int kMaxAttnLength = 2048;
@@ -117,22 +148,9 @@ void trace_clear() {
   g_trace.clear();
 }
 
-int elem_size(int dtype) { return dtype == ESA_DTYPE_F32 ? 4 : 2; }
-
 bool head_dim_supported(int dtype, int d) {
   if (dtype == ESA_DTYPE_F32) return d == 8 || d == 16 || d == 32 || d == 64 || d == 128;
   return d == 8 || d == 16 || d == 32 || d == 64 || d == 128 || d == 256;
-}
-
-int check_tensor(const char* name, const esa_tensor_t& t, int esize) {
-  if (!t.data) return fail(ESA_ERR_INVALID, "%s: null data pointer", name);
-  if (reinterpret_cast<uintptr_t>(t.data) % 16)
-    return fail(ESA_ERR_INVALID, "%s: data pointer must be 16-byte aligned", name);
-  if ((t.stride_b * esize) % 16 || (t.stride_h * esize) % 16 || (t.stride_s * esize) % 16)
-    return fail(ESA_ERR_INVALID,
-                "%s: strides (%lld, %lld, %lld) elements must be multiples of 16 bytes",
-                name, (long long)t.stride_b, (long long)t.stride_h, (long long)t.stride_s);
-  return ESA_OK;
 }
 
 int check_problem(const esa_problem_t* pb) {
@@ -257,13 +275,17 @@ int symbol_address(const void* symbol, SymbolAddresses& cache, const char* what,
 // device; sticky until esa_device_errors resets it).
 static __device__ int g_device_errors;
 
-int device_error_word(int** out) {
+}  // namespace
+
+int esa::host::device_error_word(int** out) {
   static SymbolAddresses cache;
   void* a = nullptr;
   if (int rc = symbol_address(&g_device_errors, cache, "device error word", &a)) return rc;
   *out = static_cast<int*>(a);
   return ESA_OK;
 }
+
+namespace {
 
 // Up to this many (batch, head, row) pairs the forward runs the latency kernel
 // (one CTA per pair, slots split over warps) instead of a throughput kernel.
@@ -770,7 +792,7 @@ void set_plan(esa::AttnParams& p, const void* plan, const PlanGeom& g) {
 
 extern "C" {
 
-int esa_version(void) { return 130; }
+int esa_version(void) { return 140; }
 
 const char* esa_last_error(void) { return g_last_error.c_str(); }
 
@@ -1100,26 +1122,6 @@ extern "C" int esa_backward_noalloc(const esa_problem_t* pb, esa_tensor_t q, esa
 // Decoder-layer harness entry points (include/esa_layer.h).
 // ---------------------------------------------------------------------------
 namespace {
-
-bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
-
-int check_rows_op(const char* what, int32_t dtype, int64_t n_rows, int32_t dim) {
-  if (dtype != ESA_DTYPE_F32 && dtype != ESA_DTYPE_BF16 && dtype != ESA_DTYPE_F16)
-    return fail(ESA_ERR_INVALID, "%s: unknown dtype %d", what, dtype);
-  if (n_rows < 0 || dim < 1) return fail(ESA_ERR_INVALID, "%s: bad shape", what);
-  const int es = elem_size(dtype);
-  if ((dim * es) % 16) return fail(ESA_ERR_INVALID, "%s: dim * element size must be a multiple of 16 bytes", what);
-  return ESA_OK;
-}
-
-template <typename F>
-int by_dtype(int32_t dtype, F&& f) {
-  switch (dtype) {
-    case ESA_DTYPE_F32: return f(float{});
-    case ESA_DTYPE_BF16: return f(__nv_bfloat16{});
-    default: return f(__half{});
-  }
-}
 
 int norm_threads(int32_t dtype, int32_t dim) {
   const int vecs = dim / (16 / elem_size(dtype));

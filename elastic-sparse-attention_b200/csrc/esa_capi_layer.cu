@@ -1,0 +1,550 @@
+// extern "C" entry points of include/esa_layer.h: token embedding and its
+// gradient, per-head query / key norm with the rotary embedding, activations
+// kept in 8 bits.  (RMSNorm, rotary embedding and SwiGLU are in esa_capi.cu.)
+#include <algorithm>
+#include <cmath>
+
+#include "esa_layer.h"
+#include "esa_embed.cuh"
+#include "esa_host.h"
+#include "esa_pack8.cuh"
+#include "esa_qknorm.cuh"
+
+namespace {
+
+using namespace esa::host;
+
+size_t align256(size_t x) { return (x + 255) / 256 * 256; }
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// ---------------------------------------------------------------------------
+// Token embedding.
+// ---------------------------------------------------------------------------
+namespace em = esa::embed;
+
+constexpr int64_t kMaxTokens = int64_t(1) << 30;
+constexpr int64_t kMaxVocab = (int64_t(1) << 27) - 1;   // three digits of 9 bits, one key spare
+
+int check_embedding(const char* what, int32_t dtype, int32_t id_bytes, int64_t n, int64_t vocab,
+                    int32_t dim, const void* ids, float scale) {
+  if (int rc = check_rows_op(what, dtype, n, dim)) return rc;
+  if (id_bytes != 4 && id_bytes != 8)
+    return fail(ESA_ERR_INVALID, "%s: id_bytes %d (4 or 8)", what, id_bytes);
+  if (vocab < 1) return fail(ESA_ERR_INVALID, "%s: vocab must be >= 1", what);
+  if (vocab > kMaxVocab || n > kMaxTokens)
+    return fail(ESA_ERR_UNSUPPORTED, "%s: more than 2^27 - 1 rows or 2^30 tokens", what);
+  if (!std::isfinite(scale)) return fail(ESA_ERR_INVALID, "%s: scale must be finite", what);
+  if (n > 0 && (!ids || reinterpret_cast<uintptr_t>(ids) % id_bytes))
+    return fail(ESA_ERR_INVALID, "%s: null or misaligned ids", what);
+  return ESA_OK;
+}
+
+// Geometry and workspace of the sorted gradient.
+struct GradPlan {
+  int passes, bits;          // digits of the key, bits per digit
+  int tile;                  // keys per sorting CTA
+  int64_t tiles, pieces;
+  size_t keys[2], rows[2], hist, part, owners, counter, bytes;   // offsets
+};
+
+GradPlan grad_plan(int64_t n, int64_t vocab, int32_t dim) {
+  GradPlan g;
+  int bits = 1;
+  while ((vocab >> bits) != 0) ++bits;               // keys 0 .. vocab
+  g.passes = (int)ceil_div(bits, em::kRadixBits);
+  g.bits = (int)ceil_div(bits, g.passes);
+  g.tile = (int)(ceil_div(std::max<int64_t>(ceil_div(n, em::kSortMaxTiles), em::kSortTile),
+                          em::kSortTile) * em::kSortTile);
+  g.tiles = ceil_div(n, g.tile);
+  g.pieces = ceil_div(n, em::kPiece);
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t o = at;
+    at += align256(bytes);
+    return o;
+  };
+  for (int i = 0; i < 2; ++i) {
+    g.keys[i] = take(n * 4);
+    g.rows[i] = take(n * 4);
+  }
+  g.hist = take(g.tiles * em::kRadix * 4);
+  g.owners = take(g.pieces * 4);
+  g.counter = take(4);
+  g.part = take((size_t)g.pieces * 2 * dim * sizeof(float));
+  g.bytes = at;
+  return g;
+}
+
+template <typename T>
+int embedding_grad(int64_t n, int64_t vocab, int32_t dim, const em::Ids& ids, const void* dy,
+                   float scale, int64_t pad, void* dweight, char* ws, int* err, cudaStream_t s) {
+  const uint32_t vpr = dim / esa::Vec<T>::kElems;
+  const unsigned ychunks = (unsigned)ceil_div(vpr, em::kGradThreads);
+  if (ychunks > 65535) return fail(ESA_ERR_UNSUPPORTED, "esa_embedding_backward: dim %d too large", dim);
+  if (n <= em::kDirectMax) {
+    // about four CTAs per SM over the vocabulary, 32 rows of it at most
+    const int R = (int)std::min<int64_t>(32, ceil_div(vocab * ychunks, 148 * 4));
+    em::grad_direct_kernel<T><<<dim3((unsigned)ceil_div(vocab, R), ychunks), em::kGradThreads, 0, s>>>(
+        (int)n, vocab, R, vpr, ids, static_cast<const T*>(dy), scale, pad, static_cast<T*>(dweight),
+        err);
+    return check_launch("esa_embedding_backward");
+  }
+  const GradPlan g = grad_plan(n, vocab, dim);
+  em::SortPass p;
+  p.n = n;
+  p.vocab = vocab;
+  p.pad = pad;
+  p.ids = ids;
+  p.keys = p.rows = nullptr;
+  p.bits = g.bits;
+  p.tile = g.tile;
+  p.hist = reinterpret_cast<uint32_t*>(ws + g.hist);
+  p.counter = reinterpret_cast<int*>(ws + g.counter);
+  p.err = err;
+  for (int i = 0; i < g.passes; ++i) {
+    p.shift = i * g.bits;
+    p.out_keys = reinterpret_cast<uint32_t*>(ws + g.keys[i & 1]);
+    p.out_rows = reinterpret_cast<uint32_t*>(ws + g.rows[i & 1]);
+    em::sort_hist_kernel<<<(unsigned)g.tiles, em::kSortThreads, 0, s>>>(p);
+    if (int rc = check_launch("esa_embedding_backward (histogram)")) return rc;
+    em::sort_scatter_kernel<<<(unsigned)g.tiles, em::kSortThreads, 0, s>>>(p);
+    if (int rc = check_launch("esa_embedding_backward (sort)")) return rc;
+    p.keys = p.out_keys;
+    p.rows = p.out_rows;
+  }
+  em::GradParams q;
+  q.n = n;
+  q.vocab = vocab;
+  q.vpr = vpr;
+  q.keys = p.keys;
+  q.rows = p.rows;
+  q.scale = scale;
+  q.part = reinterpret_cast<float*>(ws + g.part);
+  q.counter = p.counter;
+  q.owners = reinterpret_cast<uint32_t*>(ws + g.owners);
+  q.pieces = g.pieces;
+  q.zero_blocks = (int)ceil_div(vocab, em::kZeroRows);
+  em::grad_pieces_kernel<T><<<dim3((unsigned)(q.zero_blocks + g.pieces), ychunks), em::kGradThreads,
+                              0, s>>>(q, static_cast<const T*>(dy), static_cast<T*>(dweight));
+  if (int rc = check_launch("esa_embedding_backward (sums)")) return rc;
+  em::grad_join_kernel<T><<<148 * 4, em::kJoinWarps * 32, 0, s>>>(q, static_cast<T*>(dweight));
+  return check_launch("esa_embedding_backward (join)");
+}
+
+// ---------------------------------------------------------------------------
+// Query / key norm with the rotary embedding.
+// ---------------------------------------------------------------------------
+namespace qk = esa::qknorm;
+
+constexpr int kQkBwdCtas = 148 * 4;   // fixed, so the weight gradients' sums do not depend on the GPU
+
+int check_qk(const char* what, int32_t dtype, int32_t batch, int64_t seq_len, int32_t head_dim,
+             int32_t num_q_heads, int32_t num_k_heads, int64_t pos_stride, float eps) {
+  if (dtype != ESA_DTYPE_F32 && dtype != ESA_DTYPE_BF16 && dtype != ESA_DTYPE_F16)
+    return fail(ESA_ERR_INVALID, "%s: unknown dtype %d", what, dtype);
+  if (batch < 0 || seq_len < 0 || num_q_heads < 0 || num_k_heads < 0 || pos_stride < 0)
+    return fail(ESA_ERR_INVALID, "%s: negative size", what);
+  const int per = 2 * (16 / elem_size(dtype));     // elements a thread owns
+  if (head_dim < per || head_dim > 16 * per || (head_dim & (head_dim - 1)))
+    return fail(ESA_ERR_UNSUPPORTED, "%s: head_dim %d (a power of two in [%d, %d])", what, head_dim,
+                per, 16 * per);
+  if ((int64_t)batch * seq_len > (int64_t(1) << 31) || num_q_heads > 65535 || num_k_heads > 65535)
+    return fail(ESA_ERR_UNSUPPORTED, "%s: too many positions or heads", what);
+  if (!(eps >= 0.f) || !std::isfinite(eps))
+    return fail(ESA_ERR_INVALID, "%s: eps must be finite and not negative", what);
+  return ESA_OK;
+}
+
+template <typename T>
+int set_heads(qk::Heads<T>& s, const char* name, const esa_tensor_t& x, const esa_tensor_t* d,
+              const esa_tensor_t& o, const void* w, int H) {
+  s = qk::Heads<T>{};
+  s.H = H;
+  if (H == 0) return ESA_OK;
+  const int es = sizeof(T);
+  if (int rc = check_tensor(name, x, es)) return rc;
+  if (d)
+    if (int rc = check_tensor(name, *d, es)) return rc;
+  if (int rc = check_tensor(name, o, es)) return rc;
+  if (!w || !aligned16(w)) return fail(ESA_ERR_INVALID, "%s weight: null or misaligned pointer", name);
+  s.x = static_cast<const T*>(x.data);
+  s.xb = x.stride_b; s.xh = x.stride_h; s.xs = x.stride_s;
+  if (d) {
+    s.d = static_cast<const T*>(d->data);
+    s.db = d->stride_b; s.dh = d->stride_h; s.ds = d->stride_s;
+  }
+  s.o = static_cast<T*>(o.data);
+  s.ob = o.stride_b; s.oh = o.stride_h; s.os = o.stride_s;
+  s.w = static_cast<const T*>(w);
+  return ESA_OK;
+}
+
+// f(std::integral_constant<int, threads per row>)
+template <typename F>
+int by_threads_per_row(int tpr, F&& f) {
+  switch (tpr) {
+    case 1: return f(std::integral_constant<int, 1>{});
+    case 2: return f(std::integral_constant<int, 2>{});
+    case 4: return f(std::integral_constant<int, 4>{});
+    case 8: return f(std::integral_constant<int, 8>{});
+    default: return f(std::integral_constant<int, 16>{});
+  }
+}
+
+// Heads per warp task: all of a token's heads once there are tokens enough for
+// 16 warps per SM, a single round of the warp for few tokens.
+template <typename T>
+void set_tasks(qk::Params<T>& p, int rows_per_warp) {
+  const int most = std::max(p.q.H, p.k.H);
+  int hpt = rows_per_warp;
+  while (hpt < most && p.tokens * ceil_div(most, 2 * hpt) >= 148 * 16) hpt *= 2;
+  p.hpt = hpt;
+  p.cq = (int)ceil_div(p.q.H, hpt);
+  p.ck = (int)ceil_div(p.k.H, hpt);
+}
+
+int qk_bwd_ctas(int64_t tokens, int32_t hq, int32_t hk) {
+  return (int)std::max<int64_t>(2, std::min<int64_t>(kQkBwdCtas, ceil_div(tokens * (hq + hk), qk::kWarps)));
+}
+
+// Share of the CTAs that the query heads get (at least one for each side present).
+int qk_q_ctas(int ctas, int32_t hq, int32_t hk) {
+  if (hk == 0) return ctas;
+  if (hq == 0) return 0;
+  return std::max(1, std::min(ctas - 1, (int)((int64_t)ctas * hq / (hq + hk))));
+}
+
+// ---------------------------------------------------------------------------
+// 8-bit rows.
+// ---------------------------------------------------------------------------
+namespace p8 = esa::pack8;
+
+int check_pack(const char* what, int32_t dtype, int32_t format, int64_t n_rows, int32_t dim) {
+  if (int rc = check_rows_op(what, dtype, n_rows, dim)) return rc;
+  if (format != ESA_PACK_INT8 && format != ESA_PACK_E4M3)
+    return fail(ESA_ERR_INVALID, "%s: unknown 8-bit format %d", what, format);
+  if (dim > (1 << 28)) return fail(ESA_ERR_UNSUPPORTED, "%s: dim %d too large", what, dim);
+  return ESA_OK;
+}
+
+template <typename F>
+int by_format(int32_t format, F&& f) {
+  if (format == ESA_PACK_INT8) return f(std::integral_constant<int, p8::kInt8>{});
+  return f(std::integral_constant<int, p8::kE4m3>{});
+}
+
+// Grid of the kernels whose warps stride over units of 32 vectors.
+unsigned unit_grid(int64_t rows, int32_t dim, int elems) {
+  const int64_t units = rows * ceil_div(dim / elems, 32);
+  return (unsigned)std::min<int64_t>(ceil_div(units, p8::kWarps), 148 * 32);
+}
+
+// f(std::integral_constant<int, vectors per lane>) for a warp-per-row kernel.
+template <typename F>
+int by_vectors(int vecs, F&& f) {
+  if (vecs <= 32) return f(std::integral_constant<int, 1>{});
+  if (vecs <= 64) return f(std::integral_constant<int, 2>{});
+  if (vecs <= 128) return f(std::integral_constant<int, 4>{});
+  if (vecs <= 256) return f(std::integral_constant<int, 8>{});
+  if (vecs <= 512) return f(std::integral_constant<int, 16>{});
+  return f(std::integral_constant<int, 32>{});
+}
+
+int check_norm_rows(const char* what, int32_t dtype, int64_t n_rows, int32_t dim, float eps) {
+  if (dim > 1024 * (16 / elem_size(dtype)))
+    return fail(ESA_ERR_UNSUPPORTED, "%s: dim %d too large", what, dim);
+  if (ceil_div(n_rows, p8::kNormWarps) > INT32_MAX)
+    return fail(ESA_ERR_UNSUPPORTED, "%s: too many rows", what);
+  if (!(eps >= 0.f) || !std::isfinite(eps))
+    return fail(ESA_ERR_INVALID, "%s: eps must be finite and not negative", what);
+  return ESA_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int esa_embedding_forward(int32_t dtype, int32_t id_bytes, int64_t n_tokens, int64_t vocab,
+                          int32_t dim, const void* ids, const void* weight, float scale, void* out,
+                          void* stream) {
+  if (int rc = check_embedding("esa_embedding_forward", dtype, id_bytes, n_tokens, vocab, dim, ids,
+                               scale))
+    return rc;
+  if (n_tokens == 0) return ESA_OK;
+  if (!weight || !out || !aligned16(weight) || !aligned16(out))
+    return fail(ESA_ERR_INVALID, "esa_embedding_forward: null or misaligned pointer");
+  const int64_t vpr = dim / (16 / elem_size(dtype));
+  const int64_t ctas = ceil_div(n_tokens * vpr, em::kLookupThreads * em::kLookupUnroll);
+  if (ctas > INT32_MAX)
+    return fail(ESA_ERR_UNSUPPORTED, "esa_embedding_forward: output too large");
+  int* err = nullptr;
+  if (int rc = device_error_word(&err)) return rc;
+  const em::Ids src{ids, id_bytes == 8};
+  return by_dtype(dtype, [&](auto tag) {
+    using T = decltype(tag);
+    em::lookup_kernel<T><<<(unsigned)ctas, em::kLookupThreads, 0, (cudaStream_t)stream>>>(
+        n_tokens, vocab, (uint32_t)vpr, src, static_cast<const T*>(weight), scale,
+        static_cast<T*>(out), err);
+    return check_launch("esa_embedding_forward");
+  });
+}
+
+size_t esa_embedding_backward_workspace_size(int64_t n_tokens, int64_t vocab, int32_t dim) {
+  if (n_tokens <= em::kDirectMax || n_tokens > kMaxTokens || vocab < 1 || vocab > kMaxVocab ||
+      dim < 1)
+    return 0;
+  return grad_plan(n_tokens, vocab, dim).bytes;
+}
+
+int esa_embedding_backward(int32_t dtype, int32_t id_bytes, int64_t n_tokens, int64_t vocab,
+                           int32_t dim, const void* ids, const void* dy, float scale,
+                           int64_t padding_idx, void* dweight, void* workspace,
+                           size_t workspace_bytes, void* stream) {
+  if (int rc = check_embedding("esa_embedding_backward", dtype, id_bytes, n_tokens, vocab, dim, ids,
+                               scale))
+    return rc;
+  if ((n_tokens > 0 && (!dy || !aligned16(dy))) || !dweight || !aligned16(dweight))
+    return fail(ESA_ERR_INVALID, "esa_embedding_backward: null or misaligned pointer");
+  const size_t need = esa_embedding_backward_workspace_size(n_tokens, vocab, dim);
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(ESA_ERR_WORKSPACE, "esa_embedding_backward: workspace of %zu bytes given, %zu needed",
+                workspace_bytes, need);
+  if (need && reinterpret_cast<uintptr_t>(workspace) % 256)
+    return fail(ESA_ERR_INVALID, "esa_embedding_backward: workspace must be 256-byte aligned");
+  int* err = nullptr;
+  if (int rc = device_error_word(&err)) return rc;
+  const em::Ids src{ids, id_bytes == 8};
+  return by_dtype(dtype, [&](auto tag) {
+    return embedding_grad<decltype(tag)>(n_tokens, vocab, dim, src, dy, scale,
+                                         padding_idx < 0 ? -1 : padding_idx, dweight,
+                                         static_cast<char*>(workspace), err, (cudaStream_t)stream);
+  });
+}
+
+int esa_qk_norm_rope_forward(int32_t dtype, int32_t batch, int64_t seq_len, int32_t head_dim,
+                             esa_tensor_t q, int32_t num_q_heads, esa_tensor_t k,
+                             int32_t num_k_heads, const void* q_weight, const void* k_weight,
+                             float eps, const int64_t* positions, int64_t positions_stride_b,
+                             const float* inv_freq, esa_tensor_t q_out, esa_tensor_t k_out,
+                             void* stream) {
+  if (int rc = check_qk("esa_qk_norm_rope_forward", dtype, batch, seq_len, head_dim, num_q_heads,
+                        num_k_heads, positions_stride_b, eps))
+    return rc;
+  if (batch == 0 || seq_len == 0 || num_q_heads + num_k_heads == 0) return ESA_OK;
+  if (!inv_freq) return fail(ESA_ERR_INVALID, "esa_qk_norm_rope_forward: null inv_freq");
+  return by_dtype(dtype, [&](auto tag) {
+    using T = decltype(tag);
+    qk::Params<T> p;
+    if (int rc = set_heads(p.q, "q", q, nullptr, q_out, q_weight, num_q_heads)) return rc;
+    if (int rc = set_heads(p.k, "k", k, nullptr, k_out, k_weight, num_k_heads)) return rc;
+    p.L = seq_len;
+    p.tokens = (int64_t)batch * seq_len;
+    p.pos = positions;
+    p.pos_sb = positions_stride_b;
+    p.inv_freq = inv_freq;
+    p.eps = eps;
+    const int tpr = head_dim / (2 * esa::Vec<T>::kElems);
+    set_tasks(p, 32 / tpr);
+    const int64_t ctas = ceil_div(p.tokens * (p.cq + p.ck), qk::kWarps);
+    if (ctas > INT32_MAX)
+      return fail(ESA_ERR_UNSUPPORTED, "esa_qk_norm_rope_forward: too many positions");
+    return by_threads_per_row(tpr, [&](auto t) {
+      qk::fwd_kernel<T, decltype(t)::value>
+          <<<(unsigned)ctas, qk::kThreads, 0, (cudaStream_t)stream>>>(p);
+      return check_launch("esa_qk_norm_rope_forward");
+    });
+  });
+}
+
+size_t esa_qk_norm_rope_backward_workspace_size(int32_t batch, int64_t seq_len, int32_t num_q_heads,
+                                                int32_t num_k_heads, int32_t head_dim) {
+  if (batch <= 0 || seq_len <= 0 || num_q_heads < 0 || num_k_heads < 0 || head_dim <= 0) return 0;
+  return (size_t)qk_bwd_ctas((int64_t)batch * seq_len, num_q_heads, num_k_heads) * head_dim *
+         sizeof(float);
+}
+
+int esa_qk_norm_rope_backward(int32_t dtype, int32_t batch, int64_t seq_len, int32_t head_dim,
+                              esa_tensor_t q, int32_t num_q_heads, esa_tensor_t k,
+                              int32_t num_k_heads, const void* q_weight, const void* k_weight,
+                              float eps, const int64_t* positions, int64_t positions_stride_b,
+                              const float* inv_freq, esa_tensor_t dq_out, esa_tensor_t dk_out,
+                              esa_tensor_t dq, esa_tensor_t dk, void* dq_weight, void* dk_weight,
+                              void* workspace, size_t workspace_bytes, void* stream) {
+  if (int rc = check_qk("esa_qk_norm_rope_backward", dtype, batch, seq_len, head_dim, num_q_heads,
+                        num_k_heads, positions_stride_b, eps))
+    return rc;
+  if ((num_q_heads > 0 && !dq_weight) || (num_k_heads > 0 && !dk_weight))
+    return fail(ESA_ERR_INVALID, "esa_qk_norm_rope_backward: null weight gradient");
+  cudaStream_t s = (cudaStream_t)stream;
+  if (batch == 0 || seq_len == 0) {   // sums over no rows
+    const size_t bytes = (size_t)head_dim * elem_size(dtype);
+    if (num_q_heads > 0) cudaMemsetAsync(dq_weight, 0, bytes, s);
+    if (num_k_heads > 0) cudaMemsetAsync(dk_weight, 0, bytes, s);
+    return check_launch("esa_qk_norm_rope_backward");
+  }
+  if (num_q_heads + num_k_heads == 0) return ESA_OK;
+  if (!inv_freq) return fail(ESA_ERR_INVALID, "esa_qk_norm_rope_backward: null inv_freq");
+  const size_t need = esa_qk_norm_rope_backward_workspace_size(batch, seq_len, num_q_heads,
+                                                               num_k_heads, head_dim);
+  if (!workspace || workspace_bytes < need)
+    return fail(ESA_ERR_WORKSPACE,
+                "esa_qk_norm_rope_backward: workspace of %zu bytes given, %zu needed",
+                workspace_bytes, need);
+  if (!aligned16(workspace))
+    return fail(ESA_ERR_INVALID, "esa_qk_norm_rope_backward: workspace must be 16-byte aligned");
+  return by_dtype(dtype, [&](auto tag) {
+    using T = decltype(tag);
+    qk::Params<T> p;
+    if (int rc = set_heads(p.q, "q", q, &dq_out, dq, q_weight, num_q_heads)) return rc;
+    if (int rc = set_heads(p.k, "k", k, &dk_out, dk, k_weight, num_k_heads)) return rc;
+    p.L = seq_len;
+    p.tokens = (int64_t)batch * seq_len;
+    p.pos = positions;
+    p.pos_sb = positions_stride_b;
+    p.inv_freq = inv_freq;
+    p.eps = eps;
+    const int tpr = head_dim / (2 * esa::Vec<T>::kElems);
+    set_tasks(p, 32 / tpr);
+    const int ctas = qk_bwd_ctas(p.tokens, num_q_heads, num_k_heads);
+    const int q_ctas = qk_q_ctas(ctas, num_q_heads, num_k_heads);
+    float* part = static_cast<float*>(workspace);
+    return by_threads_per_row(tpr, [&](auto t) {
+      qk::bwd_kernel<T, decltype(t)::value><<<ctas, qk::kThreads, 0, s>>>(p, q_ctas, part);
+      if (int rc = check_launch("esa_qk_norm_rope_backward")) return rc;
+      // block row 0: query weights, 1: key weights
+      const int first = num_q_heads > 0 ? 0 : 1, sides = (num_q_heads > 0) + (num_k_heads > 0);
+      qk::sum_kernel<T><<<dim3((unsigned)ceil_div(head_dim, 32), sides), qk::kSumWarps * 32, 0, s>>>(
+          head_dim, q_ctas, ctas, first, part, static_cast<T*>(dq_weight),
+          static_cast<T*>(dk_weight));
+      return check_launch("esa_qk_norm_rope_backward (weight sums)");
+    });
+  });
+}
+
+int esa_quantize_rows(int32_t dtype, int32_t format, int64_t n_rows, int32_t dim, const void* x,
+                      void* codes, float* scales, void* stream) {
+  if (int rc = check_pack("esa_quantize_rows", dtype, format, n_rows, dim)) return rc;
+  if (n_rows == 0) return ESA_OK;
+  if (!x || !codes || !scales || !aligned16(x) || !aligned16(codes) || !aligned16(scales))
+    return fail(ESA_ERR_INVALID, "esa_quantize_rows: null or misaligned pointer");
+  return by_dtype(dtype, [&](auto tag) {
+    using T = decltype(tag);
+    return by_format(format, [&](auto f) {
+      p8::quantize_kernel<T, decltype(f)::value>
+          <<<unit_grid(n_rows, dim, esa::Vec<T>::kElems), p8::kThreads, 0, (cudaStream_t)stream>>>(
+              n_rows, dim, static_cast<const T*>(x), static_cast<uint8_t*>(codes), scales);
+      return check_launch("esa_quantize_rows");
+    });
+  });
+}
+
+int esa_dequantize_rows(int32_t dtype, int32_t format, int64_t n_rows, int32_t dim,
+                        const void* codes, const float* scales, void* x, void* stream) {
+  if (int rc = check_pack("esa_dequantize_rows", dtype, format, n_rows, dim)) return rc;
+  if (n_rows == 0) return ESA_OK;
+  if (!x || !codes || !scales || !aligned16(x) || !aligned16(codes) || !aligned16(scales))
+    return fail(ESA_ERR_INVALID, "esa_dequantize_rows: null or misaligned pointer");
+  return by_dtype(dtype, [&](auto tag) {
+    using T = decltype(tag);
+    return by_format(format, [&](auto f) {
+      p8::dequantize_kernel<T, decltype(f)::value>
+          <<<unit_grid(n_rows, dim, esa::Vec<T>::kElems), p8::kThreads, 0, (cudaStream_t)stream>>>(
+              n_rows, dim, static_cast<const uint8_t*>(codes), scales, static_cast<T*>(x));
+      return check_launch("esa_dequantize_rows");
+    });
+  });
+}
+
+int esa_rmsnorm_pack_forward(int32_t dtype, int32_t format, int64_t n_rows, int32_t dim,
+                             const void* x, const void* residual, void* h_out, const void* weight,
+                             float eps, void* y, float* rstd, void* codes, float* scales,
+                             void* stream) {
+  if (int rc = check_pack("esa_rmsnorm_pack_forward", dtype, format, n_rows, dim)) return rc;
+  if (int rc = check_norm_rows("esa_rmsnorm_pack_forward", dtype, n_rows, dim, eps)) return rc;
+  if (n_rows == 0) return ESA_OK;
+  if (!x || !weight || !y || !rstd || !codes || !scales || (residual && !h_out) || !aligned16(x) ||
+      !aligned16(weight) || !aligned16(y) || !aligned16(codes) || !aligned16(scales) ||
+      !aligned16(residual) || !aligned16(h_out))
+    return fail(ESA_ERR_INVALID, "esa_rmsnorm_pack_forward: null or misaligned pointer");
+  return by_dtype(dtype, [&](auto tag) {
+    using T = decltype(tag);
+    return by_format(format, [&](auto f) {
+      return by_vectors(dim / esa::Vec<T>::kElems, [&](auto nv) {
+        p8::norm_pack_kernel<T, decltype(f)::value, decltype(nv)::value>
+            <<<(unsigned)ceil_div(n_rows, p8::kNormWarps), p8::kNormThreads, 0,
+               (cudaStream_t)stream>>>(n_rows, dim, static_cast<const T*>(x),
+                                       static_cast<const T*>(residual), static_cast<T*>(h_out),
+                                       static_cast<const T*>(weight), eps, static_cast<T*>(y), rstd,
+                                       static_cast<uint8_t*>(codes), scales);
+        return check_launch("esa_rmsnorm_pack_forward");
+      });
+    });
+  });
+}
+
+int esa_rmsnorm_unpack_forward(int32_t dtype, int32_t format, int64_t n_rows, int32_t dim,
+                               const void* codes, const float* scales, const void* weight,
+                               float eps, void* h, void* y, float* rstd, void* stream) {
+  if (int rc = check_pack("esa_rmsnorm_unpack_forward", dtype, format, n_rows, dim)) return rc;
+  if (int rc = check_norm_rows("esa_rmsnorm_unpack_forward", dtype, n_rows, dim, eps)) return rc;
+  if (n_rows == 0) return ESA_OK;
+  if (!codes || !scales || !weight || !h || !y || !rstd || !aligned16(codes) ||
+      !aligned16(scales) || !aligned16(weight) || !aligned16(h) || !aligned16(y))
+    return fail(ESA_ERR_INVALID, "esa_rmsnorm_unpack_forward: null or misaligned pointer");
+  return by_dtype(dtype, [&](auto tag) {
+    using T = decltype(tag);
+    return by_format(format, [&](auto f) {
+      return by_vectors(dim / esa::Vec<T>::kElems, [&](auto nv) {
+        p8::unpack_norm_kernel<T, decltype(f)::value, decltype(nv)::value>
+            <<<(unsigned)ceil_div(n_rows, p8::kNormWarps), p8::kNormThreads, 0,
+               (cudaStream_t)stream>>>(n_rows, dim, static_cast<const uint8_t*>(codes), scales,
+                                       static_cast<T*>(h), static_cast<const T*>(weight), eps,
+                                       static_cast<T*>(y), rstd);
+        return check_launch("esa_rmsnorm_unpack_forward");
+      });
+    });
+  });
+}
+
+int esa_swiglu_pack_forward(int32_t dtype, int32_t format, int64_t n_rows, int32_t ffn,
+                            const void* gate_up, void* out, void* codes, float* scales,
+                            void* stream) {
+  if (int rc = check_pack("esa_swiglu_pack_forward", dtype, format, n_rows, ffn)) return rc;
+  if (n_rows == 0) return ESA_OK;
+  if (!gate_up || !out || !codes || !scales || !aligned16(gate_up) || !aligned16(out) ||
+      !aligned16(codes) || !aligned16(scales))
+    return fail(ESA_ERR_INVALID, "esa_swiglu_pack_forward: null or misaligned pointer");
+  return by_dtype(dtype, [&](auto tag) {
+    using T = decltype(tag);
+    return by_format(format, [&](auto f) {
+      p8::swiglu_pack_kernel<T, decltype(f)::value>
+          <<<unit_grid(n_rows, ffn, esa::Vec<T>::kElems), p8::kThreads, 0, (cudaStream_t)stream>>>(
+              n_rows, ffn, static_cast<const T*>(gate_up), static_cast<T*>(out),
+              static_cast<uint8_t*>(codes), scales);
+      return check_launch("esa_swiglu_pack_forward");
+    });
+  });
+}
+
+int esa_swiglu_unpack_backward(int32_t dtype, int32_t format, int64_t n_rows, int32_t ffn,
+                               const void* codes, const float* scales, const void* dout,
+                               void* dgate_up, void* out_recomputed, void* stream) {
+  if (int rc = check_pack("esa_swiglu_unpack_backward", dtype, format, n_rows, ffn)) return rc;
+  if (n_rows == 0) return ESA_OK;
+  if (!codes || !scales || !dout || !dgate_up || !aligned16(codes) || !aligned16(scales) ||
+      !aligned16(dout) || !aligned16(dgate_up) || !aligned16(out_recomputed))
+    return fail(ESA_ERR_INVALID, "esa_swiglu_unpack_backward: null or misaligned pointer");
+  return by_dtype(dtype, [&](auto tag) {
+    using T = decltype(tag);
+    return by_format(format, [&](auto f) {
+      p8::swiglu_unpack_bwd_kernel<T, decltype(f)::value>
+          <<<unit_grid(n_rows, ffn, esa::Vec<T>::kElems), p8::kThreads, 0, (cudaStream_t)stream>>>(
+              n_rows, ffn, static_cast<const uint8_t*>(codes), scales, static_cast<const T*>(dout),
+              static_cast<T*>(dgate_up), static_cast<T*>(out_recomputed));
+      return check_launch("esa_swiglu_unpack_backward");
+    });
+  });
+}
+
+}  // extern "C"

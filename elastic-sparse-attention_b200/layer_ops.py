@@ -1,10 +1,14 @@
 """Tensor-level calls of the decoder-layer harness kernels (include/esa_layer.h):
-RMSNorm with a fused residual add, rotary embedding in place, SwiGLU.
+RMSNorm with a fused residual add, rotary embedding in place, SwiGLU, token
+embedding and its gradient, per-head query / key norm with the rotary
+embedding, rows kept in 8 bits between forward and backward.
 
 Like ``ops``, torch only allocates memory and provides the stream; every
 kernel is in libesa_b200.so and there is no fallback.
 """
 from __future__ import annotations
+
+from dataclasses import dataclass
 
 import torch
 
@@ -129,4 +133,357 @@ def swiglu_backward(gate_up: torch.Tensor, dout: torch.Tensor, recompute: bool =
         _lib.check(lib.esa_swiglu_backward(_dtype_code(gate_up), n, ffn, gate_up.data_ptr(),
                                            dout.data_ptr(), dgu.data_ptr(), _lib.ptr(out),
                                            _lib.stream_handle(dev)), "esa_swiglu_backward")
+    return dgu, out
+
+
+# ---------------------------------------------------------------------------
+# Token embedding
+# ---------------------------------------------------------------------------
+def _ids(ids: torch.Tensor) -> torch.Tensor:
+    if ids.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"token ids must be int64 or int32, got {ids.dtype}")
+    return ids.contiguous()
+
+
+def embedding_forward(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+    """scale * weight[ids], [*ids.shape, dim], rounded once.  An id outside
+    [0, vocab) gives a row of zeros and sets ``_lib.DEVERR_TOKEN_RANGE`` in
+    the device error word (``ops.device_errors``); no host round trip."""
+    dev = _check_device(ids, weight)
+    ids = _ids(ids)
+    if weight.dim() != 2:
+        raise ValueError("weight must be [vocab, dim]")
+    vocab, dim = weight.shape
+    _rows(weight, dim)
+    out = torch.empty(ids.shape + (dim,), dtype=weight.dtype, device=dev)
+    lib = _lib.load()
+    with _on(dev):
+        _lib.check(lib.esa_embedding_forward(
+            _dtype_code(weight), ids.element_size(), ids.numel(), vocab, dim, ids.data_ptr(),
+            weight.data_ptr(), scale, out.data_ptr(), _lib.stream_handle(dev)),
+            "esa_embedding_forward")
+    return out
+
+
+def embedding_backward(ids: torch.Tensor, dy: torch.Tensor, vocab_size: int, scale: float = 1.0,
+                       padding_idx: int | None = None) -> torch.Tensor:
+    """dweight [vocab_size, dim] of :func:`embedding_forward` for dy
+    [*ids.shape, dim]: float32 sums over each token's rows in ascending order
+    (the same in every run), rounded once to dy's dtype.  Rows of absent
+    tokens and the row ``padding_idx`` are zero."""
+    dev = _check_device(ids, dy)
+    ids = _ids(ids)
+    dim = dy.shape[-1]
+    if dy.shape[:-1] != ids.shape:
+        raise ValueError("dy must be [*ids.shape, dim]")
+    if padding_idx is not None and not 0 <= padding_idx < vocab_size:
+        raise ValueError(f"padding_idx {padding_idx} outside [0, {vocab_size})")
+    dy = dy.contiguous()
+    dw = torch.empty((vocab_size, dim), dtype=dy.dtype, device=dev)
+    lib = _lib.load()
+    need = lib.esa_embedding_backward_workspace_size(ids.numel(), vocab_size, dim)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    with _on(dev):
+        _lib.check(lib.esa_embedding_backward(
+            _dtype_code(dy), ids.element_size(), ids.numel(), vocab_size, dim, ids.data_ptr(),
+            dy.data_ptr(), scale, -1 if padding_idx is None else padding_idx, dw.data_ptr(),
+            _lib.ptr(ws), need, _lib.stream_handle(dev)), "esa_embedding_backward")
+    return dw
+
+
+# ---------------------------------------------------------------------------
+# Query / key norm with the rotary embedding
+# ---------------------------------------------------------------------------
+_NO_TENSOR = _lib.EsaTensor(None, 0, 0, 0)
+
+
+def _t4(t: torch.Tensor | None) -> _lib.EsaTensor:
+    return _NO_TENSOR if t is None else _lib.tensor4(t)
+
+
+def _qk_checks(q, k, q_weight, k_weight, inv_freq, positions):
+    dev = _check_device(*(t for t in (q, k, q_weight, k_weight, inv_freq) if t is not None))
+    B, _, L, D = q.shape
+    sides = [("q", q, q_weight)]
+    if k is not None:
+        if k.shape[0] != B or k.shape[2] != L or k.shape[3] != D or k.dtype != q.dtype:
+            raise ValueError("q and k must share batch, length, head_dim and dtype")
+        sides.append(("k", k, k_weight))
+    for name, _, w in sides:
+        if w is None or w.shape != (D,) or w.dtype != q.dtype or not w.is_contiguous():
+            raise ValueError(f"{name}_weight must be a contiguous [head_dim] tensor of q's dtype")
+    if inv_freq.dtype != torch.float32 or inv_freq.numel() != D // 2 or not inv_freq.is_contiguous():
+        raise ValueError("inv_freq must be float32 [head_dim / 2]")
+    stride = 0
+    if positions is not None:
+        if positions.shape != (L,) and positions.shape != (B, L):
+            raise ValueError("positions must be [L] or [B, L]")
+        positions = positions.to(device=dev, dtype=torch.int64).contiguous()
+        stride = L if positions.dim() == 2 else 0
+    return dev, positions, stride
+
+
+def _like_heads(name: str, out: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
+    if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
+        raise ValueError(f"{name} must match its input's shape, dtype and device")
+    return out
+
+
+def _new_heads(q: torch.Tensor, k: torch.Tensor | None):
+    """Outputs shaped like q and k in one [B, L, Hq + Hk, D] buffer (a
+    token's heads side by side, as in a projection's output)."""
+    B, Hq, L, D = q.shape
+    buf = torch.empty((B, L, Hq + (0 if k is None else k.shape[1]), D), dtype=q.dtype,
+                      device=q.device)
+    heads = buf.transpose(1, 2)
+    return heads[:, :Hq], (None if k is None else heads[:, Hq:])
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tensor,
+                 k_weight: torch.Tensor | None, eps: float, inv_freq: torch.Tensor,
+                 positions: torch.Tensor | None = None, q_out: torch.Tensor | None = None,
+                 k_out: torch.Tensor | None = None):
+    """(q', k'): each head row of q [B, Hq, L, D] and k [B, Hk, L, D] (strided
+    views with a contiguous D axis; k may be None) RMS-normalised with its
+    side's [D] weight, then rotated at its position, in one pass.  positions:
+    [L] shared by the batch, [B, L], or None for 0 .. L-1.  ``q_out`` /
+    ``k_out`` receive the result (e.g. rows of a key cache; q / k themselves
+    for in place); by default new views of one [B, L, Hq + Hk, D] buffer."""
+    dev, positions, stride = _qk_checks(q, k, q_weight, k_weight, inv_freq, positions)
+    B, Hq, L, D = q.shape
+    Hk = 0 if k is None else k.shape[1]
+    if q_out is None or (k is not None and k_out is None):
+        new_q, new_k = _new_heads(q, k)
+    q_out = new_q if q_out is None else _like_heads("q_out", q_out, q)
+    if k is not None:
+        k_out = new_k if k_out is None else _like_heads("k_out", k_out, k)
+    elif k_out is not None:
+        raise ValueError("k_out without k")
+    lib = _lib.load()
+    with _on(dev):
+        _lib.check(lib.esa_qk_norm_rope_forward(
+            _dtype_code(q), B, L, D, _t4(q), Hq, _t4(k), Hk, q_weight.data_ptr(),
+            _lib.ptr(k_weight), eps, _lib.ptr(positions), stride, inv_freq.data_ptr(), _t4(q_out),
+            _t4(k_out), _lib.stream_handle(dev)), "esa_qk_norm_rope_forward")
+    return q_out, k_out
+
+
+def qk_norm_rope_backward(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tensor,
+                          k_weight: torch.Tensor | None, eps: float, inv_freq: torch.Tensor,
+                          dq_out: torch.Tensor, dk_out: torch.Tensor | None,
+                          positions: torch.Tensor | None = None, dq: torch.Tensor | None = None,
+                          dk: torch.Tensor | None = None):
+    """(dq, dk, dq_weight, dk_weight) of :func:`qk_norm_rope` from its inputs
+    and the gradients of its outputs.  ``dq`` / ``dk`` receive the result
+    (dq_out / dk_out themselves for in place)."""
+    dev, positions, stride = _qk_checks(q, k, q_weight, k_weight, inv_freq, positions)
+    B, Hq, L, D = q.shape
+    Hk = 0 if k is None else k.shape[1]
+    if (k is None) != (dk_out is None):
+        raise ValueError("dk_out and k must be given together")
+    _like_heads("dq_out", dq_out, q)
+    if k is not None:
+        _like_heads("dk_out", dk_out, k)
+    elif dk is not None:
+        raise ValueError("dk without k")
+    if dq is None or (k is not None and dk is None):
+        new_q, new_k = _new_heads(q, k)
+    dq = new_q if dq is None else _like_heads("dq", dq, q)
+    dwq = torch.empty_like(q_weight)
+    dwk = None
+    if k is not None:
+        dk = new_k if dk is None else _like_heads("dk", dk, k)
+        dwk = torch.empty_like(k_weight)
+    lib = _lib.load()
+    need = lib.esa_qk_norm_rope_backward_workspace_size(B, L, Hq, Hk, D)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    with _on(dev):
+        _lib.check(lib.esa_qk_norm_rope_backward(
+            _dtype_code(q), B, L, D, _t4(q), Hq, _t4(k), Hk, q_weight.data_ptr(),
+            _lib.ptr(k_weight), eps, _lib.ptr(positions), stride, inv_freq.data_ptr(),
+            _t4(dq_out), _t4(dk_out), _t4(dq), _t4(dk), dwq.data_ptr(), _lib.ptr(dwk),
+            ws.data_ptr(), need, _lib.stream_handle(dev)), "esa_qk_norm_rope_backward")
+    return dq, dk, dwq, dwk
+
+
+# ---------------------------------------------------------------------------
+# Rows in 8 bits
+# ---------------------------------------------------------------------------
+PACK_FORMATS = {"int8": 0, "e4m3": 1}
+PACK_GROUP = 128
+
+
+@dataclass(frozen=True)
+class PackedRows:
+    """Rows kept in 8 bits: ``codes`` uint8 [*shape], ``scales`` float32
+    [*shape[:-1], ceil(shape[-1] / 128)], one scale per 128 elements;
+    ``dtype`` is the type of the rows they were made from."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+    format: str
+    dtype: torch.dtype
+
+    @property
+    def shape(self) -> torch.Size:
+        return self.codes.shape
+
+    def nbytes(self) -> int:
+        return self.codes.numel() + 4 * self.scales.numel()
+
+
+def _pack_code(format: str) -> int:
+    if format not in PACK_FORMATS:
+        raise ValueError(f"unknown 8-bit format {format!r}; expected one of {sorted(PACK_FORMATS)}")
+    return PACK_FORMATS[format]
+
+
+def _new_packed(shape, format: str, dtype: torch.dtype, dev) -> PackedRows:
+    groups = -(-shape[-1] // PACK_GROUP)
+    return PackedRows(torch.empty(shape, dtype=torch.uint8, device=dev),
+                      torch.empty(tuple(shape[:-1]) + (groups,), dtype=torch.float32, device=dev),
+                      format, dtype)
+
+
+def _check_packed(p: PackedRows) -> int:
+    """The format code of a PackedRows whose parts fit together."""
+    code = _pack_code(p.format)
+    want = p.codes.shape[:-1] + (-(-p.codes.shape[-1] // PACK_GROUP),)
+    if p.codes.dtype != torch.uint8 or p.scales.dtype != torch.float32 or p.scales.shape != want:
+        raise ValueError("PackedRows: codes must be uint8 and scales float32 "
+                         "[*codes.shape[:-1], ceil(codes.shape[-1] / 128)]")
+    if not p.codes.is_contiguous() or not p.scales.is_contiguous():
+        raise ValueError("PackedRows: codes and scales must be contiguous")
+    return code
+
+
+def quantize_rows(x: torch.Tensor, format: str = "int8") -> PackedRows:
+    """x [..., dim] in 8 bits, one scale per 128 elements of the last axis:
+    ``int8`` (even steps of max|x| / 127 per group) or ``e4m3`` (relative
+    steps, power-of-two scales).  A group with an infinity or a NaN decodes to
+    NaN."""
+    code = _pack_code(format)
+    dev = _check_device(x)
+    dim = x.shape[-1]
+    n = _rows(x, dim)
+    p = _new_packed(x.shape, format, x.dtype, dev)
+    lib = _lib.load()
+    with _on(dev):
+        _lib.check(lib.esa_quantize_rows(_dtype_code(x), code, n, dim, x.data_ptr(),
+                                         p.codes.data_ptr(), p.scales.data_ptr(),
+                                         _lib.stream_handle(dev)), "esa_quantize_rows")
+    return p
+
+
+def dequantize_rows(packed: PackedRows, dtype: torch.dtype | None = None) -> torch.Tensor:
+    """The rows that the codes stand for, in ``dtype`` (default: the dtype they
+    were made from)."""
+    code = _check_packed(packed)
+    dev = _check_device(packed.codes, packed.scales)
+    x = torch.empty(packed.shape, dtype=dtype or packed.dtype, device=dev)
+    dim = x.shape[-1]
+    lib = _lib.load()
+    with _on(dev):
+        _lib.check(lib.esa_dequantize_rows(_dtype_code(x), code, _rows(x, dim), dim,
+                                           packed.codes.data_ptr(), packed.scales.data_ptr(),
+                                           x.data_ptr(), _lib.stream_handle(dev)),
+                   "esa_dequantize_rows")
+    return x
+
+
+def rmsnorm_forward_packed(x: torch.Tensor, weight: torch.Tensor, eps: float,
+                           residual: torch.Tensor | None = None, format: str = "int8"):
+    """(h, y, rstd, packed): :func:`rmsnorm_forward` and h in 8 bits, in one
+    pass."""
+    code = _pack_code(format)
+    dev = _check_device(x, weight)
+    dim = x.shape[-1]
+    n = _rows(x, dim)
+    _check_norm_weight(weight, dim, x.dtype)
+    h = x
+    if residual is not None:
+        if residual.shape != x.shape or residual.dtype != x.dtype or residual.device != dev:
+            raise ValueError("residual must match x")
+        _rows(residual, dim)
+        h = torch.empty_like(x)
+    y = torch.empty_like(x)
+    rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+    p = _new_packed(x.shape, format, x.dtype, dev)
+    lib = _lib.load()
+    with _on(dev):
+        _lib.check(lib.esa_rmsnorm_pack_forward(
+            _dtype_code(x), code, n, dim, x.data_ptr(), _lib.ptr(residual),
+            h.data_ptr() if residual is not None else None, weight.data_ptr(), eps, y.data_ptr(),
+            rstd.data_ptr(), p.codes.data_ptr(), p.scales.data_ptr(), _lib.stream_handle(dev)),
+            "esa_rmsnorm_pack_forward")
+    return h, y, rstd, p
+
+
+def rmsnorm_from_packed(packed: PackedRows, weight: torch.Tensor, eps: float):
+    """(h, y, rstd): the rows the codes stand for, in their dtype, and their
+    RMSNorm, in one pass over the codes."""
+    code = _check_packed(packed)
+    dev = _check_device(packed.codes, packed.scales, weight)
+    dim = packed.shape[-1]
+    _check_norm_weight(weight, dim, packed.dtype)
+    h = torch.empty(packed.shape, dtype=packed.dtype, device=dev)
+    n = _rows(h, dim)
+    y = torch.empty_like(h)
+    rstd = torch.empty(packed.shape[:-1], dtype=torch.float32, device=dev)
+    lib = _lib.load()
+    with _on(dev):
+        _lib.check(lib.esa_rmsnorm_unpack_forward(
+            _dtype_code(h), code, n, dim, packed.codes.data_ptr(), packed.scales.data_ptr(),
+            weight.data_ptr(), eps, h.data_ptr(), y.data_ptr(), rstd.data_ptr(),
+            _lib.stream_handle(dev)), "esa_rmsnorm_unpack_forward")
+    return h, y, rstd
+
+
+def _check_norm_weight(weight: torch.Tensor, dim: int, dtype: torch.dtype) -> None:
+    if weight.shape != (dim,) or weight.dtype != dtype or not weight.is_contiguous():
+        raise ValueError("weight must be a contiguous [dim] tensor of the rows' dtype")
+
+
+def swiglu_forward_packed(gate_up: torch.Tensor, format: str = "int8"):
+    """(out, packed): :func:`swiglu_forward` and gate_up in 8 bits, in one
+    pass.  packed has shape [..., 2, ffn]: the gate and the up half of a row
+    are rows of their own."""
+    code = _pack_code(format)
+    dev = _check_device(gate_up)
+    if gate_up.shape[-1] % 2:
+        raise ValueError("gate_up rows must hold two halves of equal width")
+    ffn = gate_up.shape[-1] // 2
+    n = _rows(gate_up, 2 * ffn)
+    lead = tuple(gate_up.shape[:-1])
+    out = torch.empty(lead + (ffn,), dtype=gate_up.dtype, device=dev)
+    p = _new_packed(lead + (2, ffn), format, gate_up.dtype, dev)
+    lib = _lib.load()
+    with _on(dev):
+        _lib.check(lib.esa_swiglu_pack_forward(
+            _dtype_code(gate_up), code, n, ffn, gate_up.data_ptr(), out.data_ptr(),
+            p.codes.data_ptr(), p.scales.data_ptr(), _lib.stream_handle(dev)),
+            "esa_swiglu_pack_forward")
+    return out, p
+
+
+def swiglu_backward_packed(packed: PackedRows, dout: torch.Tensor, recompute: bool = True):
+    """(d gate_up, output recomputed or None) of SwiGLU at the gate and up
+    values that the codes of :func:`swiglu_forward_packed` stand for."""
+    code = _check_packed(packed)
+    dev = _check_device(packed.codes, packed.scales, dout)
+    if len(packed.shape) < 2 or packed.shape[-2] != 2:
+        raise ValueError("packed must come from swiglu_forward_packed ([..., 2, ffn])")
+    ffn = packed.shape[-1]
+    lead = tuple(packed.shape[:-2])
+    if tuple(dout.shape) != lead + (ffn,) or dout.dtype != packed.dtype:
+        raise ValueError("dout must be [..., ffn] in the packed rows' dtype")
+    dout = dout.contiguous()
+    n = _rows(dout, ffn)
+    dgu = torch.empty(lead + (2 * ffn,), dtype=dout.dtype, device=dev)
+    out = torch.empty_like(dout) if recompute else None
+    lib = _lib.load()
+    with _on(dev):
+        _lib.check(lib.esa_swiglu_unpack_backward(
+            _dtype_code(dout), code, n, ffn, packed.codes.data_ptr(), packed.scales.data_ptr(),
+            dout.data_ptr(), dgu.data_ptr(), _lib.ptr(out), _lib.stream_handle(dev)),
+            "esa_swiglu_unpack_backward")
     return dgu, out

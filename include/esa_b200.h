@@ -150,11 +150,14 @@ typedef struct {
                                      its output row is zero */
 #define ESA_DEVERR_PLAN 8         /* esa_backward was given a key plan built for
                                      another problem; dk / dv not written */
+#define ESA_DEVERR_TOKEN_RANGE 16 /* a token id outside [0, vocab): its embedding
+                                     row is zero and takes no gradient */
 
 /* Library version, e.g. 130 for 0.1.3 (110 added head_offset / pattern_heads
  * to esa_problem_t, the launch trace and the gather probe; 120 the key plan:
  * key_plan / key_plan_bytes in esa_problem_t, esa_key_plan_size / _build;
- * 130 esa_copy_rows). */
+ * 130 esa_copy_rows; 140 the token embedding, the query / key norm and the
+ * 8-bit rows of esa_layer.h). */
 int esa_version(void);
 
 /* Message of the last failing call on this thread ("" if none). */
