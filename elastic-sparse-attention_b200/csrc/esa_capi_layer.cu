@@ -69,7 +69,7 @@ GradPlan grad_plan(int64_t n, int64_t vocab, int32_t dim) {
     g.rows[i] = take(n * 4);
   }
   g.hist = take(g.tiles * em::kRadix * 4);
-  g.owners = take(g.pieces * 4);
+  g.owners = take(g.pieces * sizeof(uint2));
   g.counter = take(4);
   g.part = take((size_t)g.pieces * 2 * dim * sizeof(float));
   g.bytes = at;
@@ -122,13 +122,13 @@ int embedding_grad(int64_t n, int64_t vocab, int32_t dim, const em::Ids& ids, co
   q.scale = scale;
   q.part = reinterpret_cast<float*>(ws + g.part);
   q.counter = p.counter;
-  q.owners = reinterpret_cast<uint32_t*>(ws + g.owners);
+  q.owners = reinterpret_cast<uint2*>(ws + g.owners);
   q.pieces = g.pieces;
   q.zero_blocks = (int)ceil_div(vocab, em::kZeroRows);
   em::grad_pieces_kernel<T><<<dim3((unsigned)(q.zero_blocks + g.pieces), ychunks), em::kGradThreads,
                               0, s>>>(q, static_cast<const T*>(dy), static_cast<T*>(dweight));
   if (int rc = check_launch("esa_embedding_backward (sums)")) return rc;
-  em::grad_join_kernel<T><<<148 * 4, em::kJoinWarps * 32, 0, s>>>(q, static_cast<T*>(dweight));
+  em::grad_join_kernel<T><<<148 * 8, em::kJoinWarps * 32, 0, s>>>(q, static_cast<T*>(dweight));
   return check_launch("esa_embedding_backward (join)");
 }
 

@@ -77,6 +77,7 @@ lookup_kernel(int64_t n, int64_t vocab, uint32_t vpr, Ids ids, const T* __restri
 // each row's list.
 // ---------------------------------------------------------------------------
 constexpr int kGradThreads = 128;
+constexpr int kGradUnroll = 8;  // rows in flight per thread
 constexpr int kGradWarps = kGradThreads / 32;
 constexpr int kDirectMax = 1024;
 constexpr int kDirectPerWarp = kDirectMax / kGradWarps;
@@ -116,23 +117,40 @@ grad_direct_kernel(int n, int64_t vocab, int R, uint32_t vpr, Ids ids, const T* 
   }
   if (lane == 0) count[warp] = c;
   __syncthreads();
-  const uint32_t vec = blockIdx.y * kGradThreads + threadIdx.x;
-  if (vec >= vpr) return;
+  const uint32_t mine_vec = blockIdx.y * kGradThreads + threadIdx.x;
+  const bool active = mine_vec < vpr;
+  const uint32_t vec = active ? mine_vec : 0;     // the warp stays whole for its shuffles
+  constexpr uint32_t lanes = 0xffffffffu;
   for (int r = 0; r < R && v0 + r < vocab; ++r) {
     float acc[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.f;
     for (int wi = 0; wi < kGradWarps; ++wi) {
-      for (int j = 0; j < count[wi]; ++j) {
-        const uint32_t it = list[wi][j];
-        if ((int)(it >> 16) != r) continue;
-        float f[E];
-        V::to_float(ldg16_stream(dy + ((int64_t)(it & 0xffffu) * vpr + vec) * E), f);
+      for (int j0 = 0; j0 < count[wi]; j0 += 32) {
+        const uint32_t it = j0 + lane < count[wi] ? list[wi][j0 + lane] : 0xffffffffu;
+        uint32_t m = __ballot_sync(lanes, (it >> 16) == (uint32_t)r);
+        while (m) {                       // kGradUnroll rows in flight, added in order
+          uint4 x[kGradUnroll];
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] += f[e];
+          for (int u = 0; u < kGradUnroll; ++u) {
+            x[u] = make_uint4(0, 0, 0, 0);
+            if (m) {
+              const uint32_t row = __shfl_sync(lanes, it, __ffs(m) - 1) & 0xffffu;
+              m &= m - 1;
+              x[u] = ldg16_stream(dy + ((int64_t)row * vpr + vec) * E);
+            }
+          }
+#pragma unroll
+          for (int u = 0; u < kGradUnroll; ++u) {
+            float f[E];
+            V::to_float(x[u], f);
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] += f[e];
+          }
+        }
       }
     }
-    store_scaled<T>(dw + ((v0 + r) * vpr + vec) * E, acc, scale);
+    if (active) store_scaled<T>(dw + ((v0 + r) * vpr + vec) * E, acc, scale);
   }
 }
 
@@ -140,16 +158,17 @@ grad_direct_kernel(int n, int64_t vocab, int R, uint32_t vpr, Ids ids, const T* 
 // Gradient, many tokens.  The (token, row) pairs are sorted by token with a
 // stable radix sort (digits of up to 9 bits, low digit first: a histogram and
 // a scatter launch per digit), then the sorted list is cut into pieces of
-// kPiece pairs that are summed independently, so a token's share of the work
-// does not depend on how often it occurs.  A run of one token that crosses a
-// piece border leaves float32 partial sums, which a last launch adds in order.
+// kPiece pairs that are summed independently.  A run of one token of at most
+// kPiece pairs belongs to the piece it starts in; a longer one is cut at the
+// piece borders into float32 partial sums, which a last launch adds in order,
+// so no CTA's share grows with a token's frequency.
 // Tokens that are padding or out of range get the key `vocab` and sort last.
 // ---------------------------------------------------------------------------
 constexpr int kRadixBits = 9;
 constexpr int kRadix = 1 << kRadixBits;
-constexpr int kSortThreads = 256;
+constexpr int kSortThreads = 512;
 constexpr int kSortWarps = kSortThreads / 32;
-constexpr int kSortItems = 8;
+constexpr int kSortItems = 4;
 constexpr int kSortTile = kSortThreads * kSortItems;   // keys of a CTA's inner step
 constexpr int kSortMaxTiles = 512;                     // rows of the histogram table
 constexpr int kPiece = 64;
@@ -175,7 +194,7 @@ struct SortPass {
   uint32_t* hist;             // [gridDim.x][kRadix]
   uint32_t* out_keys;
   uint32_t* out_rows;
-  int* counter;               // crossing runs found later; reset in the first pass
+  int* counter;               // of the long runs found later; reset in the first pass
   int* err;
 };
 
@@ -204,23 +223,21 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(SortPass p) 
   __shared__ uint32_t cnt[kSortWarps][kRadix];
   __shared__ uint32_t wsum[kSortWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr int C = kRadix / kSortThreads;          // digits per thread (consecutive)
-  uint32_t tot[C], before[C], run = 0;
+  static_assert(kRadix == kSortThreads, "a thread per digit");
+  uint32_t tot = 0, before = 0;
+  const uint32_t* h = p.hist + threadIdx.x;
+  for (int k0 = 0; k0 < (int)gridDim.x; k0 += 16) {
+    uint32_t x[16];
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
-    const int d = threadIdx.x * C + c;
-    uint32_t t = 0, b = 0;
-#pragma unroll 4
-    for (int k = 0; k < (int)gridDim.x; ++k) {
-      const uint32_t h = p.hist[(int64_t)k * kRadix + d];
-      t += h;
-      if (k < (int)blockIdx.x) b += h;
+    for (int u = 0; u < 16; ++u)
+      x[u] = k0 + u < (int)gridDim.x ? h[(int64_t)(k0 + u) * kRadix] : 0;
+#pragma unroll
+    for (int u = 0; u < 16; ++u) {
+      tot += x[u];
+      if (k0 + u < (int)blockIdx.x) before += x[u];
     }
-    tot[c] = t;
-    before[c] = b;
-    run += t;
   }
-  uint32_t incl = run;                              // inclusive scan over threads
+  uint32_t incl = tot;                              // inclusive scan over digits
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o);
@@ -228,13 +245,9 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(SortPass p) 
   }
   if (lane == 31) wsum[warp] = incl;
   __syncthreads();
-  uint32_t off = incl - run;
+  uint32_t off = incl - tot;
   for (int w = 0; w < warp; ++w) off += wsum[w];
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-    base[threadIdx.x * C + c] = off + before[c];
-    off += tot[c];
-  }
+  base[threadIdx.x] = off + before;
   const uint32_t mask = (1u << p.bits) - 1;
   const int64_t lo = (int64_t)blockIdx.x * p.tile;
   const int64_t hi = lo + p.tile < p.n ? lo + p.tile : p.n;
@@ -300,15 +313,14 @@ struct GradParams {
   const uint32_t* keys;       // sorted
   const uint32_t* rows;
   float scale;
-  float* part;                // [pieces][2][dim]: head / tail sums of crossing runs
-  int* counter;               // number of crossing runs
-  uint32_t* owners;           // the piece each crossing run starts in
+  float* part;                // [pieces][2][dim]: head / tail sums of long runs
+  int* counter;               // number of long runs
+  uint2* owners;              // each long run's first and last piece
   int64_t pieces;
   int zero_blocks;            // leading CTAs (x) that clear rows of absent tokens
 };
 
 constexpr int kZeroRows = 32;   // rows of dW per clearing CTA
-constexpr int kGradUnroll = 8;  // rows in flight per thread
 
 // grid.x: zero_blocks clearing CTAs, then one CTA per piece; grid.y: 128
 // vectors of the width each.
@@ -317,8 +329,9 @@ __global__ void __launch_bounds__(kGradThreads)
 grad_pieces_kernel(GradParams p, const T* __restrict__ dy, T* __restrict__ dw) {
   using V = Vec<T>;
   constexpr int E = V::kElems;
-  __shared__ uint32_t skey[kPiece + 2];   // keys of the piece and its neighbours
-  __shared__ uint32_t srow[kPiece];
+  __shared__ uint32_t skey[3 * kPiece + 1];   // keys around the piece
+  __shared__ uint32_t srow[2 * kPiece];       // rows of the piece and the next
+  static_assert(kGradThreads >= kPiece + 1 && kZeroRows <= 2 * kPiece, "");
   const uint32_t vec = blockIdx.y * kGradThreads + threadIdx.x;
   const bool active = vec < p.vpr;
   if ((int)blockIdx.x < p.zero_blocks) {
@@ -339,54 +352,66 @@ grad_pieces_kernel(GradParams p, const T* __restrict__ dy, T* __restrict__ dw) {
     return;
   }
   const int64_t piece = blockIdx.x - p.zero_blocks;
-  const int64_t first = piece * kPiece;
-  const uint32_t none = 0xffffffffu;
-  for (int i = threadIdx.x; i < kPiece + 2; i += kGradThreads) {
-    const int64_t at = first + i - 1;
-    skey[i] = at >= 0 && at < p.n ? __ldg(p.keys + at) : none;
-    if (i >= 1 && i <= kPiece && at < p.n) srow[i - 1] = __ldg(p.rows + at);
+  const int64_t a = piece * kPiece;
+  const uint32_t none = 0xffffffffu;      // outside the list, or dropped
+  for (int i = threadIdx.x; i < 3 * kPiece + 1; i += kGradThreads) {
+    const int64_t at = a - kPiece + i;
+    uint32_t key = at >= 0 && at < p.n ? __ldg(p.keys + at) : none;
+    if (key >= (uint32_t)p.vocab) key = none;
+    skey[i] = key;
+    if (i >= kPiece && i < 3 * kPiece && at < p.n) srow[i - kPiece] = __ldg(p.rows + at);
   }
   __syncthreads();
-  // entries of the piece: up to the end of the list or the dropped tokens
-  int len = p.n - first < kPiece ? (int)(p.n - first) : kPiece;
-  while (len > 0 && skey[len] >= (uint32_t)p.vocab) --len;
-  if (len == 0) return;
-  if (blockIdx.y == 0 && threadIdx.x == 0 && len == kPiece && skey[kPiece] == skey[kPiece + 1]) {
-    // the last run crosses into the next piece; listed where it starts (keys
-    // ascend: if the entry before the piece has its key, all of the piece does)
-    const bool starts = skey[0] != skey[kPiece];
-    if (starts) p.owners[atomicAdd(p.counter, 1)] = (uint32_t)piece;
-  }
+  const uint32_t* key = skey + kPiece;    // key[i]: entry a + i, i in [-kPiece, 2 kPiece]
+  if (key[0] == none) return;             // only dropped tokens from here on
+  const int t = threadIdx.x;
+  const int len = __syncthreads_count(t < kPiece && key[t] != none);
+  // entries before and from the piece's first one that share its key (64 + 65 at
+  // most are looked at); the same around its last
+  const int fb = __syncthreads_count(t < kPiece && key[t - kPiece] == key[0]);
+  const int ff = __syncthreads_count(t <= kPiece && key[t] == key[0]);
+  const int lb = __syncthreads_count(t < kPiece && key[len - 1 - t] == key[len - 1]);
+  const int lf = __syncthreads_count(t < kPiece && key[len + t] == key[len - 1]);
+  const bool long_first = fb + ff > kPiece, long_last = lb + lf > kPiece;
+  const int i0 = !long_first && fb > 0 ? ff : 0;           // skip a short run begun earlier
+  const int i1 = !long_last ? len + lf : len;              // finish a short run begun here
+  // a long run at the end that goes on; listed where it starts
+  const bool cut = long_last && lf > 0;
+  const bool starts = lb < len || key[-1] != key[0];
+  if (cut && starts && blockIdx.y == 0 && t == 0)
+    p.owners[atomicAdd(p.counter, 1)] =
+        make_uint2((uint32_t)piece,
+                   (uint32_t)((lower_bound(p.keys, p.n, key[len - 1] + 1) - 1) / kPiece));
   if (!active) return;
   const int64_t dim = (int64_t)p.vpr * E;
-  bool head = skey[0] == skey[1];         // the first run began in an earlier piece
+  bool head = long_first && fb > 0;       // the first run's sum is one of several
   float acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  for (int j0 = 0; j0 < len; j0 += kGradUnroll) {
+  for (int j0 = i0; j0 < i1; j0 += kGradUnroll) {
     uint4 x[kGradUnroll];
 #pragma unroll
     for (int u = 0; u < kGradUnroll; ++u)
-      if (j0 + u < len) x[u] = ldg16_stream(dy + ((int64_t)srow[j0 + u] * p.vpr + vec) * E);
+      if (j0 + u < i1) x[u] = ldg16_stream(dy + ((int64_t)srow[j0 + u] * p.vpr + vec) * E);
 #pragma unroll
     for (int u = 0; u < kGradUnroll; ++u) {
       const int j = j0 + u;
-      if (j < len) {
+      if (j < i1) {
         float f[E];
         V::to_float(x[u], f);
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] += f[e];
-        const uint32_t key = skey[j + 1];
-        const bool more = skey[j + 2] == key;
-        if (!more || j + 1 == len) {
-          if (head || more) {
+        const bool last = j + 1 == i1;
+        if (last || key[j + 1] != key[j]) {
+          const bool tail = last && cut;
+          if (head || tail) {
             float* dst = p.part + (piece * 2 + (head ? 0 : 1)) * dim + (int64_t)vec * E;
 #pragma unroll
             for (int e = 0; e < E; e += 4)
               *reinterpret_cast<float4*>(dst + e) =
                   make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
           } else {
-            store_scaled<T>(dw + ((int64_t)key * p.vpr + vec) * E, acc, p.scale);
+            store_scaled<T>(dw + ((int64_t)key[j] * p.vpr + vec) * E, acc, p.scale);
           }
           head = false;
 #pragma unroll
@@ -397,43 +422,55 @@ grad_pieces_kernel(GradParams p, const T* __restrict__ dy, T* __restrict__ dw) {
   }
 }
 
-// Joins the partial sums of the runs that cross pieces.  A task is (run, 128
-// columns); its warps take every kJoinWarps-th partial, then add up in order.
+// Joins the partial sums of the long runs.  A task is (run, 512 columns); its
+// warps take every kJoinWarps-th partial, then warp 0 adds theirs in order.
 constexpr int kJoinWarps = 8;
+constexpr int kJoinVecs = 4;                     // float4 per lane
+constexpr int kJoinCols = 128 * kJoinVecs;
+
+__device__ __forceinline__ void add4(float4& a, const float4& x) {
+  a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
+}
 
 template <typename T>
 __global__ void __launch_bounds__(kJoinWarps * 32)
 grad_join_kernel(GradParams p, T* __restrict__ dw) {
-  __shared__ float4 sum[kJoinWarps][32];
+  __shared__ float4 sum[kJoinWarps][kJoinVecs][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t dim = (int64_t)p.vpr * Vec<T>::kElems;
-  const int64_t chunks = (dim + 127) / 128;
+  const int64_t chunks = (dim + kJoinCols - 1) / kJoinCols;
   const int64_t tasks = (int64_t)*p.counter * chunks;
   for (int64_t t = blockIdx.x; t < tasks; t += gridDim.x) {
-    const int64_t piece = p.owners[t / chunks];
-    const int64_t col = (t % chunks) * 128 + lane * 4;
+    const uint2 run = p.owners[t / chunks];
+    const int64_t piece = run.x, last = run.y;
+    const int64_t col = (t % chunks) * kJoinCols + lane * 4;
     const uint32_t key = p.keys[piece * kPiece + kPiece - 1];
-    const int64_t last = (lower_bound(p.keys, p.n, key + 1) - 1) / kPiece;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (col < dim) {
-      for (int64_t q = piece + warp; q <= last; q += kJoinWarps) {
-        const float4 x = *reinterpret_cast<const float4*>(
-            p.part + (q * 2 + (q == piece ? 1 : 0)) * dim + col);
-        a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
-      }
+    float4 a[kJoinVecs];
+#pragma unroll
+    for (int v = 0; v < kJoinVecs; ++v) a[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+    // slot 1 of the piece it starts in, slot 0 of each later one it reaches
+#pragma unroll 4
+    for (int64_t q = piece + warp; q <= last; q += kJoinWarps) {
+      const float* src = p.part + (q * 2 + (q == piece ? 1 : 0)) * dim + col;
+#pragma unroll
+      for (int v = 0; v < kJoinVecs; ++v)
+        if (col + v * 128 < dim) add4(a[v], *reinterpret_cast<const float4*>(src + v * 128));
     }
-    sum[warp][lane] = a;
+#pragma unroll
+    for (int v = 0; v < kJoinVecs; ++v) sum[warp][v][lane] = a[v];
     __syncthreads();
-    if (warp == 0 && col < dim) {
-      for (int w = 1; w < kJoinWarps; ++w) {
-        const float4 x = sum[w][lane];
-        a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
+    if (warp < kJoinVecs) {
+      const int64_t c = col + warp * 128;
+      float4 o = sum[0][warp][lane];
+#pragma unroll
+      for (int w = 1; w < kJoinWarps; ++w) add4(o, sum[w][warp][lane]);
+      if (c < dim) {
+        T* dst = dw + (int64_t)key * dim + c;
+        dst[0] = from_f32<T>(o.x * p.scale);
+        dst[1] = from_f32<T>(o.y * p.scale);
+        dst[2] = from_f32<T>(o.z * p.scale);
+        dst[3] = from_f32<T>(o.w * p.scale);
       }
-      T* dst = dw + (int64_t)key * dim + col;
-      dst[0] = from_f32<T>(a.x * p.scale);
-      dst[1] = from_f32<T>(a.y * p.scale);
-      dst[2] = from_f32<T>(a.z * p.scale);
-      dst[3] = from_f32<T>(a.w * p.scale);
     }
     __syncthreads();
   }
