@@ -125,8 +125,10 @@ int embedding_grad(int64_t n, int64_t vocab, int32_t dim, const em::Ids& ids, co
   q.owners = reinterpret_cast<uint2*>(ws + g.owners);
   q.pieces = g.pieces;
   q.zero_blocks = (int)ceil_div(vocab, em::kZeroRows);
-  em::grad_pieces_kernel<T><<<dim3((unsigned)(q.zero_blocks + g.pieces), ychunks), em::kGradThreads,
-                              0, s>>>(q, static_cast<const T*>(dy), static_cast<T*>(dweight));
+  q.ychunks = (int)ychunks;
+  const int64_t ctas = (q.zero_blocks + g.pieces) * ychunks;
+  if (ctas > INT32_MAX) return fail(ESA_ERR_UNSUPPORTED, "esa_embedding_backward: too many tokens");
+  em::grad_pieces_kernel<T><<<(unsigned)ctas, em::kGradThreads, 0, s>>>(q, static_cast<const T*>(dy), static_cast<T*>(dweight));
   if (int rc = check_launch("esa_embedding_backward (sums)")) return rc;
   em::grad_join_kernel<T><<<148 * 8, em::kJoinWarps * 32, 0, s>>>(q, static_cast<T*>(dweight));
   return check_launch("esa_embedding_backward (join)");

@@ -317,13 +317,16 @@ struct GradParams {
   int* counter;               // number of long runs
   uint2* owners;              // each long run's first and last piece
   int64_t pieces;
-  int zero_blocks;            // leading CTAs (x) that clear rows of absent tokens
+  int zero_blocks;            // items that clear rows of absent tokens
+  int ychunks;                // CTAs per item
 };
 
 constexpr int kZeroRows = 32;   // rows of dW per clearing CTA
 
-// grid.x: zero_blocks clearing CTAs, then one CTA per piece; grid.y: 128
-// vectors of the width each.
+// One CTA per item and 128 vectors of the width, the CTAs of an item side by
+// side so that a row's parts are read together.  Items are the pieces with the
+// clearing of absent rows spread evenly among them: its searches would leave
+// HBM idle if they came first.
 template <typename T>
 __global__ void __launch_bounds__(kGradThreads)
 grad_pieces_kernel(GradParams p, const T* __restrict__ dy, T* __restrict__ dw) {
@@ -332,10 +335,14 @@ grad_pieces_kernel(GradParams p, const T* __restrict__ dy, T* __restrict__ dw) {
   __shared__ uint32_t skey[3 * kPiece + 1];   // keys around the piece
   __shared__ uint32_t srow[2 * kPiece];       // rows of the piece and the next
   static_assert(kGradThreads >= kPiece + 1 && kZeroRows <= 2 * kPiece, "");
-  const uint32_t vec = blockIdx.y * kGradThreads + threadIdx.x;
+  const int64_t item = blockIdx.x / p.ychunks;
+  const uint32_t chunk = (uint32_t)(blockIdx.x - item * p.ychunks);
+  const uint32_t vec = chunk * kGradThreads + threadIdx.x;
   const bool active = vec < p.vpr;
-  if ((int)blockIdx.x < p.zero_blocks) {
-    const int64_t v0 = (int64_t)blockIdx.x * kZeroRows;
+  const int64_t items = p.pieces + p.zero_blocks;
+  const int64_t zeros = item * p.zero_blocks / items;     // clearing items before this one
+  if ((item + 1) * p.zero_blocks / items > zeros) {
+    const int64_t v0 = zeros * kZeroRows;
     if (threadIdx.x < kZeroRows) {
       const int64_t v = v0 + threadIdx.x;
       uint32_t absent = 0;
@@ -351,7 +358,7 @@ grad_pieces_kernel(GradParams p, const T* __restrict__ dy, T* __restrict__ dw) {
         if (srow[r]) stg16(dw + ((v0 + r) * p.vpr + vec) * E, make_uint4(0, 0, 0, 0));
     return;
   }
-  const int64_t piece = blockIdx.x - p.zero_blocks;
+  const int64_t piece = item - zeros;
   const int64_t a = piece * kPiece;
   const uint32_t none = 0xffffffffu;      // outside the list, or dropped
   for (int i = threadIdx.x; i < 3 * kPiece + 1; i += kGradThreads) {
@@ -378,7 +385,7 @@ grad_pieces_kernel(GradParams p, const T* __restrict__ dy, T* __restrict__ dw) {
   // a long run at the end that goes on; listed where it starts
   const bool cut = long_last && lf > 0;
   const bool starts = lb < len || key[-1] != key[0];
-  if (cut && starts && blockIdx.y == 0 && t == 0)
+  if (cut && starts && chunk == 0 && t == 0)
     p.owners[atomicAdd(p.counter, 1)] =
         make_uint2((uint32_t)piece,
                    (uint32_t)((lower_bound(p.keys, p.n, key[len - 1] + 1) - 1) / kPiece));
