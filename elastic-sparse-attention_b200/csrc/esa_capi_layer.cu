@@ -106,10 +106,17 @@ int embedding_grad(int64_t n, int64_t vocab, int32_t dim, const em::Ids& ids, co
     p.shift = i * g.bits;
     p.out_keys = reinterpret_cast<uint32_t*>(ws + g.keys[i & 1]);
     p.out_rows = reinterpret_cast<uint32_t*>(ws + g.rows[i & 1]);
-    em::sort_hist_kernel<<<(unsigned)g.tiles, em::kSortThreads, 0, s>>>(p);
-    if (int rc = check_launch("esa_embedding_backward (histogram)")) return rc;
-    em::sort_scatter_kernel<<<(unsigned)g.tiles, em::kSortThreads, 0, s>>>(p);
-    if (int rc = check_launch("esa_embedding_backward (sort)")) return rc;
+    const dim3 grid((unsigned)g.tiles), block(em::kSortThreads);
+    if (i == 0) {
+      em::sort_hist_kernel<<<grid, block, 0, s>>>(p);
+      if (int rc = check_launch("esa_embedding_backward (histogram)")) return rc;
+    } else if (int rc = launch_after("esa_embedding_backward (histogram)", em::sort_hist_kernel,
+                                     grid, block, s, p)) {
+      return rc;
+    }
+    if (int rc = launch_after("esa_embedding_backward (sort)", em::sort_scatter_kernel, grid, block,
+                              s, p))
+      return rc;
     p.keys = p.out_keys;
     p.rows = p.out_rows;
   }
@@ -128,10 +135,12 @@ int embedding_grad(int64_t n, int64_t vocab, int32_t dim, const em::Ids& ids, co
   q.ychunks = (int)ychunks;
   const int64_t ctas = (q.zero_blocks + g.pieces) * ychunks;
   if (ctas > INT32_MAX) return fail(ESA_ERR_UNSUPPORTED, "esa_embedding_backward: too many tokens");
-  em::grad_pieces_kernel<T><<<(unsigned)ctas, em::kGradThreads, 0, s>>>(q, static_cast<const T*>(dy), static_cast<T*>(dweight));
-  if (int rc = check_launch("esa_embedding_backward (sums)")) return rc;
-  em::grad_join_kernel<T><<<148 * 8, em::kJoinWarps * 32, 0, s>>>(q, static_cast<T*>(dweight));
-  return check_launch("esa_embedding_backward (join)");
+  if (int rc = launch_after("esa_embedding_backward (sums)", em::grad_pieces_kernel<T>,
+                            dim3((unsigned)ctas), dim3(em::kGradThreads), s, q,
+                            static_cast<const T*>(dy), static_cast<T*>(dweight)))
+    return rc;
+  return launch_after("esa_embedding_backward (join)", em::grad_join_kernel<T>, dim3(148 * 8),
+                      dim3(em::kJoinWarps * 32), s, q, static_cast<T*>(dweight));
 }
 
 // ---------------------------------------------------------------------------

@@ -201,7 +201,9 @@ struct SortPass {
 // hist[tile][digit] of one pass.
 __global__ void __launch_bounds__(kSortThreads) sort_hist_kernel(SortPass p) {
   __shared__ uint32_t h[kRadix];
+  cudaTriggerProgrammaticLaunchCompletion();   // the next launch may take free SMs
   for (int i = threadIdx.x; i < kRadix; i += kSortThreads) h[i] = 0;
+  cudaGridDependencySynchronize();
   if (!p.keys && blockIdx.x == 0 && threadIdx.x == 0) *p.counter = 0;
   __syncthreads();
   const int64_t lo = (int64_t)blockIdx.x * p.tile;
@@ -223,16 +225,18 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(SortPass p) 
   __shared__ uint32_t cnt[kSortWarps][kRadix];
   __shared__ uint32_t wsum[kSortWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  cudaTriggerProgrammaticLaunchCompletion();
+  cudaGridDependencySynchronize();
   static_assert(kRadix == kSortThreads, "a thread per digit");
   uint32_t tot = 0, before = 0;
   const uint32_t* h = p.hist + threadIdx.x;
-  for (int k0 = 0; k0 < (int)gridDim.x; k0 += 16) {
-    uint32_t x[16];
+  for (int k0 = 0; k0 < (int)gridDim.x; k0 += 32) {
+    uint32_t x[32];
 #pragma unroll
-    for (int u = 0; u < 16; ++u)
+    for (int u = 0; u < 32; ++u)
       x[u] = k0 + u < (int)gridDim.x ? h[(int64_t)(k0 + u) * kRadix] : 0;
 #pragma unroll
-    for (int u = 0; u < 16; ++u) {
+    for (int u = 0; u < 32; ++u) {
       tot += x[u];
       if (k0 + u < (int)blockIdx.x) before += x[u];
     }
@@ -335,6 +339,8 @@ grad_pieces_kernel(GradParams p, const T* __restrict__ dy, T* __restrict__ dw) {
   __shared__ uint32_t skey[3 * kPiece + 1];   // keys around the piece
   __shared__ uint32_t srow[2 * kPiece];       // rows of the piece and the next
   static_assert(kGradThreads >= kPiece + 1 && kZeroRows <= 2 * kPiece, "");
+  cudaTriggerProgrammaticLaunchCompletion();
+  cudaGridDependencySynchronize();
   const int64_t item = blockIdx.x / p.ychunks;
   const uint32_t chunk = (uint32_t)(blockIdx.x - item * p.ychunks);
   const uint32_t vec = chunk * kGradThreads + threadIdx.x;
@@ -446,6 +452,7 @@ grad_join_kernel(GradParams p, T* __restrict__ dw) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t dim = (int64_t)p.vpr * Vec<T>::kElems;
   const int64_t chunks = (dim + kJoinCols - 1) / kJoinCols;
+  cudaGridDependencySynchronize();
   const int64_t tasks = (int64_t)*p.counter * chunks;
   for (int64_t t = blockIdx.x; t < tasks; t += gridDim.x) {
     const uint2 run = p.owners[t / chunks];

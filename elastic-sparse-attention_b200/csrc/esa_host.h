@@ -33,6 +33,30 @@ inline bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 1
 __attribute__((visibility("hidden"))) int check_rows_op(const char* what, int32_t dtype,
                                                         int64_t n_rows, int32_t dim);
 
+// Launches `kernel` so that its CTAs may be placed while the kernel before it
+// in the stream still runs (programmatic dependent launch).  The kernel calls
+// cudaGridDependencySynchronize() before it touches memory, which waits for
+// that kernel's end; what is saved is the launch latency between the two.
+template <typename... P, typename... A>
+int launch_after(const char* what, void (*kernel)(P...), dim3 grid, dim3 block, cudaStream_t s,
+                 A... args) {
+  cudaLaunchConfig_t c = {};
+  c.gridDim = grid;
+  c.blockDim = block;
+  c.stream = s;
+  cudaLaunchAttribute a[1];
+  a[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  a[0].val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = a;
+  c.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&c, kernel, P(args)...);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(ESA_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+  }
+  return ESA_OK;
+}
+
 template <typename F>
 int by_dtype(int32_t dtype, F&& f) {
   switch (dtype) {
