@@ -199,20 +199,29 @@ int by_threads_per_row(int tpr, F&& f) {
     case 2: return f(std::integral_constant<int, 2>{});
     case 4: return f(std::integral_constant<int, 4>{});
     case 8: return f(std::integral_constant<int, 8>{});
-    default: return f(std::integral_constant<int, 16>{});
+    case 16: return f(std::integral_constant<int, 16>{});
+    default: return f(std::integral_constant<int, 32>{});
   }
 }
 
-// Heads per warp task: all of a token's heads once there are tokens enough for
-// 16 warps per SM, a single round of the warp for few tokens.
+// Rounds per warp task: all of a token's once there are tokens enough for 16
+// warps per SM, fewer (down to one) for few tokens.
+int rounds_per_task(int rounds, int64_t tokens) {
+  if (rounds == 0) return 1;
+  const int64_t tasks = std::max<int64_t>(1, std::min<int64_t>(rounds, ceil_div(148 * 16, tokens)));
+  return (int)ceil_div(rounds, tasks);
+}
+
 template <typename T>
 void set_tasks(qk::Params<T>& p, int rows_per_warp) {
-  const int most = std::max(p.q.H, p.k.H);
-  int hpt = rows_per_warp;
-  while (hpt < most && p.tokens * ceil_div(most, 2 * hpt) >= 148 * 16) hpt *= 2;
-  p.hpt = hpt;
-  p.cq = (int)ceil_div(p.q.H, hpt);
-  p.ck = (int)ceil_div(p.k.H, hpt);
+  p.rq = (int)ceil_div(p.q.H, rows_per_warp);
+  p.rk = (int)ceil_div(p.k.H, rows_per_warp);
+  p.rpt = rounds_per_task(p.rq + p.rk, p.tokens);
+  p.tasks = (int)ceil_div(p.rq + p.rk, p.rpt);
+  p.rpt_q = rounds_per_task(p.rq, p.tokens);
+  p.rpt_k = rounds_per_task(p.rk, p.tokens);
+  p.tasks_q = (int)ceil_div(p.rq, p.rpt_q);
+  p.tasks_k = (int)ceil_div(p.rk, p.rpt_k);
 }
 
 int qk_bwd_ctas(int64_t tokens, int32_t hq, int32_t hk) {
@@ -357,7 +366,7 @@ int esa_qk_norm_rope_forward(int32_t dtype, int32_t batch, int64_t seq_len, int3
     p.eps = eps;
     const int tpr = head_dim / (2 * esa::Vec<T>::kElems);
     set_tasks(p, 32 / tpr);
-    const int64_t ctas = ceil_div(p.tokens * (p.cq + p.ck), qk::kWarps);
+    const int64_t ctas = ceil_div(p.tokens * p.tasks, qk::kWarps);
     if (ctas > INT32_MAX)
       return fail(ESA_ERR_UNSUPPORTED, "esa_qk_norm_rope_forward: too many positions");
     return by_threads_per_row(tpr, [&](auto t) {
@@ -415,7 +424,7 @@ int esa_qk_norm_rope_backward(int32_t dtype, int32_t batch, int64_t seq_len, int
     p.pos_sb = positions_stride_b;
     p.inv_freq = inv_freq;
     p.eps = eps;
-    const int tpr = head_dim / (2 * esa::Vec<T>::kElems);
+    const int tpr = head_dim / 8;   // four elements of each half per thread
     set_tasks(p, 32 / tpr);
     const int ctas = qk_bwd_ctas(p.tokens, num_q_heads, num_k_heads);
     const int q_ctas = qk_q_ctas(ctas, num_q_heads, num_k_heads);

@@ -9,11 +9,16 @@
 //
 //   dx = rstd * (w dn - xh mean(xh w dn)),   dw = sum over rows of dn xh
 //
-// A row is held by D / (2 E) threads (E elements per 16-byte vector): thread t
-// owns elements [tE, tE + E) and the same of the second half, so the rotation
-// needs no exchange.  A warp takes several heads of one token, so the angles
-// are formed once per token and thread.  HBM-bound: every element is read and
-// written once; rstd is formed again in the backward instead of being kept.
+// A row is held by D / (2 E) threads: thread t owns elements [tE, tE + E) and
+// the same of the second half, so the rotation needs no exchange.  The forward
+// has E = one 16-byte vector.  The backward, which holds twice the operands
+// and the weight gradient's sums, has E = 4, so that several rounds fit in the
+// registers of 16 warps per SM.  A warp takes the heads of one token, 32 / threads-per-row
+// at a time (a round), and loads kUnroll rounds before it works on the first:
+// the kernels are HBM-bound (every element is read and written once) and need
+// that many bytes in flight.  The D / 2 angles of a token are formed once,
+// spread over the warp's lanes, and shared through shared memory.  rstd is
+// formed again in the backward instead of being kept.
 #pragma once
 #include "esa_common.cuh"
 
@@ -37,8 +42,9 @@ struct Params {
   int64_t pos_sb;                     // 0: positions shared by the batch
   const float* inv_freq;
   float eps;
-  int hpt;                            // heads per warp task
-  int cq, ck;                         // tasks per token of the query / key heads
+  int rq, rk;                         // rounds of the query / key heads
+  int rpt, tasks;                     // forward: rounds per warp task, tasks per token
+  int rpt_q, rpt_k, tasks_q, tasks_k; // backward: the same for each side
 };
 
 // cos and sin of p * f: the product in float64 (p and f are exact there), in
@@ -58,6 +64,96 @@ __device__ __forceinline__ float row_sum(float v) {
 
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
+constexpr int kFwdUnroll = 4;
+constexpr int kBwdUnroll = 4;
+
+// Two float32 values and their packed arithmetic (one instruction for both).
+struct F2 { unsigned long long v; };
+__device__ __forceinline__ F2 f2(float lo, float hi) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void split(F2 a, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(a.v));
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
+// Sums of a and b over the TPR lanes of a row, both on every lane: even lanes
+// carry a through the levels, odd lanes b, so the pair costs one shuffle per
+// level and one more.
+template <int TPR>
+__device__ __forceinline__ void row_sum2(float& a, float& b) {
+  if constexpr (TPR == 1) return;
+  const bool odd = threadIdx.x & 1;
+  float mine = (odd ? b : a) + __shfl_xor_sync(0xffffffffu, odd ? a : b, 1);
+#pragma unroll
+  for (int o = 2; o < TPR; o <<= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  const float other = __shfl_xor_sync(0xffffffffu, mine, 1);
+  a = odd ? other : mine;
+  b = odd ? mine : other;
+}
+
+// E = 4 elements of T: 8 bytes of a 16-bit type, 16 of float32.
+template <typename T> struct Quad {
+  using Raw = uint2;
+  __device__ __forceinline__ static void to_float(const Raw& r, F2 (&f)[2]) {
+    float t[8];
+    Vec<T>::to_float(make_uint4(r.x, r.y, 0, 0), t);
+    f[0] = f2(t[0], t[1]);
+    f[1] = f2(t[2], t[3]);
+  }
+  __device__ __forceinline__ static Raw from_float(const F2 (&f)[2]) {
+    float t[4];
+    split(f[0], t[0], t[1]);
+    split(f[1], t[2], t[3]);
+    return make_uint2(Vec<T>::pack(t[0], t[1]), Vec<T>::pack(t[2], t[3]));
+  }
+  __device__ __forceinline__ static Raw zero() { return make_uint2(0, 0); }
+};
+template <> struct Quad<float> {
+  using Raw = uint4;
+  __device__ __forceinline__ static void to_float(const Raw& r, F2 (&f)[2]) {
+    f[0] = f2(__uint_as_float(r.x), __uint_as_float(r.y));
+    f[1] = f2(__uint_as_float(r.z), __uint_as_float(r.w));
+  }
+  __device__ __forceinline__ static Raw from_float(const F2 (&f)[2]) {
+    float t[4];
+    split(f[0], t[0], t[1]);
+    split(f[1], t[2], t[3]);
+    return Vec<float>::from_float(t);
+  }
+  __device__ __forceinline__ static Raw zero() { return make_uint4(0, 0, 0, 0); }
+};
+
+// cos and sin of the token at `pos` for this thread's elements, by way of the
+// warp's row cs_of_warp (cos of each angle, then sin).
+template <int D, int E>
+__device__ __forceinline__ void token_rotation(int64_t pos, const float* inv_freq, int lane, int i0,
+                                               float* cs_of_warp, float (&cs)[E], float (&sn)[E]) {
+  __syncwarp();      // the row's last readers are done
+  for (int i = lane; i < D / 2; i += 32) {
+    float c, s;
+    rotation(pos, inv_freq[i], c, s);
+    cs_of_warp[i] = c;
+    cs_of_warp[D / 2 + i] = s;
+  }
+  __syncwarp();
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    cs[e] = cs_of_warp[i0 + e];
+    sn[e] = cs_of_warp[D / 2 + i0 + e];
+  }
+}
 
 template <typename T, int TPR>
 __global__ void __launch_bounds__(kThreads) fwd_kernel(Params<T> p) {
@@ -65,46 +161,65 @@ __global__ void __launch_bounds__(kThreads) fwd_kernel(Params<T> p) {
   constexpr int E = V::kElems;
   constexpr int RPW = 32 / TPR;               // rows a warp holds at once
   constexpr int D = 2 * E * TPR;
-  const int lane = threadIdx.x & 31;
-  const int64_t task = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
-  const int64_t tok = task / (p.cq + p.ck);
+  constexpr int U = kFwdUnroll;
+  __shared__ float table[kWarps][D];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t task = (int64_t)blockIdx.x * kWarps + warp;
+  const int64_t tok = task / p.tasks;
   if (tok >= p.tokens) return;
-  int c = (int)(task - tok * (p.cq + p.ck));
-  const bool is_q = c < p.cq;
-  const Heads<T>& s = is_q ? p.q : p.k;
-  if (!is_q) c -= p.cq;
   const int64_t b = tok / p.L, l = tok - b * p.L;
-  const int i0 = (lane % TPR) * E;
-  const int64_t pos = p.pos ? p.pos[b * p.pos_sb + l] : l;
-  float cs[E], sn[E], w1[E], w2[E];
+  const int i0 = (lane % TPR) * E, hl = lane / TPR;
+  const int lo = (int)(task - tok * p.tasks) * p.rpt;
+  const int hi = min(lo + p.rpt, p.rq + p.rk);
+  float cs[E], sn[E];
+  bool first = true;
+  for (int r0 = lo; r0 < hi; r0 += U) {
+    uint4 x1[U], x2[U];
 #pragma unroll
-  for (int e = 0; e < E; ++e) rotation(pos, p.inv_freq[i0 + e], cs[e], sn[e]);
-  V::to_float(ldg16(s.w + i0), w1);
-  V::to_float(ldg16(s.w + D / 2 + i0), w2);
-  const int h1 = min((c + 1) * p.hpt, s.H);
-  for (int h0 = c * p.hpt; h0 < h1; h0 += RPW) {
-    const int h = h0 + lane / TPR;
-    const bool in = h < h1;
-    float x1[E], x2[E], ss = 0.f;
-    const T* row = s.x + b * s.xb + (int64_t)h * s.xh + l * s.xs;
-    if (in) {
-      V::to_float(*reinterpret_cast<const uint4*>(row + i0), x1);
-      V::to_float(*reinterpret_cast<const uint4*>(row + D / 2 + i0), x2);
-#pragma unroll
-      for (int e = 0; e < E; ++e) ss = fmaf(x1[e], x1[e], fmaf(x2[e], x2[e], ss));
-    }
-    const float rs = rsqrtf(row_sum<TPR>(ss) * (1.f / D) + p.eps);
-    if (in) {
-      float o1[E], o2[E];
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const float n1 = x1[e] * rs * w1[e], n2 = x2[e] * rs * w2[e];
-        o1[e] = n1 * cs[e] - n2 * sn[e];
-        o2[e] = n2 * cs[e] + n1 * sn[e];
+    for (int u = 0; u < U; ++u) {
+      const int r = r0 + u;
+      const bool is_q = r < p.rq;
+      const Heads<T>& s = is_q ? p.q : p.k;
+      const int h = (is_q ? r : r - p.rq) * RPW + hl;
+      x1[u] = x2[u] = make_uint4(0, 0, 0, 0);
+      if (r < hi && h < s.H) {
+        const T* row = s.x + b * s.xb + (int64_t)h * s.xh + l * s.xs + i0;
+        x1[u] = *reinterpret_cast<const uint4*>(row);
+        x2[u] = *reinterpret_cast<const uint4*>(row + D / 2);
       }
-      T* out = s.o + b * s.ob + (int64_t)h * s.oh + l * s.os;
-      stg16(out + i0, V::from_float(o1));
-      stg16(out + D / 2 + i0, V::from_float(o2));
+    }
+    if (first) {       // while the first rows are on their way
+      const int64_t pos = p.pos ? p.pos[b * p.pos_sb + l] : l;
+      token_rotation<D, E>(pos, p.inv_freq, lane, i0, table[warp], cs, sn);
+      first = false;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int r = r0 + u;
+      if (r >= hi) break;
+      const bool is_q = r < p.rq;
+      const Heads<T>& s = is_q ? p.q : p.k;
+      const int h = (is_q ? r : r - p.rq) * RPW + hl;
+      float a1[E], a2[E], ss = 0.f;
+      V::to_float(x1[u], a1);
+      V::to_float(x2[u], a2);
+#pragma unroll
+      for (int e = 0; e < E; ++e) ss = fmaf(a1[e], a1[e], fmaf(a2[e], a2[e], ss));
+      const float rs = rsqrtf(row_sum<TPR>(ss) * (1.f / D) + p.eps);
+      if (h < s.H) {
+        float w1[E], w2[E], o1[E], o2[E];
+        V::to_float(ldg16(s.w + i0), w1);
+        V::to_float(ldg16(s.w + D / 2 + i0), w2);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float n1 = a1[e] * rs * w1[e], n2 = a2[e] * rs * w2[e];
+          o1[e] = n1 * cs[e] - n2 * sn[e];
+          o2[e] = n2 * cs[e] + n1 * sn[e];
+        }
+        T* out = s.o + b * s.ob + (int64_t)h * s.oh + l * s.os + i0;
+        stg16(out, V::from_float(o1));
+        stg16(out + D / 2, V::from_float(o2));
+      }
     }
   }
 }
@@ -112,88 +227,130 @@ __global__ void __launch_bounds__(kThreads) fwd_kernel(Params<T> p) {
 // Backward: CTAs [0, q_ctas) stride over the query tasks, the others over the
 // key tasks, so a CTA sums one weight gradient; part[cta][D].
 template <typename T, int TPR>
-__global__ void __launch_bounds__(kThreads) bwd_kernel(Params<T> p, int q_ctas, float* part) {
-  using V = Vec<T>;
-  constexpr int E = V::kElems;
+__global__ void __launch_bounds__(kThreads, 4) bwd_kernel(Params<T> p, int q_ctas, float* part) {
+  using V = Quad<T>;
+  using Raw = typename V::Raw;
+  constexpr int E = 4;
   constexpr int RPW = 32 / TPR;
   constexpr int D = 2 * E * TPR;
-  __shared__ float red[kWarps][D];
+  constexpr int U = kBwdUnroll;
+  __shared__ float red[kWarps][D];            // angles of the warps' tokens, then sums
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const bool is_q = (int)blockIdx.x < q_ctas;
   const Heads<T>& s = is_q ? p.q : p.k;
-  const int chunks = is_q ? p.cq : p.ck;
+  const int per_tok = is_q ? p.tasks_q : p.tasks_k, rpt = is_q ? p.rpt_q : p.rpt_k;
+  const int rounds = is_q ? p.rq : p.rk;
   const int64_t cta = is_q ? blockIdx.x : blockIdx.x - q_ctas;
   const int64_t ctas = is_q ? q_ctas : gridDim.x - q_ctas;
-  const int i0 = (lane % TPR) * E;
-  float w1[E], w2[E], a1[E], a2[E];
-  V::to_float(ldg16(s.w + i0), w1);
-  V::to_float(ldg16(s.w + D / 2 + i0), w2);
+  const int i0 = (lane % TPR) * E, hl = lane / TPR;
+  F2 w1[2], w2[2], a1[2], a2[2];
+  V::to_float(__ldg(reinterpret_cast<const Raw*>(s.w + i0)), w1);
+  V::to_float(__ldg(reinterpret_cast<const Raw*>(s.w + D / 2 + i0)), w2);
 #pragma unroll
-  for (int e = 0; e < E; ++e) a1[e] = a2[e] = 0.f;
-  const int64_t tasks = p.tokens * chunks;
+  for (int v = 0; v < 2; ++v) a1[v] = a2[v] = f2(0.f, 0.f);
+  const int64_t xstep = RPW * s.xh, dstep = RPW * s.dh, ostep = RPW * s.oh;
+  const int64_t tasks = p.tokens * per_tok;
   for (int64_t task = cta * kWarps + warp; task < tasks; task += ctas * kWarps) {
-    const int64_t tok = task / chunks;
-    const int c = (int)(task - tok * chunks);
+    const int64_t tok = task / per_tok;
     const int64_t b = tok / p.L, l = tok - b * p.L;
-    const int64_t pos = p.pos ? p.pos[b * p.pos_sb + l] : l;
-    float cs[E], sn[E];
+    const int lo = (int)(task - tok * per_tok) * rpt, hi = min(lo + rpt, rounds);
+    const int64_t h0 = (int64_t)lo * RPW + hl;
+    const T* xp = s.x + b * s.xb + h0 * s.xh + l * s.xs + i0;
+    const T* dp = s.d + b * s.db + h0 * s.dh + l * s.ds + i0;
+    T* op = s.o + b * s.ob + h0 * s.oh + l * s.os + i0;
+    F2 cs[2], sn[2], ns[2];
+    bool first = true;
+    for (int r0 = lo; r0 < hi; r0 += U) {
+      Raw x1[U], x2[U], d1[U], d2[U];
 #pragma unroll
-    for (int e = 0; e < E; ++e) rotation(pos, p.inv_freq[i0 + e], cs[e], sn[e]);
-    const int h1 = min((c + 1) * p.hpt, s.H);
-    for (int h0 = c * p.hpt; h0 < h1; h0 += RPW) {
-      const int h = h0 + lane / TPR;
-      const bool in = h < h1;
-      float x1[E], x2[E], g1[E], g2[E], ss = 0.f, dot = 0.f;
-      if (in) {
-        const T* row = s.x + b * s.xb + (int64_t)h * s.xh + l * s.xs;
-        const T* drow = s.d + b * s.db + (int64_t)h * s.dh + l * s.ds;
-        float d1[E], d2[E];
-        V::to_float(*reinterpret_cast<const uint4*>(row + i0), x1);
-        V::to_float(*reinterpret_cast<const uint4*>(row + D / 2 + i0), x2);
-        V::to_float(*reinterpret_cast<const uint4*>(drow + i0), d1);
-        V::to_float(*reinterpret_cast<const uint4*>(drow + D / 2 + i0), d2);
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          g1[e] = d1[e] * cs[e] + d2[e] * sn[e];
-          g2[e] = d2[e] * cs[e] - d1[e] * sn[e];
-          ss = fmaf(x1[e], x1[e], fmaf(x2[e], x2[e], ss));
-          dot = fmaf(g1[e] * w1[e], x1[e], fmaf(g2[e] * w2[e], x2[e], dot));
+      for (int u = 0; u < U; ++u) {
+        x1[u] = x2[u] = d1[u] = d2[u] = V::zero();
+        if (r0 + u < hi && (r0 + u) * RPW + hl < s.H) {
+          x1[u] = *reinterpret_cast<const Raw*>(xp);
+          x2[u] = *reinterpret_cast<const Raw*>(xp + D / 2);
+          d1[u] = *reinterpret_cast<const Raw*>(dp);
+          d2[u] = *reinterpret_cast<const Raw*>(dp + D / 2);
         }
+        xp += xstep;
+        dp += dstep;
       }
-      ss = row_sum<TPR>(ss);
-      dot = row_sum<TPR>(dot);
-      const float rs = rsqrtf(ss * (1.f / D) + p.eps);
-      if (in) {
-        const float m = dot * rs * (1.f / D);
-        float o1[E], o2[E];
+      if (first) {       // while the first rows are on their way
+        float c[E], n[E];
+        const int64_t pos = p.pos ? p.pos[b * p.pos_sb + l] : l;
+        token_rotation<D, E>(pos, p.inv_freq, lane, i0, red[warp], c, n);
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const float h1v = x1[e] * rs, h2v = x2[e] * rs;
-          a1[e] = fmaf(g1[e], h1v, a1[e]);
-          a2[e] = fmaf(g2[e], h2v, a2[e]);
-          o1[e] = rs * (w1[e] * g1[e] - h1v * m);
-          o2[e] = rs * (w2[e] * g2[e] - h2v * m);
+        for (int v = 0; v < 2; ++v) {
+          cs[v] = f2(c[2 * v], c[2 * v + 1]);
+          sn[v] = f2(n[2 * v], n[2 * v + 1]);
+          ns[v] = f2(-n[2 * v], -n[2 * v + 1]);
         }
-        T* out = s.o + b * s.ob + (int64_t)h * s.oh + l * s.os;
-        stg16(out + i0, V::from_float(o1));
-        stg16(out + D / 2 + i0, V::from_float(o2));
+        first = false;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (r0 + u >= hi) break;
+        F2 xv1[2], xv2[2], y1[2], y2[2], g1[2], g2[2], gw1[2], gw2[2];
+        F2 ss2 = f2(0.f, 0.f), dot2 = f2(0.f, 0.f);
+        V::to_float(x1[u], xv1);
+        V::to_float(x2[u], xv2);
+        V::to_float(d1[u], y1);
+        V::to_float(d2[u], y2);
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+          g1[v] = fma2(y1[v], cs[v], mul2(y2[v], sn[v]));
+          g2[v] = fma2(y2[v], cs[v], mul2(y1[v], ns[v]));
+          gw1[v] = mul2(g1[v], w1[v]);
+          gw2[v] = mul2(g2[v], w2[v]);
+          ss2 = fma2(xv1[v], xv1[v], fma2(xv2[v], xv2[v], ss2));
+          dot2 = fma2(gw1[v], xv1[v], fma2(gw2[v], xv2[v], dot2));
+        }
+        float ss, dot, hi_ss, hi_dot;
+        split(ss2, ss, hi_ss);
+        split(dot2, dot, hi_dot);
+        ss += hi_ss;
+        dot += hi_dot;
+        row_sum2<TPR>(ss, dot);
+        // dx = rstd w g - x rstd^3 mean(x w g)
+        const float rs = rsqrtf(ss * (1.f / D) + p.eps);
+        const float c = -(dot * rs * (1.f / D)) * rs * rs;
+        const F2 rs2 = f2(rs, rs), c2 = f2(c, c);
+        F2 o1[2], o2[2];
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+          a1[v] = fma2(g1[v], mul2(xv1[v], rs2), a1[v]);
+          a2[v] = fma2(g2[v], mul2(xv2[v], rs2), a2[v]);
+          o1[v] = fma2(xv1[v], c2, mul2(gw1[v], rs2));
+          o2[v] = fma2(xv2[v], c2, mul2(gw2[v], rs2));
+        }
+        if ((r0 + u) * RPW + hl < s.H) {
+          *reinterpret_cast<Raw*>(op) = V::from_float(o1);
+          *reinterpret_cast<Raw*>(op + D / 2) = V::from_float(o2);
+        }
+        op += ostep;
       }
     }
+  }
+  __syncwarp();
+  float s1[E], s2[E];
+#pragma unroll
+  for (int v = 0; v < 2; ++v) {
+    split(a1[v], s1[2 * v], s1[2 * v + 1]);
+    split(a2[v], s2[2 * v], s2[2 * v + 1]);
   }
   // rows of the warp, then warps
 #pragma unroll
   for (int o = TPR; o < 32; o <<= 1) {
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      a1[e] += __shfl_xor_sync(0xffffffffu, a1[e], o);
-      a2[e] += __shfl_xor_sync(0xffffffffu, a2[e], o);
+      s1[e] += __shfl_xor_sync(0xffffffffu, s1[e], o);
+      s2[e] += __shfl_xor_sync(0xffffffffu, s2[e], o);
     }
   }
   if (lane < TPR) {
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      red[warp][i0 + e] = a1[e];
-      red[warp][D / 2 + i0 + e] = a2[e];
+      red[warp][i0 + e] = s1[e];
+      red[warp][D / 2 + i0 + e] = s2[e];
     }
   }
   __syncthreads();
