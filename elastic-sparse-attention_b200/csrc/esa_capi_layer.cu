@@ -148,7 +148,7 @@ int embedding_grad(int64_t n, int64_t vocab, int32_t dim, const em::Ids& ids, co
 // ---------------------------------------------------------------------------
 namespace qk = esa::qknorm;
 
-constexpr int kQkBwdCtas = 148 * 4;   // fixed, so the weight gradients' sums do not depend on the GPU
+constexpr int kQkBwdCtas = 148 * qk::kBwdCtasPerSm;   // fixed, so the weight gradients' sums do not depend on the GPU
 
 int check_qk(const char* what, int32_t dtype, int32_t batch, int64_t seq_len, int32_t head_dim,
              int32_t num_q_heads, int32_t num_k_heads, int64_t pos_stride, float eps) {
@@ -434,10 +434,10 @@ int esa_qk_norm_rope_backward(int32_t dtype, int32_t batch, int64_t seq_len, int
       if (int rc = check_launch("esa_qk_norm_rope_backward")) return rc;
       // block row 0: query weights, 1: key weights
       const int first = num_q_heads > 0 ? 0 : 1, sides = (num_q_heads > 0) + (num_k_heads > 0);
-      qk::sum_kernel<T><<<dim3((unsigned)ceil_div(head_dim, 32), sides), qk::kSumWarps * 32, 0, s>>>(
-          head_dim, q_ctas, ctas, first, part, static_cast<T*>(dq_weight),
-          static_cast<T*>(dk_weight));
-      return check_launch("esa_qk_norm_rope_backward (weight sums)");
+      return launch_after("esa_qk_norm_rope_backward (weight sums)", qk::sum_kernel<T>,
+                          dim3((unsigned)ceil_div(head_dim, 32), sides), dim3(qk::kSumWarps * 32),
+                          s, head_dim, q_ctas, ctas, first, part, static_cast<T*>(dq_weight),
+                          static_cast<T*>(dk_weight));
     });
   });
 }

@@ -13,7 +13,7 @@
 // the same of the second half, so the rotation needs no exchange.  The forward
 // has E = one 16-byte vector.  The backward, which holds twice the operands
 // and the weight gradient's sums, has E = 4, so that several rounds fit in the
-// registers of 16 warps per SM.  A warp takes the heads of one token, 32 / threads-per-row
+// registers.  A warp takes the heads of one token, 32 / threads-per-row
 // at a time (a round), and loads kUnroll rounds before it works on the first:
 // the kernels are HBM-bound (every element is read and written once) and need
 // that many bytes in flight.  The D / 2 angles of a token are formed once,
@@ -64,8 +64,15 @@ __device__ __forceinline__ float row_sum(float v) {
 
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
-constexpr int kFwdUnroll = 4;
-constexpr int kBwdUnroll = 4;
+
+// Rounds loaded together.  Forward: two, with 24 warps per SM (five took as
+// long, four 222 against 214 us on 65536 tokens of 40 heads of 128, bf16: 40
+// heads are ten rounds).  Backward: four (two in float32), the next four
+// loaded ahead, 12 warps per SM (251 us on 32768 tokens of 64 heads; two ahead
+// of two on 16 warps 268, four without loading ahead 277).
+constexpr int kFwdUnroll = 2;
+template <typename T> constexpr int kBwdUnroll = sizeof(T) == 4 ? 2 : 4;
+constexpr int kBwdCtasPerSm = 3;
 
 // Two float32 values and their packed arithmetic (one instruction for both).
 struct F2 { unsigned long long v; };
@@ -227,14 +234,15 @@ __global__ void __launch_bounds__(kThreads) fwd_kernel(Params<T> p) {
 // Backward: CTAs [0, q_ctas) stride over the query tasks, the others over the
 // key tasks, so a CTA sums one weight gradient; part[cta][D].
 template <typename T, int TPR>
-__global__ void __launch_bounds__(kThreads, 4) bwd_kernel(Params<T> p, int q_ctas, float* part) {
+__global__ void __launch_bounds__(kThreads, kBwdCtasPerSm) bwd_kernel(Params<T> p, int q_ctas, float* part) {
   using V = Quad<T>;
   using Raw = typename V::Raw;
   constexpr int E = 4;
   constexpr int RPW = 32 / TPR;
   constexpr int D = 2 * E * TPR;
-  constexpr int U = kBwdUnroll;
+  constexpr int U = kBwdUnroll<T>;
   __shared__ float red[kWarps][D];            // angles of the warps' tokens, then sums
+  cudaTriggerProgrammaticLaunchCompletion();  // the sum's CTAs may take free SMs
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const bool is_q = (int)blockIdx.x < q_ctas;
   const Heads<T>& s = is_q ? p.q : p.k;
@@ -249,43 +257,70 @@ __global__ void __launch_bounds__(kThreads, 4) bwd_kernel(Params<T> p, int q_cta
 #pragma unroll
   for (int v = 0; v < 2; ++v) a1[v] = a2[v] = f2(0.f, 0.f);
   const int64_t xstep = RPW * s.xh, dstep = RPW * s.dh, ostep = RPW * s.oh;
-  const int64_t tasks = p.tokens * per_tok;
-  for (int64_t task = cta * kWarps + warp; task < tasks; task += ctas * kWarps) {
-    const int64_t tok = task / per_tok;
+  const int64_t tasks = p.tokens * per_tok, stride = ctas * kWarps;
+  // The next U rounds are loaded while the current ones are worked on, across
+  // the border between two tokens too.
+  struct Place { int64_t task, pos; int r0, hi; const T* xp; const T* dp; T* op; };
+  auto enter = [&](Place& at) {          // first rounds of at.task
+    if (at.task >= tasks) return;
+    const int64_t tok = at.task / per_tok;
     const int64_t b = tok / p.L, l = tok - b * p.L;
-    const int lo = (int)(task - tok * per_tok) * rpt, hi = min(lo + rpt, rounds);
-    const int64_t h0 = (int64_t)lo * RPW + hl;
-    const T* xp = s.x + b * s.xb + h0 * s.xh + l * s.xs + i0;
-    const T* dp = s.d + b * s.db + h0 * s.dh + l * s.ds + i0;
-    T* op = s.o + b * s.ob + h0 * s.oh + l * s.os + i0;
-    F2 cs[2], sn[2], ns[2];
-    bool first = true;
-    for (int r0 = lo; r0 < hi; r0 += U) {
-      Raw x1[U], x2[U], d1[U], d2[U];
+    at.r0 = (int)(at.task - tok * per_tok) * rpt;
+    at.hi = min(at.r0 + rpt, rounds);
+    const int64_t h0 = (int64_t)at.r0 * RPW + hl;
+    at.xp = s.x + b * s.xb + h0 * s.xh + l * s.xs + i0;
+    at.dp = s.d + b * s.db + h0 * s.dh + l * s.ds + i0;
+    at.op = s.o + b * s.ob + h0 * s.oh + l * s.os + i0;
+    at.pos = p.pos ? p.pos[b * p.pos_sb + l] : l;
+  };
+  auto load = [&](Place& at, Raw (&x1)[U], Raw (&x2)[U], Raw (&d1)[U], Raw (&d2)[U]) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        x1[u] = x2[u] = d1[u] = d2[u] = V::zero();
-        if (r0 + u < hi && (r0 + u) * RPW + hl < s.H) {
-          x1[u] = *reinterpret_cast<const Raw*>(xp);
-          x2[u] = *reinterpret_cast<const Raw*>(xp + D / 2);
-          d1[u] = *reinterpret_cast<const Raw*>(dp);
-          d2[u] = *reinterpret_cast<const Raw*>(dp + D / 2);
-        }
-        xp += xstep;
-        dp += dstep;
+    for (int u = 0; u < U; ++u) {
+      x1[u] = x2[u] = d1[u] = d2[u] = V::zero();
+      if (at.task < tasks && at.r0 + u < at.hi && (at.r0 + u) * RPW + hl < s.H) {
+        x1[u] = *reinterpret_cast<const Raw*>(at.xp);
+        x2[u] = *reinterpret_cast<const Raw*>(at.xp + D / 2);
+        d1[u] = *reinterpret_cast<const Raw*>(at.dp);
+        d2[u] = *reinterpret_cast<const Raw*>(at.dp + D / 2);
       }
-      if (first) {       // while the first rows are on their way
-        float c[E], n[E];
-        const int64_t pos = p.pos ? p.pos[b * p.pos_sb + l] : l;
-        token_rotation<D, E>(pos, p.inv_freq, lane, i0, red[warp], c, n);
+      at.xp += xstep;
+      at.dp += dstep;
+    }
+  };
+  Place next;
+  next.task = cta * kWarps + warp;
+  Raw nx1[U], nx2[U], nd1[U], nd2[U];
+  enter(next);
+  load(next, nx1, nx2, nd1, nd2);
+  F2 cs[2], sn[2], ns[2];
+  int64_t done = -1;                     // the task whose angles are held
+  while (next.task < tasks) {
+    Raw x1[U], x2[U], d1[U], d2[U];
 #pragma unroll
-        for (int v = 0; v < 2; ++v) {
-          cs[v] = f2(c[2 * v], c[2 * v + 1]);
-          sn[v] = f2(n[2 * v], n[2 * v + 1]);
-          ns[v] = f2(-n[2 * v], -n[2 * v + 1]);
-        }
-        first = false;
+    for (int u = 0; u < U; ++u) {
+      x1[u] = nx1[u]; x2[u] = nx2[u]; d1[u] = nd1[u]; d2[u] = nd2[u];
+    }
+    const int r0 = next.r0, hi = next.hi;
+    const int64_t task = next.task, pos = next.pos;
+    T* op = next.op;
+    next.r0 += U;
+    next.op += U * ostep;
+    if (next.r0 >= hi) {
+      next.task += stride;
+      enter(next);
+    }
+    load(next, nx1, nx2, nd1, nd2);
+    if (task != done) {
+      float c[E], n[E];
+      token_rotation<D, E>(pos, p.inv_freq, lane, i0, red[warp], c, n);
+#pragma unroll
+      for (int v = 0; v < 2; ++v) {
+        cs[v] = f2(c[2 * v], c[2 * v + 1]);
+        sn[v] = f2(n[2 * v], n[2 * v + 1]);
+        ns[v] = f2(-n[2 * v], -n[2 * v + 1]);
       }
+      done = task;
+    }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (r0 + u >= hi) break;
@@ -328,7 +363,6 @@ __global__ void __launch_bounds__(kThreads, 4) bwd_kernel(Params<T> p, int q_cta
         }
         op += ostep;
       }
-    }
   }
   __syncwarp();
   float s1[E], s2[E];
@@ -372,6 +406,7 @@ sum_kernel(int D, int q_ctas, int ctas, int first, const float* __restrict__ par
            T* dwk) {
   __shared__ float red[kSumWarps][33];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  cudaGridDependencySynchronize();
   const bool keys = blockIdx.y + first > 0;
   const int lo = keys ? q_ctas : 0, hi = keys ? ctas : q_ctas;
   const int col = blockIdx.x * 32 + lane;
