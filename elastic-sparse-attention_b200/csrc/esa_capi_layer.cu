@@ -260,21 +260,23 @@ unsigned unit_grid(int64_t rows, int32_t dim, int elems) {
   return (unsigned)std::min<int64_t>(ceil_div(units, p8::kWarps), 148 * 32);
 }
 
-// f(std::integral_constant<int, vectors per lane>) for a warp-per-row kernel.
+// f(vectors per lane, warps per row) for a row of `vecs` 16-byte vectors: at
+// most four per lane, as few warps as hold the row.
 template <typename F>
-int by_vectors(int vecs, F&& f) {
-  if (vecs <= 32) return f(std::integral_constant<int, 1>{});
-  if (vecs <= 64) return f(std::integral_constant<int, 2>{});
-  if (vecs <= 128) return f(std::integral_constant<int, 4>{});
-  if (vecs <= 256) return f(std::integral_constant<int, 8>{});
-  if (vecs <= 512) return f(std::integral_constant<int, 16>{});
-  return f(std::integral_constant<int, 32>{});
+int by_row_shape(int vecs, F&& f) {
+  using std::integral_constant;
+  if (vecs <= 32) return f(integral_constant<int, 1>{}, integral_constant<int, 1>{});
+  if (vecs <= 64) return f(integral_constant<int, 2>{}, integral_constant<int, 1>{});
+  if (vecs <= 128) return f(integral_constant<int, 4>{}, integral_constant<int, 1>{});
+  if (vecs <= 256) return f(integral_constant<int, 4>{}, integral_constant<int, 2>{});
+  if (vecs <= 512) return f(integral_constant<int, 4>{}, integral_constant<int, 4>{});
+  return f(integral_constant<int, 4>{}, integral_constant<int, 8>{});
 }
 
 int check_norm_rows(const char* what, int32_t dtype, int64_t n_rows, int32_t dim, float eps) {
   if (dim > 1024 * (16 / elem_size(dtype)))
     return fail(ESA_ERR_UNSUPPORTED, "%s: dim %d too large", what, dim);
-  if (ceil_div(n_rows, p8::kNormWarps) > INT32_MAX)
+  if (n_rows > INT32_MAX)
     return fail(ESA_ERR_UNSUPPORTED, "%s: too many rows", what);
   if (!(eps >= 0.f) || !std::isfinite(eps))
     return fail(ESA_ERR_INVALID, "%s: eps must be finite and not negative", what);
@@ -490,9 +492,10 @@ int esa_rmsnorm_pack_forward(int32_t dtype, int32_t format, int64_t n_rows, int3
   return by_dtype(dtype, [&](auto tag) {
     using T = decltype(tag);
     return by_format(format, [&](auto f) {
-      return by_vectors(dim / esa::Vec<T>::kElems, [&](auto nv) {
-        p8::norm_pack_kernel<T, decltype(f)::value, decltype(nv)::value>
-            <<<(unsigned)ceil_div(n_rows, p8::kNormWarps), p8::kNormThreads, 0,
+      return by_row_shape(dim / esa::Vec<T>::kElems, [&](auto nv, auto nw) {
+        constexpr int W = decltype(nw)::value;
+        p8::norm_pack_kernel<T, decltype(f)::value, decltype(nv)::value, W>
+            <<<(unsigned)ceil_div(n_rows, p8::kNormRows<W>), p8::kNormThreads<W>, 0,
                (cudaStream_t)stream>>>(n_rows, dim, static_cast<const T*>(x),
                                        static_cast<const T*>(residual), static_cast<T*>(h_out),
                                        static_cast<const T*>(weight), eps, static_cast<T*>(y), rstd,
@@ -515,9 +518,10 @@ int esa_rmsnorm_unpack_forward(int32_t dtype, int32_t format, int64_t n_rows, in
   return by_dtype(dtype, [&](auto tag) {
     using T = decltype(tag);
     return by_format(format, [&](auto f) {
-      return by_vectors(dim / esa::Vec<T>::kElems, [&](auto nv) {
-        p8::unpack_norm_kernel<T, decltype(f)::value, decltype(nv)::value>
-            <<<(unsigned)ceil_div(n_rows, p8::kNormWarps), p8::kNormThreads, 0,
+      return by_row_shape(dim / esa::Vec<T>::kElems, [&](auto nv, auto nw) {
+        constexpr int W = decltype(nw)::value;
+        p8::unpack_norm_kernel<T, decltype(f)::value, decltype(nv)::value, W>
+            <<<(unsigned)ceil_div(n_rows, p8::kNormRows<W>), p8::kNormThreads<W>, 0,
                (cudaStream_t)stream>>>(n_rows, dim, static_cast<const uint8_t*>(codes), scales,
                                        static_cast<T*>(h), static_cast<const T*>(weight), eps,
                                        static_cast<T*>(y), rstd);

@@ -231,23 +231,39 @@ dequantize_kernel(int64_t rows, int dim, const uint8_t* __restrict__ codes,
 // ---------------------------------------------------------------------------
 // RMSNorm (with an optional residual add) that also writes h in 8 bits, and
 // its counterpart in the backward pass: h from the codes, normalised again.
-// A warp owns a row and keeps it in registers: NV vectors per lane.
+// W warps own a row and keep it in registers, NV <= 4 vectors per lane: all of
+// a row's loads are issued before the first is used, and 4 vectors leave room
+// for enough rows per SM to keep HBM busy while others are summed.
 // ---------------------------------------------------------------------------
-constexpr int kNormThreads = 128;
-constexpr int kNormWarps = kNormThreads / 32;
+template <int W> constexpr int kNormThreads = W > 4 ? 32 * W : 128;
+template <int W> constexpr int kNormRows = kNormThreads<W> / (32 * W);   // rows per CTA
 
-// h (already rounded to T, as float) -> y and rstd of one row.
-template <typename T, int NV>
-__device__ __forceinline__ void norm_row(const uint4 (&h)[NV], int vpr, int lane, int dim, float ss,
-                                         float eps, const T* __restrict__ w, T* y, float* rstd) {
+// Sum of v over the W warps of a row; red has a float per warp of the CTA.
+template <int W>
+__device__ __forceinline__ float row_total(float v, float* red) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if constexpr (W > 1) {
+    const int warp = threadIdx.x >> 5;
+    if ((threadIdx.x & 31) == 0) red[warp] = v;
+    __syncthreads();
+    const int w0 = warp / W * W;
+    v = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) v += red[w0 + w];
+  }
+  return v;
+}
+
+// h (already rounded to T) -> y of this lane's vectors.
+template <typename T, int NV, int W>
+__device__ __forceinline__ void norm_vecs(const uint4 (&h)[NV], int vpr, int vec0, float rs,
+                                          const T* __restrict__ w, T* y) {
   using V = Vec<T>;
   constexpr int E = V::kElems;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  const float rs = rsqrtf(ss / (float)dim + eps);
-#pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int vec = j * 32 + lane;
+    const int vec = vec0 + j * W * 32;
     if (vec < vpr) {
       float f[E], wv[E];
       V::to_float(h[j], f);
@@ -257,84 +273,100 @@ __device__ __forceinline__ void norm_row(const uint4 (&h)[NV], int vpr, int lane
       stg16(y + vec * E, V::from_float(f));
     }
   }
-  if (lane == 0) *rstd = rs;
 }
 
-template <typename T, int F, int NV>
-__global__ void __launch_bounds__(kNormThreads)
+template <typename T, int F, int NV, int W>
+__global__ void __launch_bounds__(kNormThreads<W>)
 norm_pack_kernel(int64_t rows, int dim, const T* __restrict__ x, const T* __restrict__ res,
                  T* __restrict__ h_out, const T* __restrict__ w, float eps, T* __restrict__ y,
                  float* __restrict__ rstd, uint8_t* __restrict__ codes,
                  float* __restrict__ scales) {
   using V = Vec<T>;
   constexpr int E = V::kElems;
-  const int lane = threadIdx.x & 31;
-  const int vpr = dim / E, groups = (dim + kGroup - 1) / kGroup;
-  const int64_t row = (int64_t)blockIdx.x * kNormWarps + (threadIdx.x >> 5);
-  if (row >= rows) return;
+  __shared__ float red[kNormThreads<W> / 32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int groups = (dim + kGroup - 1) / kGroup;
+  const int64_t row = (int64_t)blockIdx.x * kNormRows<W> + warp / W;
+  const int vpr = row < rows ? dim / E : 0;        // no vectors past the last row
+  const int vec0 = (warp % W) * 32 + lane;
   const int64_t at = row * dim;
-  uint4 h[NV];
+  uint4 h[NV], r[NV];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int vec = j * 32 + lane;
+    const int vec = vec0 + j * W * 32;
     h[j] = vec < vpr ? ldg16_stream(x + at + vec * E) : make_uint4(0, 0, 0, 0);
+    r[j] = res && vec < vpr ? ldg16_stream(res + at + vec * E) : make_uint4(0, 0, 0, 0);
   }
   float ss = 0.f;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int vec = j * 32 + lane;
+    const int vec = vec0 + j * W * 32;
     const bool in = vec < vpr;
     float f[E];
     V::to_float(h[j], f);
-    if (res && in) {
-      float r[E];
-      V::to_float(ldg16_stream(res + at + vec * E), r);
+    if (res) {
+      float rf[E];
+      V::to_float(r[j], rf);
 #pragma unroll
-      for (int e = 0; e < E; ++e) f[e] += r[e];
+      for (int e = 0; e < E; ++e) f[e] += rf[e];
       h[j] = V::from_float(f);   // the stored h is what is normed and packed
-      stg16(h_out + at + vec * E, h[j]);
+      if (in) stg16(h_out + at + vec * E, h[j]);
       V::to_float(h[j], f);
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) ss = fmaf(f[e], f[e], ss);
-    if (j * 32 < vpr)
+    if (vec - lane < vpr)        // the warp's 32 vectors begin inside the row
       pack_vec<F, T>(f, in, codes + at + vec * E, scales + row * groups + vec * E / kGroup);
   }
-  norm_row<T, NV>(h, vpr, lane, dim, ss, eps, w, y + at, rstd + row);
+  const float rs = rsqrtf(row_total<W>(ss, red) / (float)dim + eps);
+  norm_vecs<T, NV, W>(h, vpr, vec0, rs, w, y + at);
+  if (vec0 == 0 && vpr) rstd[row] = rs;
 }
 
-template <typename T, int F, int NV>
-__global__ void __launch_bounds__(kNormThreads)
+template <typename T, int F, int NV, int W>
+__global__ void __launch_bounds__(kNormThreads<W>)
 unpack_norm_kernel(int64_t rows, int dim, const uint8_t* __restrict__ codes,
                    const float* __restrict__ scales, T* __restrict__ h_out,
                    const T* __restrict__ w, float eps, T* __restrict__ y,
                    float* __restrict__ rstd) {
   using V = Vec<T>;
-  using W = typename Codes<T>::Word;
+  using C = typename Codes<T>::Word;
   constexpr int E = V::kElems;
-  const int lane = threadIdx.x & 31;
-  const int vpr = dim / E, groups = (dim + kGroup - 1) / kGroup;
-  const int64_t row = (int64_t)blockIdx.x * kNormWarps + (threadIdx.x >> 5);
-  if (row >= rows) return;
+  __shared__ float red[kNormThreads<W> / 32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int groups = (dim + kGroup - 1) / kGroup;
+  const int64_t row = (int64_t)blockIdx.x * kNormRows<W> + warp / W;
+  const int vpr = row < rows ? dim / E : 0;
+  const int vec0 = (warp % W) * 32 + lane;
   const int64_t at = row * dim;
+  C c[NV];
+  float s[NV];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int vec = vec0 + j * W * 32;
+    c[j] = C{};
+    s[j] = 0.f;
+    if (vec < vpr) {
+      c[j] = *reinterpret_cast<const C*>(codes + at + vec * E);
+      s[j] = __ldg(scales + row * groups + vec * E / kGroup);
+    }
+  }
   uint4 h[NV];
   float ss = 0.f;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int vec = j * 32 + lane;
-    h[j] = make_uint4(0, 0, 0, 0);
-    if (vec < vpr) {
-      float f[E];
-      decode<F, E>(*reinterpret_cast<const W*>(codes + at + vec * E),
-                   __ldg(scales + row * groups + vec * E / kGroup), f);
-      h[j] = V::from_float(f);
-      stg16(h_out + at + vec * E, h[j]);
-      V::to_float(h[j], f);
+    const int vec = vec0 + j * W * 32;
+    float f[E];
+    decode<F, E>(c[j], s[j], f);
+    h[j] = V::from_float(f);
+    if (vec < vpr) stg16(h_out + at + vec * E, h[j]);
+    V::to_float(h[j], f);
 #pragma unroll
-      for (int e = 0; e < E; ++e) ss = fmaf(f[e], f[e], ss);
-    }
+    for (int e = 0; e < E; ++e) ss = fmaf(f[e], f[e], ss);
   }
-  norm_row<T, NV>(h, vpr, lane, dim, ss, eps, w, y + at, rstd + row);
+  const float rs = rsqrtf(row_total<W>(ss, red) / (float)dim + eps);
+  norm_vecs<T, NV, W>(h, vpr, vec0, rs, w, y + at);
+  if (vec0 == 0 && vpr) rstd[row] = rs;
 }
 
 // ---------------------------------------------------------------------------
