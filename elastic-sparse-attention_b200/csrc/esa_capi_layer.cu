@@ -245,6 +245,9 @@ int check_pack(const char* what, int32_t dtype, int32_t format, int64_t n_rows, 
   if (format != ESA_PACK_INT8 && format != ESA_PACK_E4M3)
     return fail(ESA_ERR_INVALID, "%s: unknown 8-bit format %d", what, format);
   if (dim > (1 << 28)) return fail(ESA_ERR_UNSUPPORTED, "%s: dim %d too large", what, dim);
+  const int64_t units = ceil_div(dim / (16 / elem_size(dtype)), 32);   // of 32 vectors, per row
+  if (n_rows > (int64_t(1) << 31) / units)
+    return fail(ESA_ERR_UNSUPPORTED, "%s: too many rows", what);
   return ESA_OK;
 }
 
@@ -254,10 +257,9 @@ int by_format(int32_t format, F&& f) {
   return f(std::integral_constant<int, p8::kE4m3>{});
 }
 
-// Grid of the kernels whose warps stride over units of 32 vectors.
-unsigned unit_grid(int64_t rows, int32_t dim, int elems) {
-  const int64_t units = rows * ceil_div(dim / elems, 32);
-  return (unsigned)std::min<int64_t>(ceil_div(units, p8::kWarps), 148 * 32);
+// Grid of the kernels whose warps take K * 32 vectors of a row.
+unsigned part_grid(int64_t rows, int32_t dim, int elems, int K) {
+  return (unsigned)ceil_div(rows * ceil_div(dim / elems, 32 * K), p8::kWarps);
 }
 
 // f(vectors per lane, warps per row) for a row of `vecs` 16-byte vectors: at
@@ -454,7 +456,7 @@ int esa_quantize_rows(int32_t dtype, int32_t format, int64_t n_rows, int32_t dim
     using T = decltype(tag);
     return by_format(format, [&](auto f) {
       p8::quantize_kernel<T, decltype(f)::value>
-          <<<unit_grid(n_rows, dim, esa::Vec<T>::kElems), p8::kThreads, 0, (cudaStream_t)stream>>>(
+          <<<part_grid(n_rows, dim, esa::Vec<T>::kElems, p8::kRowUnits), p8::kThreads, 0, (cudaStream_t)stream>>>(
               n_rows, dim, static_cast<const T*>(x), static_cast<uint8_t*>(codes), scales);
       return check_launch("esa_quantize_rows");
     });
@@ -471,7 +473,7 @@ int esa_dequantize_rows(int32_t dtype, int32_t format, int64_t n_rows, int32_t d
     using T = decltype(tag);
     return by_format(format, [&](auto f) {
       p8::dequantize_kernel<T, decltype(f)::value>
-          <<<unit_grid(n_rows, dim, esa::Vec<T>::kElems), p8::kThreads, 0, (cudaStream_t)stream>>>(
+          <<<part_grid(n_rows, dim, esa::Vec<T>::kElems, p8::kRowUnits), p8::kThreads, 0, (cudaStream_t)stream>>>(
               n_rows, dim, static_cast<const uint8_t*>(codes), scales, static_cast<T*>(x));
       return check_launch("esa_dequantize_rows");
     });
@@ -543,7 +545,7 @@ int esa_swiglu_pack_forward(int32_t dtype, int32_t format, int64_t n_rows, int32
     using T = decltype(tag);
     return by_format(format, [&](auto f) {
       p8::swiglu_pack_kernel<T, decltype(f)::value>
-          <<<unit_grid(n_rows, ffn, esa::Vec<T>::kElems), p8::kThreads, 0, (cudaStream_t)stream>>>(
+          <<<part_grid(n_rows, ffn, esa::Vec<T>::kElems, p8::kSwigluFwdUnits), p8::kThreads, 0, (cudaStream_t)stream>>>(
               n_rows, ffn, static_cast<const T*>(gate_up), static_cast<T*>(out),
               static_cast<uint8_t*>(codes), scales);
       return check_launch("esa_swiglu_pack_forward");
@@ -563,7 +565,7 @@ int esa_swiglu_unpack_backward(int32_t dtype, int32_t format, int64_t n_rows, in
     using T = decltype(tag);
     return by_format(format, [&](auto f) {
       p8::swiglu_unpack_bwd_kernel<T, decltype(f)::value>
-          <<<unit_grid(n_rows, ffn, esa::Vec<T>::kElems), p8::kThreads, 0, (cudaStream_t)stream>>>(
+          <<<part_grid(n_rows, ffn, esa::Vec<T>::kElems, p8::kSwigluBwdUnits), p8::kThreads, 0, (cudaStream_t)stream>>>(
               n_rows, ffn, static_cast<const uint8_t*>(codes), scales, static_cast<const T*>(dout),
               static_cast<T*>(dgate_up), static_cast<T*>(out_recomputed));
       return check_launch("esa_swiglu_unpack_backward");

@@ -20,7 +20,7 @@
 // spread over the warp's lanes, and shared through shared memory.  rstd is
 // formed again in the backward instead of being kept.
 #pragma once
-#include "esa_common.cuh"
+#include "esa_f32x2.cuh"
 
 namespace esa {
 namespace qknorm {
@@ -73,27 +73,6 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kFwdUnroll = 2;
 template <typename T> constexpr int kBwdUnroll = sizeof(T) == 4 ? 2 : 4;
 constexpr int kBwdCtasPerSm = 3;
-
-// Two float32 values and their packed arithmetic (one instruction for both).
-struct F2 { unsigned long long v; };
-__device__ __forceinline__ F2 f2(float lo, float hi) {
-  F2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ void split(F2 a, float& lo, float& hi) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(a.v));
-}
-__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
-  F2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-  F2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return r;
-}
 
 // Sums of a and b over the TPR lanes of a row, both on every lane: even lanes
 // carry a through the levels, odd lanes b, so the pair costs one shuffle per
