@@ -160,7 +160,7 @@ int check_qk(const char* what, int32_t dtype, int32_t batch, int64_t seq_len, in
   if (head_dim < per || head_dim > 16 * per || (head_dim & (head_dim - 1)))
     return fail(ESA_ERR_UNSUPPORTED, "%s: head_dim %d (a power of two in [%d, %d])", what, head_dim,
                 per, 16 * per);
-  if ((int64_t)batch * seq_len > (int64_t(1) << 31) || num_q_heads > 65535 || num_k_heads > 65535)
+  if ((int64_t)batch * seq_len > INT32_MAX || num_q_heads > 65535 || num_k_heads > 65535)
     return fail(ESA_ERR_UNSUPPORTED, "%s: too many positions or heads", what);
   if (!(eps >= 0.f) || !std::isfinite(eps))
     return fail(ESA_ERR_INVALID, "%s: eps must be finite and not negative", what);
@@ -191,17 +191,14 @@ int set_heads(qk::Heads<T>& s, const char* name, const esa_tensor_t& x, const es
   return ESA_OK;
 }
 
-// f(std::integral_constant<int, threads per row>)
-template <typename F>
+// f(std::integral_constant<int, threads per row>) for a power of two in [Least, 16 * Least]
+template <int Least, typename F>
 int by_threads_per_row(int tpr, F&& f) {
-  switch (tpr) {
-    case 1: return f(std::integral_constant<int, 1>{});
-    case 2: return f(std::integral_constant<int, 2>{});
-    case 4: return f(std::integral_constant<int, 4>{});
-    case 8: return f(std::integral_constant<int, 8>{});
-    case 16: return f(std::integral_constant<int, 16>{});
-    default: return f(std::integral_constant<int, 32>{});
-  }
+  if (tpr == Least) return f(std::integral_constant<int, Least>{});
+  if (tpr == 2 * Least) return f(std::integral_constant<int, 2 * Least>{});
+  if (tpr == 4 * Least) return f(std::integral_constant<int, 4 * Least>{});
+  if (tpr == 8 * Least) return f(std::integral_constant<int, 8 * Least>{});
+  return f(std::integral_constant<int, 16 * Least>{});
 }
 
 // Rounds per warp task: all of a token's once there are tokens enough for 16
@@ -373,7 +370,7 @@ int esa_qk_norm_rope_forward(int32_t dtype, int32_t batch, int64_t seq_len, int3
     const int64_t ctas = ceil_div(p.tokens * p.tasks, qk::kWarps);
     if (ctas > INT32_MAX)
       return fail(ESA_ERR_UNSUPPORTED, "esa_qk_norm_rope_forward: too many positions");
-    return by_threads_per_row(tpr, [&](auto t) {
+    return by_threads_per_row<1>(tpr, [&](auto t) {
       qk::fwd_kernel<T, decltype(t)::value>
           <<<(unsigned)ctas, qk::kThreads, 0, (cudaStream_t)stream>>>(p);
       return check_launch("esa_qk_norm_rope_forward");
@@ -433,7 +430,7 @@ int esa_qk_norm_rope_backward(int32_t dtype, int32_t batch, int64_t seq_len, int
     const int ctas = qk_bwd_ctas(p.tokens, num_q_heads, num_k_heads);
     const int q_ctas = qk_q_ctas(ctas, num_q_heads, num_k_heads);
     float* part = static_cast<float*>(workspace);
-    return by_threads_per_row(tpr, [&](auto t) {
+    return by_threads_per_row<esa::Vec<T>::kElems / 4>(tpr, [&](auto t) {
       qk::bwd_kernel<T, decltype(t)::value><<<ctas, qk::kThreads, 0, s>>>(p, q_ctas, part);
       if (int rc = check_launch("esa_qk_norm_rope_backward")) return rc;
       // block row 0: query weights, 1: key weights

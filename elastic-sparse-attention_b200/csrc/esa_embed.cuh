@@ -42,31 +42,40 @@ lookup_kernel(int64_t n, int64_t vocab, uint32_t vpr, Ids ids, const T* __restri
   const int64_t base = (int64_t)blockIdx.x * (kLookupThreads * kLookupUnroll);
   const int64_t tok0 = base / vpr;
   const uint32_t rem0 = (uint32_t)(base - tok0 * vpr);
+  // vector and token of this thread, then steps of kLookupThreads vectors
+  uint32_t dt = (rem0 + threadIdx.x) / vpr, col = rem0 + threadIdx.x - dt * vpr;
+  const uint32_t dt_step = kLookupThreads / vpr, col_step = kLookupThreads - dt_step * vpr;
   uint4 v[kLookupUnroll];
 #pragma unroll
   for (int u = 0; u < kLookupUnroll; ++u) {
-    const uint32_t local = rem0 + u * kLookupThreads + threadIdx.x;
     v[u] = make_uint4(0, 0, 0, 0);
     if (base + u * kLookupThreads + threadIdx.x < total) {
-      const uint32_t dt = local / vpr;
       const int64_t id = ids.get(tok0 + dt);
       if (id >= 0 && id < vocab) {
-        v[u] = ldg16(w + (id * vpr + (local - dt * vpr)) * E);
-      } else if (local - dt * vpr == 0) {
+        v[u] = ldg16(w + (id * vpr + col) * E);
+      } else if (col == 0) {
         atomicOr(err, kErrTokenRange);
       }
+    }
+    dt += dt_step;
+    col += col_step;
+    if (col >= vpr) {
+      col -= vpr;
+      ++dt;
     }
   }
 #pragma unroll
   for (int u = 0; u < kLookupUnroll; ++u) {
     const int64_t i = base + u * kLookupThreads + threadIdx.x;
-    if (i < total) {
+    if (i >= total) break;
+    if (scale != 1.f) {          // 1 needs no arithmetic
       float f[E];
       V::to_float(v[u], f);
 #pragma unroll
       for (int e = 0; e < E; ++e) f[e] *= scale;
-      stg16(out + i * E, V::from_float(f));
+      v[u] = V::from_float(f);
     }
+    __stcs(reinterpret_cast<uint4*>(out + i * E), v[u]);
   }
 }
 

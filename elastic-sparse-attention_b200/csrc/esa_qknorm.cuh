@@ -65,12 +65,15 @@ __device__ __forceinline__ float row_sum(float v) {
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 
-// Rounds loaded together.  Forward: two, with 24 warps per SM (five took as
-// long, four 222 against 214 us on 65536 tokens of 40 heads of 128, bf16: 40
-// heads are ten rounds).  Backward: four (two in float32), the next four
-// loaded ahead, 12 warps per SM (251 us on 32768 tokens of 64 heads; two ahead
-// of two on 16 warps 268, four without loading ahead 277).
+// Rounds loaded together and CTAs per SM.  Forward: two rounds on 32 warps per
+// SM (65536 tokens of 40 heads of 128, bf16: 205 us; on 24 warps 222, five
+// rounds on 20 warps 208).  Backward: four (two in float32), the next four
+// loaded ahead, on 12 warps (32768 tokens of 64 heads: 251 us; two ahead of two
+// on 16 warps 268, four without loading ahead 277).  In long runs the power
+// limit lowers the SM clock and these become 225 and 283 us; a plain copy of
+// as many bytes (209 us) does not reach it.
 constexpr int kFwdUnroll = 2;
+constexpr int kFwdCtasPerSm = 8;
 template <typename T> constexpr int kBwdUnroll = sizeof(T) == 4 ? 2 : 4;
 constexpr int kBwdCtasPerSm = 3;
 
@@ -141,23 +144,41 @@ __device__ __forceinline__ void token_rotation(int64_t pos, const float* inv_fre
   }
 }
 
+// Pairs of a 16-byte vector.
+template <typename T>
+__device__ __forceinline__ void to_pairs(const uint4& raw, F2 (&f)[Vec<T>::kElems / 2]) {
+  float t[Vec<T>::kElems];
+  Vec<T>::to_float(raw, t);
+#pragma unroll
+  for (int v = 0; v < Vec<T>::kElems / 2; ++v) f[v] = f2(t[2 * v], t[2 * v + 1]);
+}
+template <typename T>
+__device__ __forceinline__ uint4 from_pairs(const F2 (&f)[Vec<T>::kElems / 2]) {
+  float t[Vec<T>::kElems];
+#pragma unroll
+  for (int v = 0; v < Vec<T>::kElems / 2; ++v) split(f[v], t[2 * v], t[2 * v + 1]);
+  return Vec<T>::from_float(t);
+}
+
 template <typename T, int TPR>
-__global__ void __launch_bounds__(kThreads) fwd_kernel(Params<T> p) {
-  using V = Vec<T>;
-  constexpr int E = V::kElems;
+__global__ void __launch_bounds__(kThreads, kFwdCtasPerSm) fwd_kernel(Params<T> p) {
+  constexpr int E = Vec<T>::kElems;
+  constexpr int P = E / 2;
   constexpr int RPW = 32 / TPR;               // rows a warp holds at once
   constexpr int D = 2 * E * TPR;
   constexpr int U = kFwdUnroll;
   __shared__ float table[kWarps][D];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t task = (int64_t)blockIdx.x * kWarps + warp;
-  const int64_t tok = task / p.tasks;
+  // 64-bit divisions here would be an eighth of the kernel's instructions
+  const uint32_t task = blockIdx.x * kWarps + warp;
+  const uint32_t tok = task / (uint32_t)p.tasks;
   if (tok >= p.tokens) return;
-  const int64_t b = tok / p.L, l = tok - b * p.L;
+  const uint32_t bu = tok / (uint32_t)p.L;
+  const int64_t b = bu, l = tok - bu * (uint32_t)p.L;
   const int i0 = (lane % TPR) * E, hl = lane / TPR;
   const int lo = (int)(task - tok * p.tasks) * p.rpt;
   const int hi = min(lo + p.rpt, p.rq + p.rk);
-  float cs[E], sn[E];
+  F2 cs[P], sn[P];
   bool first = true;
   for (int r0 = lo; r0 < hi; r0 += U) {
     uint4 x1[U], x2[U];
@@ -175,8 +196,14 @@ __global__ void __launch_bounds__(kThreads) fwd_kernel(Params<T> p) {
       }
     }
     if (first) {       // while the first rows are on their way
+      float c[E], n[E];
       const int64_t pos = p.pos ? p.pos[b * p.pos_sb + l] : l;
-      token_rotation<D, E>(pos, p.inv_freq, lane, i0, table[warp], cs, sn);
+      token_rotation<D, E>(pos, p.inv_freq, lane, i0, table[warp], c, n);
+#pragma unroll
+      for (int v = 0; v < P; ++v) {
+        cs[v] = f2(c[2 * v], c[2 * v + 1]);
+        sn[v] = f2(n[2 * v], n[2 * v + 1]);
+      }
       first = false;
     }
 #pragma unroll
@@ -186,25 +213,28 @@ __global__ void __launch_bounds__(kThreads) fwd_kernel(Params<T> p) {
       const bool is_q = r < p.rq;
       const Heads<T>& s = is_q ? p.q : p.k;
       const int h = (is_q ? r : r - p.rq) * RPW + hl;
-      float a1[E], a2[E], ss = 0.f;
-      V::to_float(x1[u], a1);
-      V::to_float(x2[u], a2);
+      F2 a1[P], a2[P], ss2 = f2(0.f, 0.f);
+      to_pairs<T>(x1[u], a1);
+      to_pairs<T>(x2[u], a2);
 #pragma unroll
-      for (int e = 0; e < E; ++e) ss = fmaf(a1[e], a1[e], fmaf(a2[e], a2[e], ss));
-      const float rs = rsqrtf(row_sum<TPR>(ss) * (1.f / D) + p.eps);
+      for (int v = 0; v < P; ++v) ss2 = fma2(a1[v], a1[v], fma2(a2[v], a2[v], ss2));
+      float ss, ss_hi;
+      split(ss2, ss, ss_hi);
+      const float rs = rsqrtf(row_sum<TPR>(ss + ss_hi) * (1.f / D) + p.eps);
       if (h < s.H) {
-        float w1[E], w2[E], o1[E], o2[E];
-        V::to_float(ldg16(s.w + i0), w1);
-        V::to_float(ldg16(s.w + D / 2 + i0), w2);
+        const F2 rs2 = f2(rs, rs), minus = f2(-1.f, -1.f);
+        F2 w1[P], w2[P], o1[P], o2[P];
+        to_pairs<T>(ldg16(s.w + i0), w1);
+        to_pairs<T>(ldg16(s.w + D / 2 + i0), w2);
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const float n1 = a1[e] * rs * w1[e], n2 = a2[e] * rs * w2[e];
-          o1[e] = n1 * cs[e] - n2 * sn[e];
-          o2[e] = n2 * cs[e] + n1 * sn[e];
+        for (int v = 0; v < P; ++v) {
+          const F2 n1 = mul2(mul2(a1[v], rs2), w1[v]), n2 = mul2(mul2(a2[v], rs2), w2[v]);
+          o1[v] = fma2(n1, cs[v], mul2(mul2(n2, sn[v]), minus));
+          o2[v] = fma2(n2, cs[v], mul2(n1, sn[v]));
         }
         T* out = s.o + b * s.ob + (int64_t)h * s.oh + l * s.os + i0;
-        stg16(out, V::from_float(o1));
-        stg16(out + D / 2, V::from_float(o2));
+        stg16(out, from_pairs<T>(o1));
+        stg16(out + D / 2, from_pairs<T>(o2));
       }
     }
   }
@@ -242,9 +272,10 @@ __global__ void __launch_bounds__(kThreads, kBwdCtasPerSm) bwd_kernel(Params<T> 
   struct Place { int64_t task, pos; int r0, hi; const T* xp; const T* dp; T* op; };
   auto enter = [&](Place& at) {          // first rounds of at.task
     if (at.task >= tasks) return;
-    const int64_t tok = at.task / per_tok;
-    const int64_t b = tok / p.L, l = tok - b * p.L;
-    at.r0 = (int)(at.task - tok * per_tok) * rpt;
+    const uint32_t task = (uint32_t)at.task;
+    const uint32_t tok = task / (uint32_t)per_tok, bu = tok / (uint32_t)p.L;
+    const int64_t b = bu, l = tok - bu * (uint32_t)p.L;
+    at.r0 = (int)(task - tok * per_tok) * rpt;
     at.hi = min(at.r0 + rpt, rounds);
     const int64_t h0 = (int64_t)at.r0 * RPW + hl;
     at.xp = s.x + b * s.xb + h0 * s.xh + l * s.xs + i0;
