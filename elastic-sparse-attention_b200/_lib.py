@@ -189,13 +189,33 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 def tensor4(t: torch.Tensor) -> EsaTensor:
     """[B, H, L, D] tensor with a contiguous last axis -> EsaTensor."""
-    if t.stride(-1) != 1:
+    st = t.stride()
+    if st[-1] != 1:
         raise ValueError("the head_dim axis must be contiguous")
-    return EsaTensor(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2))
+    return EsaTensor(t.data_ptr(), st[0], st[1], st[2])
+
+
+# The handle of torch's current stream without building a Stream object (2 us
+# of a call's host time); the public way where torch does not offer it.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def stream_handle(device: torch.device) -> int:
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def launch(fn, device: torch.device, *args) -> None:
+    """fn(*args, stream) with ``device`` current, on its current stream; raises
+    EsaError when it fails."""
+    if device.index == torch.cuda.current_device():
+        rc = fn(*args, stream_handle(device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, stream_handle(device))
+    if rc != ESA_OK:
+        check(rc, fn.__name__)
 
 
 def problem(*, dtype: torch.dtype, batch: int, num_heads: int, num_kv_heads: int, head_dim: int,

@@ -139,6 +139,17 @@ def swiglu_backward(gate_up: torch.Tensor, dout: torch.Tensor, recompute: bool =
 # ---------------------------------------------------------------------------
 # Token embedding
 # ---------------------------------------------------------------------------
+def _empty(shape, dtype: torch.dtype, dev: torch.device) -> torch.Tensor:
+    """torch.empty of a contiguous tensor; with the strides given torch takes a
+    third less host time, which single-token calls feel."""
+    strides, n = [], 1
+    for d in reversed(shape):
+        strides.append(n)
+        n *= d if d > 1 else 1
+    strides.reverse()
+    return torch.empty_strided(shape, strides, dtype=dtype, device=dev)
+
+
 def _ids(ids: torch.Tensor) -> torch.Tensor:
     if ids.dtype not in (torch.int64, torch.int32):
         raise TypeError(f"token ids must be int64 or int32, got {ids.dtype}")
@@ -155,13 +166,9 @@ def embedding_forward(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.
         raise ValueError("weight must be [vocab, dim]")
     vocab, dim = weight.shape
     _rows(weight, dim)
-    out = torch.empty(ids.shape + (dim,), dtype=weight.dtype, device=dev)
-    lib = _lib.load()
-    with _on(dev):
-        _lib.check(lib.esa_embedding_forward(
-            _dtype_code(weight), ids.element_size(), ids.numel(), vocab, dim, ids.data_ptr(),
-            weight.data_ptr(), scale, out.data_ptr(), _lib.stream_handle(dev)),
-            "esa_embedding_forward")
+    out = _empty(tuple(ids.shape) + (dim,), weight.dtype, dev)
+    _lib.launch(_lib.load().esa_embedding_forward, dev, _dtype_code(weight), ids.element_size(),
+                ids.numel(), vocab, dim, ids.data_ptr(), weight.data_ptr(), scale, out.data_ptr())
     return out
 
 
@@ -178,16 +185,16 @@ def embedding_backward(ids: torch.Tensor, dy: torch.Tensor, vocab_size: int, sca
         raise ValueError("dy must be [*ids.shape, dim]")
     if padding_idx is not None and not 0 <= padding_idx < vocab_size:
         raise ValueError(f"padding_idx {padding_idx} outside [0, {vocab_size})")
+    code = _dtype_code(dy)
     dy = dy.contiguous()
-    dw = torch.empty((vocab_size, dim), dtype=dy.dtype, device=dev)
+    dw = _empty((vocab_size, dim), dy.dtype, dev)
     lib = _lib.load()
-    need = lib.esa_embedding_backward_workspace_size(ids.numel(), vocab_size, dim)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    with _on(dev):
-        _lib.check(lib.esa_embedding_backward(
-            _dtype_code(dy), ids.element_size(), ids.numel(), vocab_size, dim, ids.data_ptr(),
-            dy.data_ptr(), scale, -1 if padding_idx is None else padding_idx, dw.data_ptr(),
-            _lib.ptr(ws), need, _lib.stream_handle(dev)), "esa_embedding_backward")
+    n = ids.numel()
+    need = lib.esa_embedding_backward_workspace_size(n, vocab_size, dim)
+    ws = _empty((need,), torch.uint8, dev) if need else None
+    _lib.launch(lib.esa_embedding_backward, dev, code, ids.element_size(), n, vocab_size, dim,
+                ids.data_ptr(), dy.data_ptr(), scale, -1 if padding_idx is None else padding_idx,
+                dw.data_ptr(), _lib.ptr(ws), need)
     return dw
 
 
@@ -201,42 +208,48 @@ def _t4(t: torch.Tensor | None) -> _lib.EsaTensor:
     return _NO_TENSOR if t is None else _lib.tensor4(t)
 
 
+def _check_head_weight(name: str, w, like: torch.Tensor, dev: torch.device) -> None:
+    if (w is None or w.shape != like.shape[-1:] or w.dtype != like.dtype or w.device != dev
+            or not w.is_contiguous()):
+        raise ValueError(f"{name}_weight must be a contiguous [head_dim] tensor of q's dtype and "
+                         "device")
+
+
 def _qk_checks(q, k, q_weight, k_weight, inv_freq, positions):
-    dev = _check_device(*(t for t in (q, k, q_weight, k_weight, inv_freq) if t is not None))
-    B, _, L, D = q.shape
-    sides = [("q", q, q_weight)]
+    """(device, B, Hq, Hk, L, D, positions, their batch stride)."""
+    dev = _check_device(q, inv_freq)
+    B, Hq, L, D = q.shape
+    _check_head_weight("q", q_weight, q, dev)
+    Hk = 0
     if k is not None:
-        if k.shape[0] != B or k.shape[2] != L or k.shape[3] != D or k.dtype != q.dtype:
-            raise ValueError("q and k must share batch, length, head_dim and dtype")
-        sides.append(("k", k, k_weight))
-    for name, _, w in sides:
-        if w is None or w.shape != (D,) or w.dtype != q.dtype or not w.is_contiguous():
-            raise ValueError(f"{name}_weight must be a contiguous [head_dim] tensor of q's dtype")
+        kB, Hk, kL, kD = k.shape
+        if kB != B or kL != L or kD != D or k.dtype != q.dtype or k.device != dev:
+            raise ValueError("q and k must share batch, length, head_dim, dtype and device")
+        _check_head_weight("k", k_weight, k, dev)
     if inv_freq.dtype != torch.float32 or inv_freq.numel() != D // 2 or not inv_freq.is_contiguous():
         raise ValueError("inv_freq must be float32 [head_dim / 2]")
     stride = 0
     if positions is not None:
-        if positions.shape != (L,) and positions.shape != (B, L):
+        shape = tuple(positions.shape)
+        if shape != (L,) and shape != (B, L):
             raise ValueError("positions must be [L] or [B, L]")
-        positions = positions.to(device=dev, dtype=torch.int64).contiguous()
-        stride = L if positions.dim() == 2 else 0
-    return dev, positions, stride
+        if positions.dtype != torch.int64 or positions.device != dev:
+            positions = positions.to(device=dev, dtype=torch.int64)
+        positions = positions.contiguous()
+        stride = L if len(shape) == 2 else 0
+    return dev, B, Hq, Hk, L, D, positions, stride
 
 
-def _like_heads(name: str, out: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
+def _heads_out(name: str, out: torch.Tensor | None, x: torch.Tensor) -> torch.Tensor:
+    """``out`` if it fits x [B, H, L, D]; by default a new tensor whose heads
+    of a token lie side by side (storage [B, L, H, D])."""
+    if out is None:
+        B, H, L, D = x.shape
+        return torch.empty_strided((B, H, L, D), (L * H * D, D, H * D, 1), dtype=x.dtype,
+                                   device=x.device)
     if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
         raise ValueError(f"{name} must match its input's shape, dtype and device")
     return out
-
-
-def _new_heads(q: torch.Tensor, k: torch.Tensor | None):
-    """Outputs shaped like q and k in one [B, L, Hq + Hk, D] buffer (a
-    token's heads side by side, as in a projection's output)."""
-    B, Hq, L, D = q.shape
-    buf = torch.empty((B, L, Hq + (0 if k is None else k.shape[1]), D), dtype=q.dtype,
-                      device=q.device)
-    heads = buf.transpose(1, 2)
-    return heads[:, :Hq], (None if k is None else heads[:, Hq:])
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tensor,
@@ -248,23 +261,17 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tensor
     side's [D] weight, then rotated at its position, in one pass.  positions:
     [L] shared by the batch, [B, L], or None for 0 .. L-1.  ``q_out`` /
     ``k_out`` receive the result (e.g. rows of a key cache; q / k themselves
-    for in place); by default new views of one [B, L, Hq + Hk, D] buffer."""
-    dev, positions, stride = _qk_checks(q, k, q_weight, k_weight, inv_freq, positions)
-    B, Hq, L, D = q.shape
-    Hk = 0 if k is None else k.shape[1]
-    if q_out is None or (k is not None and k_out is None):
-        new_q, new_k = _new_heads(q, k)
-    q_out = new_q if q_out is None else _like_heads("q_out", q_out, q)
+    for in place); by default new [B, H, L, D] views of [B, L, H, D] storage."""
+    dev, B, Hq, Hk, L, D, positions, stride = _qk_checks(q, k, q_weight, k_weight, inv_freq,
+                                                         positions)
+    q_out = _heads_out("q_out", q_out, q)
     if k is not None:
-        k_out = new_k if k_out is None else _like_heads("k_out", k_out, k)
+        k_out = _heads_out("k_out", k_out, k)
     elif k_out is not None:
         raise ValueError("k_out without k")
-    lib = _lib.load()
-    with _on(dev):
-        _lib.check(lib.esa_qk_norm_rope_forward(
-            _dtype_code(q), B, L, D, _t4(q), Hq, _t4(k), Hk, q_weight.data_ptr(),
-            _lib.ptr(k_weight), eps, _lib.ptr(positions), stride, inv_freq.data_ptr(), _t4(q_out),
-            _t4(k_out), _lib.stream_handle(dev)), "esa_qk_norm_rope_forward")
+    _lib.launch(_lib.load().esa_qk_norm_rope_forward, dev, _dtype_code(q), B, L, D, _t4(q), Hq,
+                _t4(k), Hk, q_weight.data_ptr(), _lib.ptr(k_weight), eps, _lib.ptr(positions),
+                stride, inv_freq.data_ptr(), _t4(q_out), _t4(k_out))
     return q_out, k_out
 
 
@@ -276,33 +283,29 @@ def qk_norm_rope_backward(q: torch.Tensor, k: torch.Tensor | None, q_weight: tor
     """(dq, dk, dq_weight, dk_weight) of :func:`qk_norm_rope` from its inputs
     and the gradients of its outputs.  ``dq`` / ``dk`` receive the result
     (dq_out / dk_out themselves for in place)."""
-    dev, positions, stride = _qk_checks(q, k, q_weight, k_weight, inv_freq, positions)
-    B, Hq, L, D = q.shape
-    Hk = 0 if k is None else k.shape[1]
+    dev, B, Hq, Hk, L, D, positions, stride = _qk_checks(q, k, q_weight, k_weight, inv_freq,
+                                                         positions)
     if (k is None) != (dk_out is None):
         raise ValueError("dk_out and k must be given together")
-    _like_heads("dq_out", dq_out, q)
-    if k is not None:
-        _like_heads("dk_out", dk_out, k)
-    elif dk is not None:
-        raise ValueError("dk without k")
-    if dq is None or (k is not None and dk is None):
-        new_q, new_k = _new_heads(q, k)
-    dq = new_q if dq is None else _like_heads("dq", dq, q)
+    if dq_out is None:
+        raise ValueError("dq_out is required")
+    _heads_out("dq_out", dq_out, q)
+    dq = _heads_out("dq", dq, q)
     dwq = torch.empty_like(q_weight)
     dwk = None
     if k is not None:
-        dk = new_k if dk is None else _like_heads("dk", dk, k)
+        _heads_out("dk_out", dk_out, k)
+        dk = _heads_out("dk", dk, k)
         dwk = torch.empty_like(k_weight)
+    elif dk is not None:
+        raise ValueError("dk without k")
     lib = _lib.load()
     need = lib.esa_qk_norm_rope_backward_workspace_size(B, L, Hq, Hk, D)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    with _on(dev):
-        _lib.check(lib.esa_qk_norm_rope_backward(
-            _dtype_code(q), B, L, D, _t4(q), Hq, _t4(k), Hk, q_weight.data_ptr(),
-            _lib.ptr(k_weight), eps, _lib.ptr(positions), stride, inv_freq.data_ptr(),
-            _t4(dq_out), _t4(dk_out), _t4(dq), _t4(dk), dwq.data_ptr(), _lib.ptr(dwk),
-            ws.data_ptr(), need, _lib.stream_handle(dev)), "esa_qk_norm_rope_backward")
+    ws = _empty((need,), torch.uint8, dev)
+    _lib.launch(lib.esa_qk_norm_rope_backward, dev, _dtype_code(q), B, L, D, _t4(q), Hq, _t4(k), Hk,
+                q_weight.data_ptr(), _lib.ptr(k_weight), eps, _lib.ptr(positions), stride,
+                inv_freq.data_ptr(), _t4(dq_out), _t4(dk_out), _t4(dq), _t4(dk), dwq.data_ptr(),
+                _lib.ptr(dwk), ws.data_ptr(), need)
     return dq, dk, dwq, dwk
 
 
@@ -313,7 +316,7 @@ PACK_FORMATS = {"int8": 0, "e4m3": 1}
 PACK_GROUP = 128
 
 
-@dataclass(frozen=True)
+@dataclass
 class PackedRows:
     """Rows kept in 8 bits: ``codes`` uint8 [*shape], ``scales`` float32
     [*shape[:-1], ceil(shape[-1] / 128)], one scale per 128 elements;
@@ -332,23 +335,24 @@ class PackedRows:
 
 
 def _pack_code(format: str) -> int:
-    if format not in PACK_FORMATS:
+    code = PACK_FORMATS.get(format)
+    if code is None:
         raise ValueError(f"unknown 8-bit format {format!r}; expected one of {sorted(PACK_FORMATS)}")
-    return PACK_FORMATS[format]
+    return code
 
 
-def _new_packed(shape, format: str, dtype: torch.dtype, dev) -> PackedRows:
-    groups = -(-shape[-1] // PACK_GROUP)
-    return PackedRows(torch.empty(shape, dtype=torch.uint8, device=dev),
-                      torch.empty(tuple(shape[:-1]) + (groups,), dtype=torch.float32, device=dev),
+def _new_packed(shape: tuple, format: str, dtype: torch.dtype, dev) -> PackedRows:
+    return PackedRows(_empty(shape, torch.uint8, dev),
+                      _empty(shape[:-1] + (-(-shape[-1] // PACK_GROUP),), torch.float32, dev),
                       format, dtype)
 
 
 def _check_packed(p: PackedRows) -> int:
     """The format code of a PackedRows whose parts fit together."""
     code = _pack_code(p.format)
-    want = p.codes.shape[:-1] + (-(-p.codes.shape[-1] // PACK_GROUP),)
-    if p.codes.dtype != torch.uint8 or p.scales.dtype != torch.float32 or p.scales.shape != want:
+    shape = p.codes.shape
+    if (p.codes.dtype != torch.uint8 or p.scales.dtype != torch.float32
+            or p.scales.shape != shape[:-1] + (-(-shape[-1] // PACK_GROUP),)):
         raise ValueError("PackedRows: codes must be uint8 and scales float32 "
                          "[*codes.shape[:-1], ceil(codes.shape[-1] / 128)]")
     if not p.codes.is_contiguous() or not p.scales.is_contiguous():
@@ -363,14 +367,12 @@ def quantize_rows(x: torch.Tensor, format: str = "int8") -> PackedRows:
     NaN."""
     code = _pack_code(format)
     dev = _check_device(x)
-    dim = x.shape[-1]
-    n = _rows(x, dim)
-    p = _new_packed(x.shape, format, x.dtype, dev)
-    lib = _lib.load()
-    with _on(dev):
-        _lib.check(lib.esa_quantize_rows(_dtype_code(x), code, n, dim, x.data_ptr(),
-                                         p.codes.data_ptr(), p.scales.data_ptr(),
-                                         _lib.stream_handle(dev)), "esa_quantize_rows")
+    shape = tuple(x.shape)
+    n = _rows(x, shape[-1])
+    dtype_code = _dtype_code(x)
+    p = _new_packed(shape, format, x.dtype, dev)
+    _lib.launch(_lib.load().esa_quantize_rows, dev, dtype_code, code, n, shape[-1], x.data_ptr(),
+                p.codes.data_ptr(), p.scales.data_ptr())
     return p
 
 
@@ -379,14 +381,10 @@ def dequantize_rows(packed: PackedRows, dtype: torch.dtype | None = None) -> tor
     were made from)."""
     code = _check_packed(packed)
     dev = _check_device(packed.codes, packed.scales)
-    x = torch.empty(packed.shape, dtype=dtype or packed.dtype, device=dev)
+    x = torch.empty_like(packed.codes, dtype=dtype or packed.dtype)
     dim = x.shape[-1]
-    lib = _lib.load()
-    with _on(dev):
-        _lib.check(lib.esa_dequantize_rows(_dtype_code(x), code, _rows(x, dim), dim,
-                                           packed.codes.data_ptr(), packed.scales.data_ptr(),
-                                           x.data_ptr(), _lib.stream_handle(dev)),
-                   "esa_dequantize_rows")
+    _lib.launch(_lib.load().esa_dequantize_rows, dev, _dtype_code(x), code, _rows(x, dim), dim,
+                packed.codes.data_ptr(), packed.scales.data_ptr(), x.data_ptr())
     return x
 
 
@@ -396,8 +394,10 @@ def rmsnorm_forward_packed(x: torch.Tensor, weight: torch.Tensor, eps: float,
     pass."""
     code = _pack_code(format)
     dev = _check_device(x, weight)
-    dim = x.shape[-1]
+    shape = tuple(x.shape)
+    dim = shape[-1]
     n = _rows(x, dim)
+    dtype_code = _dtype_code(x)
     _check_norm_weight(weight, dim, x.dtype)
     h = x
     if residual is not None:
@@ -406,15 +406,11 @@ def rmsnorm_forward_packed(x: torch.Tensor, weight: torch.Tensor, eps: float,
         _rows(residual, dim)
         h = torch.empty_like(x)
     y = torch.empty_like(x)
-    rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
-    p = _new_packed(x.shape, format, x.dtype, dev)
-    lib = _lib.load()
-    with _on(dev):
-        _lib.check(lib.esa_rmsnorm_pack_forward(
-            _dtype_code(x), code, n, dim, x.data_ptr(), _lib.ptr(residual),
-            h.data_ptr() if residual is not None else None, weight.data_ptr(), eps, y.data_ptr(),
-            rstd.data_ptr(), p.codes.data_ptr(), p.scales.data_ptr(), _lib.stream_handle(dev)),
-            "esa_rmsnorm_pack_forward")
+    rstd = _empty(shape[:-1], torch.float32, dev)
+    p = _new_packed(shape, format, x.dtype, dev)
+    _lib.launch(_lib.load().esa_rmsnorm_pack_forward, dev, dtype_code, code, n, dim, x.data_ptr(),
+                _lib.ptr(residual), None if residual is None else h.data_ptr(), weight.data_ptr(),
+                eps, y.data_ptr(), rstd.data_ptr(), p.codes.data_ptr(), p.scales.data_ptr())
     return h, y, rstd, p
 
 
@@ -423,18 +419,14 @@ def rmsnorm_from_packed(packed: PackedRows, weight: torch.Tensor, eps: float):
     RMSNorm, in one pass over the codes."""
     code = _check_packed(packed)
     dev = _check_device(packed.codes, packed.scales, weight)
-    dim = packed.shape[-1]
-    _check_norm_weight(weight, dim, packed.dtype)
-    h = torch.empty(packed.shape, dtype=packed.dtype, device=dev)
-    n = _rows(h, dim)
+    shape = tuple(packed.shape)
+    _check_norm_weight(weight, shape[-1], packed.dtype)
+    h = torch.empty_like(packed.codes, dtype=packed.dtype)
     y = torch.empty_like(h)
-    rstd = torch.empty(packed.shape[:-1], dtype=torch.float32, device=dev)
-    lib = _lib.load()
-    with _on(dev):
-        _lib.check(lib.esa_rmsnorm_unpack_forward(
-            _dtype_code(h), code, n, dim, packed.codes.data_ptr(), packed.scales.data_ptr(),
-            weight.data_ptr(), eps, h.data_ptr(), y.data_ptr(), rstd.data_ptr(),
-            _lib.stream_handle(dev)), "esa_rmsnorm_unpack_forward")
+    rstd = _empty(shape[:-1], torch.float32, dev)
+    _lib.launch(_lib.load().esa_rmsnorm_unpack_forward, dev, _dtype_code(h), code,
+                _rows(h, shape[-1]), shape[-1], packed.codes.data_ptr(), packed.scales.data_ptr(),
+                weight.data_ptr(), eps, h.data_ptr(), y.data_ptr(), rstd.data_ptr())
     return h, y, rstd
 
 
@@ -449,19 +441,16 @@ def swiglu_forward_packed(gate_up: torch.Tensor, format: str = "int8"):
     are rows of their own."""
     code = _pack_code(format)
     dev = _check_device(gate_up)
-    if gate_up.shape[-1] % 2:
+    shape = tuple(gate_up.shape)
+    if shape[-1] % 2:
         raise ValueError("gate_up rows must hold two halves of equal width")
-    ffn = gate_up.shape[-1] // 2
+    ffn = shape[-1] // 2
     n = _rows(gate_up, 2 * ffn)
-    lead = tuple(gate_up.shape[:-1])
-    out = torch.empty(lead + (ffn,), dtype=gate_up.dtype, device=dev)
-    p = _new_packed(lead + (2, ffn), format, gate_up.dtype, dev)
-    lib = _lib.load()
-    with _on(dev):
-        _lib.check(lib.esa_swiglu_pack_forward(
-            _dtype_code(gate_up), code, n, ffn, gate_up.data_ptr(), out.data_ptr(),
-            p.codes.data_ptr(), p.scales.data_ptr(), _lib.stream_handle(dev)),
-            "esa_swiglu_pack_forward")
+    dtype_code = _dtype_code(gate_up)
+    out = _empty(shape[:-1] + (ffn,), gate_up.dtype, dev)
+    p = _new_packed(shape[:-1] + (2, ffn), format, gate_up.dtype, dev)
+    _lib.launch(_lib.load().esa_swiglu_pack_forward, dev, dtype_code, code, n, ffn,
+                gate_up.data_ptr(), out.data_ptr(), p.codes.data_ptr(), p.scales.data_ptr())
     return out, p
 
 
@@ -470,20 +459,17 @@ def swiglu_backward_packed(packed: PackedRows, dout: torch.Tensor, recompute: bo
     values that the codes of :func:`swiglu_forward_packed` stand for."""
     code = _check_packed(packed)
     dev = _check_device(packed.codes, packed.scales, dout)
-    if len(packed.shape) < 2 or packed.shape[-2] != 2:
+    shape = tuple(packed.shape)
+    if len(shape) < 2 or shape[-2] != 2:
         raise ValueError("packed must come from swiglu_forward_packed ([..., 2, ffn])")
-    ffn = packed.shape[-1]
-    lead = tuple(packed.shape[:-2])
+    ffn = shape[-1]
+    lead = shape[:-2]
     if tuple(dout.shape) != lead + (ffn,) or dout.dtype != packed.dtype:
         raise ValueError("dout must be [..., ffn] in the packed rows' dtype")
     dout = dout.contiguous()
-    n = _rows(dout, ffn)
-    dgu = torch.empty(lead + (2 * ffn,), dtype=dout.dtype, device=dev)
+    dgu = _empty(lead + (2 * ffn,), dout.dtype, dev)
     out = torch.empty_like(dout) if recompute else None
-    lib = _lib.load()
-    with _on(dev):
-        _lib.check(lib.esa_swiglu_unpack_backward(
-            _dtype_code(dout), code, n, ffn, packed.codes.data_ptr(), packed.scales.data_ptr(),
-            dout.data_ptr(), dgu.data_ptr(), _lib.ptr(out), _lib.stream_handle(dev)),
-            "esa_swiglu_unpack_backward")
+    _lib.launch(_lib.load().esa_swiglu_unpack_backward, dev, _dtype_code(dout), code,
+                _rows(dout, ffn), ffn, packed.codes.data_ptr(), packed.scales.data_ptr(),
+                dout.data_ptr(), dgu.data_ptr(), _lib.ptr(out))
     return dgu, out
