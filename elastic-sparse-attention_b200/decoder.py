@@ -28,6 +28,22 @@ Built for B200 without layout copies:
 
 ``activation_checkpointing=True`` recomputes each layer in the backward
 (keeps only its input), for lengths whose activations do not fit.
+
+Options (all off by default):
+
+* ``embed_scale`` / ``padding_idx``: the token embedding runs in the library's
+  lookup (times ``embed_scale``) and its gradient in the sorted-token kernels,
+  which leave the row ``padding_idx`` without a gradient; ids outside the
+  vocabulary give zero rows and a device error bit instead of an assert.
+* ``qk_norm``: RMSNorm of each query and key head (weights ``q_norm``,
+  ``k_norm`` of head_dim) before the rotary embedding, both in one pass; the
+  backward normalises again instead of keeping the result.
+* ``activation_storage`` = "int8" or "e4m3": what the backward needs is kept
+  in 8 bits.  With ``activation_checkpointing`` that is each layer's input
+  (written by the norm that precedes the layer, restored together with that
+  norm), instead of two full rows; without, the MLP's gate / up rows, the
+  largest activation of a layer.  The forward pass is unchanged; gradients are
+  taken at the decoded values.
 """
 from __future__ import annotations
 
@@ -38,7 +54,24 @@ import torch.utils.checkpoint
 
 from . import layer_ops, ops
 from .attention import KeyPlanCache, _ensure_monotone
+from .layer_ops import PACK_FORMATS, PackedRows
 from .ops import PatternSpec
+
+
+class _Embedding(torch.autograd.Function):
+    """scale * w[ids]."""
+
+    @staticmethod
+    def forward(ctx, ids, w, scale: float, padding_idx):
+        ctx.save_for_backward(ids)
+        ctx.meta = (w.shape[0], scale, padding_idx)
+        return layer_ops.embedding_forward(ids, w, scale)
+
+    @staticmethod
+    def backward(ctx, dy):
+        ids, = ctx.saved_tensors
+        vocab, scale, padding_idx = ctx.meta
+        return None, layer_ops.embedding_backward(ids, dy, vocab, scale, padding_idx), None, None
 
 
 class _RMSNorm(torch.autograd.Function):
@@ -54,6 +87,27 @@ class _RMSNorm(torch.autograd.Function):
         x, w, rstd = ctx.saved_tensors
         dx, dw = layer_ops.rmsnorm_backward(x, w, rstd, dy)
         return dx, dw, None
+
+
+class _PackedRMSNorm(torch.autograd.Function):
+    """(y, codes, scales) of x: its norm and its 8-bit form, which is what the
+    backward keeps of it."""
+
+    @staticmethod
+    def forward(ctx, x, w, eps: float, fmt: str):
+        _, y, _, p = layer_ops.rmsnorm_forward_packed(x.contiguous(), w, eps, format=fmt)
+        ctx.save_for_backward(p.codes, p.scales, w)
+        ctx.meta = (fmt, x.dtype)
+        ctx.eps = eps
+        ctx.mark_non_differentiable(p.codes, p.scales)
+        return y, p.codes, p.scales
+
+    @staticmethod
+    def backward(ctx, dy, _codes, _scales):
+        codes, scales, w = ctx.saved_tensors
+        x, _, rstd = layer_ops.rmsnorm_from_packed(PackedRows(codes, scales, *ctx.meta), w, ctx.eps)
+        dx, dw = layer_ops.rmsnorm_backward(x, w, rstd, dy)
+        return dx, dw, None, None
 
 
 class _AddRMSNorm(torch.autograd.Function):
@@ -75,35 +129,44 @@ class _AddRMSNorm(torch.autograd.Function):
 
 
 class _AttentionBlock(torch.autograd.Function):
-    """a = attention(rope(y Wqkv^T)) Wo^T with the layouts described above."""
+    """a = attention(rope(y Wqkv^T)) Wo^T with the layouts described above;
+    with q_norm / k_norm, attention(rope(norm(y Wqkv^T)))."""
 
     @staticmethod
     def forward(ctx, y, wqkv, wo, spec: PatternSpec, heads: tuple, inv_freq, positions,
-                plans=None):
+                plans=None, q_norm=None, k_norm=None, eps: float = 0.0):
         Hq, Hkv, D = heads
         B, L, d = y.shape
         qkv = torch.matmul(y, wqkv.t())                       # [B, L, (Hq + 2 Hkv) D]
         q, k, v = _split_heads(qkv, B, L, Hq, Hkv, D)
-        layer_ops.rope_(q, k, inv_freq, positions)
+        if q_norm is None:
+            layer_ops.rope_(q, k, inv_freq, positions)
+        else:
+            q, k = layer_ops.qk_norm_rope(q, k, q_norm, k_norm, eps, inv_freq, positions)
         scale = D ** -0.5
         probs = ops.probs_buffer(q, k, spec)                  # kept for the backward
         o, lse = ops.forward(q, k, v, spec, scale, probs=probs)   # o: view of [B, L, Hq, D]
         o_rows = o.transpose(1, 2).reshape(B, L, Hq * D)      # a view, no copy
         a = torch.matmul(o_rows, wo.t())
-        ctx.save_for_backward(y, wqkv, wo, qkv, o_rows, lse, inv_freq, positions, probs)
-        ctx.meta = (spec, heads, scale)
+        ctx.save_for_backward(y, wqkv, wo, qkv, o_rows, lse, inv_freq, positions, probs, q_norm,
+                              k_norm)
+        ctx.meta = (spec, heads, scale, eps)
         ctx.plans = plans
         return a
 
     @staticmethod
     def backward(ctx, da):
-        y, wqkv, wo, qkv, o_rows, lse, inv_freq, positions, probs = ctx.saved_tensors
-        spec, (Hq, Hkv, D), scale = ctx.meta
+        (y, wqkv, wo, qkv, o_rows, lse, inv_freq, positions, probs, q_norm,
+         k_norm) = ctx.saved_tensors
+        spec, (Hq, Hkv, D), scale, eps = ctx.meta
         B, L, d = y.shape
         da = da.contiguous()
         do_rows = torch.matmul(da, wo)                        # [B, L, Hq D]
         dwo = torch.matmul(da.reshape(-1, d).t(), o_rows.reshape(-1, Hq * D))
         q, k, v = _split_heads(qkv, B, L, Hq, Hkv, D)
+        raw_q, raw_k = q, k
+        if q_norm is not None:
+            q, k = layer_ops.qk_norm_rope(q, k, q_norm, k_norm, eps, inv_freq, positions)
         o = o_rows.view(B, L, Hq, D).transpose(1, 2)
         dqkv = torch.empty_like(qkv)
         dq, dk, dv = _split_heads(dqkv, B, L, Hq, Hkv, D)
@@ -112,10 +175,15 @@ class _AttentionBlock(torch.autograd.Function):
         ops.backward(q, k, v, o, lse, do_rows.view(B, L, Hq, D).transpose(1, 2), spec, scale,
                      dq=dq, dk=dk, dv=dv, probs=probs, key_plan=plan)
         del do_rows
-        layer_ops.rope_(dq, dk, inv_freq, positions, inverse=True)
+        dq_norm = dk_norm = None
+        if q_norm is None:
+            layer_ops.rope_(dq, dk, inv_freq, positions, inverse=True)
+        else:
+            _, _, dq_norm, dk_norm = layer_ops.qk_norm_rope_backward(
+                raw_q, raw_k, q_norm, k_norm, eps, inv_freq, dq, dk, positions, dq=dq, dk=dk)
         dy = torch.matmul(dqkv, wqkv)
         dwqkv = torch.matmul(dqkv.reshape(-1, dqkv.shape[-1]).t(), y.reshape(-1, d))
-        return dy, dwqkv, dwo, None, None, None, None, None
+        return dy, dwqkv, dwo, None, None, None, None, None, dq_norm, dk_norm, None
 
 
 def _split_heads(qkv, B, L, Hq, Hkv, D):
@@ -149,6 +217,67 @@ class _MLPBlock(torch.autograd.Function):
         dy = torch.matmul(dgu, wgu)
         dwgu = torch.matmul(dgu.reshape(-1, dgu.shape[-1]).t(), y.reshape(-1, d))
         return dy, dwgu, dwd
+
+
+class _PackedMLPBlock(torch.autograd.Function):
+    """:class:`_MLPBlock` whose gate / up rows are kept in 8 bits."""
+
+    @staticmethod
+    def forward(ctx, y, wgu, wd, fmt: str):
+        m, p = layer_ops.swiglu_forward_packed(torch.matmul(y, wgu.t()), fmt)
+        ctx.save_for_backward(y, wgu, wd, p.codes, p.scales)
+        ctx.meta = (fmt, m.dtype)
+        return torch.matmul(m, wd.t())
+
+    @staticmethod
+    def backward(ctx, dout):
+        y, wgu, wd, codes, scales = ctx.saved_tensors
+        d = y.shape[-1]
+        dout = dout.contiguous()
+        dm = torch.matmul(dout, wd)
+        dgu, m = layer_ops.swiglu_backward_packed(PackedRows(codes, scales, *ctx.meta), dm)
+        del dm
+        dwd = torch.matmul(dout.reshape(-1, d).t(), m.reshape(-1, m.shape[-1]))
+        del m
+        dy = torch.matmul(dgu, wgu)
+        dwgu = torch.matmul(dgu.reshape(-1, dgu.shape[-1]).t(), y.reshape(-1, d))
+        return dy, dwgu, dwd, None
+
+
+class _PackedLayer(torch.autograd.Function):
+    """One decoder layer that keeps its input h in 8 bits (codes, scales) and
+    nothing else: (h', y', codes', scales') = layer(h, y), codes' / scales' the
+    8-bit form of h'.  The backward restores h and y = norm(h) from the codes,
+    runs the layer again and differentiates that run."""
+
+    @staticmethod
+    def forward(ctx, stack, i: int, h, y, codes, scales, positions, *params):
+        ctx.stack, ctx.i, ctx.dtype = stack, i, h.dtype
+        ctx.save_for_backward(codes, scales, positions, *params)
+        fmt = stack.activation_storage
+        h, m, w = stack._layer_body(i, h, y, positions)
+        h, m = h.contiguous(), m.contiguous()
+        if i + 1 == len(stack.layers):      # no layer follows that would keep h
+            h, y, _ = layer_ops.rmsnorm_forward(h, w, stack.eps, residual=m)
+            return h, y, None, None
+        h, y, _, p = layer_ops.rmsnorm_forward_packed(h, w, stack.eps, residual=m, format=fmt)
+        ctx.mark_non_differentiable(p.codes, p.scales)
+        return h, y, p.codes, p.scales
+
+    @staticmethod
+    def backward(ctx, dh, dy, _codes, _scales):
+        stack, i = ctx.stack, ctx.i
+        codes, scales, positions, *params = ctx.saved_tensors
+        h, y, _ = layer_ops.rmsnorm_from_packed(
+            PackedRows(codes, scales, stack.activation_storage, ctx.dtype),
+            stack._input_norm(i), stack.eps)
+        wanted = [h.requires_grad_(), y.requires_grad_()] + [p for p in params if p.requires_grad]
+        with torch.enable_grad():
+            out = stack._layer(i, h, y, positions)
+        grads = iter(torch.autograd.grad(out, wanted, (dh, dy), allow_unused=True))
+        gh, gy = next(grads), next(grads)
+        return (None, None, gh, gy, None, None, None,
+                *(next(grads) if p.requires_grad else None for p in params))
 
 
 class _LMHeadCrossEntropy(torch.autograd.Function):
@@ -196,7 +325,8 @@ class _LMHeadCrossEntropy(torch.autograd.Function):
 class ElasticDecoderLayerWeights(nn.Module):
     """The parameters of one decoder layer (pre-norm, fused QKV and gate/up)."""
 
-    def __init__(self, hidden: int, Hq: int, Hkv: int, D: int, ffn: int, dtype, device):
+    def __init__(self, hidden: int, Hq: int, Hkv: int, D: int, ffn: int, dtype, device,
+                 qk_norm: bool = False):
         super().__init__()
         kw = dict(dtype=dtype, device=device)
         self.input_norm = nn.Parameter(torch.ones(hidden, **kw))
@@ -205,6 +335,8 @@ class ElasticDecoderLayerWeights(nn.Module):
         self.post_attention_norm = nn.Parameter(torch.ones(hidden, **kw))
         self.gate_up_proj = nn.Parameter(torch.empty(2 * ffn, hidden, **kw))
         self.down_proj = nn.Parameter(torch.empty(hidden, ffn, **kw))
+        self.q_norm = nn.Parameter(torch.ones(D, **kw)) if qk_norm else None
+        self.k_norm = nn.Parameter(torch.ones(D, **kw)) if qk_norm else None
 
 
 class ElasticDecoderStack(nn.Module):
@@ -213,7 +345,9 @@ class ElasticDecoderStack(nn.Module):
 
     Defaults are the C4 configuration: 4 layers, hidden 4096, 32 heads of
     128, SwiGLU 11008, RoPE base 10000, vocabulary 32000, attention_length 64.
-    Weights are random N(0, 0.02) (norm weights 1) in ``dtype``.
+    Weights are random N(0, 0.02) (norm weights 1) in ``dtype``.  The options
+    ``embed_scale``, ``padding_idx``, ``qk_norm`` and ``activation_storage`` are
+    described at the top of this file.
     """
 
     def __init__(self, vocab_size: int = 32000, hidden_size: int = 4096,
@@ -222,8 +356,17 @@ class ElasticDecoderStack(nn.Module):
                  intermediate_size: int = 11008, rope_theta: float = 10000.0,
                  rms_norm_eps: float = 1e-6, attention_length: int = 64,
                  max_seq_len: int = 262144, activation_checkpointing: bool = False,
-                 loss_chunk_rows: int = 8192, dtype=torch.bfloat16, device=None, seed: int = 0):
+                 loss_chunk_rows: int = 8192, dtype=torch.bfloat16, device=None, seed: int = 0,
+                 embed_scale: float | None = None, padding_idx: int | None = None,
+                 qk_norm: bool = False, activation_storage: str | None = None):
         super().__init__()
+        if activation_storage is not None and activation_storage not in PACK_FORMATS:
+            raise ValueError(f"activation_storage must be one of {sorted(PACK_FORMATS)} or None")
+        if padding_idx is not None and not 0 <= padding_idx < vocab_size:
+            raise ValueError(f"padding_idx {padding_idx} outside [0, {vocab_size})")
+        self.embed_scale = embed_scale
+        self.padding_idx = padding_idx
+        self.activation_storage = activation_storage
         self.Hq = num_attention_heads
         self.Hkv = num_key_value_heads or num_attention_heads
         if self.Hq % self.Hkv:
@@ -243,7 +386,7 @@ class ElasticDecoderStack(nn.Module):
         self.embed = nn.Parameter(torch.empty(vocab_size, hidden_size, **kw))
         self.layers = nn.ModuleList(
             ElasticDecoderLayerWeights(hidden_size, self.Hq, self.Hkv, self.D, intermediate_size,
-                                       dtype, device) for _ in range(num_hidden_layers))
+                                       dtype, device, qk_norm) for _ in range(num_hidden_layers))
         self.final_norm = nn.Parameter(torch.ones(hidden_size, **kw))
         self.lm_head = nn.Parameter(torch.empty(vocab_size, hidden_size, **kw))
         self.register_buffer("inv_freq", layer_ops.rope_inv_freq(self.D, rope_theta, device),
@@ -254,15 +397,42 @@ class ElasticDecoderStack(nn.Module):
                 if p.dim() == 2:
                     p.copy_(torch.randn(p.shape, generator=g) * 0.02)
 
-    def _layer(self, i: int, h, y, positions):
+    def _input_norm(self, i: int) -> nn.Parameter:
+        """The weight of the norm before layer i (the final norm after the last)."""
+        return self.layers[i].input_norm if i < len(self.layers) else self.final_norm
+
+    def _layer_body(self, i: int, h, y, positions):
+        """Layer i up to its last residual add: (h, m, weight of the norm of h + m)."""
         lw = self.layers[i]
         a = _AttentionBlock.apply(y, lw.qkv_proj, lw.o_proj, self.specs[i],
                                   (self.Hq, self.Hkv, self.D), self.inv_freq, positions,
-                                  self.key_plans[i])
+                                  self.key_plans[i], lw.q_norm, lw.k_norm, self.eps)
         h, y2 = _AddRMSNorm.apply(h, a, lw.post_attention_norm, self.eps)
-        m = _MLPBlock.apply(y2, lw.gate_up_proj, lw.down_proj)
-        next_w = self.layers[i + 1].input_norm if i + 1 < len(self.layers) else self.final_norm
+        if (self.activation_storage is not None and not self.checkpointing
+                and torch.is_grad_enabled()):
+            m = _PackedMLPBlock.apply(y2, lw.gate_up_proj, lw.down_proj, self.activation_storage)
+        else:
+            m = _MLPBlock.apply(y2, lw.gate_up_proj, lw.down_proj)
+        return h, m, self._input_norm(i + 1)
+
+    def _layer(self, i: int, h, y, positions):
+        h, m, next_w = self._layer_body(i, h, y, positions)
         return _AddRMSNorm.apply(h, m, next_w, self.eps)
+
+    def _layer_params(self, i: int) -> list:
+        """The parameters that layer i's outputs depend on besides h and y."""
+        lw = self.layers[i]
+        ps = [lw.qkv_proj, lw.o_proj, lw.post_attention_norm, lw.gate_up_proj, lw.down_proj]
+        if lw.q_norm is not None:
+            ps += [lw.q_norm, lw.k_norm]
+        return ps + [self._input_norm(i + 1)]
+
+    def _embed(self, ids):
+        if self.embed_scale is None and self.padding_idx is None:
+            return F.embedding(ids, self.embed)
+        return _Embedding.apply(ids, self.embed,
+                                1.0 if self.embed_scale is None else self.embed_scale,
+                                self.padding_idx)
 
     def forward(self, input_ids: torch.Tensor, labels: torch.Tensor | None = None,
                 positions: torch.Tensor | None = None):
@@ -274,14 +444,21 @@ class ElasticDecoderStack(nn.Module):
             raise ValueError(f"sequence length {L} exceeds max_seq_len {self.max_seq_len}")
         if positions is None:
             positions = torch.arange(L, device=input_ids.device)
-        h = F.embedding(input_ids, self.embed)
-        y = _RMSNorm.apply(h, self.layers[0].input_norm, self.eps)
-        for i in range(len(self.layers)):
-            if self.checkpointing and torch.is_grad_enabled():
-                h, y = torch.utils.checkpoint.checkpoint(self._layer, i, h, y, positions,
-                                                         use_reentrant=False)
-            else:
-                h, y = self._layer(i, h, y, positions)
+        h = self._embed(input_ids)
+        if self.checkpointing and self.activation_storage is not None and torch.is_grad_enabled():
+            y, codes, scales = _PackedRMSNorm.apply(h, self._input_norm(0), self.eps,
+                                                    self.activation_storage)
+            for i in range(len(self.layers)):
+                h, y, codes, scales = _PackedLayer.apply(self, i, h, y, codes, scales, positions,
+                                                         *self._layer_params(i))
+        else:
+            y = _RMSNorm.apply(h, self._input_norm(0), self.eps)
+            for i in range(len(self.layers)):
+                if self.checkpointing and torch.is_grad_enabled():
+                    h, y = torch.utils.checkpoint.checkpoint(self._layer, i, h, y, positions,
+                                                             use_reentrant=False)
+                else:
+                    h, y = self._layer(i, h, y, positions)
         if labels is None:
             return y
         targets = torch.full_like(labels, -100)
