@@ -925,7 +925,9 @@ def bench_c4(args):
     dev = torch.device("cuda", 0)
     L4 = args.c4_seq_len
     m = esa.ElasticDecoderStack(max_seq_len=L4, device=dev, seed=0,
-                                activation_checkpointing=args.checkpoint)
+                                activation_checkpointing=args.checkpoint,
+                                activation_storage=args.activation_storage,
+                                qk_norm=args.qk_norm, embed_scale=args.embed_scale)
     g = torch.Generator().manual_seed(4)
     ids_host = torch.randint(0, 32000, (1, L4), generator=g).pin_memory()
     ids = ids_host.to(dev)
@@ -966,6 +968,8 @@ def bench_c4(args):
                                    "RMSNorm, RoPE 1e4, vocab 32000, elastic attention w=64 nl=4",
                        "global_batch": 1, "seq_len": L4,
                        "activation_checkpointing": bool(args.checkpoint),
+                       "activation_storage": args.activation_storage,
+                       "qk_norm": bool(args.qk_norm), "embed_scale": args.embed_scale,
                        "l2": "activations of GBs per step, far above the 126 MB L2"},
             "loss": round(loss_val, 4), "peak_memory_gb": round(peak_gb, 1),
             "gemm_flops_per_step": m.flops_per_token(L4) * L4,
@@ -1128,6 +1132,11 @@ def main():
     ap.add_argument("--c4-seq-len", type=int, default=262144)
     ap.add_argument("--checkpoint", action="store_true",
                     help="c4: recompute each decoder layer in the backward")
+    ap.add_argument("--activation-storage", choices=["int8", "e4m3"], default=None,
+                    help="c4: keep layer inputs (--checkpoint) or the MLP's gate / up rows in 8 bits")
+    ap.add_argument("--qk-norm", action="store_true", help="c4: normalise query and key heads")
+    ap.add_argument("--embed-scale", type=float, default=None,
+                    help="c4: scaled embedding with the library's lookup and gradient")
     ap.add_argument("--case", choices=["step", "one-layer", "rows"], default="step",
                     help="one-layer: a single fwd+bwd at --seq-len/--layer, for profilers; "
                          "rows: the sequence split's layout copies at C5's 2-rank shapes")

@@ -271,13 +271,19 @@ class _PackedLayer(torch.autograd.Function):
         h, y, _ = layer_ops.rmsnorm_from_packed(
             PackedRows(codes, scales, stack.activation_storage, ctx.dtype),
             stack._input_norm(i), stack.eps)
-        wanted = [h.requires_grad_(), y.requires_grad_()] + [p for p in params if p.requires_grad]
+        params_in = [p for p in params[:-1] if p.requires_grad]
+        wanted = [h.requires_grad_(), y.requires_grad_()] + params_in
         with torch.enable_grad():
-            out = stack._layer(i, h, y, positions)
-        grads = iter(torch.autograd.grad(out, wanted, (dh, dy), allow_unused=True))
+            h1, m, w = stack._layer_body(i, h, y, positions)
+        del h, y
+        # the last add and norm by hand: its outputs are gone before the rest runs backward
+        h2, _, rstd = layer_ops.rmsnorm_forward(h1.detach(), w, stack.eps, residual=m.detach())
+        ds, dw = layer_ops.rmsnorm_backward(h2, w, rstd, dy, dh_in=dh)
+        del h2, rstd, dh, dy
+        grads = iter(torch.autograd.grad((h1, m), wanted, (ds, ds)))
         gh, gy = next(grads), next(grads)
-        return (None, None, gh, gy, None, None, None,
-                *(next(grads) if p.requires_grad else None for p in params))
+        by_param = [next(grads) if p.requires_grad else None for p in params[:-1]]
+        return (None, None, gh, gy, None, None, None, *by_param, dw if w.requires_grad else None)
 
 
 class _LMHeadCrossEntropy(torch.autograd.Function):
@@ -420,7 +426,8 @@ class ElasticDecoderStack(nn.Module):
         return _AddRMSNorm.apply(h, m, next_w, self.eps)
 
     def _layer_params(self, i: int) -> list:
-        """The parameters that layer i's outputs depend on besides h and y."""
+        """The parameters that layer i's outputs depend on besides h and y, the
+        weight of the norm after it last."""
         lw = self.layers[i]
         ps = [lw.qkv_proj, lw.o_proj, lw.post_attention_norm, lw.gate_up_proj, lw.down_proj]
         if lw.q_norm is not None:
