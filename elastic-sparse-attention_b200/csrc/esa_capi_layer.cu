@@ -42,6 +42,7 @@ int check_embedding(const char* what, int32_t dtype, int32_t id_bytes, int64_t n
 
 // Geometry and workspace of the sorted gradient.
 struct GradPlan {
+  int key_bits;              // keys are 0 .. vocab
   int passes, bits;          // digits of the key, bits per digit
   int tile;                  // keys per sorting CTA
   int64_t tiles, pieces;
@@ -50,10 +51,10 @@ struct GradPlan {
 
 GradPlan grad_plan(int64_t n, int64_t vocab, int32_t dim) {
   GradPlan g;
-  int bits = 1;
-  while ((vocab >> bits) != 0) ++bits;               // keys 0 .. vocab
-  g.passes = (int)ceil_div(bits, em::kRadixBits);
-  g.bits = (int)ceil_div(bits, g.passes);
+  g.key_bits = 1;
+  while ((vocab >> g.key_bits) != 0) ++g.key_bits;
+  g.passes = (int)ceil_div(g.key_bits, em::kRadixBits);
+  g.bits = (int)ceil_div(g.key_bits, g.passes);
   g.tile = (int)(ceil_div(std::max<int64_t>(ceil_div(n, em::kSortMaxTiles), em::kSortTile),
                           em::kSortTile) * em::kSortTile);
   g.tiles = ceil_div(n, g.tile);
@@ -81,54 +82,86 @@ int embedding_grad(int64_t n, int64_t vocab, int32_t dim, const em::Ids& ids, co
                    float scale, int64_t pad, void* dweight, char* ws, int* err, cudaStream_t s) {
   const uint32_t vpr = dim / esa::Vec<T>::kElems;
   const unsigned ychunks = (unsigned)ceil_div(vpr, em::kGradThreads);
-  if (ychunks > 65535) return fail(ESA_ERR_UNSUPPORTED, "esa_embedding_backward: dim %d too large", dim);
+  if (vpr > 32 * 65535) return fail(ESA_ERR_UNSUPPORTED, "esa_embedding_backward: dim %d too large", dim);
   if (n <= em::kDirectMax) {
-    // about four CTAs per SM over the vocabulary, 32 rows of it at most
-    const int R = (int)std::min<int64_t>(32, ceil_div(vocab * ychunks, 148 * 4));
-    em::grad_direct_kernel<T><<<dim3((unsigned)ceil_div(vocab, R), ychunks), em::kGradThreads, 0, s>>>(
-        (int)n, vocab, R, vpr, ids, static_cast<const T*>(dy), scale, pad, static_cast<T*>(dweight),
-        err);
-    return check_launch("esa_embedding_backward");
+    auto direct = [&](auto nv) {
+      constexpr int NV = decltype(nv)::value;
+      // about eight CTAs per SM over the vocabulary, 32 rows of it at most
+      const unsigned chunks = (unsigned)ceil_div(vpr, 32 * NV);
+      const int R = (int)std::min<int64_t>(32, ceil_div(vocab * chunks, 148 * 8));
+      em::grad_direct_kernel<T, NV>
+          <<<dim3((unsigned)ceil_div(vocab, R), chunks), em::kDirectThreads, 0, s>>>(
+              (int)n, vocab, R, vpr, ids, static_cast<const T*>(dy), scale, pad,
+              static_cast<T*>(dweight), err);
+      return check_launch("esa_embedding_backward");
+    };
+    if (vpr > 64) return direct(std::integral_constant<int, 4>{});
+    return direct(std::integral_constant<int, 1>{});
   }
   const GradPlan g = grad_plan(n, vocab, dim);
-  em::SortPass p;
-  p.n = n;
-  p.vocab = vocab;
-  p.pad = pad;
-  p.ids = ids;
-  p.keys = p.rows = nullptr;
-  p.bits = g.bits;
-  p.tile = g.tile;
-  p.hist = reinterpret_cast<uint32_t*>(ws + g.hist);
-  p.counter = reinterpret_cast<int*>(ws + g.counter);
-  p.err = err;
-  for (int i = 0; i < g.passes; ++i) {
-    p.shift = i * g.bits;
-    p.out_keys = reinterpret_cast<uint32_t*>(ws + g.keys[i & 1]);
-    p.out_rows = reinterpret_cast<uint32_t*>(ws + g.rows[i & 1]);
-    const dim3 grid((unsigned)g.tiles), block(em::kSortThreads);
-    if (i == 0) {
-      em::sort_hist_kernel<<<grid, block, 0, s>>>(p);
-      if (int rc = check_launch("esa_embedding_backward (histogram)")) return rc;
-    } else if (int rc = launch_after("esa_embedding_backward (histogram)", em::sort_hist_kernel,
-                                     grid, block, s, p)) {
-      return rc;
+  uint32_t* keys[2];
+  uint32_t* rows[2];
+  for (int i = 0; i < 2; ++i) {
+    keys[i] = reinterpret_cast<uint32_t*>(ws + g.keys[i]);
+    rows[i] = reinterpret_cast<uint32_t*>(ws + g.rows[i]);
+  }
+  int* counter = reinterpret_cast<int*>(ws + g.counter);
+  int last = 0;                          // which buffer holds the sorted pairs
+  if (n <= em::kSmallMax) {
+    em::SmallSort p;
+    p.vocab = vocab;
+    p.pad = pad;
+    p.ids = ids;
+    p.n = (int)n;
+    p.passes = (int)ceil_div(g.key_bits, em::kSmallBits);
+    p.bits = (int)ceil_div(g.key_bits, p.passes);
+    p.out_keys = keys[0];
+    p.out_rows = rows[0];
+    p.counter = counter;
+    p.err = err;
+    em::sort_small_kernel<<<1, em::kSmallThreads, 0, s>>>(p);
+    if (int rc = check_launch("esa_embedding_backward (sort)")) return rc;
+  } else {
+    em::SortPass p;
+    p.n = n;
+    p.vocab = vocab;
+    p.pad = pad;
+    p.ids = ids;
+    p.keys = p.rows = nullptr;
+    p.bits = g.bits;
+    p.tile = g.tile;
+    p.hist = reinterpret_cast<uint32_t*>(ws + g.hist);
+    p.counter = counter;
+    p.err = err;
+    for (int i = 0; i < g.passes; ++i) {
+      p.shift = i * g.bits;
+      p.out_keys = keys[i & 1];
+      p.out_rows = rows[i & 1];
+      const dim3 grid((unsigned)g.tiles), block(em::kSortThreads);
+      if (i == 0) {
+        em::sort_hist_kernel<<<grid, block, 0, s>>>(p);
+        if (int rc = check_launch("esa_embedding_backward (histogram)")) return rc;
+      } else if (int rc = launch_after("esa_embedding_backward (histogram)", em::sort_hist_kernel,
+                                       grid, block, s, p)) {
+        return rc;
+      }
+      if (int rc = launch_after("esa_embedding_backward (sort)", em::sort_scatter_kernel, grid,
+                                block, s, p))
+        return rc;
+      p.keys = p.out_keys;
+      p.rows = p.out_rows;
+      last = i & 1;
     }
-    if (int rc = launch_after("esa_embedding_backward (sort)", em::sort_scatter_kernel, grid, block,
-                              s, p))
-      return rc;
-    p.keys = p.out_keys;
-    p.rows = p.out_rows;
   }
   em::GradParams q;
   q.n = n;
   q.vocab = vocab;
   q.vpr = vpr;
-  q.keys = p.keys;
-  q.rows = p.rows;
+  q.keys = keys[last];
+  q.rows = rows[last];
   q.scale = scale;
   q.part = reinterpret_cast<float*>(ws + g.part);
-  q.counter = p.counter;
+  q.counter = counter;
   q.owners = reinterpret_cast<uint2*>(ws + g.owners);
   q.pieces = g.pieces;
   q.zero_blocks = (int)ceil_div(vocab, em::kZeroRows);
