@@ -83,7 +83,7 @@ int embedding_grad(int64_t n, int64_t vocab, int32_t dim, const em::Ids& ids, co
   const uint32_t vpr = dim / esa::Vec<T>::kElems;
   const unsigned ychunks = (unsigned)ceil_div(vpr, em::kGradThreads);
   if (vpr > 32 * 65535) return fail(ESA_ERR_UNSUPPORTED, "esa_embedding_backward: dim %d too large", dim);
-  if (n <= em::kDirectMax) {
+  if (n <= em::direct_max(dim)) {
     auto direct = [&](auto nv) {
       constexpr int NV = decltype(nv)::value;
       // about eight CTAs per SM over the vocabulary, 32 rows of it at most
@@ -345,7 +345,7 @@ int esa_embedding_forward(int32_t dtype, int32_t id_bytes, int64_t n_tokens, int
 }
 
 size_t esa_embedding_backward_workspace_size(int64_t n_tokens, int64_t vocab, int32_t dim) {
-  if (n_tokens <= em::kDirectMax || n_tokens > kMaxTokens || vocab < 1 || vocab > kMaxVocab ||
+  if (n_tokens <= em::direct_max(dim) || n_tokens > kMaxTokens || vocab < 1 || vocab > kMaxVocab ||
       dim < 1)
     return 0;
   return grad_plan(n_tokens, vocab, dim).bytes;
