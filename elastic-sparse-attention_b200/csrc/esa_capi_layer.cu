@@ -242,8 +242,22 @@ int rounds_per_task(int rounds, int64_t tokens) {
   return (int)ceil_div(rounds, tasks);
 }
 
+// Tokens of a task that takes several because a token's heads fill less than
+// one of its rounds, or a quarter of them (1: they fill more).  With half of
+// them filled a task of one token is faster (16 / 4 heads of 128, bf16
+// backward, 9910 tokens: 43 against 54 us).  No more than leaves 16 warps per
+// SM a task.
+int tokens_per_task(int heads, int rows_per_warp, int rounds, int64_t tokens) {
+  if (heads == 0 || (heads >= rows_per_warp && rounds < 4 * ceil_div(heads, rows_per_warp))) return 1;
+  return (int)std::max<int64_t>(1, std::min<int64_t>(rounds * rows_per_warp / heads,
+                                                     tokens / (148 * 16)));
+}
+
 template <typename T>
 void set_tasks(qk::Params<T>& p, int rows_per_warp) {
+  p.nt = tokens_per_task(p.q.H + p.k.H, rows_per_warp, qk::kFewRounds, p.tokens);
+  p.nt_q = tokens_per_task(p.q.H, rows_per_warp, qk::kBwdUnroll<T>, p.tokens);
+  p.nt_k = tokens_per_task(p.k.H, rows_per_warp, qk::kBwdUnroll<T>, p.tokens);
   p.rq = (int)ceil_div(p.q.H, rows_per_warp);
   p.rk = (int)ceil_div(p.k.H, rows_per_warp);
   p.rpt = rounds_per_task(p.rq + p.rk, p.tokens);
@@ -258,11 +272,18 @@ int qk_bwd_ctas(int64_t tokens, int32_t hq, int32_t hk) {
   return (int)std::max<int64_t>(2, std::min<int64_t>(kQkBwdCtas, ceil_div(tokens * (hq + hk), qk::kWarps)));
 }
 
-// Share of the CTAs that the query heads get (at least one for each side present).
-int qk_q_ctas(int ctas, int32_t hq, int32_t hk) {
-  if (hk == 0) return ctas;
-  if (hq == 0) return 0;
-  return std::max(1, std::min(ctas - 1, (int)((int64_t)ctas * hq / (hq + hk))));
+// Share of the CTAs that the query heads get (at least one for each side
+// present): by the loop steps of the two sides, which take about as long
+// whether their U rounds are full or not.
+template <typename T>
+int qk_q_ctas(const qk::Params<T>& p, int ctas) {
+  if (p.k.H == 0) return ctas;
+  if (p.q.H == 0) return 0;
+  auto steps = [&](int nt, int tasks, int rpt) {
+    return nt > 1 ? ceil_div(p.tokens, nt) : p.tokens * tasks * ceil_div(rpt, qk::kBwdUnroll<T>);
+  };
+  const int64_t q = steps(p.nt_q, p.tasks_q, p.rpt_q), k = steps(p.nt_k, p.tasks_k, p.rpt_k);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(ctas - 1, ctas * q / (q + k)));
 }
 
 // ---------------------------------------------------------------------------
@@ -400,12 +421,17 @@ int esa_qk_norm_rope_forward(int32_t dtype, int32_t batch, int64_t seq_len, int3
     p.eps = eps;
     const int tpr = head_dim / (2 * esa::Vec<T>::kElems);
     set_tasks(p, 32 / tpr);
-    const int64_t ctas = ceil_div(p.tokens * p.tasks, qk::kWarps);
+    const int64_t ctas = p.nt > 1 ? ceil_div(p.tokens, (int64_t)p.nt * qk::kWarps)
+                                  : ceil_div(p.tokens * p.tasks, qk::kWarps);
     if (ctas > INT32_MAX)
       return fail(ESA_ERR_UNSUPPORTED, "esa_qk_norm_rope_forward: too many positions");
     return by_threads_per_row<1>(tpr, [&](auto t) {
-      qk::fwd_kernel<T, decltype(t)::value>
-          <<<(unsigned)ctas, qk::kThreads, 0, (cudaStream_t)stream>>>(p);
+      constexpr int TPR = decltype(t)::value;
+      cudaStream_t s = (cudaStream_t)stream;
+      if (p.nt > 1)
+        qk::fwd_few_kernel<T, TPR><<<(unsigned)ctas, qk::kThreads, 0, s>>>(p);
+      else
+        qk::fwd_kernel<T, TPR><<<(unsigned)ctas, qk::kThreads, 0, s>>>(p);
       return check_launch("esa_qk_norm_rope_forward");
     });
   });
@@ -461,7 +487,7 @@ int esa_qk_norm_rope_backward(int32_t dtype, int32_t batch, int64_t seq_len, int
     const int tpr = head_dim / 8;   // four elements of each half per thread
     set_tasks(p, 32 / tpr);
     const int ctas = qk_bwd_ctas(p.tokens, num_q_heads, num_k_heads);
-    const int q_ctas = qk_q_ctas(ctas, num_q_heads, num_k_heads);
+    const int q_ctas = qk_q_ctas(p, ctas);
     float* part = static_cast<float*>(workspace);
     return by_threads_per_row<esa::Vec<T>::kElems / 4>(tpr, [&](auto t) {
       qk::bwd_kernel<T, decltype(t)::value><<<ctas, qk::kThreads, 0, s>>>(p, q_ctas, part);

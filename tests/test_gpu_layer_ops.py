@@ -171,7 +171,11 @@ def qk_case(dtype, B, L, Hq, Hk, D, seed, far=False):
 
 
 QK_SHAPES = [(1, 1, 32, 8, 128), (2, 333, 4, 2, 64), (3, 5, 3, 1, 16), (1, 70, 5, 5, 32),
-             (2, 40, 6, 2, 128), (1, 3, 1, 1, 64), (1, 2100, 8, 2, 128)]
+             (2, 40, 6, 2, 128), (1, 3, 1, 1, 64), (1, 2100, 8, 2, 128),
+             # few heads, several tokens per warp: whole and partial last tasks, odd heads,
+             # tasks across the batch border
+             (3, 2400, 1, 1, 16), (2, 5003, 3, 1, 32), (1, 9001, 2, 1, 128), (5, 1900, 5, 2, 64),
+             (1, 4800, 8, 1, 32)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
