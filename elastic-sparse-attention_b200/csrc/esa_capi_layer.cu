@@ -457,13 +457,11 @@ int esa_qk_norm_rope_backward(int32_t dtype, int32_t batch, int64_t seq_len, int
   if ((num_q_heads > 0 && !dq_weight) || (num_k_heads > 0 && !dk_weight))
     return fail(ESA_ERR_INVALID, "esa_qk_norm_rope_backward: null weight gradient");
   cudaStream_t s = (cudaStream_t)stream;
-  if (batch == 0 || seq_len == 0) {   // sums over no rows
-    const size_t bytes = (size_t)head_dim * elem_size(dtype);
-    if (num_q_heads > 0) cudaMemsetAsync(dq_weight, 0, bytes, s);
-    if (num_k_heads > 0) cudaMemsetAsync(dk_weight, 0, bytes, s);
-    return check_launch("esa_qk_norm_rope_backward");
-  }
-  if (num_q_heads + num_k_heads == 0) return ESA_OK;
+  const bool no_tokens = batch == 0 || seq_len == 0;   // sums over no rows are zero
+  const size_t weight_bytes = (size_t)head_dim * elem_size(dtype);
+  if (dq_weight && (no_tokens || num_q_heads == 0)) cudaMemsetAsync(dq_weight, 0, weight_bytes, s);
+  if (dk_weight && (no_tokens || num_k_heads == 0)) cudaMemsetAsync(dk_weight, 0, weight_bytes, s);
+  if (no_tokens || num_q_heads + num_k_heads == 0) return check_launch("esa_qk_norm_rope_backward");
   if (!inv_freq) return fail(ESA_ERR_INVALID, "esa_qk_norm_rope_backward: null inv_freq");
   const size_t need = esa_qk_norm_rope_backward_workspace_size(batch, seq_len, num_q_heads,
                                                                num_k_heads, head_dim);

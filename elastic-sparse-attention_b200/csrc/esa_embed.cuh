@@ -1,7 +1,7 @@
 // Token embedding: lookup with a scale, and the weight gradient by sorted tokens.
 //
 //   out[r]  = scale * W[id_r]                                (one rounding)
-//   dW[v]   = scale * sum over r ascending, id_r = v, of dy[r]   (float32 sums)
+//   dW[v]   = scale * sum over r with id_r = v of dy[r]        (float32 sums)
 //
 // Both move rows and do almost no arithmetic: they are bound by HBM.  The
 // gradient sums the rows of each token in a fixed order without atomics, so

@@ -175,7 +175,7 @@ def embedding_forward(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.
 def embedding_backward(ids: torch.Tensor, dy: torch.Tensor, vocab_size: int, scale: float = 1.0,
                        padding_idx: int | None = None) -> torch.Tensor:
     """dweight [vocab_size, dim] of :func:`embedding_forward` for dy
-    [*ids.shape, dim]: float32 sums over each token's rows in ascending order
+    [*ids.shape, dim]: float32 sums over each token's rows in a fixed order
     (the same in every run), rounded once to dy's dtype.  Rows of absent
     tokens and the row ``padding_idx`` are zero."""
     dev = _check_device(ids, dy)

@@ -16,7 +16,8 @@
  * (ESA_DTYPE_F32 / _BF16 / _F16); rows are contiguous vectors of `dim`
  * elements (row stride = dim) unless stated otherwise; every pointer is
  * 16-byte aligned and dim * element size is a multiple of 16 bytes.
- * Arithmetic is float32; each output is rounded once to dtype.
+ * Arithmetic is float32; each output is rounded once to dtype.  Outputs do not
+ * overlap inputs or each other unless an entry point allows it.
  */
 #ifndef ESA_LAYER_H
 #define ESA_LAYER_H
@@ -106,8 +107,9 @@ size_t esa_embedding_backward_workspace_size(int64_t n_tokens, int64_t vocab, in
 
 /*
  * Gradient of esa_embedding_forward:
- *   dweight[v] = scale * sum over ascending r with ids[r] = v of dy[r]
- * (float32 sums without atomics: the same in every run; rounded once).  All
+ *   dweight[v] = scale * sum over r with ids[r] = v of dy[r]
+ * (float32 sums in a fixed order, without atomics: the same in every run;
+ * rounded once).  All
  * of dweight [vocab, dim] is written; rows of absent tokens and row
  * padding_idx (none if negative) are zero.  Ids outside [0, vocab) are left
  * out and set ESA_DEVERR_TOKEN_RANGE.  workspace: 256-byte aligned, its
@@ -152,7 +154,8 @@ size_t esa_qk_norm_rope_backward_workspace_size(int32_t batch, int64_t seq_len,
  *   dx = rstd * (weight * g - xhat * mean(xhat * weight * g))
  *   dweight = sum over batch, heads and positions of g * xhat   (in dtype)
  * dq / dk may be dq_out / dk_out themselves.  Sums are float32 in a fixed
- * order.  With no rows the weight gradients are zero.
+ * order.  With no rows the weight gradients are zero; so is a given dq_weight
+ * / dk_weight of a side without heads.
  */
 int esa_qk_norm_rope_backward(int32_t dtype, int32_t batch, int64_t seq_len, int32_t head_dim,
                               esa_tensor_t q, int32_t num_q_heads, esa_tensor_t k,

@@ -314,6 +314,20 @@ def test_qk_norm_rope_gradient_is_the_difference_quotient(lops):
     assert abs(got - quotient) <= 1e-5 * scale
 
 
+def test_qk_norm_rope_side_without_heads(lops):
+    inv = lops.rope_inv_freq(64, 10000.0, DEV)
+    w = torch.ones(64, device=DEV)
+    q = torch.randn(1, 3, 5, 64, device=DEV)
+    none = q[:, :0]
+    for a, b in ((q, none), (none, q)):
+        a2, b2 = lops.qk_norm_rope(a, b, w, w, 1e-6, inv)
+        da, db, dwa, dwb = lops.qk_norm_rope_backward(a, b, w, w, 1e-6, inv, a2, b2)
+        assert a2.shape == a.shape and db.shape == b.shape
+        assert (dwa.abs().max() > 0) == (a is q) and (dwb.abs().max() > 0) == (b is q)
+    alone, _ = lops.qk_norm_rope(q, None, w, None, 1e-6, inv)
+    assert torch.equal(lops.qk_norm_rope(none, q, w, w, 1e-6, inv)[1], alone)
+
+
 def test_qk_norm_rope_no_rows(lops):
     inv = lops.rope_inv_freq(64, 10000.0, DEV)
     w = torch.ones(64, device=DEV)
@@ -560,7 +574,10 @@ def all_ops(lops, seed):
         dgu, _ = lops.swiglu_backward_packed(pm, out)
         h2, y2, _ = lops.rmsnorm_from_packed(p, nw, 1e-6)
         dw = lops.embedding_backward(ids, dgu, 300, 2.0)
-        return [e, h, y, q2, k2, dq, dk, dwq, dwk, out, dgu, h2, y2, dw]
+        # more tokens than one launch takes: the one-CTA sort, and the general one
+        dws = [lops.embedding_backward(ids.repeat(1, n), dgu.repeat(1, n, 1), 300, 2.0)
+               for n in (2, 3)]
+        return [e, h, y, q2, k2, dq, dk, dwq, dwk, out, dgu, h2, y2, dw] + dws
 
     return run, (ids, w)
 
@@ -595,6 +612,54 @@ def test_operators_on_another_stream_and_captured(lops):
     graphs[0].replay()
     torch.cuda.synchronize()
     assert torch.equal(outs[0][0], lops.embedding_forward(ids, w, 2.0))
+
+
+def test_offsets_beyond_32_bits(lops):
+    """Tensors of more than 2^32 bytes and 2^31 elements: the last rows come
+    out as from a small tensor that holds them alone."""
+    dt = torch.bfloat16
+    rows, d = 540_000, 4096
+    big = torch.empty(rows, d, device=DEV, dtype=dt)
+    big[-40:] = torch.randn(40, d, device=DEV).to(dt)
+    tail = big[-40:].clone()
+    ids = torch.tensor([rows - 1, rows - 40, 0, rows - 7], device=DEV)
+    out = lops.embedding_forward(ids, big, 1.0)
+    assert torch.equal(out[[0, 1, 3]], tail[[39, 0, 33]])
+    for n in (1, 3000):       # one launch, and sorted tokens
+        dw = lops.embedding_backward(ids.repeat(n), tail[:4].repeat(n, 1), rows)
+        small = lops.embedding_backward((ids - (rows - 40)).clamp_min(0)[[0, 1, 3]].repeat(n),
+                                        tail[[0, 1, 3]].repeat(n, 1), 40)
+        assert torch.equal(dw[-40:], small) and not dw[-60:-40].any() and dw[0].any()
+        del dw
+    for fmt in ("int8", "e4m3"):
+        p, q = lops.quantize_rows(big, fmt), lops.quantize_rows(tail, fmt)
+        assert torch.equal(p.codes[-40:], q.codes) and torch.equal(p.scales[-40:], q.scales)
+        assert torch.equal(lops.dequantize_rows(p)[-40:], lops.dequantize_rows(q))
+        del p
+    w = torch.ones(d, device=DEV, dtype=dt)
+    got = lops.rmsnorm_forward_packed(big, w, 1e-6)
+    want = lops.rmsnorm_forward_packed(tail, w, 1e-6)
+    assert torch.equal(got[1][-40:], want[1]) and torch.equal(got[3].codes[-40:], want[3].codes)
+    back = lops.rmsnorm_from_packed(got[3], w, 1e-6)[1][-40:]
+    assert torch.equal(back, lops.rmsnorm_from_packed(want[3], w, 1e-6)[1])
+    del got
+    out, p = lops.swiglu_forward_packed(big)
+    out2, p2 = lops.swiglu_forward_packed(tail)
+    assert torch.equal(out[-40:], out2)
+    dgu, _ = lops.swiglu_backward_packed(p, out)
+    assert torch.equal(dgu[-40:], lops.swiglu_backward_packed(p2, out2)[0])
+    del dgu, out, p
+    hw = torch.ones(128, device=DEV, dtype=dt)
+    inv = lops.rope_inv_freq(128, 10000.0, DEV)
+    q = big.view(rows, 32, 128).transpose(0, 1)[None]
+    pos = torch.arange(rows, device=DEV)
+    q2, _ = lops.qk_norm_rope(q, None, hw, None, 1e-6, inv, positions=pos)
+    want, _ = lops.qk_norm_rope(q[:, :, -40:], None, hw, None, 1e-6, inv, positions=pos[-40:])
+    assert torch.equal(q2[:, :, -40:], want)
+    dq, _, _, _ = lops.qk_norm_rope_backward(q, None, hw, None, 1e-6, inv, q2, None, positions=pos)
+    want, _, _, _ = lops.qk_norm_rope_backward(q[:, :, -40:], None, hw, None, 1e-6, inv, want, None,
+                                               positions=pos[-40:])
+    assert torch.equal(dq[:, :, -40:], want)
 
 
 def test_refusals(lops, esa_mod):
