@@ -84,8 +84,8 @@ constexpr int kWarps = kThreads / 32;
 // rounds on 20 warps 208).  Backward: four (two in float32), the next four
 // loaded ahead, on 12 warps (32768 tokens of 64 heads: 251 us; two ahead of two
 // on 16 warps 268, four without loading ahead 277).  In long runs the power
-// limit lowers the SM clock and these become 225 and 283 us; a plain copy of
-// as many bytes (209 us) does not reach it.
+// limit lowers the SM clock and these become 213-225 and 269-283 us; a plain
+// copy of as many bytes (209 us) does not reach it.
 constexpr int kFwdUnroll = 2;
 constexpr int kFwdCtasPerSm = 8;
 template <typename T> constexpr int kBwdUnroll = sizeof(T) == 4 ? 2 : 4;
