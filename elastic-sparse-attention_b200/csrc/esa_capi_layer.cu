@@ -55,10 +55,12 @@ GradPlan grad_plan(int64_t n, int64_t vocab, int32_t dim) {
   while ((vocab >> g.key_bits) != 0) ++g.key_bits;
   g.passes = (int)ceil_div(g.key_bits, em::kRadixBits);
   g.bits = (int)ceil_div(g.key_bits, g.passes);
-  g.tile = (int)(ceil_div(std::max<int64_t>(ceil_div(n, em::kSortMaxTiles), em::kSortTile),
-                          em::kSortTile) * em::kSortTile);
+  g.tile = em::kSortTile;
+  while (ceil_div(n, g.tile) > em::kSortTiles &&
+         (g.tile < 2 * em::kSortTile || ceil_div(n, g.tile) > em::kSortMaxTiles))
+    g.tile += em::kSortTile;
   g.tiles = ceil_div(n, g.tile);
-  g.pieces = ceil_div(n, em::kPiece);
+  g.pieces = ceil_div(n, em::piece_len(n, dim));
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t o = at;
@@ -81,7 +83,6 @@ template <typename T>
 int embedding_grad(int64_t n, int64_t vocab, int32_t dim, const em::Ids& ids, const void* dy,
                    float scale, int64_t pad, void* dweight, char* ws, int* err, cudaStream_t s) {
   const uint32_t vpr = dim / esa::Vec<T>::kElems;
-  const unsigned ychunks = (unsigned)ceil_div(vpr, em::kGradThreads);
   if (vpr > 32 * 65535) return fail(ESA_ERR_UNSUPPORTED, "esa_embedding_backward: dim %d too large", dim);
   if (n <= em::direct_max(dim)) {
     auto direct = [&](auto nv) {
@@ -165,13 +166,28 @@ int embedding_grad(int64_t n, int64_t vocab, int32_t dim, const em::Ids& ids, co
   q.owners = reinterpret_cast<uint2*>(ws + g.owners);
   q.pieces = g.pieces;
   q.zero_blocks = (int)ceil_div(vocab, em::kZeroRows);
-  q.ychunks = (int)ychunks;
-  const int64_t ctas = (q.zero_blocks + g.pieces) * ychunks;
-  if (ctas > INT32_MAX) return fail(ESA_ERR_UNSUPPORTED, "esa_embedding_backward: too many tokens");
-  if (int rc = launch_after("esa_embedding_backward (sums)", em::grad_pieces_kernel<T>,
-                            dim3((unsigned)ctas), dim3(em::kGradThreads), s, q,
-                            static_cast<const T*>(dy), static_cast<T*>(dweight)))
-    return rc;
+  q.piece = em::piece_len(n, dim);
+  auto pieces = [&](auto piece, auto threads) {
+    constexpr int P = decltype(piece)::value, TH = decltype(threads)::value;
+    q.ychunks = (int)ceil_div(vpr, TH);
+    const int64_t ctas = (q.zero_blocks + g.pieces) * q.ychunks;
+    if (ctas > INT32_MAX)
+      return fail(ESA_ERR_UNSUPPORTED, "esa_embedding_backward: too many tokens");
+    return launch_after("esa_embedding_backward (sums)", em::grad_pieces_kernel<T, P, TH>,
+                        dim3((unsigned)ctas), dim3(TH), s, q, static_cast<const T*>(dy),
+                        static_cast<T*>(dweight));
+  };
+  using std::integral_constant;
+  int rc;
+  if (em::narrow_rows(dim))
+    rc = pieces(integral_constant<int, 16>{}, integral_constant<int, 32>{});
+  else if (q.piece == 16)
+    rc = pieces(integral_constant<int, 16>{}, integral_constant<int, 128>{});
+  else if (q.piece == 32)
+    rc = pieces(integral_constant<int, 32>{}, integral_constant<int, 128>{});
+  else
+    rc = pieces(integral_constant<int, 64>{}, integral_constant<int, 128>{});
+  if (rc) return rc;
   return launch_after("esa_embedding_backward (join)", em::grad_join_kernel<T>, dim3(148 * 8),
                       dim3(em::kJoinWarps * 32), s, q, static_cast<T*>(dweight));
 }

@@ -93,7 +93,9 @@ constexpr int kDirectMax = 2048;
 // Up to how many tokens: against the sort, vocabulary 32000 in bf16, 2048
 // tokens take 20 and 28 us at width 64, 67 and 71 at 4096, where 2048 times the
 // same token, which one CTA per 128 vectors then sums, would take 200 and 62.
-__host__ __device__ constexpr int direct_max(int dim) { return dim <= 256 ? kDirectMax : kDirectMax / 2; }
+__host__ __device__ constexpr int direct_max(int dim) {
+  return dim <= 256 ? kDirectMax : kDirectMax / 2;
+}
 
 constexpr int kDirectThreads = 128;
 constexpr int kDirectWarps = kDirectThreads / 32;
@@ -235,21 +237,30 @@ grad_direct_kernel(int n, int64_t vocab, int R, uint32_t vpr, Ids ids, const T* 
 // Gradient, many tokens.  The (token, row) pairs are sorted by token with a
 // stable radix sort (digits of up to 9 bits, low digit first: a histogram and
 // a scatter launch per digit), then the sorted list is cut into pieces of
-// kPiece pairs that are summed independently.  A run of one token of at most
-// kPiece pairs belongs to the piece it starts in; a longer one is cut at the
-// piece borders into float32 partial sums, which a last launch adds in order,
-// so no CTA's share grows with a token's frequency.
+// P pairs that are summed independently.  A run of one token of at most P
+// pairs belongs to the piece it starts in; a longer one is cut at the piece
+// borders into float32 partial sums, which a last launch adds in order, so no
+// CTA's share grows with a token's frequency.
 // Tokens that are padding or out of range get the key `vocab` and sort last.
 // ---------------------------------------------------------------------------
 constexpr int kRadixBits = 9;
 constexpr int kRadix = 1 << kRadixBits;
 constexpr int kSortThreads = 512;
 constexpr int kSortWarps = kSortThreads / 32;
-constexpr int kSortItems = 4;
+constexpr int kSortItems = 2;
 constexpr int kSortTile = kSortThreads * kSortItems;   // keys of a CTA's inner step
-constexpr int kSortMaxTiles = 512;                     // rows of the histogram table
-constexpr int kPiece = 64;
-constexpr int kGradThreads = 128;
+constexpr int kSortTiles = 128;       // with more keys than fill them, longer tiles first
+constexpr int kSortMaxTiles = 512;    // rows of the histogram table
+
+// Pairs per piece: 64, so that partial sums are few; less for narrow rows and
+// fewer tokens, whose time is a piece's chain of loads.  Vocabulary 32000 in
+// bf16, P = 16 / 32 / 64: 8192 x 4096 73 / 76 / 80 us, 32768 x 1024 43 / 44 /
+// 50, 65536 x 1024 62 / 58 / 61, 131072 x 4096 288 / 256 / 247; 8192 x 64 (with a
+// warp per piece) 22 against 32 with 64.
+__host__ __device__ constexpr bool narrow_rows(int dim) { return dim <= 256; }
+__host__ __device__ constexpr int piece_len(int64_t n, int dim) {
+  return narrow_rows(dim) || n <= 8192 ? 16 : n <= 65536 ? 32 : 64;
+}
 constexpr int kGradUnroll = 8;          // rows in flight per thread
 
 // Key of token i in the first pass.
@@ -300,15 +311,35 @@ __global__ void __launch_bounds__(kSortThreads) sort_hist_kernel(SortPass p) {
 // Stable scatter of one pass: a warp ranks its contiguous keys round by round
 // (equal digits of a round by lane), warps and CTAs follow in order.
 __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(SortPass p) {
-  __shared__ uint32_t base[kRadix];                 // next output slot of each digit
-  __shared__ uint32_t cnt[kSortWarps][kRadix];
+  __shared__ uint32_t cnt[kSortWarps][kRadix];      // of a warp's keys; then their places
   __shared__ uint32_t wsum[kSortWarps];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  cudaTriggerProgrammaticLaunchCompletion();
-  cudaGridDependencySynchronize();
   static_assert(kRadix == kSortThreads, "a thread per digit");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, digit = threadIdx.x;
+  cudaTriggerProgrammaticLaunchCompletion();
+  auto clear = [&] {
+    for (int i = threadIdx.x; i < kSortWarps * kRadix / 4; i += kSortThreads)
+      reinterpret_cast<uint4*>(&cnt[0][0])[i] = make_uint4(0, 0, 0, 0);
+  };
+  clear();
+  cudaGridDependencySynchronize();
+  const uint32_t mask = (1u << p.bits) - 1;
+  const int64_t lo = (int64_t)blockIdx.x * p.tile;
+  const int64_t hi = lo + p.tile < p.n ? lo + p.tile : p.n;
+  uint32_t key[kSortItems], row[kSortItems], rank[kSortItems];
+  auto load = [&](int64_t t0) {
+#pragma unroll
+    for (int r = 0; r < kSortItems; ++r) {
+      const int64_t i = t0 + warp * (32 * kSortItems) + r * 32 + lane;
+      key[r] = row[r] = 0;
+      if (i < hi) {
+        key[r] = p.keys ? p.keys[i] : token_key(p.ids, i, p.vocab, p.pad, nullptr);
+        row[r] = p.keys ? p.rows[i] : (uint32_t)i;
+      }
+    }
+  };
+  load(lo);                                         // on their way during the sums
   uint32_t tot = 0, before = 0;
-  const uint32_t* h = p.hist + threadIdx.x;
+  const uint32_t* h = p.hist + digit;
   for (int k0 = 0; k0 < (int)gridDim.x; k0 += 32) {
     uint32_t x[32];
 #pragma unroll
@@ -328,25 +359,12 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(SortPass p) 
   }
   if (lane == 31) wsum[warp] = incl;
   __syncthreads();
-  uint32_t off = incl - tot;
-  for (int w = 0; w < warp; ++w) off += wsum[w];
-  base[threadIdx.x] = off + before;
-  const uint32_t mask = (1u << p.bits) - 1;
-  const int64_t lo = (int64_t)blockIdx.x * p.tile;
-  const int64_t hi = lo + p.tile < p.n ? lo + p.tile : p.n;
+  uint32_t base = incl - tot + before;              // next output slot of this digit
+  for (int w = 0; w < warp; ++w) base += wsum[w];
   for (int64_t t0 = lo; t0 < hi; t0 += kSortTile) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < kSortWarps * kRadix; i += kSortThreads) (&cnt[0][0])[i] = 0;
-    __syncthreads();
-    uint32_t key[kSortItems], row[kSortItems], rank[kSortItems];
 #pragma unroll
     for (int r = 0; r < kSortItems; ++r) {
-      const int64_t i = t0 + warp * (32 * kSortItems) + r * 32 + lane;
-      const bool in = i < hi;
-      if (in) {
-        key[r] = p.keys ? p.keys[i] : token_key(p.ids, i, p.vocab, p.pad, nullptr);
-        row[r] = p.keys ? p.rows[i] : (uint32_t)i;
-      }
+      const bool in = t0 + warp * (32 * kSortItems) + r * 32 + lane < hi;
       const uint32_t d = in ? (key[r] >> p.shift) & mask : kRadix;   // kRadix: no key
       const uint32_t same = __match_any_sync(0xffffffffu, d);
       const int before_me = __popc(same & ((1u << lane) - 1));
@@ -356,25 +374,26 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(SortPass p) 
       __syncwarp();
     }
     __syncthreads();
-    for (int d = threadIdx.x; d < kRadix; d += kSortThreads) {
-      uint32_t o = base[d];
 #pragma unroll
-      for (int w = 0; w < kSortWarps; ++w) {
-        const uint32_t x = cnt[w][d];
-        cnt[w][d] = o;
-        o += x;
-      }
-      base[d] = o;
+    for (int w = 0; w < kSortWarps; ++w) {
+      const uint32_t x = cnt[w][digit];
+      cnt[w][digit] = base;
+      base += x;
     }
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < kSortItems; ++r) {
-      const int64_t i = t0 + warp * (32 * kSortItems) + r * 32 + lane;
-      if (i < hi) {
+      if (t0 + warp * (32 * kSortItems) + r * 32 + lane < hi) {
         const uint32_t pos = cnt[warp][(key[r] >> p.shift) & mask] + rank[r];
         p.out_keys[pos] = key[r];
         p.out_rows[pos] = row[r];
       }
+    }
+    if (t0 + kSortTile < hi) {
+      load(t0 + kSortTile);
+      __syncthreads();
+      clear();
+      __syncthreads();
     }
   }
 }
@@ -507,29 +526,30 @@ struct GradParams {
   int* counter;               // number of long runs
   uint2* owners;              // each long run's first and last piece
   int64_t pieces;
+  int piece;                  // pairs per piece
   int zero_blocks;            // items that clear rows of absent tokens
   int ychunks;                // CTAs per item
 };
 
 constexpr int kZeroRows = 32;   // rows of dW per clearing CTA
 
-// One CTA per item and 128 vectors of the width, the CTAs of an item side by
-// side so that a row's parts are read together.  Items are the pieces with the
+// One CTA of TH threads per item and TH vectors of the width (TH = 32 for narrow
+// rows), the CTAs of an item side by side so that a row's parts are read together.  Items are the pieces with the
 // clearing of absent rows spread evenly among them: its searches would leave
 // HBM idle if they came first.
-template <typename T>
-__global__ void __launch_bounds__(kGradThreads)
+template <typename T, int P, int TH>
+__global__ void __launch_bounds__(TH)
 grad_pieces_kernel(GradParams p, const T* __restrict__ dy, T* __restrict__ dw) {
   using V = Vec<T>;
   constexpr int E = V::kElems;
-  __shared__ uint32_t skey[3 * kPiece + 1];   // keys around the piece
-  __shared__ uint32_t srow[2 * kPiece];       // rows of the piece and the next
-  static_assert(kGradThreads >= kPiece + 1 && kZeroRows <= 2 * kPiece, "");
+  __shared__ uint32_t skey[3 * P + 1];   // keys around the piece
+  __shared__ uint32_t srow[2 * P];       // rows of the piece and the next
+  static_assert(TH > P && kZeroRows <= 2 * P && kZeroRows <= TH, "");
   cudaTriggerProgrammaticLaunchCompletion();
   cudaGridDependencySynchronize();
   const int64_t item = blockIdx.x / p.ychunks;
   const uint32_t chunk = (uint32_t)(blockIdx.x - item * p.ychunks);
-  const uint32_t vec = chunk * kGradThreads + threadIdx.x;
+  const uint32_t vec = chunk * TH + threadIdx.x;
   const bool active = vec < p.vpr;
   const int64_t items = p.pieces + p.zero_blocks;
   const int64_t zeros = item * p.zero_blocks / items;     // clearing items before this one
@@ -551,27 +571,27 @@ grad_pieces_kernel(GradParams p, const T* __restrict__ dy, T* __restrict__ dw) {
     return;
   }
   const int64_t piece = item - zeros;
-  const int64_t a = piece * kPiece;
+  const int64_t a = piece * P;
   const uint32_t none = 0xffffffffu;      // outside the list, or dropped
-  for (int i = threadIdx.x; i < 3 * kPiece + 1; i += kGradThreads) {
-    const int64_t at = a - kPiece + i;
+  for (int i = threadIdx.x; i < 3 * P + 1; i += TH) {
+    const int64_t at = a - P + i;
     uint32_t key = at >= 0 && at < p.n ? __ldg(p.keys + at) : none;
     if (key >= (uint32_t)p.vocab) key = none;
     skey[i] = key;
-    if (i >= kPiece && i < 3 * kPiece && at < p.n) srow[i - kPiece] = __ldg(p.rows + at);
+    if (i >= P && i < 3 * P && at < p.n) srow[i - P] = __ldg(p.rows + at);
   }
   __syncthreads();
-  const uint32_t* key = skey + kPiece;    // key[i]: entry a + i, i in [-kPiece, 2 kPiece]
+  const uint32_t* key = skey + P;    // key[i]: entry a + i, i in [-P, 2 P]
   if (key[0] == none) return;             // only dropped tokens from here on
   const int t = threadIdx.x;
-  const int len = __syncthreads_count(t < kPiece && key[t] != none);
+  const int len = __syncthreads_count(t < P && key[t] != none);
   // entries before and from the piece's first one that share its key (64 + 65 at
   // most are looked at); the same around its last
-  const int fb = __syncthreads_count(t < kPiece && key[t - kPiece] == key[0]);
-  const int ff = __syncthreads_count(t <= kPiece && key[t] == key[0]);
-  const int lb = __syncthreads_count(t < kPiece && key[len - 1 - t] == key[len - 1]);
-  const int lf = __syncthreads_count(t < kPiece && key[len + t] == key[len - 1]);
-  const bool long_first = fb + ff > kPiece, long_last = lb + lf > kPiece;
+  const int fb = __syncthreads_count(t < P && key[t - P] == key[0]);
+  const int ff = __syncthreads_count(t <= P && key[t] == key[0]);
+  const int lb = __syncthreads_count(t < P && key[len - 1 - t] == key[len - 1]);
+  const int lf = __syncthreads_count(t < P && key[len + t] == key[len - 1]);
+  const bool long_first = fb + ff > P, long_last = lb + lf > P;
   const int i0 = !long_first && fb > 0 ? ff : 0;           // skip a short run begun earlier
   const int i1 = !long_last ? len + lf : len;              // finish a short run begun here
   // a long run at the end that goes on; listed where it starts
@@ -580,7 +600,7 @@ grad_pieces_kernel(GradParams p, const T* __restrict__ dy, T* __restrict__ dw) {
   if (cut && starts && chunk == 0 && t == 0)
     p.owners[atomicAdd(p.counter, 1)] =
         make_uint2((uint32_t)piece,
-                   (uint32_t)((lower_bound(p.keys, a, p.n, key[len - 1] + 1) - 1) / kPiece));
+                   (uint32_t)((lower_bound(p.keys, a, p.n, key[len - 1] + 1) - 1) / P));
   if (!active) return;
   const int64_t dim = (int64_t)p.vpr * E;
   bool head = long_first && fb > 0;       // the first run's sum is one of several
@@ -644,7 +664,7 @@ grad_join_kernel(GradParams p, T* __restrict__ dw) {
     const uint2 run = p.owners[t / chunks];
     const int64_t piece = run.x, last = run.y;
     const int64_t col = (t % chunks) * kJoinCols + lane * 4;
-    const uint32_t key = p.keys[piece * kPiece + kPiece - 1];
+    const uint32_t key = p.keys[(piece + 1) * p.piece - 1];
     float4 a[kJoinVecs];
 #pragma unroll
     for (int v = 0; v < kJoinVecs; ++v) a[v] = make_float4(0.f, 0.f, 0.f, 0.f);

@@ -96,7 +96,9 @@ def test_embedding_out_of_range_ids(lops, esa_mod):
 @pytest.mark.parametrize("n,V,d", [
     (0, 3, 8), (1, 1, 16), (5, 700, 264), (63, 9, 8), (1023, 50, 1032), (1024, 33000, 16),
     (1025, 40, 1024), (2048, 33000, 64), (2049, 600, 256), (4096, 70000, 8), (4099, 2, 264),
-    (4160, 512, 8), (9000, 70000, 24), (20001, 300000, 8)])
+    (4160, 512, 8), (9000, 70000, 24), (20001, 300000, 8),
+    # the other piece lengths of wide rows
+    (5000, 90, 264), (12001, 900, 264), (70001, 5000, 264)])
 def test_embedding_backward(lops, dtype, kind, n, V, d):
     g = torch.Generator().manual_seed(n + V)
     ids = make_ids(kind, n, V, g).to(DEV)
