@@ -90,9 +90,10 @@ lookup_kernel(int64_t n, int64_t vocab, uint32_t vpr, Ids ids, const T* __restri
 // ---------------------------------------------------------------------------
 constexpr int kDirectMax = 2048;
 
-// Up to how many tokens: against the sort, vocabulary 32000 in bf16, 2048
-// tokens take 20 and 28 us at width 64, 67 and 71 at 4096, where 2048 times the
-// same token, which one CTA per 128 vectors then sums, would take 200 and 62.
+// Up to how many tokens: against the sort, vocabulary 32000 in bf16, a call with
+// 2048 tokens takes 15 and 22 us at width 64, 67 and 64 at 4096, with 1024 52
+// and 58 there.  (1024 times the same token, which one CTA per 128 vectors then
+// sums, take 109 us at 4096.)
 __host__ __device__ constexpr int direct_max(int dim) {
   return dim <= 256 ? kDirectMax : kDirectMax / 2;
 }
@@ -109,6 +110,29 @@ __device__ __forceinline__ void store_scaled(T* dst, const float* acc, float sca
 #pragma unroll
   for (int e = 0; e < V::kElems; ++e) o[e] = acc[e] * scale;
   stg16(dst, V::from_float(o));
+}
+
+// Clears the rows of dW in [v0, v0 + rows) whose bit in `which` is set, all of
+// their width (whole: by the CTA's threads through the contiguous block, which
+// keeps lanes busy on narrow rows) or 32 * NV vectors from vec0 on (a warp a row).
+template <typename T, int Threads, int NV>
+__device__ __forceinline__ void clear_rows(T* dw, int64_t v0, int rows, uint32_t which,
+                                           uint32_t vpr, uint32_t vec0, bool whole) {
+  constexpr int E = Vec<T>::kElems;
+  T* dst = dw + v0 * vpr * E;
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  if (whole) {
+    for (uint32_t i = threadIdx.x; i < rows * vpr; i += Threads)
+      if (which >> (i / vpr) & 1) stg16(dst + (int64_t)i * E, zero);
+  } else {
+    const uint32_t vec = vec0 + (threadIdx.x & 31);
+    for (int r = threadIdx.x >> 5; r < rows; r += Threads / 32) {
+      if (!(which >> r & 1)) continue;
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+        if (vec + v * 32 < vpr) stg16(dst + ((int64_t)r * vpr + vec + v * 32) * E, zero);
+    }
+  }
 }
 
 // acc += the rows of a warp's list that belong to row r, in order; lane's
@@ -191,21 +215,17 @@ grad_direct_kernel(int n, int64_t vocab, int R, uint32_t vpr, Ids ids, const T* 
     any |= present[w];
   }
   const uint32_t vec = blockIdx.y * (32 * NV) + lane;
-  T* dst = dw + (v0 * vpr + vec) * E;
-  // rows without tokens, and rows that one warp has alone
-  for (int r = 0; r < R && v0 + r < vocab; ++r, dst += (int64_t)vpr * E) {
-    if (!(any >> r & 1)) {
-      if (r % kDirectWarps != warp) continue;
+  clear_rows<T, kDirectThreads, NV>(dw, v0, (int)(vocab - v0 < R ? vocab - v0 : R), ~any, vpr,
+                                    blockIdx.y * (32 * NV), gridDim.y == 1);
+  // rows that this warp has alone
+  for (uint32_t own = rows_seen & ~several; own; own &= own - 1) {
+    const int r = __ffs(own) - 1;
+    float acc[NV][E] = {};
+    add_listed<T, NV>(list[warp], count, r, dy, vpr, vec, acc);
 #pragma unroll
-      for (int v = 0; v < NV; ++v)
-        if (vec + v * 32 < vpr) stg16(dst + v * 32 * E, make_uint4(0, 0, 0, 0));
-    } else if ((rows_seen >> r & 1) && !(several >> r & 1)) {
-      float acc[NV][E] = {};
-      add_listed<T, NV>(list[warp], count, r, dy, vpr, vec, acc);
-#pragma unroll
-      for (int v = 0; v < NV; ++v)
-        if (vec + v * 32 < vpr) store_scaled<T>(dst + v * 32 * E, acc[v], scale);
-    }
+    for (int v = 0; v < NV; ++v)
+      if (vec + v * 32 < vpr)
+        store_scaled<T>(dw + ((v0 + r) * vpr + vec + v * 32) * E, acc[v], scale);
   }
   while (several) {
     const int r = __ffs(several) - 1;
@@ -544,7 +564,7 @@ grad_pieces_kernel(GradParams p, const T* __restrict__ dy, T* __restrict__ dw) {
   constexpr int E = V::kElems;
   __shared__ uint32_t skey[3 * P + 1];   // keys around the piece
   __shared__ uint32_t srow[2 * P];       // rows of the piece and the next
-  static_assert(TH > P && kZeroRows <= 2 * P && kZeroRows <= TH, "");
+  static_assert(TH > P && kZeroRows == 32, "");
   cudaTriggerProgrammaticLaunchCompletion();
   cudaGridDependencySynchronize();
   const int64_t item = blockIdx.x / p.ychunks;
@@ -555,19 +575,20 @@ grad_pieces_kernel(GradParams p, const T* __restrict__ dy, T* __restrict__ dw) {
   const int64_t zeros = item * p.zero_blocks / items;     // clearing items before this one
   if ((item + 1) * p.zero_blocks / items > zeros) {
     const int64_t v0 = zeros * kZeroRows;
-    if (threadIdx.x < kZeroRows) {
+    uint32_t absent = 0;
+    if (threadIdx.x < 32) {
       const int64_t v = v0 + threadIdx.x;
-      uint32_t absent = 0;
+      bool none_of_it = false;
       if (v < p.vocab) {
         const int64_t at = lower_bound(p.keys, 0, p.n, (uint32_t)v);
-        absent = at == p.n || p.keys[at] != (uint32_t)v;
+        none_of_it = at == p.n || p.keys[at] != (uint32_t)v;
       }
-      srow[threadIdx.x] = absent;
+      absent = __ballot_sync(0xffffffffu, none_of_it);
+      if (threadIdx.x == 0) srow[0] = absent;
     }
     __syncthreads();
-    if (active)
-      for (int r = 0; r < kZeroRows; ++r)
-        if (srow[r]) stg16(dw + ((v0 + r) * p.vpr + vec) * E, make_uint4(0, 0, 0, 0));
+    const int64_t rows = p.vocab - v0 < kZeroRows ? p.vocab - v0 : kZeroRows;
+    clear_rows<T, TH, TH / 32>(dw, v0, (int)rows, srow[0], p.vpr, chunk * TH, p.ychunks == 1);
     return;
   }
   const int64_t piece = item - zeros;
