@@ -316,7 +316,7 @@ PACK_FORMATS = {"int8": 0, "e4m3": 1}
 PACK_GROUP = 128
 
 
-@dataclass
+@dataclass(eq=False)
 class PackedRows:
     """Rows kept in 8 bits: ``codes`` uint8 [*shape], ``scales`` float32
     [*shape[:-1], ceil(shape[-1] / 128)], one scale per 128 elements;
