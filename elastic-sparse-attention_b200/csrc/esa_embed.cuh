@@ -85,14 +85,14 @@ lookup_kernel(int64_t n, int64_t vocab, uint32_t vpr, Ids ids, const T* __restri
 // the tokens of these rows in a contiguous quarter of the input, in order, and
 // sums its own list; what several warps have of a row is added in warp order.
 // NV = 4 for wide rows, whose clearing wants long stores (vocabulary 32000 x
-// 4096 bf16 with 8 tokens: 46 us, NV = 1 86, torch's zero_ of dW alone 70), 1
-// for narrow ones, whose CTAs would be too few.
+// 4096 bf16: with 1024 tokens 50 us, NV = 1 78; with 8 tokens 40 and 41, torch's
+// zero_ of dW alone 70), 1 for narrow ones, whose CTAs would be too few.
 // ---------------------------------------------------------------------------
 constexpr int kDirectMax = 2048;
 
 // Up to how many tokens: against the sort, vocabulary 32000 in bf16, a call with
-// 2048 tokens takes 15 and 22 us at width 64, 67 and 64 at 4096, with 1024 52
-// and 58 there.  (1024 times the same token, which one CTA per 128 vectors then
+// 2048 tokens takes 12 and 17 us at width 64, 63 and 60 at 4096, with 1024 50
+// and 54 there.  (1024 times the same token, which one CTA per 128 vectors then
 // sums, take 109 us at 4096.)
 __host__ __device__ constexpr int direct_max(int dim) {
   return dim <= 256 ? kDirectMax : kDirectMax / 2;
@@ -420,11 +420,13 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(SortPass p) 
 
 // The whole sort in one launch of one CTA for up to kSmallMax keys: the same
 // passes (digits of up to 8 bits) with keys, rows and counts in shared memory.
-// At 4096 keys it takes 15 us against 16 for the four launches of the general
-// sort, but three launches less on the host; at 8192 24 against 16.
+// It saves three launches, but its one CTA takes longer with every key.  A
+// gradient call (32000 x 1024, bf16) with this and with the general sort, in a
+// graph: 24 and 28 us with 1025 keys, 29 and 30 with 2048, 31 and 31 with 2560,
+// 37 and 31 with 4096; called singly 37 and 44, 42 and 46, 45 and 46, 50 and 46.
 constexpr int kSmallThreads = 1024;
-constexpr int kSmallItems = 4;
-constexpr int kSmallMax = kSmallThreads * kSmallItems;
+constexpr int kSmallMax = 2560;
+constexpr int kSmallItems = (kSmallMax + kSmallThreads - 1) / kSmallThreads;
 constexpr int kSmallBits = 8;
 
 struct SmallSort {

@@ -98,7 +98,9 @@ def test_embedding_out_of_range_ids(lops, esa_mod):
     (1025, 40, 1024), (2048, 33000, 64), (2049, 600, 256), (4096, 70000, 8), (4099, 2, 264),
     (4160, 512, 8), (9000, 70000, 24), (20001, 300000, 8),
     # the other piece lengths of wide rows
-    (5000, 90, 264), (12001, 900, 264), (70001, 5000, 264)])
+    (5000, 90, 264), (12001, 900, 264), (70001, 5000, 264),
+    # around the most keys that one CTA sorts
+    (2305, 70000, 8), (2559, 33000, 264), (2560, 300, 264), (2561, 33000, 264)])
 def test_embedding_backward(lops, dtype, kind, n, V, d):
     g = torch.Generator().manual_seed(n + V)
     ids = make_ids(kind, n, V, g).to(DEV)
@@ -576,7 +578,7 @@ def all_ops(lops, seed):
         dgu, _ = lops.swiglu_backward_packed(pm, out)
         h2, y2, _ = lops.rmsnorm_from_packed(p, nw, 1e-6)
         dw = lops.embedding_backward(ids, dgu, 300, 2.0)
-        # more tokens than one launch takes: the one-CTA sort, and the general one
+        # more tokens than one launch takes: the general sort
         dws = [lops.embedding_backward(ids.repeat(1, n), dgu.repeat(1, n, 1), 300, 2.0)
                for n in (2, 3)]
         return [e, h, y, q2, k2, dq, dk, dwq, dwk, out, dgu, h2, y2, dw] + dws
@@ -614,6 +616,24 @@ def test_operators_on_another_stream_and_captured(lops):
     graphs[0].replay()
     torch.cuda.synchronize()
     assert torch.equal(outs[0][0], lops.embedding_forward(ids, w, 2.0))
+
+
+@pytest.mark.parametrize("n", [2560, 2561])       # sorted by one CTA, by several
+def test_sorted_embedding_gradient_captured(lops, n):
+    """Replays follow the ids and gradients that the inputs hold by then."""
+    g = torch.Generator().manual_seed(n)
+    cases = [(torch.randint(0, 5000, (n,), generator=g).to(DEV),
+              torch.randn(n, 264, generator=g).to(DEV)) for _ in range(3)]
+    want = [lops.embedding_backward(i, d, 5000, 0.5) for i, d in cases]
+    ids, dy = (t.clone() for t in cases[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        dw = lops.embedding_backward(ids, dy, 5000, 0.5)
+    for (i, d), w in list(zip(cases, want)) * 2:
+        ids.copy_(i)
+        dy.copy_(d)
+        graph.replay()
+        assert torch.equal(dw, w)
 
 
 def test_offsets_beyond_32_bits(lops):
