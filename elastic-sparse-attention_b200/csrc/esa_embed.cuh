@@ -528,12 +528,15 @@ __global__ void __launch_bounds__(kSmallThreads) sort_small_kernel(SmallSort p) 
   }
 }
 
-// First position in [lo, hi) of the sorted keys that is not below `key`.
-__device__ __forceinline__ int64_t lower_bound(const uint32_t* __restrict__ keys, int64_t lo,
-                                               int64_t hi, uint32_t key) {
+// First position in [lo, hi) of the sorted keys that is not below `key`.  The
+// sorted pairs are read with ordinary loads here and in the kernels below: the
+// sort may still be writing them when those kernels start, and loads through
+// the read-only path want memory that does not change while a kernel runs.
+__device__ __forceinline__ int64_t lower_bound(const uint32_t* keys, int64_t lo, int64_t hi,
+                                               uint32_t key) {
   while (lo < hi) {
     const int64_t mid = (lo + hi) >> 1;
-    if (__ldg(keys + mid) < key) lo = mid + 1; else hi = mid;
+    if (keys[mid] < key) lo = mid + 1; else hi = mid;
   }
   return lo;
 }
@@ -598,10 +601,10 @@ grad_pieces_kernel(GradParams p, const T* __restrict__ dy, T* __restrict__ dw) {
   const uint32_t none = 0xffffffffu;      // outside the list, or dropped
   for (int i = threadIdx.x; i < 3 * P + 1; i += TH) {
     const int64_t at = a - P + i;
-    uint32_t key = at >= 0 && at < p.n ? __ldg(p.keys + at) : none;
+    uint32_t key = at >= 0 && at < p.n ? p.keys[at] : none;
     if (key >= (uint32_t)p.vocab) key = none;
     skey[i] = key;
-    if (i >= P && i < 3 * P && at < p.n) srow[i - P] = __ldg(p.rows + at);
+    if (i >= P && i < 3 * P && at < p.n) srow[i - P] = p.rows[at];
   }
   __syncthreads();
   const uint32_t* key = skey + P;    // key[i]: entry a + i, i in [-P, 2 P]

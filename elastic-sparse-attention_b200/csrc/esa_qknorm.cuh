@@ -599,13 +599,14 @@ bwd_kernel(Params<T> p, int q_ctas, float* part) {
 }
 
 // dw of the query side (y = 0) and the key side (y = 1; y = 0 when there are
-// keys only: first = 1) from the CTAs' partials, in a fixed order.
+// keys only: first = 1) from the CTAs' partials, in a fixed order.  The partials
+// may still be written when this kernel starts: no __restrict__ on them, so that
+// they are not read through the read-only path.
 constexpr int kSumWarps = 32;
 
 template <typename T>
 __global__ void __launch_bounds__(kSumWarps * 32)
-sum_kernel(int D, int q_ctas, int ctas, int first, const float* __restrict__ part, T* dwq,
-           T* dwk) {
+sum_kernel(int D, int q_ctas, int ctas, int first, const float* part, T* dwq, T* dwk) {
   __shared__ float red[kSumWarps][33];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   cudaGridDependencySynchronize();
