@@ -331,7 +331,8 @@ __global__ void __launch_bounds__(kSortThreads) sort_hist_kernel(SortPass p) {
 // Stable scatter of one pass: a warp ranks its contiguous keys round by round
 // (equal digits of a round by lane), warps and CTAs follow in order.
 __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(SortPass p) {
-  __shared__ uint32_t cnt[kSortWarps][kRadix];      // of a warp's keys; then their places
+  // of a warp's keys, then their places; cleared 16 bytes at a time
+  __shared__ __align__(16) uint32_t cnt[kSortWarps][kRadix];
   __shared__ uint32_t wsum[kSortWarps];
   static_assert(kRadix == kSortThreads, "a thread per digit");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, digit = threadIdx.x;
@@ -443,7 +444,8 @@ __global__ void __launch_bounds__(kSmallThreads) sort_small_kernel(SmallSort p) 
   constexpr int W = kSmallThreads / 32, R = 1 << kSmallBits;
   __shared__ uint32_t skey[kSmallMax];
   __shared__ uint16_t srow[kSmallMax];
-  __shared__ uint16_t cnt[W][R];         // of a warp's keys; then their places
+  // of a warp's keys, then their places; cleared two at a time
+  __shared__ __align__(4) uint16_t cnt[W][R];
   __shared__ uint32_t wsum[R / 32];
   cudaTriggerProgrammaticLaunchCompletion();
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
