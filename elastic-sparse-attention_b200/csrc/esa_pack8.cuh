@@ -143,13 +143,12 @@ __device__ __forceinline__ W encode(const float (&x)[E], float s) {
       off = fmaxf(off, fmaxf(fabsf(d0), fabsf(d1)));
     }
     if (off > 0.49997f) {
-      const float half = 0.5f * s;
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const float r = __fsub_rn(__uint_as_float(code[e]), kMagic);
         const float d = fmaf(-r, s, x[e]);
-        const float ad = fabsf(d);
-        if (ad > half || (ad == half && (code[e] & 1))) code[e] += d > 0.f ? 1u : 0xffffffffu;
+        const float ad2 = fabsf(d) + fabsf(d);   // exact, unlike s / 2 next to 2^-126
+        if (ad2 > s || (ad2 == s && (code[e] & 1))) code[e] += d > 0.f ? 1u : 0xffffffffu;
       }
     }
 #pragma unroll

@@ -63,3 +63,37 @@ def test_qk_weight_gradients_in_a_row(lops):
     got = [call(do) for do in douts]
     for (a, b), (c, d) in zip(got, want):
         assert torch.equal(a, c) and torch.equal(b, d)
+
+
+def border_rows(dtype):
+    """Rows of one group whose int8 scale is just above 2^-126 with an odd last
+    bit, so that half of it is no float32, and values next to the border between
+    two codes; and the codes by float64, whose quotients keep a distance of
+    2^-25 from the border that float64 resolves."""
+    g = torch.Generator().manual_seed(21)
+    rows = 256
+    m = (1 << 23) + 2 * torch.randint(0, 1 << 22, (rows, 1), generator=g) + 1   # s = m 2^-149
+    k = torch.randint(0, 126, (rows, 128), generator=g)
+    x = ((2 * k + 1) * m + torch.randint(0, 2, k.shape, generator=g) * 2 - 1).double() * 2.0 ** -150
+    x = x * (torch.randint(0, 2, k.shape, generator=g) * 2 - 1)
+    x[:, :1] = 127 * m.double() * 2.0 ** -149
+    x = x.to(dtype)
+    s = (x.double().abs().amax(-1, keepdim=True) / 127).float().double().clamp_min(2.0 ** -126)
+    return x, torch.round(x.double() / s), s
+
+
+def test_border_rows_reach_the_border():
+    x, _, s = border_rows(torch.float32)
+    steps = (x.double().abs() / s - 0.5).frac().sub(0.5).abs()
+    odd = (s * 2.0 ** 149).long() & 1 == 1
+    assert (odd & (s < 2.0 ** -125)).sum() > 100
+    assert (0.5 - steps < 2.0 ** -23).sum() > 2000
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_int8_borders_at_the_smallest_scales(lops, dtype):
+    x, codes, s = border_rows(dtype)
+    p = lops.quantize_rows(x.to(DEV), "int8")
+    assert torch.equal(p.scales.cpu().double(), s)
+    assert torch.equal(p.codes.view(torch.int8).cpu().double(), codes)
