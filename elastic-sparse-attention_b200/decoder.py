@@ -248,42 +248,47 @@ class _PackedLayer(torch.autograd.Function):
     """One decoder layer that keeps its input h in 8 bits (codes, scales) and
     nothing else: (h', y', codes', scales') = layer(h, y), codes' / scales' the
     8-bit form of h'.  The backward restores h and y = norm(h) from the codes,
-    runs the layer again and differentiates that run."""
+    runs the layer again and differentiates that run, with the format and the
+    weights of the forward pass.  ``weights``: :meth:`ElasticDecoderStack._layer_weights`."""
 
     @staticmethod
-    def forward(ctx, stack, i: int, h, y, codes, scales, positions, *params):
-        ctx.stack, ctx.i, ctx.dtype = stack, i, h.dtype
-        ctx.save_for_backward(codes, scales, positions, *params)
-        fmt = stack.activation_storage
-        h, m, w = stack._layer_body(i, h, y, positions)
+    def forward(ctx, stack, i: int, fmt: str, h, y, codes, scales, positions, *weights):
+        ctx.stack, ctx.i, ctx.meta = stack, i, (fmt, h.dtype)
+        ctx.save_for_backward(codes, scales, positions, *weights)
+        *of_layer, _, next_norm = weights
+        h, m = stack._layer_body(i, h, y, positions, of_layer)
         h, m = h.contiguous(), m.contiguous()
         if i + 1 == len(stack.layers):      # no layer follows that would keep h
-            h, y, _ = layer_ops.rmsnorm_forward(h, w, stack.eps, residual=m)
+            h, y, _ = layer_ops.rmsnorm_forward(h, next_norm, stack.eps, residual=m)
             return h, y, None, None
-        h, y, _, p = layer_ops.rmsnorm_forward_packed(h, w, stack.eps, residual=m, format=fmt)
+        h, y, _, p = layer_ops.rmsnorm_forward_packed(h, next_norm, stack.eps, residual=m,
+                                                      format=fmt)
         ctx.mark_non_differentiable(p.codes, p.scales)
         return h, y, p.codes, p.scales
 
     @staticmethod
     def backward(ctx, dh, dy, _codes, _scales):
         stack, i = ctx.stack, ctx.i
-        codes, scales, positions, *params = ctx.saved_tensors
-        h, y, _ = layer_ops.rmsnorm_from_packed(
-            PackedRows(codes, scales, stack.activation_storage, ctx.dtype),
-            stack._input_norm(i), stack.eps)
-        params_in = [p for p in params[:-1] if p.requires_grad]
-        wanted = [h.requires_grad_(), y.requires_grad_()] + params_in
+        codes, scales, positions, *weights = ctx.saved_tensors
+        *of_layer, input_norm, next_norm = weights
+        h, y, _ = layer_ops.rmsnorm_from_packed(PackedRows(codes, scales, *ctx.meta), input_norm,
+                                                stack.eps)
+        wants = [w is not None and w.requires_grad for w in of_layer]
+        wanted = [h.requires_grad_(), y.requires_grad_()]
+        wanted += [w for w, want in zip(of_layer, wants) if want]
         with torch.enable_grad():
-            h1, m, w = stack._layer_body(i, h, y, positions)
+            h1, m = stack._layer_body(i, h, y, positions, of_layer)
         del h, y
         # the last add and norm by hand: its outputs are gone before the rest runs backward
-        h2, _, rstd = layer_ops.rmsnorm_forward(h1.detach(), w, stack.eps, residual=m.detach())
-        ds, dw = layer_ops.rmsnorm_backward(h2, w, rstd, dy, dh_in=dh)
+        h2, _, rstd = layer_ops.rmsnorm_forward(h1.detach(), next_norm, stack.eps,
+                                                residual=m.detach())
+        ds, dw = layer_ops.rmsnorm_backward(h2, next_norm, rstd, dy, dh_in=dh)
         del h2, rstd, dh, dy
         grads = iter(torch.autograd.grad((h1, m), wanted, (ds, ds)))
         gh, gy = next(grads), next(grads)
-        by_param = [next(grads) if p.requires_grad else None for p in params[:-1]]
-        return (None, None, gh, gy, None, None, None, *by_param, dw if w.requires_grad else None)
+        by_weight = [next(grads) if want else None for want in wants]
+        return (None, None, None, gh, gy, None, None, None, *by_weight, None,
+                dw if next_norm.requires_grad else None)
 
 
 class _LMHeadCrossEntropy(torch.autograd.Function):
@@ -407,32 +412,34 @@ class ElasticDecoderStack(nn.Module):
         """The weight of the norm before layer i (the final norm after the last)."""
         return self.layers[i].input_norm if i < len(self.layers) else self.final_norm
 
-    def _layer_body(self, i: int, h, y, positions):
-        """Layer i up to its last residual add: (h, m, weight of the norm of h + m)."""
+    def _layer_weights(self, i: int) -> list:
+        """What layer i multiplies with, in the order :meth:`_layer_body` takes it (the
+        query / key norms None without ``qk_norm``); then the weights of the norms
+        before and after the layer."""
         lw = self.layers[i]
-        a = _AttentionBlock.apply(y, lw.qkv_proj, lw.o_proj, self.specs[i],
+        return [lw.qkv_proj, lw.o_proj, lw.q_norm, lw.k_norm, lw.post_attention_norm,
+                lw.gate_up_proj, lw.down_proj, self._input_norm(i), self._input_norm(i + 1)]
+
+    def _layer_body(self, i: int, h, y, positions, weights, mlp_format: str | None = None):
+        """Layer i up to its last residual add: (h, m), whose sum the next norm
+        takes.  ``mlp_format``: keep the gate / up rows in that 8-bit format."""
+        qkv_proj, o_proj, q_norm, k_norm, post_attention_norm, gate_up_proj, down_proj = weights
+        a = _AttentionBlock.apply(y, qkv_proj, o_proj, self.specs[i],
                                   (self.Hq, self.Hkv, self.D), self.inv_freq, positions,
-                                  self.key_plans[i], lw.q_norm, lw.k_norm, self.eps)
-        h, y2 = _AddRMSNorm.apply(h, a, lw.post_attention_norm, self.eps)
-        if (self.activation_storage is not None and not self.checkpointing
-                and torch.is_grad_enabled()):
-            m = _PackedMLPBlock.apply(y2, lw.gate_up_proj, lw.down_proj, self.activation_storage)
+                                  self.key_plans[i], q_norm, k_norm, self.eps)
+        h, y2 = _AddRMSNorm.apply(h, a, post_attention_norm, self.eps)
+        if mlp_format is not None:
+            m = _PackedMLPBlock.apply(y2, gate_up_proj, down_proj, mlp_format)
         else:
-            m = _MLPBlock.apply(y2, lw.gate_up_proj, lw.down_proj)
-        return h, m, self._input_norm(i + 1)
+            m = _MLPBlock.apply(y2, gate_up_proj, down_proj)
+        return h, m
 
     def _layer(self, i: int, h, y, positions):
-        h, m, next_w = self._layer_body(i, h, y, positions)
-        return _AddRMSNorm.apply(h, m, next_w, self.eps)
-
-    def _layer_params(self, i: int) -> list:
-        """The parameters that layer i's outputs depend on besides h and y, the
-        weight of the norm after it last."""
-        lw = self.layers[i]
-        ps = [lw.qkv_proj, lw.o_proj, lw.post_attention_norm, lw.gate_up_proj, lw.down_proj]
-        if lw.q_norm is not None:
-            ps += [lw.q_norm, lw.k_norm]
-        return ps + [self._input_norm(i + 1)]
+        *of_layer, _, next_norm = self._layer_weights(i)
+        keeps = not self.checkpointing and torch.is_grad_enabled()
+        h, m = self._layer_body(i, h, y, positions, of_layer,
+                                self.activation_storage if keeps else None)
+        return _AddRMSNorm.apply(h, m, next_norm, self.eps)
 
     def _embed(self, ids):
         if self.embed_scale is None and self.padding_idx is None:
@@ -456,8 +463,9 @@ class ElasticDecoderStack(nn.Module):
             y, codes, scales = _PackedRMSNorm.apply(h, self._input_norm(0), self.eps,
                                                     self.activation_storage)
             for i in range(len(self.layers)):
-                h, y, codes, scales = _PackedLayer.apply(self, i, h, y, codes, scales, positions,
-                                                         *self._layer_params(i))
+                h, y, codes, scales = _PackedLayer.apply(self, i, self.activation_storage, h, y,
+                                                         codes, scales, positions,
+                                                         *self._layer_weights(i))
         else:
             y = _RMSNorm.apply(h, self._input_norm(0), self.eps)
             for i in range(len(self.layers)):
