@@ -95,6 +95,7 @@ class _PackedRMSNorm(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w, eps: float, fmt: str):
+        ctx.set_materialize_grads(False)     # no zeros for the codes' gradients
         _, y, _, p = layer_ops.rmsnorm_forward_packed(x.contiguous(), w, eps, format=fmt)
         ctx.save_for_backward(p.codes, p.scales, w)
         ctx.meta = (fmt, x.dtype)
@@ -245,20 +246,42 @@ class _PackedMLPBlock(torch.autograd.Function):
 
 
 class _PackedLayer(torch.autograd.Function):
-    """One decoder layer that keeps its input h in 8 bits (codes, scales) and
-    nothing else: (h', y', codes', scales') = layer(h, y), codes' / scales' the
-    8-bit form of h'.  The backward restores h and y = norm(h) from the codes,
-    runs the layer again and differentiates that run, with the format and the
-    weights of the forward pass.  ``weights``: :meth:`ElasticDecoderStack._layer_weights`."""
+    """A decoder layer of which nothing but its input in 8 bits is kept, up to its
+    last residual add: (h', m) with h' + m what :class:`_PackedLayerNorm` takes.
+    That class's backward runs the layer again and leaves the run in ``run`` (a
+    list that the two share) for the backward here to differentiate: as two
+    nodes, because a node's incoming gradients live until it returns, and the
+    norm's two rows per token are not needed while the layer runs backward."""
 
     @staticmethod
-    def forward(ctx, stack, i: int, fmt: str, h, y, codes, scales, positions, *weights):
-        ctx.stack, ctx.i, ctx.meta = stack, i, (fmt, h.dtype)
-        ctx.save_for_backward(codes, scales, positions, *weights)
-        *of_layer, _, next_norm = weights
-        h, m = stack._layer_body(i, h, y, positions, of_layer)
-        h, m = h.contiguous(), m.contiguous()
-        if i + 1 == len(stack.layers):      # no layer follows that would keep h
+    def forward(ctx, run: list, stack, i: int, h, y, positions, *weights):
+        ctx.run = run
+        h, m = stack._layer_body(i, h, y, positions, weights)
+        return h.contiguous(), m.contiguous()
+
+    @staticmethod
+    def backward(ctx, dh, dm):
+        edges, wanted, wants = ctx.run.pop()
+        grads = iter(torch.autograd.grad(edges, wanted, (dh, dm)))
+        gh, gy = next(grads), next(grads)
+        return (None, None, None, gh, gy, None,
+                *(next(grads) if want else None for want in wants))
+
+
+class _PackedLayerNorm(torch.autograd.Function):
+    """The add and norm after a :class:`_PackedLayer`: (h', y', codes', scales'),
+    codes' / scales' the 8-bit form of h' = h + m (None after the last layer).
+    The backward restores the layer's input h and y = norm(h) from its codes and
+    runs the layer again, with the format and the weights of the forward pass.
+    ``layer``: (codes, scales, positions, weight of the norm before the layer,
+    the layer's own weights)."""
+
+    @staticmethod
+    def forward(ctx, run: list, stack, i: int, fmt: str, h, m, next_norm, layer: tuple):
+        ctx.set_materialize_grads(False)     # no zeros for the codes' gradients
+        ctx.run, ctx.stack, ctx.i, ctx.meta = run, stack, i, (fmt, h.dtype)
+        ctx.save_for_backward(next_norm, *layer)
+        if i + 1 == len(stack.layers):       # no layer follows that would keep h
             h, y, _ = layer_ops.rmsnorm_forward(h, next_norm, stack.eps, residual=m)
             return h, y, None, None
         h, y, _, p = layer_ops.rmsnorm_forward_packed(h, next_norm, stack.eps, residual=m,
@@ -268,27 +291,24 @@ class _PackedLayer(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dh, dy, _codes, _scales):
-        stack, i = ctx.stack, ctx.i
-        codes, scales, positions, *weights = ctx.saved_tensors
-        *of_layer, input_norm, next_norm = weights
+        next_norm, codes, scales, positions, input_norm, *weights = ctx.saved_tensors
+        stack = ctx.stack
         h, y, _ = layer_ops.rmsnorm_from_packed(PackedRows(codes, scales, *ctx.meta), input_norm,
                                                 stack.eps)
-        wants = [w is not None and w.requires_grad for w in of_layer]
+        wants = [w is not None and w.requires_grad for w in weights]
         wanted = [h.requires_grad_(), y.requires_grad_()]
-        wanted += [w for w, want in zip(of_layer, wants) if want]
+        wanted += [w for w, want in zip(weights, wants) if want]
         with torch.enable_grad():
-            h1, m = stack._layer_body(i, h, y, positions, of_layer)
-        del h, y
-        # the last add and norm by hand: its outputs are gone before the rest runs backward
-        h2, _, rstd = layer_ops.rmsnorm_forward(h1.detach(), next_norm, stack.eps,
-                                                residual=m.detach())
-        ds, dw = layer_ops.rmsnorm_backward(h2, next_norm, rstd, dy, dh_in=dh)
-        del h2, rstd, dh, dy
-        grads = iter(torch.autograd.grad((h1, m), wanted, (ds, ds)))
-        gh, gy = next(grads), next(grads)
-        by_weight = [next(grads) if want else None for want in wants]
-        return (None, None, None, gh, gy, None, None, None, *by_weight, None,
-                dw if next_norm.requires_grad else None)
+            h, m = stack._layer_body(ctx.i, h, y, positions, weights)
+        edges = [torch.autograd.graph.get_gradient_edge(t) for t in (h, m)]
+        ctx.run[:] = [(edges, wanted, wants)]
+        h, _, rstd = layer_ops.rmsnorm_forward(h.detach(), next_norm, stack.eps,
+                                               residual=m.detach())
+        del y, m
+        if dy is None:
+            dy = torch.zeros_like(h)
+        ds, dw = layer_ops.rmsnorm_backward(h, next_norm, rstd, dy, dh_in=dh)
+        return None, None, None, None, ds, ds, dw if next_norm.requires_grad else None, None
 
 
 class _LMHeadCrossEntropy(torch.autograd.Function):
@@ -463,9 +483,13 @@ class ElasticDecoderStack(nn.Module):
             y, codes, scales = _PackedRMSNorm.apply(h, self._input_norm(0), self.eps,
                                                     self.activation_storage)
             for i in range(len(self.layers)):
-                h, y, codes, scales = _PackedLayer.apply(self, i, self.activation_storage, h, y,
-                                                         codes, scales, positions,
-                                                         *self._layer_weights(i))
+                *weights, input_norm, next_norm = self._layer_weights(i)
+                run = []
+                layer = (codes, scales, positions, input_norm, *weights)
+                h, m = _PackedLayer.apply(run, self, i, h, y, positions, *weights)
+                h, y, codes, scales = _PackedLayerNorm.apply(
+                    run, self, i, self.activation_storage, h, m, next_norm, layer)
+                del m
         else:
             y = _RMSNorm.apply(h, self._input_norm(0), self.eps)
             for i in range(len(self.layers)):

@@ -52,3 +52,83 @@ def test_functional_call_with_8_bit_checkpoints():
     assert torch.equal(loss, want)
     for n, grad in gradients(m).items():
         assert torch.equal(other[n].grad, grad), n
+
+
+@pytest.mark.parametrize("nl", [2, 4])
+def test_8_bit_checkpoints_lower_the_peak_of_a_step(nl):
+    """Where a row per token is the unit (8 MiB here, the weights 15 MiB a layer),
+    the whole step's peak stays below the one of checkpoints that keep two full
+    rows per layer, from two layers on."""
+    cfg = dict(CFG, d=512, F=1024, nl=nl, L=8192, B=1, chunk=512)
+
+    def peak(**kw):
+        m, ids = build(torch.bfloat16, cfg, **kw)
+        m(ids, labels=ids).backward()      # the key plans and gradients are there
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        m(ids, labels=ids).backward()
+        return torch.cuda.max_memory_allocated() - before
+
+    full, packed = peak(activation_checkpointing=True), peak(**CKPT8)
+    assert packed < full, (packed, full)
+
+
+def test_8_bit_checkpoints_backward_twice():
+    """A graph that is kept runs again; a backward that stops at the last norm
+    leaves nothing behind that a later one takes for its own."""
+    m, ids = build(qk_norm=True, **CKPT8)
+    m(ids, labels=ids).backward()
+    want = gradients(m)
+    m.zero_grad(set_to_none=True)
+    loss = m(ids, labels=ids)
+    dw, = torch.autograd.grad(loss, m.final_norm, retain_graph=True)
+    assert torch.equal(dw, want["final_norm"])
+    loss.backward(retain_graph=True)
+    for n, grad in gradients(m).items():
+        assert torch.equal(grad, want[n]), n
+    m.zero_grad(set_to_none=True)
+    loss.backward()
+    for n, grad in gradients(m).items():
+        assert torch.equal(grad, want[n]), n
+
+
+def test_8_bit_checkpoints_of_hidden_states():
+    """Without labels: the last layer's residual sum takes no gradient."""
+    m, ids = build(**CKPT8)
+    y = m(ids)
+    g = torch.Generator().manual_seed(3)
+    c = torch.randn(y.shape, generator=g).to(y.device)
+    (y * c).sum().backward()
+    want, ids = build(activation_checkpointing=True)
+    (want(ids) * c).sum().backward()
+    for (n, p), q in zip(m.named_parameters(), want.parameters()):
+        if n == "lm_head":
+            assert p.grad is None
+            continue
+        # gradients at inputs off by at most 1/254 of their group's largest
+        assert torch.nn.functional.cosine_similarity(p.grad.flatten(), q.grad.flatten(), 0) > 0.99
+
+
+def test_captured_step_with_8_bit_checkpoints():
+    """A step captured in a graph, an eager step of the same stack before and
+    between its replays."""
+    m, ids = build(**CKPT8)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            m.zero_grad(set_to_none=True)
+            m(ids, labels=ids).backward()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    want = gradients(m)
+    m.zero_grad(set_to_none=True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        m(ids, labels=ids).backward()
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        for n, grad in gradients(m).items():
+            assert torch.equal(grad, want[n]), n
