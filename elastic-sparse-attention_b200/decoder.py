@@ -47,6 +47,8 @@ Options (all off by default):
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
@@ -56,6 +58,38 @@ from . import layer_ops, ops
 from .attention import KeyPlanCache, _ensure_monotone
 from .layer_ops import PACK_FORMATS, PackedRows
 from .ops import PatternSpec
+
+
+class _NoSecondDerivative(torch.autograd.Function):
+    """Gradients as they are, whose own derivative is an error."""
+
+    @staticmethod
+    def forward(ctx, root, *grads):
+        return tuple(g.detach() for g in grads)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("ElasticDecoderStack has no second derivatives: its gradients are "
+                           "computed by kernels that autograd does not see through")
+
+
+def _first_derivative_only(backward):
+    """For a backward made of kernels: under create_graph=True its gradients come
+    with a graph that raises when it is used, instead of none or a part of one
+    (torch's once_differentiable looks at the incoming gradients alone, and the
+    first of those takes none)."""
+    @functools.wraps(backward)
+    def wrapped(ctx, *grads):
+        graph = torch.is_grad_enabled()
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        if not graph:
+            return out
+        out = out if isinstance(out, tuple) else (out,)
+        root = torch.zeros((), requires_grad=True)
+        marked = iter(_NoSecondDerivative.apply(root, *(g for g in out if g is not None)))
+        return tuple(None if g is None else next(marked) for g in out)
+    return wrapped
 
 
 class _Embedding(torch.autograd.Function):
@@ -68,6 +102,7 @@ class _Embedding(torch.autograd.Function):
         return layer_ops.embedding_forward(ids, w, scale)
 
     @staticmethod
+    @_first_derivative_only
     def backward(ctx, dy):
         ids, = ctx.saved_tensors
         vocab, scale, padding_idx = ctx.meta
@@ -83,6 +118,7 @@ class _RMSNorm(torch.autograd.Function):
         return y
 
     @staticmethod
+    @_first_derivative_only
     def backward(ctx, dy):
         x, w, rstd = ctx.saved_tensors
         dx, dw = layer_ops.rmsnorm_backward(x, w, rstd, dy)
@@ -104,6 +140,7 @@ class _PackedRMSNorm(torch.autograd.Function):
         return y, p.codes, p.scales
 
     @staticmethod
+    @_first_derivative_only
     def backward(ctx, dy, _codes, _scales):
         codes, scales, w = ctx.saved_tensors
         x, _, rstd = layer_ops.rmsnorm_from_packed(PackedRows(codes, scales, *ctx.meta), w, ctx.eps)
@@ -121,6 +158,7 @@ class _AddRMSNorm(torch.autograd.Function):
         return h, y
 
     @staticmethod
+    @_first_derivative_only
     def backward(ctx, dh, dy):
         h, w, rstd = ctx.saved_tensors
         if dy is None:
@@ -156,6 +194,7 @@ class _AttentionBlock(torch.autograd.Function):
         return a
 
     @staticmethod
+    @_first_derivative_only
     def backward(ctx, da):
         (y, wqkv, wo, qkv, o_rows, lse, inv_freq, positions, probs, q_norm,
          k_norm) = ctx.saved_tensors
@@ -206,6 +245,7 @@ class _MLPBlock(torch.autograd.Function):
         return out
 
     @staticmethod
+    @_first_derivative_only
     def backward(ctx, dout):
         y, wgu, wd, gu = ctx.saved_tensors
         d = y.shape[-1]
@@ -231,6 +271,7 @@ class _PackedMLPBlock(torch.autograd.Function):
         return torch.matmul(m, wd.t())
 
     @staticmethod
+    @_first_derivative_only
     def backward(ctx, dout):
         y, wgu, wd, codes, scales = ctx.saved_tensors
         d = y.shape[-1]
@@ -260,6 +301,7 @@ class _PackedLayer(torch.autograd.Function):
         return h.contiguous(), m.contiguous()
 
     @staticmethod
+    @_first_derivative_only
     def backward(ctx, dh, dm):
         edges, wanted, wants = ctx.run.pop()
         grads = iter(torch.autograd.grad(edges, wanted, (dh, dm)))
@@ -290,6 +332,7 @@ class _PackedLayerNorm(torch.autograd.Function):
         return h, y, p.codes, p.scales
 
     @staticmethod
+    @_first_derivative_only
     def backward(ctx, dh, dy, _codes, _scales):
         next_norm, codes, scales, positions, input_norm, *weights = ctx.saved_tensors
         stack = ctx.stack
@@ -347,6 +390,7 @@ class _LMHeadCrossEntropy(torch.autograd.Function):
         return loss_sum * inv
 
     @staticmethod
+    @_first_derivative_only
     def backward(ctx, dloss):
         dy, dw, inv = ctx.saved_tensors
         s = dloss * inv

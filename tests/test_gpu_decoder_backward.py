@@ -132,3 +132,18 @@ def test_captured_step_with_8_bit_checkpoints():
         torch.cuda.synchronize()
         for n, grad in gradients(m).items():
             assert torch.equal(grad, want[n]), n
+
+
+@pytest.mark.parametrize("kw", [{}, dict(embed_scale=2.0), dict(qk_norm=True),
+                                dict(activation_storage="int8"), CKPT8],
+                         ids=lambda kw: "-".join(kw) or "plain")
+@pytest.mark.parametrize("of", ["embed", "layers.0.down_proj", "final_norm", "lm_head"])
+def test_second_derivatives_are_refused(kw, of):
+    """The kernels have none; a graph of the gradient would lack their part."""
+    m, ids = build(**kw)
+    p = dict(m.named_parameters())[of]
+    want, = torch.autograd.grad(m(ids, labels=ids), p)
+    got, = torch.autograd.grad(m(ids, labels=ids), p, create_graph=True)
+    assert torch.equal(got, want)
+    with pytest.raises(RuntimeError, match="no second derivatives"):
+        got.square().sum().backward()
