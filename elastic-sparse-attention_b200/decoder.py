@@ -33,8 +33,9 @@ Options (all off by default):
 
 * ``embed_scale`` / ``padding_idx``: the token embedding runs in the library's
   lookup (times ``embed_scale``) and its gradient in the sorted-token kernels,
-  which leave the row ``padding_idx`` without a gradient; ids outside the
-  vocabulary give zero rows and a device error bit instead of an assert.
+  which leave the row ``padding_idx`` without a gradient; an id outside the
+  vocabulary makes its hidden state NaN, and so the loss and the gradients, and
+  sets a device error bit, instead of an assert.
 * ``qk_norm``: RMSNorm of each query and key head (weights ``q_norm``,
   ``k_norm`` of head_dim) before the rotary embedding, both in one pass; the
   backward normalises again instead of keeping the result.
@@ -93,13 +94,16 @@ def _first_derivative_only(backward):
 
 
 class _Embedding(torch.autograd.Function):
-    """scale * w[ids]."""
+    """scale * w[ids]; the row of an id that has none in w starts with a NaN, which
+    the norm after it spreads over the row: a step on wrong ids is not silent."""
 
     @staticmethod
     def forward(ctx, ids, w, scale: float, padding_idx):
         ctx.save_for_backward(ids)
         ctx.meta = (w.shape[0], scale, padding_idx)
-        return layer_ops.embedding_forward(ids, w, scale)
+        out = layer_ops.embedding_forward(ids, w, scale)
+        out[..., 0].masked_fill_((ids < 0) | (ids >= w.shape[0]), float("nan"))
+        return out
 
     @staticmethod
     @_first_derivative_only

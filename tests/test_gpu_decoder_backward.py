@@ -147,3 +147,24 @@ def test_second_derivatives_are_refused(kw, of):
     assert torch.equal(got, want)
     with pytest.raises(RuntimeError, match="no second derivatives"):
         got.square().sum().backward()
+
+
+@pytest.mark.parametrize("bad", [-1, CFG["V"], 1 << 40])
+@pytest.mark.parametrize("kw", [{}, CKPT8], ids=["kept", "checkpoints"])
+def test_a_token_outside_the_vocabulary_shows_in_the_loss(kw, bad):
+    """With the library's lookup such a token is no device assert, but no silent
+    zero row either (the labels here are valid)."""
+    import elastic_sparse_attention_b200 as esa
+    m, ids = build(embed_scale=2.0, padding_idx=0, **kw)
+    esa.ops.device_errors()
+    clean = m(ids, labels=ids)
+    assert clean.isfinite() and esa.ops.device_errors() == 0
+    wrong = ids.clone()
+    wrong[1, 7] = bad
+    hidden = m(wrong)
+    assert hidden[1, 7].isnan().all() and hidden[0].isfinite().all()
+    loss = m(wrong, labels=ids)
+    assert loss.isnan()
+    loss.backward()
+    assert not m.layers[0].qkv_proj.grad.isfinite().all()
+    assert esa.ops.device_errors() == esa._lib.DEVERR_TOKEN_RANGE
