@@ -22,9 +22,18 @@ def _dtype_code(t: torch.Tensor) -> int:
     return _lib.DTYPES[t.dtype]
 
 
+def _shape(t: torch.Tensor) -> tuple:
+    """The shape of a row operand; its last axis is the feature axis."""
+    if t.dim() == 0:
+        raise ValueError("row operands need a feature axis")
+    return tuple(t.shape)
+
+
 def _rows(t: torch.Tensor, dim: int) -> int:
     if not t.is_contiguous() or t.shape[-1] != dim:
         raise ValueError("row operands must be contiguous with the feature axis last")
+    if dim == 0:
+        raise ValueError("rows need at least one element")
     return t.numel() // dim
 
 
@@ -350,7 +359,7 @@ def _new_packed(shape: tuple, format: str, dtype: torch.dtype, dev) -> PackedRow
 def _check_packed(p: PackedRows) -> int:
     """The format code of a PackedRows whose parts fit together."""
     code = _pack_code(p.format)
-    shape = p.codes.shape
+    shape = _shape(p.codes)
     if (p.codes.dtype != torch.uint8 or p.scales.dtype != torch.float32
             or p.scales.shape != shape[:-1] + (-(-shape[-1] // PACK_GROUP),)):
         raise ValueError("PackedRows: codes must be uint8 and scales float32 "
@@ -367,7 +376,7 @@ def quantize_rows(x: torch.Tensor, format: str = "int8") -> PackedRows:
     NaN."""
     code = _pack_code(format)
     dev = _check_device(x)
-    shape = tuple(x.shape)
+    shape = _shape(x)
     n = _rows(x, shape[-1])
     dtype_code = _dtype_code(x)
     p = _new_packed(shape, format, x.dtype, dev)
@@ -394,7 +403,7 @@ def rmsnorm_forward_packed(x: torch.Tensor, weight: torch.Tensor, eps: float,
     pass."""
     code = _pack_code(format)
     dev = _check_device(x, weight)
-    shape = tuple(x.shape)
+    shape = _shape(x)
     dim = shape[-1]
     n = _rows(x, dim)
     dtype_code = _dtype_code(x)
@@ -441,7 +450,7 @@ def swiglu_forward_packed(gate_up: torch.Tensor, format: str = "int8"):
     are rows of their own."""
     code = _pack_code(format)
     dev = _check_device(gate_up)
-    shape = tuple(gate_up.shape)
+    shape = _shape(gate_up)
     if shape[-1] % 2:
         raise ValueError("gate_up rows must hold two halves of equal width")
     ffn = shape[-1] // 2
