@@ -97,3 +97,198 @@ def test_int8_borders_at_the_smallest_scales(lops, dtype):
     p = lops.quantize_rows(x.to(DEV), "int8")
     assert torch.equal(p.scales.cpu().double(), s)
     assert torch.equal(p.codes.view(torch.int8).cpu().double(), codes)
+
+
+# ---------------------------------------------------------------------------
+# every row of the embedding gradient, at the borders of the pieces
+# ---------------------------------------------------------------------------
+def pieces_case(P, lengths, n_max, seed):
+    """Token ids, shuffled, whose sorted list has a run of each length beginning at
+    each offset within a piece of P entries; every second vocabulary entry is
+    absent.  (ids, V)"""
+    g = torch.Generator().manual_seed(seed)
+    runs, at = [], 0
+    for length in lengths:
+        for offset in range(P):
+            fill = (offset - at) % P
+            while fill > 0:                       # short runs up to the offset
+                step = min(fill, int(torch.randint(1, P, (), generator=g)))
+                runs.append(step)
+                fill -= step
+                at += step
+            runs.append(length)
+            at += length
+    assert at <= n_max, at
+    tokens = 2 * torch.arange(len(runs)) + 1
+    ids = tokens.repeat_interleave(torch.tensor(runs))
+    return ids[torch.randperm(at, generator=g)], 2 * len(runs) + 2
+
+
+def odd_rows(n, d, g):
+    """Rows of +-1: no sum without one of them is the same."""
+    return (2 * torch.randint(0, 2, (n, d), generator=g) - 1).float()
+
+
+# Pieces of 16, 32 and 64 entries: by width and token count.  Each with runs of
+# up to three pieces; and long runs, which several pieces share.
+PIECES = {
+    "narrow-16": (16, 64, 1 << 20, 2561), "wide-16": (16, 264, 8192, 2561),
+    "wide-32": (32, 264, 65536, 8193), "wide-64": (64, 264, 1 << 20, 65537),
+    "one-cta-16": (16, 264, 2560, 1025),
+}
+
+
+def pieces_ids(name):
+    P, d, n_max, n_min = PIECES[name]
+    lengths = [P - 1, P, P + 1, 2 * P - 1, 2 * P, 2 * P + 1, 3 * P, 3 * P + 1, 1]
+    if name == "one-cta-16":
+        lengths = [P - 1, P, P + 1, 2 * P + 1]
+    ids, V = pieces_case(P, lengths, n_max, P + d)
+    g = torch.Generator().manual_seed(d)
+    more = max(n_min - ids.numel(), 0)            # one long run brings it to the length wanted
+    room = n_max - ids.numel() - more
+    more += min(room, 40 * P + 3)
+    ids = torch.cat([ids, torch.full((more,), V - 2)])
+    ids = ids[torch.randperm(ids.numel(), generator=g)]
+    assert n_min <= ids.numel() <= n_max
+    return ids, V, d
+
+
+def lost_unseen(ids, dy, V, scale, dtype):
+    """Rows of dy without which the rounded gradient would be the same: without a
+    row it differs from the whole by that row, in its token's entry alone."""
+    whole = exact_gradient(ids, dy, V, 1.0, torch.float64)[ids]
+    without = ((whole - dy.double()) * scale).to(dtype)
+    return (without == (whole * scale).to(dtype)).all(1).nonzero().flatten()
+
+
+@pytest.mark.parametrize("name", PIECES)
+def test_every_lost_row_would_show(name):
+    """The oracle without any one of the rows differs from the whole."""
+    ids, V, d = pieces_ids(name)
+    dy = odd_rows(ids.numel(), 8, torch.Generator().manual_seed(1))
+    for dtype in (torch.float32, torch.bfloat16):
+        assert not lost_unseen(ids, dy, V, 0.25, dtype).numel()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("name", PIECES)
+def test_embedding_gradient_at_piece_borders(lops, name, dtype):
+    ids, V, d = pieces_ids(name)
+    ids = ids.to(DEV)
+    dy = odd_rows(ids.numel(), d, torch.Generator().manual_seed(2)).to(DEV)
+    for pad in (None, 7):
+        want = exact_gradient(ids, dy, V, 0.25, dtype)
+        if pad is not None:
+            want[pad] = 0
+        got = lops.embedding_backward(ids, dy.to(dtype), V, 0.25, padding_idx=pad)
+        assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,V,d", [
+    (1, 40, 8), (31, 7, 64), (130, 3, 520), (1000, 33, 520), (1024, 900, 1032), (1024, 1, 264),
+    (2047, 64, 64), (2048, 5, 256), (2048, 3000, 8),
+    # the general sort with one digit, two and three, all tokens the same
+    (70001, 1, 264), (9000, 2, 1032), (20000, 511, 16), (20000, 262143, 8), (66000, 300000, 264)])
+def test_embedding_gradient_is_exact_on_integers(lops, dtype, n, V, d):
+    g = torch.Generator().manual_seed(n + V + d)
+    ids = torch.randint(0, V, (n,), generator=g).to(DEV)
+    dy = odd_rows(n, d, g).to(DEV)
+    assert torch.equal(lops.embedding_backward(ids, dy.to(dtype), V, 2.0),
+                       exact_gradient(ids, dy, V, 2.0, dtype))
+
+
+# ---------------------------------------------------------------------------
+# every row of the query / key norm's weight gradients
+# ---------------------------------------------------------------------------
+U = 2.0 ** -24
+WEIGHT_SHAPES = [(1, 1, 32, 8, 128), (2, 333, 4, 2, 64), (3, 5, 3, 1, 16), (2, 40, 6, 2, 128),
+                 (1, 2100, 8, 2, 128), (3, 2400, 1, 1, 16), (2, 5003, 3, 1, 32),
+                 (1, 9001, 2, 1, 128), (5, 1500, 5, 2, 64), (1, 4800, 5, 1, 32),
+                 (2, 700, 16, 4, 128), (1, 900, 40, 8, 64)]
+
+
+def weight_case(dtype, B, L, H, D, seed, only=None):
+    """(x, dout), [B, H, L, D]; ``only``: the tokens b * L + l whose dout is not zero."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(B, L, H, D, generator=g).to(dtype)
+    dout = torch.randn(B, L, H, D, generator=g).to(dtype)
+    if only is not None:
+        keep = torch.zeros(B * L, dtype=torch.bool)
+        keep[only] = True
+        dout[~keep.view(B, L)] = 0
+    return x.transpose(1, 2), dout.transpose(1, 2)
+
+
+def weight_gradient64(x, dout, inv, eps=1e-6):
+    """(terms of dw [B, H, L, D], bound of each one's float32 error over U)."""
+    xh = x.double() * (x.double().square().mean(-1, keepdim=True) + eps).rsqrt()
+    ang = torch.arange(x.shape[2], device=x.device).double()[:, None] * inv.double()
+    c, s = ang.cos(), ang.sin()
+    a, b = dout.double().chunk(2, -1)
+    gr = torch.cat([a * c + b * s, b * c - a * s], -1)
+    mag = torch.cat([a.abs() + b.abs()] * 2, -1) * xh.abs()
+    return gr * xh, mag
+
+
+def summation_depth(B, L, Hq, Hk, D, side):
+    """Additions that a term of dw passes through at most: a lane's own rows (one
+    in every 32 / threads-per-row of a warp's, over the side's warps, of which a
+    CTA has 4; whole rounds of up to 4), the lanes of a warp (5), its CTA's warps
+    (4), a warp's share of the CTAs' sums and the 32 warps of that."""
+    rows = B * L * (Hq if side == 0 else Hk)
+    ctas = max(2, min(444, -(-B * L * (Hq + Hk) // 4)))
+    share = ctas * (Hq if side == 0 else Hk) / (Hq + Hk)     # at least half of it: see below
+    lanes = max(1, share / 2) * 4 * 32 / (D / 8)
+    return rows / lanes + 32 + 5 + 4 + ctas / 32 + 1 + 32
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,L,Hq,Hk,D", WEIGHT_SHAPES)
+def test_qk_weight_gradient_of_single_tokens(lops, dtype, B, L, Hq, Hk, D):
+    """dout is zero but for a few tokens, at the ends of the sequences and in
+    between: a sum that misses one of them is off by a large part of itself."""
+    inv = lops.rope_inv_freq(D, 10000.0, DEV)
+    w = torch.ones(D, device=DEV, dtype=dtype)
+    n = B * L
+    for seed in range(4):
+        g = torch.Generator().manual_seed(100 + seed)
+        picks = torch.cat([torch.tensor([0, n - 1, L - 1, n - L]),
+                           torch.randint(0, n, (2,), generator=g)]).unique()
+        if seed == 3:
+            picks = torch.arange(max(0, n - 9), n)            # the last tasks
+        (q, dq), (k, dk) = (tuple(t.to(DEV) for t in weight_case(dtype, B, L, H, D, seed + H, picks))
+                            for H in (Hq, Hk))
+        _, _, dwq, dwk = lops.qk_norm_rope_backward(q, k, w, w, 1e-6, inv, dq, dk)
+        for side, (dw, x, do) in enumerate(((dwq, q, dq), (dwk, k, dk))):
+            terms, mag = weight_gradient64(x, do, inv)
+            want, mag = terms.sum((0, 1, 2)), mag.sum((0, 1, 2))
+            # 64 u of each term (as for dx), the sums, the one rounding
+            slack = (64 + summation_depth(B, L, Hq, Hk, D, side)) * U * mag
+            bound = slack + torch.finfo(dtype).eps / 2 * (want.abs() + slack)
+            assert ((dw.double() - want).abs() <= bound).all(), (seed, side)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,L,Hq,Hk,D", WEIGHT_SHAPES)
+def test_qk_weight_gradient_misses_no_row(lops, B, L, Hq, Hk, D):
+    """Full dout in float32: the bound by the depth of the sums is smaller than
+    what the mean row adds, so that the sum without any one row exceeds it."""
+    inv = lops.rope_inv_freq(D, 10000.0, DEV)
+    w = torch.ones(D, device=DEV)
+    (q, dq), (k, dk) = (tuple(t.to(DEV) for t in weight_case(torch.float32, B, L, H, D, 7 * H))
+                        for H in (Hq, Hk))
+    _, _, dwq, dwk = lops.qk_norm_rope_backward(q, k, w, w, 1e-6, inv, dq, dk)
+    for side, (dw, x, do) in enumerate(((dwq, q, dq), (dwk, k, dk))):
+        terms, mag = weight_gradient64(x, do, inv)
+        want, mag = terms.sum((0, 1, 2)), mag.sum((0, 1, 2))
+        slack = (64 + summation_depth(B, L, Hq, Hk, D, side)) * U * mag
+        bound = slack + U * (want.abs() + slack)
+        # what a lost row would leave, in the column where it is largest over its bound
+        lost = (terms.abs() / (2 * bound)).amax(-1)
+        assert (lost > 1).all(), float(lost.min())
+        assert ((dw.double() - want).abs() <= bound).all(), side
