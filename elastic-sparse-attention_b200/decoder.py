@@ -43,8 +43,10 @@ Options (all off by default):
   in 8 bits.  With ``activation_checkpointing`` that is each layer's input
   (written by the norm that precedes the layer, restored together with that
   norm), instead of two full rows; without, the MLP's gate / up rows, the
-  largest activation of a layer.  The forward pass is unchanged; gradients are
-  taken at the decoded values.
+  largest activation of a layer.  The forward pass works on the activations
+  themselves, not on their 8-bit form; its results are within a rounding of
+  those without the option (the norm sums in another order, SwiGLU forms its
+  sigmoid another way).  Gradients are taken at the decoded values.
 """
 from __future__ import annotations
 

@@ -399,8 +399,8 @@ def dequantize_rows(packed: PackedRows, dtype: torch.dtype | None = None) -> tor
 
 def rmsnorm_forward_packed(x: torch.Tensor, weight: torch.Tensor, eps: float,
                            residual: torch.Tensor | None = None, format: str = "int8"):
-    """(h, y, rstd, packed): :func:`rmsnorm_forward` and h in 8 bits, in one
-    pass."""
+    """(h, y, rstd, packed): :func:`rmsnorm_forward` (h bit for bit, y and rstd
+    within a rounding) and h in 8 bits, in one pass."""
     code = _pack_code(format)
     dev = _check_device(x, weight)
     shape = _shape(x)
@@ -445,8 +445,8 @@ def _check_norm_weight(weight: torch.Tensor, dim: int, dtype: torch.dtype) -> No
 
 
 def swiglu_forward_packed(gate_up: torch.Tensor, format: str = "int8"):
-    """(out, packed): :func:`swiglu_forward` and gate_up in 8 bits, in one
-    pass.  packed has shape [..., 2, ffn]: the gate and the up half of a row
+    """(out, packed): :func:`swiglu_forward` (within a rounding) and gate_up in 8
+    bits, in one pass.  packed has shape [..., 2, ffn]: the gate and the up half of a row
     are rows of their own."""
     code = _pack_code(format)
     dev = _check_device(gate_up)

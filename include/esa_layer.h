@@ -190,7 +190,9 @@ int esa_dequantize_rows(int32_t dtype, int32_t format, int64_t n_rows, int32_t d
                         const void* codes, const float* scales, void* x, void* stream);
 
 /* esa_rmsnorm_forward that also writes the 8-bit form of h (as stored in
- * h_out, or of x without a residual) in the same pass. */
+ * h_out, or of x without a residual) in the same pass.  h_out is the same bit
+ * for bit; rstd and y may differ from that entry point's by the order of the
+ * float32 sum, so that y is a step of dtype off where that moves its rounding. */
 int esa_rmsnorm_pack_forward(int32_t dtype, int32_t format, int64_t n_rows, int32_t dim,
                              const void* x, const void* residual, void* h_out, const void* weight,
                              float eps, void* y, float* rstd, void* codes, float* scales,
@@ -203,7 +205,8 @@ int esa_rmsnorm_unpack_forward(int32_t dtype, int32_t format, int64_t n_rows, in
                                const void* codes, const float* scales, const void* weight,
                                float eps, void* h, void* y, float* rstd, void* stream);
 
-/* esa_swiglu_forward that also writes gate_up in 8 bits.  The gate and the up
+/* esa_swiglu_forward (within a rounding: the sigmoid's float32 arithmetic is
+ * another) that also writes gate_up in 8 bits.  The gate and the up
  * half of a row are two rows of ffn elements with groups of their own: codes
  * [n_rows, 2, ffn], scales [n_rows, 2, ceil(ffn / 128)]. */
 int esa_swiglu_pack_forward(int32_t dtype, int32_t format, int64_t n_rows, int32_t ffn,
