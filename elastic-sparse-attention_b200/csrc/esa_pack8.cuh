@@ -12,7 +12,10 @@
 //
 // and a code stands for code * s (float32).  A group that holds an infinity or
 // a NaN gets s = NaN, so all of it decodes to NaN: what overflowed in the
-// forward pass stays visible in the backward pass.
+// forward pass stays visible in the backward pass.  int8 has one more value that
+// does not come back finite: for a = 2^128 - 2^104, the largest float32, s is
+// 8454660 * 2^98, and 127 s = 2^128 - 4 * 2^98 rounds to infinity.  (The float32
+// below it, 2^128 - 2^105, has s = 8454659 * 2^98 and stays finite.)
 //
 // int8 is the finer of the two on rows whose groups have no outliers (steps
 // of a / 127 against 2^-4 relative), e4m3 keeps small elements next to large

@@ -373,7 +373,7 @@ def quantize_rows(x: torch.Tensor, format: str = "int8") -> PackedRows:
     """x [..., dim] in 8 bits, one scale per 128 elements of the last axis:
     ``int8`` (even steps of max|x| / 127 per group) or ``e4m3`` (relative
     steps, power-of-two scales).  A group with an infinity or a NaN decodes to
-    NaN."""
+    NaN, and in ``int8`` the largest float32 itself to an infinity."""
     code = _pack_code(format)
     dev = _check_device(x)
     shape = _shape(x)

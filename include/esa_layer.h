@@ -175,7 +175,9 @@ int esa_qk_norm_rope_backward(int32_t dtype, int32_t batch, int64_t seq_len, int
  *                  code = x / s to the nearest e4m3 value, ties to even (the
  *                  next smaller where code * s passes dtype's largest value)
  * A code stands for code * s.  A group with an infinity or a NaN gets s = NaN
- * and codes 0, so it decodes to NaN.  codes: n_rows * dim bytes; scales:
+ * and codes 0, so it decodes to NaN.  Every other group decodes to finite values
+ * with one exception: where a is the largest float32, 127 * s rounds past it in
+ * ESA_PACK_INT8, so codes of 127 decode to infinity there.  codes: n_rows * dim bytes; scales:
  * n_rows * ceil(dim / 128) floats.
  */
 #define ESA_PACK_INT8 0

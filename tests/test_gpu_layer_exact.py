@@ -292,3 +292,32 @@ def test_qk_weight_gradient_misses_no_row(lops, B, L, Hq, Hk, D):
         lost = (terms.abs() / (2 * bound)).amax(-1)
         assert (lost > 1).all(), float(lost.min())
         assert ((dw.double() - want).abs() <= bound).all(), side
+
+
+def test_the_largest_scale_by_arithmetic():
+    """127 * f32(a / 127) passes the largest float32 for that value alone: in units
+    of 2^98 it is 2^30 - 64 and its neighbours are 64 apart; 127 s rounds to
+    infinity from 2^30 - 32 on, which takes s >= 8454660, so a / 127 >= 8454659.5,
+    so a >= 2^30 - 67.5."""
+    big = torch.tensor(torch.finfo(torch.float32).max)
+    below = torch.nextafter(big, torch.tensor(0.0))
+    for a, finite in ((big, False), (below, True)):
+        s = (a.double() / 127).float()
+        assert (127 * s).isfinite().item() == finite
+    assert 127 * 8454660 >= 2 ** 30 - 32 > 127 * 8454659
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_the_largest_values_come_back_finite(lops, fmt):
+    """All but the largest float32 in int8, whose documented value is infinite."""
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        big = torch.tensor(torch.finfo(dtype).max, dtype=dtype)
+        x = torch.randn(4, 128, generator=torch.Generator().manual_seed(1)).to(dtype)
+        x[0, 5], x[1, 9] = big, -big
+        x[2, 3] = x[2, 4] = torch.nextafter(big, torch.tensor(0, dtype=dtype))
+        back = lops.dequantize_rows(lops.quantize_rows(x.to(DEV), fmt)).cpu()
+        if fmt == "int8" and dtype == torch.float32:
+            assert back[0, 5] == float("inf") and back[1, 9] == float("-inf")
+            back[0, 5] = back[1, 9] = 0
+        assert back.isfinite().all()
