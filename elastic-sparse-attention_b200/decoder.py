@@ -344,13 +344,18 @@ class _PackedLayerNorm(torch.autograd.Function):
         stack = ctx.stack
         h, y, _ = layer_ops.rmsnorm_from_packed(PackedRows(codes, scales, *ctx.meta), input_norm,
                                                 stack.eps)
+        below = ctx.needs_input_grad[4]      # the layer runs backward too
         wants = [w is not None and w.requires_grad for w in weights]
         wanted = [h.requires_grad_(), y.requires_grad_()]
         wanted += [w for w, want in zip(weights, wants) if want]
-        with torch.enable_grad():
+        with torch.set_grad_enabled(below):
             h, m = stack._layer_body(ctx.i, h, y, positions, weights)
-        edges = [torch.autograd.graph.get_gradient_edge(t) for t in (h, m)]
-        ctx.run[:] = [(edges, wanted, wants)]
+        if below:
+            edges = [torch.autograd.graph.get_gradient_edge(t) for t in (h, m)]
+            ctx.run[:] = [(edges, wanted, wants)]
+            # a call that asks for gradients above this layer alone never takes it
+            torch.autograd.Variable._execution_engine.queue_callback(ctx.run.clear)
+        del wanted
         h, _, rstd = layer_ops.rmsnorm_forward(h.detach(), next_norm, stack.eps,
                                                residual=m.detach())
         del y, m

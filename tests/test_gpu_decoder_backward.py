@@ -168,3 +168,25 @@ def test_a_token_outside_the_vocabulary_shows_in_the_loss(kw, bad):
     loss.backward()
     assert not m.layers[0].qkv_proj.grad.isfinite().all()
     assert esa.ops.device_errors() == esa._lib.DEVERR_TOKEN_RANGE
+
+
+def test_8_bit_checkpoints_keep_no_run_that_nothing_differentiates():
+    """Only the last norm's weight takes a gradient: the layer runs again for its
+    input, and nothing of that run outlives the backward."""
+    m, ids = build(**CKPT8)
+    for p in m.parameters():
+        p.requires_grad_(p is m.final_norm)
+    want, _ = build(activation_checkpointing=True)
+    want(ids, labels=ids).backward()
+    m(ids, labels=ids).backward()
+    assert torch.nn.functional.cosine_similarity(m.final_norm.grad, want.final_norm.grad, 0) > 0.99
+    loss = m(ids, labels=ids)
+    held = torch.cuda.memory_allocated()
+    loss.backward()
+    assert torch.cuda.memory_allocated() <= held
+    # the same where all may take gradients, but the call asks for one alone
+    m, ids = build(**CKPT8)
+    loss = m(ids, labels=ids)
+    held = torch.cuda.memory_allocated()
+    torch.autograd.grad(loss, m.final_norm)
+    assert torch.cuda.memory_allocated() <= held
