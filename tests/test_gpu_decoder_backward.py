@@ -3,6 +3,7 @@ belongs to, whatever happens to the stack in between, and what it holds while
 it runs."""
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from test_gpu_decoder_options import CFG, build
 
@@ -190,3 +191,22 @@ def test_8_bit_checkpoints_keep_no_run_that_nothing_differentiates():
     held = torch.cuda.memory_allocated()
     torch.autograd.grad(loss, m.final_norm)
     assert torch.cuda.memory_allocated() <= held
+
+
+def test_8_bit_checkpoints_inside_other_savers():
+    """Saved tensors that a hook moves to the host, and the whole stack inside a
+    checkpoint of the caller's: the layers' weights are still the ones that get
+    the gradients."""
+    m, ids = build(qk_norm=True, embed_scale=2.0, **CKPT8)
+    m(ids, labels=ids).backward()
+    want = gradients(m)
+    m.zero_grad(set_to_none=True)
+    with torch.autograd.graph.save_on_cpu():
+        loss = m(ids, labels=ids)
+    loss.backward()
+    for n, grad in gradients(m).items():
+        assert torch.equal(grad, want[n]), n
+    m.zero_grad(set_to_none=True)
+    torch.utils.checkpoint.checkpoint(lambda: m(ids, labels=ids), use_reentrant=False).backward()
+    for n, grad in gradients(m).items():
+        assert torch.equal(grad, want[n]), n

@@ -321,3 +321,42 @@ def test_the_largest_values_come_back_finite(lops, fmt):
             assert back[0, 5] == float("inf") and back[1, 9] == float("-inf")
             back[0, 5] = back[1, 9] = 0
         assert back.isfinite().all()
+
+
+@pytest.mark.gpu
+def test_calls_on_two_streams_and_threads(lops):
+    """Calls in flight at the same time have their workspaces to themselves."""
+    import threading
+    g = torch.Generator().manual_seed(6)
+    w = (1 + 0.1 * torch.randn(64, generator=g)).to(DEV)
+    inv = lops.rope_inv_freq(64, 10000.0, DEV)
+    jobs = []
+    for n in (3000, 9000):
+        ids = torch.randint(0, 5000, (n,), generator=g).to(DEV)
+        dy = odd_rows(n, 264, g).to(DEV)
+        q = torch.randn(1, 4, n, 64, generator=g).to(DEV)
+
+        def job(ids=ids, dy=dy, q=q):
+            return (lops.embedding_backward(ids, dy, 5000, 0.5),
+                    *lops.qk_norm_rope_backward(q, q, w, w, 1e-6, inv, q, q))
+        jobs.append(job)
+    want = [j() for j in jobs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in jobs]
+    got = [[], []]
+
+    def go(k):
+        with torch.cuda.stream(streams[k]):
+            for _ in range(20):
+                got[k].append(jobs[k]())
+        streams[k].synchronize()
+
+    threads = [threading.Thread(target=go, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for k in range(2):
+        assert len(got[k]) == 20
+        for out in got[k]:
+            assert all(torch.equal(a, b) for a, b in zip(out, want[k]))
