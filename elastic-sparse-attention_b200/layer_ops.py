@@ -90,6 +90,12 @@ def rope_inv_freq(head_dim: int, base: float, device) -> torch.Tensor:
     return (1.0 / (base ** exps)).to(device=device, dtype=torch.float32)
 
 
+def _check_inv_freq(inv_freq: torch.Tensor, head_dim: int) -> None:
+    if (inv_freq.dtype != torch.float32 or inv_freq.numel() != head_dim // 2
+            or not inv_freq.is_contiguous()):
+        raise ValueError("inv_freq must be float32 [head_dim / 2]")
+
+
 def rope_(q: torch.Tensor, k: torch.Tensor | None, inv_freq: torch.Tensor,
           positions: torch.Tensor | None = None, inverse: bool = False) -> None:
     """Rotate q [B, Hq, L, D] and k [B, Hk, L, D] (strided views with a
@@ -100,6 +106,7 @@ def rope_(q: torch.Tensor, k: torch.Tensor | None, inv_freq: torch.Tensor,
     if k is not None and (k.shape[0] != B or k.shape[2] != L or k.shape[3] != D or
                           k.dtype != q.dtype):
         raise ValueError("q and k must share batch, length, head_dim and dtype")
+    _check_inv_freq(inv_freq, D)
     if positions is not None:
         positions = positions.to(device=dev, dtype=torch.int64).contiguous()
         if positions.numel() != L:
@@ -235,8 +242,7 @@ def _qk_checks(q, k, q_weight, k_weight, inv_freq, positions):
         if kB != B or kL != L or kD != D or k.dtype != q.dtype or k.device != dev:
             raise ValueError("q and k must share batch, length, head_dim, dtype and device")
         _check_head_weight("k", k_weight, k, dev)
-    if inv_freq.dtype != torch.float32 or inv_freq.numel() != D // 2 or not inv_freq.is_contiguous():
-        raise ValueError("inv_freq must be float32 [head_dim / 2]")
+    _check_inv_freq(inv_freq, D)
     stride = 0
     if positions is not None:
         shape = tuple(positions.shape)

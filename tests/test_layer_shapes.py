@@ -32,3 +32,23 @@ def test_operators_refuse_such_rows(esa, shape):
                  lambda: lops.rmsnorm_from_packed(packed, w, 1e-6)):
         with pytest.raises(ValueError):
             call()
+
+
+def test_rotation_tables_of_another_kind(esa):
+    """A stack cast with ``.half()`` has a half table, which the kernels would read
+    as float32, past its end."""
+    check = esa.layer_ops._check_inv_freq
+    table = esa.layer_ops.rope_inv_freq(64, 10000.0, "cpu")
+    check(table, 64)
+    for bad in (table.half(), table[:16], table.repeat(2)[::2], table.double()):
+        with pytest.raises(ValueError, match="inv_freq"):
+            check(bad, 64)
+
+
+@pytest.mark.gpu
+def test_rope_refuses_such_tables(esa):
+    q = torch.randn(1, 2, 3, 64, device=DEV)
+    inv = esa.layer_ops.rope_inv_freq(64, 10000.0, DEV)
+    for bad in (inv.half(), inv[:16]):
+        with pytest.raises(ValueError, match="inv_freq"):
+            esa.layer_ops.rope_(q, None, bad)
