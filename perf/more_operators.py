@@ -102,12 +102,12 @@ def draw(rng):
         N = _log(rng, 8, min(32768, (1 << 26) // K))
         case.update(M=_log(rng, 1, 64), K=K, N=N, group=rng.choice([32, 64, 128, 128]))
     elif kind == "cache_write":
-        D = rng.choice([32, 64, 128, 128, 256])
+        D = rng.choice([64, 128, 128, 256])
         B, Hkv = rng.choice([1, 2, 3, 8, 33]), rng.choice([1, 2, 8])
         L = _log(rng, 1, min(32768, (1 << 25) // (B * Hkv * D)))
         case.update(B=B, L=L, Hkv=Hkv, D=D, S=L + _log(rng, 1, 2048), ragged=rng.random() < 0.5)
     else:
-        D = rng.choice([32, 64, 128, 128, 256])
+        D = rng.choice([64, 128, 128, 256])
         Hkv = rng.choice([1, 2, 4, 8])
         Hq = Hkv * rng.choice([1, 2, 4])
         w = rng.choice([16, 33, 64, 64, 100, 256])
