@@ -7,12 +7,13 @@ directory).
 """
 from . import _lib, layer_ops, ops
 from .attention import ElasticSparseAttention, ElasticSparseAttentionFunction, KeyPlanCache
+from .cache import PackedKVCache
 from .decoder import ElasticDecoderStack
 from .head_split import HeadShardedElasticSparseAttention, head_share
 from .ops import PatternSpec
 from .sharded import SequenceShardedElasticSparseAttention
 
 __all__ = ["ElasticSparseAttention", "ElasticSparseAttentionFunction", "ElasticDecoderStack",
-           "HeadShardedElasticSparseAttention", "KeyPlanCache", "PatternSpec",
+           "HeadShardedElasticSparseAttention", "KeyPlanCache", "PackedKVCache", "PatternSpec",
            "SequenceShardedElasticSparseAttention", "head_share", "layer_ops", "ops", "_lib"]
 __version__ = "0.1.4"

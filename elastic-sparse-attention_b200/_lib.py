@@ -35,7 +35,10 @@ EXPORTED = ("esa_version", "esa_last_error", "esa_device_errors", "esa_forward_w
             "esa_embedding_backward", "esa_qk_norm_rope_forward",
             "esa_qk_norm_rope_backward_workspace_size", "esa_qk_norm_rope_backward",
             "esa_quantize_rows", "esa_dequantize_rows", "esa_rmsnorm_pack_forward",
-            "esa_rmsnorm_unpack_forward", "esa_swiglu_pack_forward", "esa_swiglu_unpack_backward")
+            "esa_rmsnorm_unpack_forward", "esa_swiglu_pack_forward", "esa_swiglu_unpack_backward",
+            "esa_token_logprobs_forward", "esa_token_logprobs_backward", "esa_weight4_codes_size",
+            "esa_quantize_weight4", "esa_dequantize_weight4", "esa_linear4", "esa_cache4_write",
+            "esa_cache4_read", "esa_cache4_forward")
 
 # ESA_DEVERR_* bits of the per-device error word
 DEVERR_KV_RANGE = 1
@@ -55,6 +58,13 @@ class EsaRows(ctypes.Structure):
                 ("src_dtype", ctypes.c_int32), ("dst_dtype", ctypes.c_int32),
                 ("row_elems", ctypes.c_int64), ("count", ctypes.c_int64 * 3),
                 ("src_stride", ctypes.c_int64 * 3), ("dst_stride", ctypes.c_int64 * 3)]
+
+
+class EsaCache4(ctypes.Structure):
+    _fields_ = [("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p),
+                ("batch", ctypes.c_int32), ("num_kv_heads", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("reserved", ctypes.c_int32),
+                ("max_len", ctypes.c_int64)]
 
 
 class EsaProblem(ctypes.Structure):
@@ -173,6 +183,28 @@ def load() -> ctypes.CDLL:
         lib.esa_swiglu_pack_forward.restype = ctypes.c_int
         lib.esa_swiglu_unpack_backward.argtypes = [i32, i32, i64, i32, P, P, P, P, P, P]
         lib.esa_swiglu_unpack_backward.restype = ctypes.c_int
+        lib.esa_token_logprobs_forward.argtypes = [i32, i32, i64, i64, i64, P, P, i32, P, P, P, P, P,
+                                                   P]
+        lib.esa_token_logprobs_forward.restype = ctypes.c_int
+        lib.esa_token_logprobs_backward.argtypes = [i32, i32, i64, i64, i64, P, P, P, P, P, P, i64,
+                                                    P, P]
+        lib.esa_token_logprobs_backward.restype = ctypes.c_int
+        lib.esa_weight4_codes_size.argtypes = [i64, i64]
+        lib.esa_weight4_codes_size.restype = S
+        lib.esa_quantize_weight4.argtypes = [i32, i64, i64, i32, P, P, P, P]
+        lib.esa_quantize_weight4.restype = ctypes.c_int
+        lib.esa_dequantize_weight4.argtypes = [i32, i64, i64, i32, P, P, P, P]
+        lib.esa_dequantize_weight4.restype = ctypes.c_int
+        lib.esa_linear4.argtypes = [i32, i64, i64, i64, i32, P, P, P, P, P]
+        lib.esa_linear4.restype = ctypes.c_int
+        C = ctypes.POINTER(EsaCache4)
+        lib.esa_cache4_write.argtypes = [i32, C, i64, T, T, P, i64, P, P]
+        lib.esa_cache4_write.restype = ctypes.c_int
+        lib.esa_cache4_read.argtypes = [i32, C, i64, T, T, P, i64, P]
+        lib.esa_cache4_read.restype = ctypes.c_int
+        lib.esa_cache4_forward.argtypes = [i32, C, i32, i64, i32, i32, i32, i32, i32, F, T, P, i64,
+                                           P, T, P, P]
+        lib.esa_cache4_forward.restype = ctypes.c_int
         _lib = lib
     return _lib
 

@@ -81,21 +81,9 @@ namespace {
 
 using namespace esa::host;
 
-constexpr int64_t kMaxPosition = int64_t(1) << 24;  // float32 index math is exact below 2^24
-constexpr int kMaxAttnLength = 2048;
-
-esa::Pattern make_pattern(int num_heads, int w, int layer_idx, int num_hidden_layers,
-                          int head_offset = 0) {
-  esa::Pattern P;
-  const int denominator = num_hidden_layers > 1 ? num_hidden_layers - 1 : 1;   // :488
-  const double alpha = (double)layer_idx / (double)denominator;                // :489
-  P.w = w;
-  P.num_heads = num_heads;
-  P.a = (float)alpha;
-  P.c = (float)((double)w * (1.0 - alpha));                                    // :496
-  P.head_offset = head_offset;
-  return P;
-}
+using esa::kMaxAttnLength;
+using esa::kMaxPosition;
+using esa::make_pattern;
 
 // Query heads of the pattern a problem's heads belong to.
 int pattern_heads(const esa_problem_t* pb) {

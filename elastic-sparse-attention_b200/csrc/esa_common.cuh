@@ -28,6 +28,22 @@ struct Pattern {
                     // caller runs a subset of the heads, e.g. one GPU's share)
 };
 
+constexpr int64_t kMaxPosition = int64_t(1) << 24;  // float32 index math is exact below 2^24
+constexpr int kMaxAttnLength = 2048;
+
+inline Pattern make_pattern(int num_heads, int w, int layer_idx, int num_hidden_layers,
+                            int head_offset = 0) {
+  Pattern P;
+  const int denominator = num_hidden_layers > 1 ? num_hidden_layers - 1 : 1;   // :488
+  const double alpha = (double)layer_idx / (double)denominator;                // :489
+  P.w = w;
+  P.num_heads = num_heads;
+  P.a = (float)alpha;
+  P.c = (float)((double)w * (1.0 - alpha));                                    // :496
+  P.head_offset = head_offset;
+  return P;
+}
+
 // Start and spacing of the window of one query position (reference :482-499).
 struct RowWin {
   int st;    // start_ids_base                                                :497

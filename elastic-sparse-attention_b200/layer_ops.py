@@ -1,7 +1,8 @@
 """Tensor-level calls of the decoder-layer harness kernels (include/esa_layer.h):
 RMSNorm with a fused residual add, rotary embedding in place, SwiGLU, token
 embedding and its gradient, per-head query / key norm with the rotary
-embedding, rows kept in 8 bits between forward and backward.
+embedding, rows kept in 8 bits between forward and backward, log probabilities
+of tokens and their gradient, products with weights in 4 bits.
 
 Like ``ops``, torch only allocates memory and provides the stream; every
 kernel is in libesa_b200.so and there is no fallback.
@@ -488,3 +489,188 @@ def swiglu_backward_packed(packed: PackedRows, dout: torch.Tensor, recompute: bo
                 _rows(dout, ffn), ffn, packed.codes.data_ptr(), packed.scales.data_ptr(),
                 dout.data_ptr(), dgu.data_ptr(), _lib.ptr(out))
     return dgu, out
+
+
+# ---------------------------------------------------------------------------
+# Log probabilities of tokens
+# ---------------------------------------------------------------------------
+MAX_TOP = 32
+IGNORED_TOKEN = -100
+
+
+@dataclass(eq=False)
+class TokenLogProbs:
+    """What :func:`token_logprobs` found in rows of logits [..., vocab], all
+    float32 but the ids: ``logprobs`` and ``entropy`` [...], ``stats`` [..., 2]
+    (the row's maximum m and ln of the sum of exp(x - m)), ``top_ids`` int64 and
+    ``top_logprobs`` [..., top_k] (None without alternatives)."""
+    logprobs: torch.Tensor
+    entropy: torch.Tensor
+    stats: torch.Tensor
+    top_ids: torch.Tensor | None
+    top_logprobs: torch.Tensor | None
+
+    @property
+    def logsumexp(self) -> torch.Tensor:
+        return self.stats.sum(-1)
+
+
+def _logit_rows(name: str, x: torch.Tensor) -> tuple:
+    """(rows, vocab, elements between rows) of [..., vocab] rows that lie evenly
+    spaced in memory (contiguous, or a 2-D view such as a slice of columns)."""
+    if x.dim() == 0:
+        raise ValueError(f"{name} need a vocabulary axis")
+    vocab = x.shape[-1]
+    if vocab == 0:
+        raise ValueError(f"{name} need at least one element per row")
+    if x.is_contiguous():
+        return x.numel() // vocab, vocab, vocab
+    if x.dim() == 2 and x.stride(1) == 1 and (x.stride(0) >= vocab or x.shape[0] <= 1):
+        return x.shape[0], vocab, max(x.stride(0), vocab)
+    raise ValueError(f"{name} must be contiguous, or 2-D with contiguous rows")
+
+
+def _score_args(logits: torch.Tensor, tokens: torch.Tensor):
+    dev = _check_device(logits, tokens)
+    code = _dtype_code(logits)
+    n, vocab, stride = _logit_rows("logits", logits)
+    if tokens.shape != logits.shape[:-1]:
+        raise ValueError("tokens must be [*logits.shape[:-1]]")
+    return dev, code, n, vocab, stride, _ids(tokens)
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0) -> TokenLogProbs:
+    """Log probability of one token per row of ``logits`` [..., vocab], the
+    entropy of the row and, with ``top_k`` (up to 32), its most likely tokens
+    with their log probabilities, in one pass over the logits: descending, equal
+    ones by ascending id.  Logits of -infinity (a mask) have probability 0; a
+    row with a NaN or +infinity, or of -infinity alone, gives NaN.  Token -100
+    (a row to ignore) gives 0; another one outside [0, vocab) gives NaN and sets
+    ``_lib.DEVERR_TOKEN_RANGE`` (``ops.device_errors``)."""
+    dev, code, n, vocab, stride, tokens = _score_args(logits, tokens)
+    if not 0 <= top_k <= min(MAX_TOP, vocab):
+        raise ValueError(f"top_k {top_k} outside [0, {min(MAX_TOP, vocab)}]")
+    shape = tuple(tokens.shape)
+    r = TokenLogProbs(_empty(shape, torch.float32, dev), _empty(shape, torch.float32, dev),
+                      _empty(shape + (2,), torch.float32, dev), None, None)
+    if top_k:
+        r.top_ids = _empty(shape + (top_k,), torch.int64, dev)
+        r.top_logprobs = _empty(shape + (top_k,), torch.float32, dev)
+    _lib.launch(_lib.load().esa_token_logprobs_forward, dev, code, tokens.element_size(), n, vocab,
+                stride, logits.data_ptr(), tokens.data_ptr(), top_k, r.logprobs.data_ptr(),
+                r.entropy.data_ptr(), r.stats.data_ptr(), _lib.ptr(r.top_ids),
+                _lib.ptr(r.top_logprobs))
+    return r
+
+
+def token_logprobs_backward(logits: torch.Tensor, tokens: torch.Tensor, scores: TokenLogProbs,
+                            dlogprobs: torch.Tensor | None, dentropy: torch.Tensor | None = None,
+                            out: torch.Tensor | None = None) -> torch.Tensor:
+    """d logits from the gradients (float32 [...]; None = zeros) of the
+    ``logprobs`` and ``entropy`` that :func:`token_logprobs` gave as ``scores``
+    for the same logits and tokens.  The alternatives have no gradient.  ``out``
+    receives the result (``logits`` itself for in place)."""
+    dev, code, n, vocab, stride, tokens = _score_args(logits, tokens)
+    shape = tokens.shape
+    for name, t, want in (("scores.stats", scores.stats, shape + (2,)),
+                          ("scores.entropy", scores.entropy, shape),
+                          ("dlogprobs", dlogprobs, shape), ("dentropy", dentropy, shape)):
+        if t is not None and (t.dtype != torch.float32 or t.shape != want or t.device != dev):
+            raise ValueError(f"{name} must be float32 [{', '.join(map(str, want))}] on {dev}")
+    stats, entropy = scores.stats.contiguous(), scores.entropy.contiguous()
+    dlogprobs = None if dlogprobs is None else dlogprobs.contiguous()
+    dentropy = None if dentropy is None else dentropy.contiguous()
+    if out is None:
+        out = _empty(tuple(logits.shape), logits.dtype, dev)
+    elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != dev:
+        raise ValueError("out must match logits")
+    out_stride = _logit_rows("out", out)[2]
+    _lib.launch(_lib.load().esa_token_logprobs_backward, dev, code, tokens.element_size(), n, vocab,
+                stride, logits.data_ptr(), tokens.data_ptr(), stats.data_ptr(), entropy.data_ptr(),
+                _lib.ptr(dlogprobs), _lib.ptr(dentropy), out_stride, out.data_ptr())
+    return out
+
+
+# ---------------------------------------------------------------------------
+# Weights in 4 bits
+# ---------------------------------------------------------------------------
+WEIGHT4_GROUPS = (32, 64, 128)
+# Up to this many rows linear4 reads the codes; beyond, a product with the
+# decoded weight is faster.
+LINEAR4_ROWS = 64
+
+
+@dataclass(eq=False)
+class PackedWeight4:
+    """A weight [n, k] in 4 bits: ``codes`` uint8 in the order of the product,
+    ``scales`` bfloat16 [ceil(n / 16), ceil(k / group), 16], ``shape`` (n, k) and
+    ``dtype`` those of the weight it was made from."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+    shape: tuple
+    group: int
+    dtype: torch.dtype
+
+    def nbytes(self) -> int:
+        return self.codes.numel() + 2 * self.scales.numel()
+
+
+def quantize_weight4(weight: torch.Tensor, group: int = 128) -> PackedWeight4:
+    """``weight`` [n, k] (a projection's, rows of outputs) in 4 bits: even steps
+    of max|w| / 7 within ``group`` (32, 64 or 128) consecutive inputs of a row,
+    the step a bfloat16.  A group with an infinity or a NaN decodes to NaN."""
+    dev = _check_device(weight)
+    if weight.dim() != 2:
+        raise ValueError("weight must be [n, k]")
+    n, k = weight.shape
+    _rows(weight, k)
+    if n == 0:
+        raise ValueError("weight needs at least one row")
+    if group not in WEIGHT4_GROUPS:
+        raise ValueError(f"group must be one of {WEIGHT4_GROUPS}")
+    code = _dtype_code(weight)
+    lib = _lib.load()
+    p = PackedWeight4(_empty((lib.esa_weight4_codes_size(n, k),), torch.uint8, dev),
+                      _empty((-(-n // 16), -(-k // group), 16), torch.bfloat16, dev), (n, k), group,
+                      weight.dtype)
+    _lib.launch(lib.esa_quantize_weight4, dev, code, n, k, group, weight.data_ptr(),
+                p.codes.data_ptr(), p.scales.data_ptr())
+    return p
+
+
+def _check_weight4(p: PackedWeight4) -> tuple:
+    n, k = p.shape
+    if (p.group not in WEIGHT4_GROUPS or p.codes.dtype != torch.uint8
+            or p.codes.numel() != -(-n // 16) * -(-k // 64) * 512
+            or p.scales.dtype != torch.bfloat16
+            or p.scales.shape != (-(-n // 16), -(-k // p.group), 16)):
+        raise ValueError("PackedWeight4: codes, scales, shape and group do not fit together")
+    if not p.codes.is_contiguous() or not p.scales.is_contiguous():
+        raise ValueError("PackedWeight4: codes and scales must be contiguous")
+    return n, k
+
+
+def dequantize_weight4(packed: PackedWeight4, dtype: torch.dtype | None = None) -> torch.Tensor:
+    """The weight [n, k] that the codes stand for, in ``dtype`` (default: the
+    dtype it was made from)."""
+    n, k = _check_weight4(packed)
+    dev = _check_device(packed.codes, packed.scales)
+    w = _empty((n, k), dtype or packed.dtype, dev)
+    _lib.launch(_lib.load().esa_dequantize_weight4, dev, _dtype_code(w), n, k, packed.group,
+                packed.codes.data_ptr(), packed.scales.data_ptr(), w.data_ptr())
+    return w
+
+
+def linear4(x: torch.Tensor, packed: PackedWeight4) -> torch.Tensor:
+    """x [..., k] times the transposed weight: [..., n].  Exact products of x and
+    the codes, float32 sums, rounded once.  Made for few rows (decoding: up to
+    ``LINEAR4_ROWS``); it takes any number."""
+    n, k = _check_weight4(packed)
+    dev = _check_device(x, packed.codes, packed.scales)
+    shape = _shape(x)
+    rows = _rows(x, k)
+    code = _dtype_code(x)
+    y = _empty(shape[:-1] + (n,), x.dtype, dev)
+    _lib.launch(_lib.load().esa_linear4, dev, code, rows, n, k, packed.group, x.data_ptr(),
+                packed.codes.data_ptr(), packed.scales.data_ptr(), y.data_ptr())
+    return y

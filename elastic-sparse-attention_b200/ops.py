@@ -272,3 +272,56 @@ def copy_rows(dst: torch.Tensor, src: torch.Tensor) -> torch.Tensor:
         _lib.check(_lib.load().esa_copy_rows(ctypes.byref(r), _lib.stream_handle(dev)),
                    "esa_copy_rows")
     return dst
+
+
+def _span_args(batch: int, start, counts, dev: torch.device) -> tuple:
+    """(start tensor or None, start value, counts tensor or None) of a call on
+    rows start[b] + l, l < counts[b]: device int64 [batch] tensors, or one
+    non-negative int for all sequences."""
+    def per_sequence(name, t):
+        if t.shape != (batch,):
+            raise ValueError(f"{name} must be [batch]")
+        if t.dtype != torch.int64 or t.device != dev:
+            t = t.to(device=dev, dtype=torch.int64)
+        return t.contiguous()
+
+    if counts is not None:
+        counts = per_sequence("counts", counts)
+    if isinstance(start, torch.Tensor):
+        return per_sequence("start", start), 0, counts
+    if start < 0:
+        raise ValueError(f"start {start} is negative")
+    return None, int(start), counts
+
+
+def forward_packed(q: torch.Tensor, cache, spec: PatternSpec, scale: float, start, counts=None,
+                   out: torch.Tensor | None = None):
+    """Elastic attention of q [B, Hq, L, D] over a :class:`~.cache.PackedKVCache`: row l of
+    sequence b attends, at position start[b] + l, to the cached rows that
+    :func:`forward` would take there (``cache_position``).  Returns (o
+    [B, Hq, L, D] as a view of a [B, L, Hq, D] buffer, lse float32 [B, Hq, L] base
+    2).  Rows l >= counts[b] are padding: zeros and -infinity; so is a row whose
+    position is beyond the cache, which also sets
+    ``_lib.DEVERR_QUERY_RANGE``."""
+    dev = _check_device(q, cache.codes)
+    if q.dim() != 4:
+        raise ValueError("q must be [batch, num_heads, L, head_dim]")
+    B, Hq, L, D = q.shape
+    if B != cache.batch or D != cache.head_dim or Hq % cache.num_kv_heads or Hq == 0:
+        raise ValueError(f"q {list(q.shape)} does not fit a cache of batch {cache.batch}, "
+                         f"{cache.num_kv_heads} heads of {cache.head_dim}")
+    if q.dtype not in _lib.DTYPES:
+        raise TypeError(f"unsupported dtype {q.dtype}")
+    if out is None:
+        out = torch.empty_strided((B, Hq, L, D), (L * Hq * D, D, Hq * D, 1), dtype=q.dtype,
+                                  device=dev)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev:
+        raise ValueError("out must match q")
+    start, start0, counts = _span_args(B, start, counts, dev)
+    lse = torch.empty((B, Hq, L), dtype=torch.float32, device=dev)
+    _lib.launch(_lib.load().esa_cache4_forward, dev, _lib.DTYPES[q.dtype],
+                ctypes.byref(cache.struct()), Hq, L, spec.attention_length, spec.layer_idx,
+                spec.num_hidden_layers, spec.pattern_heads, spec.head_offset, scale,
+                _lib.tensor4(q), _lib.ptr(start), start0, _lib.ptr(counts), _lib.tensor4(out),
+                lse.data_ptr())
+    return out, lse

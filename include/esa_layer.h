@@ -221,6 +221,107 @@ int esa_swiglu_unpack_backward(int32_t dtype, int32_t format, int64_t n_rows, in
                                const void* codes, const float* scales, const void* dout,
                                void* dgate_up, void* out_recomputed, void* stream);
 
+/*
+ * Log probabilities of given tokens.  logits: n_rows rows of vocab elements,
+ * row_stride elements apart (>= vocab; neither rows nor their ends need be
+ * aligned beyond an element).  tokens: device integers of id_bytes 4 or 8, one
+ * per row.  With m the row's maximum and S = sum of exp(x - m), float32:
+ *   logprobs[r] = x[token] - m - ln S
+ *   entropy[r]  = -sum of p ln p
+ *   stats[r]    = (m, ln S), what the gradient needs of the row
+ *   top_ids / top_logprobs [n_rows, top_k]: the top_k largest logits in
+ *       descending order (NaN above all, equal ones by ascending index) with
+ *       their log probabilities; top_k 0 .. 32, at most vocab; 0: may be NULL.
+ * Logits of -infinity have probability 0.  A row with a NaN or +infinity, or of
+ * -infinity alone, has no distribution: its log probability and entropy are
+ * NaN.  Token -100 gives 0 (a row to be ignored); another token outside
+ * [0, vocab) gives NaN and sets ESA_DEVERR_TOKEN_RANGE.  vocab < 2^31.
+ */
+int esa_token_logprobs_forward(int32_t dtype, int32_t id_bytes, int64_t n_rows, int64_t vocab,
+                               int64_t row_stride, const void* logits, const void* tokens,
+                               int32_t top_k, float* logprobs, float* entropy, float* stats,
+                               int64_t* top_ids, float* top_logprobs, void* stream);
+
+/*
+ * Gradient of esa_token_logprobs_forward's logprobs and entropy: with g =
+ * dlogprobs[r] (0 for token -100) and h = dentropy[r] (either may be NULL: 0)
+ *   dlogits[j] = g ([j = token] - p_j) - h p_j (ln p_j + entropy)
+ * rounded to dtype.  A row with g = h = 0 is cleared without being read.
+ * dlogits may be logits (then with the same stride); rows dlogits_stride apart.
+ */
+int esa_token_logprobs_backward(int32_t dtype, int32_t id_bytes, int64_t n_rows, int64_t vocab,
+                                int64_t row_stride, const void* logits, const void* tokens,
+                                const float* stats, const float* entropy, const float* dlogprobs,
+                                const float* dentropy, int64_t dlogits_stride, void* dlogits,
+                                void* stream);
+
+/*
+ * Weights in 4 bits.  Each group of `group` (32, 64 or 128) consecutive inputs of
+ * a row of weight [n, k] (the last may be shorter) has the scale s = the bfloat16
+ * nearest to f32(max|w| / 7), at least 2^-126; a code is the integer nearest to
+ * w / s (ties to even, the quotient taken exactly) and stands for code * s.  A
+ * group with an infinity or a NaN decodes to NaN.  codes: esa_weight4_codes_size(
+ * n, k) bytes in the order the product reads them; scales: bfloat16 [ceil(n / 16),
+ * ceil(k / group), 16].  k * element size is a multiple of 16 bytes.
+ */
+size_t esa_weight4_codes_size(int64_t n, int64_t k);
+int esa_quantize_weight4(int32_t dtype, int64_t n, int64_t k, int32_t group, const void* weight,
+                         void* codes, void* scales, void* stream);
+/* weight [n, k] = code * s, rounded to dtype (any dtype). */
+int esa_dequantize_weight4(int32_t dtype, int64_t n, int64_t k, int32_t group, const void* codes,
+                           const void* scales, void* weight, void* stream);
+/* y [n_rows, n] = x [n_rows, k] times the transposed weight: exact products of x
+ * and the codes, float32 sums, one rounding to dtype.  Made for few rows (up to
+ * some 64); it takes any number. */
+int esa_linear4(int32_t dtype, int64_t n_rows, int64_t n, int64_t k, int32_t group, const void* x,
+                const void* codes, const void* scales, void* y, void* stream);
+
+/*
+ * A key / value cache in 4 bits, groups of 32 along the head dimension, format as
+ * above.  codes: [batch, num_kv_heads, max_len, 2, head_dim / 2] bytes (keys, then
+ * values; the order within a row is the library's), scales: bfloat16 [batch,
+ * num_kv_heads, max_len, 2, head_dim / 32].  head_dim 64, 128 or 256; max_len at
+ * most 2^24.  Both 16-byte aligned.
+ *
+ * A call's rows l < seq_len of sequence b are positions start[b] + l (start0 + l
+ * where start is NULL) as long as l < counts[b] (NULL: all of them; below 0 as 0,
+ * above seq_len as seq_len); the rest is padding.
+ */
+typedef struct {
+  void* codes;
+  void* scales;
+  int32_t batch;
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  int32_t reserved;
+  int64_t max_len;
+} esa_cache4_t;
+
+/* k, v [batch, num_kv_heads, seq_len, head_dim] into the cache.  Padding is not
+ * written; a position outside [0, max_len) is not written and sets
+ * ESA_DEVERR_KV_RANGE. */
+int esa_cache4_write(int32_t dtype, const esa_cache4_t* cache, int64_t seq_len, esa_tensor_t k,
+                     esa_tensor_t v, const int64_t* start, int64_t start0, const int64_t* counts,
+                     void* stream);
+/* The rows that positions start + l hold, rounded to dtype, into k and v; zeros
+ * (and ESA_DEVERR_KV_RANGE) for a position outside the cache. */
+int esa_cache4_read(int32_t dtype, const esa_cache4_t* cache, int64_t seq_len, esa_tensor_t k,
+                    esa_tensor_t v, const int64_t* start, int64_t start0, void* stream);
+/*
+ * Elastic attention of q [batch, num_heads, q_len, head_dim] over the cache: row l
+ * of sequence b attends, as position start[b] + l, to the cached rows of its
+ * pattern (as esa_forward's query at that position).  o like q, lse float32
+ * [batch, num_heads, q_len] (base 2).  Scores, softmax and sums are float32; for
+ * 16-bit dtypes a softmax weight keeps 22 bits below the largest of 32 slots.  A
+ * padding row, and one whose position is outside the cache (which sets
+ * ESA_DEVERR_QUERY_RANGE), gets zeros and -infinity.
+ */
+int esa_cache4_forward(int32_t dtype, const esa_cache4_t* cache, int32_t num_heads, int64_t q_len,
+                       int32_t attn_length, int32_t layer_idx, int32_t num_hidden_layers,
+                       int32_t pattern_heads, int32_t head_offset, float scale, esa_tensor_t q,
+                       const int64_t* start, int64_t start0, const int64_t* counts, esa_tensor_t o,
+                       float* lse, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
