@@ -5,25 +5,29 @@
 // codes (one 128-byte line for D = 128) and 2 x D / 32 bf16 scales.  The codes
 // lie in the order in which the matrix instructions take them:
 //   key:   word t * (D / 32) + c of a row (t < 4, c < D / 32) holds the elements
-//          c * 32 + t * 8 + i, nibble i
+//          (c / 2) * 64 + (i & 1) * 32 + t * 8 + (c & 1) * 4 + i / 2, nibble i: the low
+//          nibbles of two words are one group, the high ones the next; the nibbles
+//          of keys are two's complement (the code, not code + 8)
 //   value: word g * (D / 64) + c (g < 8, c < D / 64) holds the elements
 //          c * 64 + i * 8 + g, nibble i
 //
 // Attention: every (query row, head) pair has w keys of its own, so nothing is
 // shared between pairs and the work is decoding 2 w D codes.  The products run
-// on mma.sync m16n8k16 (f16, float32 sums) with the codes as A and the query,
-// or the weights, in the columns of B that one vector leaves free otherwise:
-//   scores: A = 16 keys x 16 elements, B column = the query in f16 (its float32
-//           form in three parts), per group of 32 a sum of its own, times the scale
-//   output: A = 16 elements x 16 keys, B column = (group, part) with the weight
-//           times that group's scale in two or three f16 parts; an output element
+// on mma.sync m16n8k32 of 8-bit integers (exact, the same rate as f16 with twice
+// the elements) with the stored codes (n = code + 8, one AND per four) as A and
+// the query, or the softmax weights, as fixed-point numbers in the columns of B
+// that one vector leaves free otherwise, a column per digit of 8 bits:
+//   scores: A = 16 keys x 32 elements (one group), B column = digit of the query,
+//           four digits (30 bits below the query's largest element); the sum of a
+//           group times its scale in float32
+//   output: A = 16 elements x 32 keys, B column = (group, digit) of the weight
+//           times that group's scale, two digits (16 bits below the largest of
+//           the 32 keys) for 16-bit types and four for float32; an output element
 //           reads the columns of its group
-// A code is used as the f16 denormal that its nibble is (n 2^-24, or n 2^-20 one
-// nibble up, taken back in B or in the result), so decoding costs one AND per two
-// codes and no conversion; what the stored + 8 adds is 8 times the sum of the
-// column, formed by one product with a matrix of ones.  Queries and weights are
-// scaled by a power of two to just below 2^15 before they are cut to f16: 22 bits
-// (two parts) or 33 (three) below the largest.
+// Keys are signed bytes, 16 times the code; what the stored + 8 of the values adds
+// is taken out exactly by one product with a matrix of eights.
+// (f16 products with the nibbles as denormals need as little decoding, but lose
+// 9 bits when the tensor core aligns them: the output was 2^-11 off.)
 //
 // A warp takes 32 slots of a pair at a time, all their loads in flight, with an
 // online softmax in float32; with few pairs a pair's slots are split over the
@@ -102,7 +106,9 @@ template <int D> struct Unit {          // which 8 elements a thread owns
     b = (int)(bl / p.span.L);
     l = bl % p.span.L;
   }
-  __device__ __forceinline__ int key_word() const { return (part & 3) * (D / 32) + (part >> 2); }
+  // The words of keys hold 4 elements of this thread and 4 of the thread with the
+  // next group: two words, shared by two threads.
+  __device__ __forceinline__ int key_word() const { return (part & 3) * (D / 32) + (part >> 3) * 2; }
   __device__ __forceinline__ int value_word() const { return (part & 7) * (D / 64) + (part >> 3); }
 };
 
@@ -119,6 +125,31 @@ __device__ __forceinline__ uint32_t encode8(const float (&f)[8], float& s) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) w |= int4::code_of(f[e], s, inv) << (4 * e);
   return w;
+}
+
+// Two threads, four lanes apart, with the nibbles of their 8 elements <-> the first
+// (second) of the two key words that hold them.
+__device__ __forceinline__ uint32_t mix_keys(uint32_t w, int part) {
+  const uint32_t o = __shfl_xor_sync(0xffffffffu, w, 4);
+  const uint32_t a = part & 4 ? o : w, b = part & 4 ? w : o;      // the lower group, the higher
+  // the first word takes nibbles 0 .. 3 of both, the second 4 .. 7
+  const uint32_t x = part & 4 ? a >> 16 : a & 0xffffu, y = part & 4 ? b >> 16 : b & 0xffffu;
+  auto spread = [](uint32_t v) {                                  // nibbles to bytes
+    v = (v | v << 8) & 0x00ff00ffu;
+    return (v | v << 4) & 0x0f0f0f0fu;
+  };
+  return spread(x) | spread(y) << 4;
+}
+__device__ __forceinline__ uint32_t unmix_keys(uint32_t w, int part) {
+  const uint32_t o = __shfl_xor_sync(0xffffffffu, w, 4);
+  const uint32_t a = part & 4 ? o : w, b = part & 4 ? w : o;      // the first word, the second
+  auto gather = [](uint32_t v) {                                  // low nibbles of bytes together
+    v &= 0x0f0f0f0fu;
+    v = (v | v >> 4) & 0x00ff00ffu;
+    return (v | v >> 8) & 0xffffu;
+  };
+  const int s = part & 4 ? 4 : 0;
+  return gather(a >> s) | gather(b >> s) << 16;
 }
 
 template <typename T>
@@ -143,13 +174,13 @@ write_kernel(const RowParams<T> p) {
   const bool go = in && pos >= 0;
   float f[8], sk, sv;
   load8<T>(p.k, e.b, e.h, e.l, e.part, go, f);
-  const uint32_t kw = encode8(f, sk);
+  const uint32_t kw = mix_keys(encode8(f, sk), e.part) ^ 0x88888888u;
   load8<T>(p.v, e.b, e.h, e.l, e.part, go, f);
   const uint32_t vw = transpose8(encode8(f, sv), e.part & 7);
   if (!go) return;
   const int64_t row = ((int64_t)e.b * p.c.Hkv + e.h) * p.c.S + pos;
   uint32_t* codes = reinterpret_cast<uint32_t*>(p.c.codes + row * D);
-  codes[e.key_word()] = kw;
+  codes[e.key_word() + (e.part >> 2 & 1)] = kw;
   codes[D / 8 + e.value_word()] = vw;
   if ((e.part & 3) == 0) {
     __nv_bfloat16* s = p.c.scales + row * (2 * D / kGroup) + (e.part >> 2);
@@ -180,17 +211,18 @@ read_kernel(const RowParams<T> p) {
   const int64_t pos = p.span.position(e.b, e.l, p.c.S);
   const bool go = in && pos >= 0;
   if (pos == -2 && in && p.err) atomicOr(p.err, kErrKvRange);
-  uint32_t kw = 0x88888888u, vw = kw;
+  uint32_t kw = 0u, vw = 0x88888888u;
   float sk = 0.f, sv = 0.f;
   if (go) {
     const int64_t row = ((int64_t)e.b * p.c.Hkv + e.h) * p.c.S + pos;
     const uint32_t* codes = reinterpret_cast<const uint32_t*>(p.c.codes + row * D);
-    kw = __ldg(codes + e.key_word());
+    kw = __ldg(codes + e.key_word() + (e.part >> 2 & 1));
     vw = __ldg(codes + D / 8 + e.value_word());
     const __nv_bfloat16* s = p.c.scales + row * (2 * D / kGroup) + (e.part >> 2);
     sk = __bfloat162float(s[0]);
     sv = __bfloat162float(s[D / kGroup]);
   }
+  kw = unmix_keys(kw, e.part) ^ 0x88888888u;
   vw = transpose8(vw, e.part & 7);
   if (!in) return;
   store8<T>(p.k, e.b, e.h, e.l, e.part, kw, sk);
@@ -200,41 +232,53 @@ read_kernel(const RowParams<T> p) {
 // ---------------------------------------------------------------------------
 // Attention.
 // ---------------------------------------------------------------------------
-__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
-                                    uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-      "{%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+// d = A B, m16n8k32 of 8-bit integers, both signed or both unsigned.  The
+// instructions that all lanes of a warp execute together are volatile: without it
+// the compiler may move one under a condition that only uses its result on some
+// lanes, where it waits for the others for good.
+template <bool SIGNED>
+__device__ __forceinline__ void mma(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                    const uint32_t (&b)[2]) {
+#define ESA_MMA(T)                                                                          \
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32." T "." T ".s32 {%0,%1,%2,%3}, "      \
+               "{%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"                                 \
+               : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])                             \
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b[0]), "r"(b[1]), "r"(0))
+  if constexpr (SIGNED) ESA_MMA("s8");
+  else ESA_MMA("u8");
+#undef ESA_MMA
 }
 
-// 2^e with x 2^e in [2^14, 2^15) for the float bits of x >= 0 (x = 0, or too
-// small for that: 2^126), and its inverse.
-__device__ __forceinline__ float lift(uint32_t bits, float& inverse) {
-  const int field = min(253, 14 + 254 - (int)(bits >> 23));
+// Largest of the warp's values (a NaN is above all): their bits in the order of
+// signed integers.
+__device__ __forceinline__ float max_of_warp(float x) {
+  const int b = __float_as_int(x);
+  const int m = __reduce_max_sync(0xffffffffu, b ^ ((b >> 31) & 0x7fffffff));
+  return __int_as_float(m ^ ((m >> 31) & 0x7fffffff));
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// 2^e with x 2^e in [2^TOP, 2^(TOP + 1)) for the float bits of x >= 0 (2^126 where x
+// is 0 or too small for that), and its inverse.
+template <int TOP> __device__ __forceinline__ float lift(uint32_t bits, float& inverse) {
+  const int field = min(253, TOP + 254 - (int)(bits >> 23));
   inverse = __uint_as_float((uint32_t)(254 - field) << 23);
   return __uint_as_float((uint32_t)field << 23);
 }
 
-__device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-// Part `part` of (lo, hi) in f16: what the parts before it leave, rounded.
-template <int PARTS>
-__device__ __forceinline__ uint32_t half_part(float lo, float hi, int part) {
-  uint32_t h = half2_bits(lo, hi);
-#pragma unroll
-  for (int i = 1; i < PARTS; ++i) {
-    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h));
-    if (part >= i) {
-      lo -= v.x;
-      hi -= v.y;
-      h = half2_bits(lo, hi);
-    }
-  }
-  return part < PARTS ? h : 0u;
+// Byte j of four words, in x[j].
+__device__ __forceinline__ void transpose_bytes(const uint32_t (&w)[4], uint32_t (&x)[4]) {
+  const uint32_t a = __byte_perm(w[0], w[1], 0x5140), b = __byte_perm(w[2], w[3], 0x5140);
+  const uint32_t c = __byte_perm(w[0], w[1], 0x7362), d = __byte_perm(w[2], w[3], 0x7362);
+  x[0] = __byte_perm(a, b, 0x5410);
+  x[1] = __byte_perm(a, b, 0x7632);
+  x[2] = __byte_perm(c, d, 0x5410);
+  x[3] = __byte_perm(c, d, 0x7632);
 }
 
 template <typename T> struct AttendParams {
@@ -242,27 +286,44 @@ template <typename T> struct AttendParams {
   Span span;
   Heads q, o;
   int Hq, G;                  // query heads, query heads per K/V head
-  int64_t pairs;              // B * L * Hq
-  int warps_per_pair;         // 1, 2, 4 or 8
+  unsigned rows;              // G * L: pairs of one K/V head
+  int warps_per_pair;         // 1, 2 or 4
+  int pairs_per_warp;         // one after the other; 1 where warps share a pair
   Pattern pat;
   float scale_log2;
   float* lse;                 // [B, Hq, L]
   int* err;
 };
 
-constexpr int kAttendWarps = 8;
+constexpr int kAttendWarps = 4;
 
-template <int N> __device__ __forceinline__ void load_words(const void* at, bool in, uint32_t (&w)[N]) {
+// row_window with inv_w = f32(1 / w): the quotient of two integers is rounded
+// correctly by one step from q = n inv_w with the exact remainder n - q w (Markstein,
+// IBM J. Res. Dev. 34, 1990), without the branches of a general division.
+__device__ __forceinline__ RowWin row_window_inv(const Pattern& P, int pos, float inv_w) {
+  const int end = pos > P.w - 1 ? pos : P.w - 1;
+  const float E = __int2float_rn(end + 1);
+  const float pd = __fadd_rn(P.c, __fmul_rn(E, P.a));
+  const float s = fmaxf(rintf(__fsub_rn(E, pd)), 0.f);
+  RowWin r;
+  r.st = __float2int_rz(s);
+  const float n = __int2float_rn(end + 1 - r.st), w = __int2float_rn(P.w);
+  const float q = __fmul_rn(n, inv_w);
+  r.sp = fmaf(fmaf(-w, q, n), inv_w, q);
+  return r;
+}
+
+template <int N> __device__ __forceinline__ void load_words(const void* at, uint32_t (&w)[N]) {
   const uint32_t* p = static_cast<const uint32_t*>(at);
   if constexpr (N == 1) {
-    w[0] = in ? __ldg(p) : 0u;
+    w[0] = __ldg(p);
   } else if constexpr (N == 2) {
-    const uint2 v = in ? __ldg(reinterpret_cast<const uint2*>(p)) : make_uint2(0, 0);
+    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
     w[0] = v.x; w[1] = v.y;
   } else {
 #pragma unroll
     for (int i = 0; i < N; i += 4) {
-      const uint4 v = in ? ldg16(p + i) : make_uint4(0, 0, 0, 0);
+      const uint4 v = ldg16(p + i);
       w[i] = v.x; w[i + 1] = v.y; w[i + 2] = v.z; w[i + 3] = v.w;
     }
   }
@@ -273,257 +334,350 @@ template <int N> __device__ __forceinline__ float scale_at(const uint32_t (&w)[N
   return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
 }
 
-constexpr uint32_t kEven = 0x000f000fu, kOdd = 0x00f000f0u;   // n 2^-24, n 2^-20 as f16
+// Nibbles as 8-bit numbers: the low ones n, the high ones 16 n, and what the + 8 of
+// a value's code is then.
+constexpr uint32_t kLow = 0x0f0f0f0fu, kHigh = 0xf0f0f0f0u;
+constexpr uint32_t kEight = 0x08080808u, kEightHigh = 0x80808080u;     // 8, 128
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kAttendWarps * 32, D == 256 ? 1 : 2)
+// SPLIT: the warps of a CTA share pairs, one pair at a time; else each warp has
+// pairs of its own, one after the other.
+template <typename T, int D, bool SPLIT>
+__global__ void __launch_bounds__(kAttendWarps * 32, D == 256 ? 2 : 5)
 attend_kernel(const AttendParams<T> p) {
   constexpr int NG = D / kGroup;                     // groups of a row
-  constexpr int QP = sizeof(T) == 4 ? 3 : 1;         // f16 parts of the query
-  constexpr int VP = sizeof(T) == 4 ? 3 : 2;         // f16 parts of a weight
-  constexpr int VC = VP == 3 ? 4 : 2;                // B columns of a group
+  constexpr int VC = sizeof(T) == 4 ? 4 : 2;         // digits (B columns) of a weight
   constexpr int GT = 8 / VC;                         // groups per set of 8 columns
   constexpr int NV = (NG + GT - 1) / GT;             // sets of columns
   constexpr int KW = D / 32, VW = D / 64;            // words per lane of a key / value row
   constexpr int MT = D / 16;                         // tiles of 16 output elements
   constexpr int E = Vec<T>::kElems;
+  constexpr int QS = NG * 8 + 8;                     // words of a digit's plane, offset by 8 banks
   __shared__ float s_ml[kAttendWarps][2];
-  __shared__ __align__(16) float s_out[kAttendWarps][D];
+  // query, then weights [group][digit][32 keys] in bytes, then output
+  constexpr int BUF = 4 * QS > D ? 4 * QS : D;
+  static_assert(NG * VC * 32 <= BUF * 4, "the digits of the weights fit the buffer");
+  __shared__ __align__(16) uint32_t s_buf[kAttendWarps][BUF];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
-  const int wpp = p.warps_per_pair, sub = warp % wpp;
-  // pairs in the order [B, Hkv, L, G]: neighbouring warps read neighbouring keys
-  const int64_t pair = (int64_t)blockIdx.x * (kAttendWarps / wpp) + warp / wpp;
-  const bool live = pair < p.pairs;
-  const int64_t pr = live ? pair : p.pairs - 1;
-  const int64_t rest = pr / p.G, bh = rest / p.span.L;
-  const int64_t l = rest % p.span.L;
-  const int hkv = (int)(bh % p.c.Hkv), b = (int)(bh / p.c.Hkv);
-  const int h = hkv * p.G + (int)(pr % p.G);
-  const int pos = live ? (int)p.span.position(b, l, p.c.S) : -1;   // < 2^24
-  if (pos == -2 && sub == 0 && lane == 0 && p.err) atomicOr(p.err, kErrQueryRange);
+  const int wpp = SPLIT ? p.warps_per_pair : 1, sub = SPLIT ? warp & (wpp - 1) : 0;
+  // grid = (pairs of a K/V head, B * Hkv); pairs in the order [G, L]: neighbouring
+  // rows of a head attend to the same or neighbouring keys
+  const unsigned L = (unsigned)p.span.L;
+  const unsigned step = SPLIT ? (unsigned)(kAttendWarps / wpp) : kAttendWarps;   // pairs a CTA has at a time
+  unsigned pair = blockIdx.x * step * (unsigned)p.pairs_per_warp + (unsigned)(SPLIT ? warp / wpp : warp);
+  const int b = (int)(blockIdx.y / (unsigned)p.c.Hkv);
+  int h = (int)(blockIdx.y % (unsigned)p.c.Hkv) * p.G + (int)(pair / L);
+  unsigned l = pair % L;
+  const int64_t begin = p.span.begin(b), count = p.span.count(b);
+  const int64_t row0 = (int64_t)blockIdx.y * p.c.S;
+  // rows of this K/V head lie within 2^32 bytes: max_len <= 2^24, D <= 256
+  const uint8_t* codes = p.c.codes + row0 * D;
+  const uint8_t* scales = reinterpret_cast<const uint8_t*>(p.c.scales + row0 * (2 * NG));
+  const T* q = static_cast<const T*>(p.q.data) + b * p.q.sb;
+  constexpr int SETS = (NG * 8 + 31) / 32;           // 4 elements of the query per lane and set
+  using QV = typename std::conditional<E == 4, uint4, uint2>::type;
+  QV qv[SETS];
+  auto load_query = [&](bool in) {
+#pragma unroll
+    for (int i = 0; i < SETS; ++i) {
+      const int set = i * 32 + lane;
+      qv[i] = QV{};
+      if (in && (NG * 8 % 32 == 0 || set < NG * 8))
+        qv[i] = __ldg(reinterpret_cast<const QV*>(q + h * p.q.sh + (int64_t)l * p.q.ss + set * 4));
+    }
+  };
+  load_query(pair < p.rows);
+  float ht = head_weight(p.pat, h), omt = __fsub_rn(1.f, ht);
+  const float inv_w = __frcp_rn((float)p.pat.w);
 
-  // The query as B columns 0 .. QP - 1: this lane's 8 elements of each group, as
-  // the nibbles of a word pair up: (0, 4), (1, 5) / 16, (2, 6), (3, 7) / 16.
-  uint32_t qb[NG][4];
-  float qoff[NG];                                    // what the codes' + 8 adds
+  for (int it = 0; it < p.pairs_per_warp; ++it) {
+  const bool live = pair < p.rows;
+  if (!SPLIT && !live) break;
+  const int my_h = h;
+  const unsigned my_l = l;
+  const float my_ht = ht, my_omt = omt;
+  // < 2^24; padding and positions outside the cache have no slots
+  const bool inside = begin >= 0 && begin < p.c.S - (int64_t)l;
+  const int pos = live && inside && (int64_t)l < count ? (int)(begin + l) : -1;
+  if (live && !inside && (int64_t)l < count && sub == 0 && lane == 0 && p.err)
+    atomicOr(p.err, kErrQueryRange);
+
+  // The query in fixed point, as columns of balanced digits -128 .. 127.  Four
+  // neighbouring elements of one lane make a B word; shared memory brings the words
+  // of digit g to lanes 4 g + t.
+  uint32_t qb[NG][2];
   float unit;                                        // of the scores
   {
-    float f[NG][8];
+    float f[SETS][4];
     uint32_t top = 0;
-    const T* q = static_cast<const T*>(p.q.data) + b * p.q.sb + h * p.q.sh + l * p.q.ss + t * 8;
 #pragma unroll
-    for (int c = 0; c < NG; ++c) {
+    for (int i = 0; i < SETS; ++i) {
+      if constexpr (E == 4) {
+        Vec<T>::to_float(qv[i], f[i]);
+      } else {
+        float w[8];
+        Vec<T>::to_float(make_uint4(qv[i].x, qv[i].y, 0u, 0u), w);
 #pragma unroll
-      for (int i = 0; i < 8; i += E) Vec<T>::to_float(ldg16(q + c * kGroup + i), f[c] + i);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) top = max(top, int4::abs_bits(f[c][i]));
-    }
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    float down;
-    const float up = lift(min(top, 0x7f7fffffu), down);
-    unit = down * p.scale_log2;
-#pragma unroll
-    for (int c = 0; c < NG; ++c) {
-      float s[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float f16 = i & 1 ? up * 0.0625f : up;
-        qb[c][i] = half_part<QP>(f[c][i] * f16, f[c][i + 4] * f16, g);
+        for (int k = 0; k < 4; ++k) f[i][k] = w[k];
       }
-      // 1 and 16 in f16: the sum of the group
-      mma(s, 0x3c003c00u, 0x3c003c00u, 0x4c004c00u, 0x4c004c00u, qb[c][0], qb[c][1]);
-      mma(s, 0x3c003c00u, 0x3c003c00u, 0x4c004c00u, 0x4c004c00u, qb[c][2], qb[c][3]);
-      qoff[c] = (s[0] + s[1]) * 0x1p-21f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) top = max(top, int4::abs_bits(f[i][k]));
     }
+    // the next pair's query is on its way while this one is worked on
+    pair += step;
+    l += step;
+    if (l >= L) {
+      do {
+        l -= L;
+        ++h;
+      } while (l >= L);
+      ht = head_weight(p.pat, h);
+      omt = __fsub_rn(1.f, ht);
+    }
+    if (it + 1 < p.pairs_per_warp) load_query(pair < p.rows);
+    top = __reduce_max_sync(0xffffffffu, top);
+    float down;
+    const float up = lift<29>(min(top, 0x7f7fffffu), down);
+    // an infinity or a NaN in the query: no score is a number
+    unit = top >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : down * 0.0625f * p.scale_log2;
+#pragma unroll
+    for (int i = 0; i < SETS; ++i) {
+      // digits are the bytes of x + 0x80808080, less 0x80 each
+      uint32_t d[4], x[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) d[k] = (uint32_t)__float2int_rn(f[i][k] * up) + 0x80808080u;
+      transpose_bytes(d, x);
+      if (NG * 8 % 32 == 0 || i * 32 + lane < NG * 8)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s_buf[warp][k * QS + i * 32 + lane] = x[k] ^ 0x80808080u;
+    }
+    __syncwarp();
+#pragma unroll
+    for (int c = 0; c < NG; ++c) {
+      uint2 v = make_uint2(0, 0);                    // no digits in columns 4 .. 7
+      if (g < 4) v = *reinterpret_cast<const uint2*>(&s_buf[warp][g * QS + c * 8 + t * 2]);
+      qb[c][0] = v.x;
+      qb[c][1] = v.y;
+    }
+    __syncwarp();                                    // the buffer is used again
   }
+  const float digit_unit = t == 1 ? 65536.f : 1.f;   // t = 0 has digits 0 and 1, t = 1 the others
 
-  const RowWin rw = row_window(p.pat, pos < 0 ? 0 : pos);
-  const float ht = head_weight(p.pat, h), omt = __fsub_rn(1.f, ht);
-  const int64_t row0 = ((int64_t)b * p.c.Hkv + hkv) * p.c.S;
-  const uint8_t* codes = p.c.codes + row0 * D;
-  const __nv_bfloat16* scales = p.c.scales + row0 * (2 * NG);
+  const RowWin rw = row_window_inv(p.pat, pos < 0 ? 0 : pos, inv_w);
   const int nchunks = pos < 0 ? 0 : (p.pat.w + 31) >> 5;
 
   // this lane's columns in the output products: column set nv holds group
-  // nv * GT + g / VC, part g % VC; results in columns 2 t and 2 t + 1
+  // nv * GT + g / VC, digit g % VC; results in columns 2 t and 2 t + 1
   const int owner = VC == 2 ? t : t >> 1;
   float total[NV][2][2];
+  uint32_t nans = 0;                                 // groups of values with a NaN
 #pragma unroll
   for (int i = 0; i < NV * 4; ++i) (&total[0][0][0])[i] = 0.f;
-  float m_run = -INFINITY, l_run = 0.f;
+  float m_run = -INFINITY, l_lane = 0.f;
 
   for (int chunk = sub; chunk < nchunks; chunk += wpp) {
-    const int slot = chunk * 32 + lane;
-    int myrow = -1;
-    if (slot < p.pat.w) {
-      const int raw = raw_index(rw, slot, ht, omt);
-      if (raw <= pos && raw >= 0) myrow = raw;       // causal
-    }
-    if (__ballot_sync(0xffffffffu, myrow >= 0) == 0) continue;
+    // lane (g, t) looks after slot t * 8 + g
+    const int slot = chunk * 32 + t * 8 + g;
+    const int raw = raw_index(rw, slot, my_ht, my_omt);
+    const bool valid = slot < p.pat.w && raw <= pos && raw >= 0;   // causal
+    const uint32_t any = __ballot_sync(0xffffffffu, valid);
+    if (any == 0) continue;
+    // masked slots read the row of one that is not: what they hold is in use anyway
+    const int safe = __shfl_sync(0xffffffffu, raw, __ffs(any) - 1);
+    const int myrow = valid ? raw : safe;
     // ---- all loads of the 32 slots ----
-    uint32_t kw[2][2][KW], ks[2][2][NG / 2], vw[2][4][VW];
-    float vs[2][4][NV];
+    uint32_t kw[4][KW], sw[NG], vw[8][VW];           // sw: the own key's scales, its value's scales
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int k = 0; k < 4; ++k) {                    // keys k * 8 + g
+      const uint32_t row = (uint32_t)__shfl_sync(0xffffffffu, myrow, (lane & 28) + k);
+      load_words<KW>(codes + (row * (uint32_t)D + t * (KW * 4)), kw[k]);
+    }
+    load_words<NG>(scales + (uint32_t)myrow * (uint32_t)(NG * 4), sw);
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int row = __shfl_sync(0xffffffffu, myrow, i * 16 + r * 8 + g);
-        load_words<KW>(codes + (int64_t)row * D + t * (KW * 4), row >= 0, kw[i][r]);
-        load_words<NG / 2>(scales + (int64_t)row * (2 * NG), row >= 0, ks[i][r]);
-      }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int row = __shfl_sync(0xffffffffu, myrow, i * 16 + 2 * t + (k & 1) + (k >> 1) * 8);
-        load_words<VW>(codes + (int64_t)row * D + D / 2 + g * (VW * 4), row >= 0, vw[i][k]);
-#pragma unroll
-        for (int nv = 0; nv < NV; ++nv) {
-          const int gi = nv * GT + g / VC;
-          vs[i][k][nv] = row >= 0 && gi < NG
-                             ? __bfloat162float(scales[(int64_t)row * (2 * NG) + NG + gi]) : 0.f;
-        }
-      }
+    for (int k = 0; k < 8; ++k) {                    // keys t * 8 + k
+      const uint32_t row = (uint32_t)__shfl_sync(0xffffffffu, myrow, k * 4 + t);
+      load_words<VW>(codes + (row * (uint32_t)D + D / 2 + g * (VW * 4)), vw[k]);
+    }
     // ---- scores ----
-    float sc[2][2];
+    float sc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      sc[i][0] = sc[i][1] = 0.f;
+    for (int c = 0; c < NG; c += 2) {
+      uint32_t f[4];                                 // scales of groups c and c + 1 of keys k * 8 + g
+#pragma unroll
+      for (int k = 0; k < 4; ++k) f[k] = __shfl_sync(0xffffffffu, sw[c / 2], (lane & 28) + k);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          // 16 times the codes as signed bytes
+          int a[4];
+          const int up = u ? 1 : 16;
+          mma<true>(a, kw[2 * i][c] * up & kHigh, kw[2 * i + 1][c] * up & kHigh,
+                    kw[2 * i][c + 1] * up & kHigh, kw[2 * i + 1][c + 1] * up & kHigh, qb[c + u]);
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const uint32_t w = f[2 * i + r];
+            sc[2 * i + r] = fmaf(__uint_as_float(u ? w & 0xffff0000u : w << 16),
+                                 (float)(a[2 * r] + a[2 * r + 1] * 256), sc[2 * i + r]);
+          }
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) sc[k] *= digit_unit;
+    transpose_reduce<4>(sc, lane);                   // lane (g, t): slot t * 8 + g
+    const float s = valid ? sc[0] * unit : -INFINITY;
+    const float mn = fmaxf(m_run, max_of_warp(s));
+    const float ref = mn == -INFINITY ? 0.f : mn;
+    const float corr = ex2(m_run - ref);              // 0 on the first chunk
+    const float e = ex2(s - ref);
+    l_lane = fmaf(l_lane, corr, e);
+    m_run = mn;
+    // ---- weight times the scales of the own key's value, in fixed point ----
+    float vs[NG];
+    uint32_t top = 0;
+#pragma unroll
+    for (int c = 0; c < NG; ++c) {
+      const uint32_t w = sw[(NG + c) / 2];
+      vs[c] = e * __uint_as_float(c & 1 ? w & 0xffff0000u : w << 16);
+      // a masked slot's scale is one that is in use, so 0 times it is 0 or a NaN that
+      // the key in use brings anyway
+      top = max(top, __float_as_uint(vs[c]));         // none is negative
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (top >= 0x7f800000u) {       // a group with a NaN: its elements come out as NaN
+      top = 0;
 #pragma unroll
       for (int c = 0; c < NG; ++c) {
-        float a[4] = {0.f, 0.f, 0.f, 0.f};
-        const uint32_t x = kw[i][0][c], y = kw[i][1][c], x8 = x >> 8, y8 = y >> 8;
-        mma(a, x & kEven, y & kEven, x & kOdd, y & kOdd, qb[c][0], qb[c][1]);
-        mma(a, x8 & kEven, y8 & kEven, x8 & kOdd, y8 & kOdd, qb[c][2], qb[c][3]);
-        sc[i][0] = fmaf(scale_at(ks[i][0], c), a[0] + a[1] - qoff[c], sc[i][0]);
-        sc[i][1] = fmaf(scale_at(ks[i][1], c), a[2] + a[3] - qoff[c], sc[i][1]);
+        const bool bad = vs[c] != vs[c];
+        if (bad) vs[c] = 0.f;
+        top = max(top, __float_as_uint(vs[c]));
+        if (__any_sync(0xffffffffu, bad)) nans |= 1u << c;
       }
-      if constexpr (QP == 3) {                        // the third part is with lane t = 1
-        sc[i][0] += __shfl_xor_sync(0xffffffffu, sc[i][0], 1);
-        sc[i][1] += __shfl_xor_sync(0xffffffffu, sc[i][1], 1);
-      }
+      top = __reduce_max_sync(0xffffffffu, top);
     }
-    // lanes t = 0 hold slots g and g + 8 of each 16: one slot per lane
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const float v = __shfl_sync(0xffffffffu, sc[i][r], (lane & 7) * 4);
-        if ((lane >> 3) == i * 2 + r) s = v;
-      }
-    s = myrow >= 0 ? s * 0x1p24f * unit : -INFINITY;
-    const float mn = fmaxf(m_run, warp_max(s));
-    const float ref = mn == -INFINITY ? 0.f : mn;
-    const float corr = exp2f(m_run - ref);            // 0 on the first chunk
-    const float e = exp2f(s - ref);
-    l_run = l_run * corr + warp_sum(e);
-    m_run = mn;
-    // ---- weighted values ----
-    float top = 0.f;
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float w = __shfl_sync(0xffffffffu, e, i * 16 + 2 * t + (k & 1) + (k >> 1) * 8);
-#pragma unroll
-        for (int nv = 0; nv < NV; ++nv) {
-          vs[i][k][nv] *= w;
-          top = fmaxf(top, vs[i][k][nv]);             // passes over NaN
-        }
-      }
     float down;
-    const float up = lift(__reduce_max_sync(0xffffffffu, min(__float_as_uint(top), 0x7f7fffffu)), down);
-    float acc[MT][4], ones[NV][4];
+    float up = lift<VC == 4 ? 31 : 15>(top, down);
+    if constexpr (VC == 2) {        // below 65535 after the rounding, so two digits hold it
+      up *= 0.9999847412109375f;    // 1 - 2^-16
+      down *= 1.00001525902189f;
+    }
+    uint8_t* digits = reinterpret_cast<uint8_t*>(s_buf[warp]);
 #pragma unroll
-    for (int i = 0; i < MT * 4; ++i) (&acc[0][0])[i] = 0.f;
+    for (int c = 0; c < NG; ++c) {
+      uint32_t d;
+      // the product plus 2^23 has the rounded product as its low bits
+      if constexpr (VC == 2) d = __float_as_uint(fmaf(vs[c], up, 8388608.f));
+      else d = __float2uint_rn(vs[c] * up);
 #pragma unroll
-    for (int i = 0; i < NV * 4; ++i) (&ones[0][0])[i] = 0.f;
+      for (int i = 0; i < VC; ++i) digits[(c * VC + i) * 32 + t * 8 + g] = (uint8_t)(d >> (8 * i));
+    }
+    __syncwarp();
+    int acc[MT][4], eights[NV][4];
+    uint32_t vb[NV][2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      uint32_t vb[NV][2];
+    for (int nv = 0; nv < NV; ++nv) {
+      uint2 v = make_uint2(0, 0);
+      if (NG % GT == 0 || g < NG * VC)
+        v = *reinterpret_cast<const uint2*>(digits + (nv * 8 + g) * 32 + t * 8);
+      vb[nv][0] = v.x;
+      vb[nv][1] = v.y;
+      mma<false>(eights[nv], kEight, kEightHigh, kEight, kEightHigh, vb[nv]);
+    }
+    __syncwarp();
 #pragma unroll
-      for (int nv = 0; nv < NV; ++nv) {
-        vb[nv][0] = half_part<VP>(vs[i][0][nv] * up, vs[i][1][nv] * up, g % VC);
-        vb[nv][1] = half_part<VP>(vs[i][2][nv] * up, vs[i][3][nv] * up, g % VC);
-        mma(ones[nv], 0x00010001u, 0x00010001u, 0x00010001u, 0x00010001u, vb[nv][0], vb[nv][1]);
+    for (int c = 0; c < VW; ++c) {
+      uint32_t x[2][4];                               // byte j of four keys
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t w[4] = {vw[4 * i][c], vw[4 * i + 1][c], vw[4 * i + 2][c], vw[4 * i + 3][c]};
+        transpose_bytes(w, x[i]);
       }
 #pragma unroll
-      for (int c = 0; c < VW; ++c)
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {        // nibbles 0 .. 3, 4 .. 7: 32 elements, one group
-          const uint32_t sel = half ? 0x7632u : 0x5410u;
-          const uint32_t x = __byte_perm(vw[i][0][c], vw[i][1][c], sel), x8 = x >> 8;
-          const uint32_t y = __byte_perm(vw[i][2][c], vw[i][3][c], sel), y8 = y >> 8;
-          const int gr = 2 * c + half, nv = gr / GT;
-          mma(acc[2 * gr], x & kEven, x & kOdd, y & kEven, y & kOdd, vb[nv][0], vb[nv][1]);
-          mma(acc[2 * gr + 1], x8 & kEven, x8 & kOdd, y8 & kEven, y8 & kOdd, vb[nv][0], vb[nv][1]);
-        }
+      for (int j = 0; j < 4; ++j)
+        mma<false>(acc[4 * c + j], x[0][j] & kLow, x[0][j] & kHigh, x[1][j] & kLow,
+                          x[1][j] & kHigh, vb[(2 * c + j / 2) / GT]);
     }
     // the columns of this lane belong to one group of each set
 #pragma unroll
     for (int nv = 0; nv < NV; ++nv) {
-      const float off = 8.f * (ones[nv][0] + ones[nv][1]);
+      const int off = eights[nv][0] + eights[nv][1] * 256, off16 = eights[nv][2] + eights[nv][3] * 256;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        float lo = 0.f, hi = 0.f;
+        int lo = 0, hi = 0;
 #pragma unroll
         for (int o = 0; o < GT; ++o) {
-          const int gr = nv * GT + o;
-          if (gr < NG && owner == o) {
-            lo = acc[2 * (gr < NG ? gr : 0) + j][0] + acc[2 * (gr < NG ? gr : 0) + j][1];
-            hi = acc[2 * (gr < NG ? gr : 0) + j][2] + acc[2 * (gr < NG ? gr : 0) + j][3];
+          const int mt = 2 * (nv * GT + o) + j;
+          if (mt < MT) {
+            const int(&a)[4] = acc[mt < MT ? mt : 0];
+            lo = owner == o ? a[0] + a[1] * 256 : lo;
+            hi = owner == o ? a[2] + a[3] * 256 : hi;
           }
         }
-        total[nv][j][0] = fmaf(lo - off, down, total[nv][j][0] * corr);
-        total[nv][j][1] = fmaf(fmaf(hi, 0.0625f, -off), down, total[nv][j][1] * corr);
+        total[nv][j][0] = fmaf((float)(lo - off), down, total[nv][j][0] * corr);
+        total[nv][j][1] = fmaf((float)(hi - off16), down * 0.0625f, total[nv][j][1] * corr);
       }
     }
   }
 
   // ---- the warps of a pair ----
 #pragma unroll
-  for (int nv = 0; nv < NV; ++nv)
+  for (int nv = 0; nv < NV; ++nv) {
+    const bool bad = (nans >> (nv * GT + owner)) & 1u;
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        float v = total[nv][j][r] * 0x1p24f;
-        if constexpr (VC == 4) v += __shfl_xor_sync(0xffffffffu, v, 1);
+        float v = total[nv][j][r];
+        if constexpr (VC == 4)                        // digits 2 and 3 are with the odd lanes
+          v = fmaf(__shfl_xor_sync(0xffffffffu, v, 1), 65536.f, v);
+        if (bad) v = __uint_as_float(0x7fffffffu);
         const int gr = nv * GT + owner;
         if (gr < NG && (VC == 2 || (t & 1) == 0))
-          s_out[warp][gr * kGroup + j * 16 + r * 8 + g] = v;
+          s_buf[warp][gr * kGroup + j * 16 + r * 8 + g] = __float_as_uint(v);
       }
-  if (lane == 0) {
+  }
+  const float l_run = warp_sum(l_lane);
+  if (SPLIT && lane == 0) {
     s_ml[warp][0] = m_run;
     s_ml[warp][1] = l_run;
   }
-  if (wpp > 1) __syncthreads(); else __syncwarp();
-  if (sub != 0 || !live) return;
-  float mx = -INFINITY;
-  for (int i = 0; i < wpp; ++i) mx = fmaxf(mx, s_ml[warp + i][0]);
-  const float ref = mx == -INFINITY ? 0.f : mx;
-  float sum = 0.f;
+  if constexpr (SPLIT) __syncthreads(); else __syncwarp();
+  if (sub == 0 && live) {
+  float ref = m_run == -INFINITY ? 0.f : m_run, sum = l_run;
   constexpr int PL = D / 32;                          // elements per lane
   float out[PL];
+  if constexpr (SPLIT) {
+    float mx = -INFINITY;
+    for (int i = 0; i < wpp; ++i) mx = fmaxf(mx, s_ml[warp + i][0]);
+    ref = mx == -INFINITY ? 0.f : mx;
+    sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < PL; ++i) out[i] = 0.f;
-  for (int i = 0; i < wpp; ++i) {
-    const float f = exp2f(s_ml[warp + i][0] - ref);
-    sum = fmaf(s_ml[warp + i][1], f, sum);
+    for (int i = 0; i < PL; ++i) out[i] = 0.f;
+    for (int i = 0; i < wpp; ++i) {
+      const float f = ex2(s_ml[warp + i][0] - ref);
+      sum = fmaf(s_ml[warp + i][1], f, sum);
 #pragma unroll
-    for (int e = 0; e < PL; ++e) out[e] = fmaf(s_out[warp + i][lane * PL + e], f, out[e]);
+      for (int e = 0; e < PL; ++e)
+        out[e] = fmaf(__uint_as_float(s_buf[warp + i][lane * PL + e]), f, out[e]);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < PL; ++e) out[e] = __uint_as_float(s_buf[warp][lane * PL + e]);
   }
-  const float inv = sum != 0.f ? 1.f / sum : 0.f;
-  T* o = static_cast<T*>(const_cast<void*>(p.o.data)) + b * p.o.sb + h * p.o.sh + l * p.o.ss + lane * PL;
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(sum));
+  if (sum == 0.f) inv = 0.f;
+  T* o = static_cast<T*>(const_cast<void*>(p.o.data)) + b * p.o.sb + my_h * p.o.sh +
+         (int64_t)my_l * p.o.ss + lane * PL;
   struct alignas(PL * sizeof(T) < 16 ? PL * sizeof(T) : 16) Pack { T v[PL]; } pack;
 #pragma unroll
   for (int e = 0; e < PL; ++e) pack.v[e] = from_f32<T>(out[e] * inv);
   *reinterpret_cast<Pack*>(o) = pack;
-  if (lane == 0) p.lse[((int64_t)b * p.Hq + h) * p.span.L + l] = ref + log2f(sum);
+  if (lane == 0) p.lse[((int64_t)b * p.Hq + my_h) * p.span.L + my_l] = ref + log2f(sum);
+  }
+  __syncwarp();                                      // the buffer holds a query next
+  }
 }
 
 }  // namespace cache4

@@ -396,20 +396,31 @@ int esa_cache4_forward(int32_t dtype, const esa_cache4_t* cache, int32_t num_hea
     p.o = heads_of(o);
     p.Hq = num_heads;
     p.G = num_heads / cache->num_kv_heads;
-    p.pairs = (int64_t)cache->batch * num_heads * q_len;
+    const int64_t pairs = (int64_t)cache->batch * num_heads * q_len;
+    const int64_t rows = p.G * q_len, kv = (int64_t)cache->batch * cache->num_kv_heads;
+    if (rows > kMaxGrid || kv > 65535)
+      return fail(ESA_ERR_UNSUPPORTED, "%s: more than 2^31 rows per K/V head, or 65535 K/V heads",
+                  what);
+    p.rows = (unsigned)rows;
     p.pat = esa::make_pattern(heads, attn_length, layer_idx, num_hidden_layers, head_offset);
     p.scale_log2 = scale * esa::kLog2e;
     p.lse = lse;
     p.err = err;
     // few pairs: the slots of a pair over several warps, up to one chunk of 32 each
     int wpp = 1;
-    while (wpp < c4::kAttendWarps && wpp * 32 < attn_length && p.pairs * wpp < kSms * 16) wpp *= 2;
+    while (wpp < c4::kAttendWarps && wpp * 32 < attn_length && pairs * wpp < kSms * 16) wpp *= 2;
     p.warps_per_pair = wpp;
-    const int64_t grid = ceil_div(p.pairs, c4::kAttendWarps / wpp);
-    if (grid > kMaxGrid) return fail(ESA_ERR_UNSUPPORTED, "%s: too many rows", what);
+    // many pairs: several per warp, as long as every SM has its CTAs
+    int ppw = 1;
+    while (wpp == 1 && ppw < 16 && pairs >= (int64_t)kSms * 20 * ppw * 4) ppw *= 2;
+    p.pairs_per_warp = ppw;
+    const dim3 grid((unsigned)ceil_div(rows, c4::kAttendWarps / wpp * ppw), (unsigned)kv);
     return by_head_dim(cache->head_dim, [&](auto d) {
-      c4::attend_kernel<T, decltype(d)::value>
-          <<<(unsigned)grid, c4::kAttendWarps * 32, 0, (cudaStream_t)stream>>>(p);
+      constexpr int D = decltype(d)::value;
+      if (wpp > 1)
+        c4::attend_kernel<T, D, true><<<grid, c4::kAttendWarps * 32, 0, (cudaStream_t)stream>>>(p);
+      else
+        c4::attend_kernel<T, D, false><<<grid, c4::kAttendWarps * 32, 0, (cudaStream_t)stream>>>(p);
       return check_launch(what);
     });
   });
