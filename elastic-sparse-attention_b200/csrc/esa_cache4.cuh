@@ -10,6 +10,8 @@
 //          of keys are two's complement (the code, not code + 8)
 //   value: word g * (D / 64) + c (g < 8, c < D / 64) holds the elements
 //          c * 64 + i * 8 + g, nibble i
+// and the 32-byte sectors of a row are turned by its number (turn_of), so that
+// lanes which read the same part of different rows mostly meet different banks.
 //
 // Attention: every (query row, head) pair has w keys of its own, so nothing is
 // shared between pairs and the work is decoding 2 w D codes.  The products run
@@ -66,6 +68,11 @@ struct Span {
     return s < 0 || s >= S - l ? -2 : s + l;
   }
 };
+
+// What the byte offsets within a row of 128-byte lines are combined with by XOR.
+template <int D> __device__ __forceinline__ uint32_t turn_of(uint32_t row) {
+  return D == 64 ? (row & 2u) << 4 : (row & 3u) << 5;
+}
 
 // 8 lanes with 8 nibbles each: nibble i of lane j <-> nibble j of lane i.
 __device__ __forceinline__ uint32_t transpose8(uint32_t w, int j) {
@@ -180,8 +187,9 @@ write_kernel(const RowParams<T> p) {
   if (!go) return;
   const int64_t row = ((int64_t)e.b * p.c.Hkv + e.h) * p.c.S + pos;
   uint32_t* codes = reinterpret_cast<uint32_t*>(p.c.codes + row * D);
-  codes[e.key_word() + (e.part >> 2 & 1)] = kw;
-  codes[D / 8 + e.value_word()] = vw;
+  const int turn = (int)turn_of<D>((uint32_t)pos) / 4;
+  codes[(e.key_word() + (e.part >> 2 & 1)) ^ turn] = kw;
+  codes[(D / 8 + e.value_word()) ^ turn] = vw;
   if ((e.part & 3) == 0) {
     __nv_bfloat16* s = p.c.scales + row * (2 * D / kGroup) + (e.part >> 2);
     s[0] = __float2bfloat16_rn(sk);
@@ -216,8 +224,9 @@ read_kernel(const RowParams<T> p) {
   if (go) {
     const int64_t row = ((int64_t)e.b * p.c.Hkv + e.h) * p.c.S + pos;
     const uint32_t* codes = reinterpret_cast<const uint32_t*>(p.c.codes + row * D);
-    kw = __ldg(codes + e.key_word() + (e.part >> 2 & 1));
-    vw = __ldg(codes + D / 8 + e.value_word());
+    const int turn = (int)turn_of<D>((uint32_t)pos) / 4;
+    kw = __ldg(codes + ((e.key_word() + (e.part >> 2 & 1)) ^ turn));
+    vw = __ldg(codes + ((D / 8 + e.value_word()) ^ turn));
     const __nv_bfloat16* s = p.c.scales + row * (2 * D / kGroup) + (e.part >> 2);
     sk = __bfloat162float(s[0]);
     sv = __bfloat162float(s[D / kGroup]);
@@ -488,16 +497,17 @@ attend_kernel(const AttendParams<T> p) {
     const int myrow = valid ? raw : safe;
     // ---- all loads of the 32 slots ----
     uint32_t kw[4][KW], sw[NG], vw[8][VW];           // sw: the own key's scales, its value's scales
+    const uint32_t at = (uint32_t)myrow * (uint32_t)D | turn_of<D>((uint32_t)myrow);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {                    // keys k * 8 + g
-      const uint32_t row = (uint32_t)__shfl_sync(0xffffffffu, myrow, (lane & 28) + k);
-      load_words<KW>(codes + (row * (uint32_t)D + t * (KW * 4)), kw[k]);
+      const uint32_t row = __shfl_sync(0xffffffffu, at, (lane & 28) + k);
+      load_words<KW>(codes + (row ^ (uint32_t)(t * (KW * 4))), kw[k]);
     }
     load_words<NG>(scales + (uint32_t)myrow * (uint32_t)(NG * 4), sw);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {                    // keys t * 8 + k
-      const uint32_t row = (uint32_t)__shfl_sync(0xffffffffu, myrow, k * 4 + t);
-      load_words<VW>(codes + (row * (uint32_t)D + D / 2 + g * (VW * 4)), vw[k]);
+      const uint32_t row = __shfl_sync(0xffffffffu, at, k * 4 + t);
+      load_words<VW>(codes + (row ^ (uint32_t)(D / 2 + g * (VW * 4))), vw[k]);
     }
     // ---- scores ----
     float sc[4] = {0.f, 0.f, 0.f, 0.f};
