@@ -21,22 +21,26 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 bool known_dtype(int32_t d) { return d == ESA_DTYPE_F32 || d == ESA_DTYPE_BF16 || d == ESA_DTYPE_F16; }
 
-// Launches `kernel` with clusters of `ctas` neighbouring CTAs.
-template <typename... P, typename... A>
-int launch_clusters(const char* what, void (*kernel)(P...), dim3 grid, dim3 block, int ctas,
-                    cudaStream_t s, A... args) {
+// Launches `kernel` with clusters of `ctas` neighbouring CTAs; its CTAs may be placed
+// while the kernel before it still runs (see launch_after).
+template <typename Q>
+int launch_clusters(const char* what, void (*kernel)(const Q), dim3 grid, dim3 block, int ctas,
+                    cudaStream_t s, const Q& params, size_t shared = 0) {
   cudaLaunchConfig_t c = {};
   c.gridDim = grid;
   c.blockDim = block;
+  c.dynamicSmemBytes = shared;
   c.stream = s;
-  cudaLaunchAttribute a[1];
-  a[0].id = cudaLaunchAttributeClusterDimension;
-  a[0].val.clusterDim.x = ctas;
-  a[0].val.clusterDim.y = 1;
-  a[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute a[2];
+  a[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  a[0].val.programmaticStreamSerializationAllowed = 1;
+  a[1].id = cudaLaunchAttributeClusterDimension;
+  a[1].val.clusterDim.x = ctas;
+  a[1].val.clusterDim.y = 1;
+  a[1].val.clusterDim.z = 1;
   c.attrs = a;
-  c.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&c, kernel, P(args)...);
+  c.numAttrs = 2;
+  const cudaError_t e = cudaLaunchKernelEx(&c, kernel, params);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return fail(ESA_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
@@ -93,25 +97,57 @@ w4::Packed packed(int64_t n, int64_t k, int32_t group, const void* codes, const 
   p.K = (int)k;
   p.group = group;
   p.tiles = (int)ceil_div(n, w4::kTileRows);
-  p.blocks = (int)ceil_div(k, w4::kBlockK);
-  p.groups = (int)ceil_div(k, group);
+  p.chunks = (int)ceil_div(k, w4::kTileK);
+  p.groups = p.chunks * (w4::kTileK / group);
   return p;
 }
 
-template <typename T, int NT, int RT, int WR>
-int linear(const w4::LinearParams<T>& p, cudaStream_t s) {
-  constexpr int kTokens = NT * 8 / w4::Operand<T>::kParts;
-  const int64_t row_ctas = ceil_div(p.tiles, RT * WR), col_ctas = ceil_div(p.M, kTokens);
+// Up to 8 columns: as many warps on a tile of rows as leave all of them resident
+// (32 per SM), with two tiles of K per warp at least.
+template <typename T, int G>
+int linear_vector(const w4::LinearParams<T>& p, cudaStream_t s) {
+  auto go = [&](auto wk) {
+    constexpr int WK = decltype(wk)::value;
+    return launch_after("esa_linear4", w4::vector_kernel<T, G, WK>, dim3((unsigned)p.tiles),
+                        dim3(WK * 32), s, p);
+  };
+  int wk = 2;
+  while (wk < 16 && p.tiles * wk * 2 <= kSms * 32 && p.chunks >= wk * 4) wk *= 2;
+  switch (wk) {
+    case 2: return go(std::integral_constant<int, 2>{});
+    case 4: return go(std::integral_constant<int, 4>{});
+    case 8: return go(std::integral_constant<int, 8>{});
+    default: return go(std::integral_constant<int, 16>{});
+  }
+}
+
+// More columns: K is split over a cluster until there are two CTAs per SM, with two
+// tiles of K per warp at least.
+template <typename T, int G, int NT, int WR>
+int linear_rows(const w4::LinearParams<T>& p, cudaStream_t s) {
+  using S = w4::Shape<T, NT, WR>;
+  const int64_t row_ctas = ceil_div(p.tiles, WR), col_ctas = ceil_div(p.M, S::kTokens);
   if (col_ctas > 65535) return fail(ESA_ERR_UNSUPPORTED, "esa_linear4: too many rows");
-  // K is split over a cluster until there are about four CTAs per SM, with two
-  // pairs of blocks per warp at least
   int ctas = 1;
-  while (ctas < 8 && row_ctas * col_ctas * ctas < kSms * 2 &&
-         p.blocks >= ctas * 2 * (w4::kWarps / WR) * 4)
+  while (ctas < 8 && row_ctas * col_ctas * ctas * 2 <= kSms * 2 && p.chunks >= ctas * 2 * S::kWK * 2)
     ctas *= 2;
-  return launch_clusters("esa_linear4", w4::linear_kernel<T, NT, RT, WR>,
-                         dim3((unsigned)(row_ctas * ctas), (unsigned)col_ctas),
-                         dim3(w4::kWarps * 32), ctas, s, p);
+  auto* kernel = w4::rows_kernel<T, G, NT, WR>;
+  if (S::kShared > 48 * 1024 &&
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kShared) != cudaSuccess) {
+    cudaGetLastError();
+    return fail(ESA_ERR_CUDA, "esa_linear4: cannot reserve %d bytes of shared memory", S::kShared);
+  }
+  return launch_clusters("esa_linear4", kernel, dim3((unsigned)(row_ctas * ctas), (unsigned)col_ctas),
+                         dim3(w4::kWarps * 32), ctas, s, p, S::kShared);
+}
+
+template <typename T, int G>
+int linear(const w4::LinearParams<T>& p, cudaStream_t s) {
+  const int64_t cols = (int64_t)p.M * w4::Operand<T>::kParts;
+  if (cols <= 8) return linear_vector<T, G>(p, s);
+  if (cols <= 16) return linear_rows<T, G, 2, 4>(p, s);
+  if (cols <= 32) return linear_rows<T, G, 4, 4>(p, s);
+  return linear_rows<T, G, 8, 4>(p, s);
 }
 
 // ---------------------------------------------------------------------------
@@ -283,7 +319,7 @@ int esa_token_logprobs_backward(int32_t dtype, int32_t id_bytes, int64_t n_rows,
 
 size_t esa_weight4_codes_size(int64_t n, int64_t k) {
   if (n < 1 || k < 1) return 0;
-  return (size_t)ceil_div(n, w4::kTileRows) * ceil_div(k, w4::kBlockK) * w4::kBlockBytes;
+  return (size_t)ceil_div(n, w4::kTileRows) * ceil_div(k, w4::kTileK) * w4::kTileBytes;
 }
 
 int esa_quantize_weight4(int32_t dtype, int64_t n, int64_t k, int32_t group, const void* weight,
@@ -336,15 +372,14 @@ int esa_linear4(int32_t dtype, int64_t n_rows, int64_t n, int64_t k, int32_t gro
     p.M = (int)n_rows;
     p.N = w.N;
     p.K = w.K;
-    p.group = group;
     p.tiles = w.tiles;
-    p.blocks = w.blocks;
-    p.groups = w.groups;
-    const int64_t cols = n_rows * w4::Operand<T>::kParts;
+    p.chunks = w.chunks;
     cudaStream_t s = (cudaStream_t)stream;
-    if (cols <= 8) return linear<T, 1, 1, 1>(p, s);
-    if (cols <= 16) return linear<T, 2, 2, 1>(p, s);
-    return linear<T, 4, 2, 1>(p, s);
+    switch (group) {
+      case 32: return linear<T, 32>(p, s);
+      case 64: return linear<T, 64>(p, s);
+      default: return linear<T, 128>(p, s);
+    }
   });
 }
 

@@ -178,6 +178,7 @@ fwd_kernel(const FwdParams<T> p) {
   __shared__ Stats s_cta;                       // read by the other CTAs of the row
   __shared__ float s_max[TOP ? NW : 1][32];
   __shared__ uint64_t s_list[TOP ? NW : 1][32];
+  cudaGridDependencySynchronize();
   const cg::cluster_group cluster = cg::this_cluster();
   const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;

@@ -11,14 +11,14 @@
 // as 8 columns.)  float32 rows of x are split into three bf16 parts (8 bits
 // each, exact), three columns whose sums are added at the end.
 //
-// Layout, made once by quantize_kernel: tiles of 16 weight rows x 64 inputs in
-// 512 bytes, 16 per lane (one load), tiles of a row side by side.  Lane 4 g + t
-// holds rows g and g + 8, inputs t * 8 .. + 8 of each half of 32; word (half, s)
-// holds inputs t * 8 + 4 s + {0, 1, 2, 3} of both rows as the four A registers
-// of one mma: nibble j is the low and nibble j + 4 the high element of register
-// j.  The same inputs of x are 16 contiguous bytes, so B needs no shared
-// memory.  One AND/OR per register makes 128 + n (bf16) or 1024 + n (fp16), one
-// subtraction the code.
+// Layout, made once by quantize_kernel: 16 weight rows x 128 inputs in 1024 bytes
+// (the tiles of a row side by side, padded with zeros to whole tiles), twice 16
+// bytes per lane.  Lane 4 g + t holds rows g and g + 8, inputs t * 8 .. + 8 of each
+// 32; word (32, s) holds inputs t * 8 + 4 s + {0, 1, 2, 3} of both rows as the four
+// A registers of one mma: nibble j is the low and nibble j + 4 the high element of
+// register j.  The same inputs of x are 16 contiguous bytes: one load is the B
+// operand of two products.  One AND/OR per register makes 128 + n (bf16) or
+// 1024 + n (fp16), one subtraction the code.
 #pragma once
 #include <cooperative_groups.h>
 
@@ -27,18 +27,21 @@
 namespace esa {
 namespace w4 {
 
-constexpr int kTileRows = 16, kBlockK = 64, kBlockBytes = 512;
+constexpr int kTileRows = 16, kTileK = 128, kTileBytes = 1024;
 
 // ---------------------------------------------------------------------------
 // Weights -> codes and scales, and back.  CTA = one tile of rows x 128 inputs;
 // thread = 8 inputs of one row.
 // ---------------------------------------------------------------------------
 struct Packed {
-  uint8_t* codes;             // [tiles][blocks][512]
-  __nv_bfloat16* scales;      // [tiles][groups][16]
+  uint8_t* codes;             // [tiles][chunks][1024]
+  __nv_bfloat16* scales;      // [tiles][groups][16]: rows 0, 8, 1, 9, ...
   int N, K, group;
-  int tiles, blocks, groups;  // of 16 rows, of 64 inputs, of `group` inputs
+  int tiles, chunks, groups;  // of 16 rows, of 128 inputs, chunks * 128 / group
 };
+
+// Place of row r of 16 among the scales of a group.
+__device__ __forceinline__ int scale_place(int r) { return (r & 7) * 2 + (r >> 3); }
 
 constexpr int kPackThreads = 256;
 
@@ -72,8 +75,8 @@ quantize_kernel(const Packed p, const T* w) {
   for (int o = 1; o < p.group / 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
   const float s = int4::group_scale(top), inv = 1.f / s;
   const int g = k / p.group;
-  if (part % (p.group / 8) == 0 && g < p.groups)
-    p.scales[(tile * p.groups + g) * kTileRows + r] = __float2bfloat16_rn(s);
+  if (part % (p.group / 8) == 0)
+    p.scales[(tile * p.groups + g) * kTileRows + scale_place(r)] = __float2bfloat16_rn(s);
   const int shift = r >= 8 ? 4 : 0;                  // registers 1 and 3 hold rows 8 .. 15
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -83,14 +86,13 @@ quantize_kernel(const Packed p, const T* w) {
     s_words[threadIdx.x][i] = (c[0] | c[1] << 16 | c[2] << 8 | c[3] << 24) << shift;
   }
   __syncthreads();
-  const int block = (int)blockIdx.x * 2 + (part >> 3);
-  if (r >= 8 || block >= p.blocks) return;
+  if (r >= 8) return;
   const int lane = (r << 2) | (part & 3), half = (part >> 2) & 1;
   uint2 out;
   out.x = s_words[threadIdx.x][0] | s_words[threadIdx.x + 128][0];
   out.y = s_words[threadIdx.x][1] | s_words[threadIdx.x + 128][1];
-  *reinterpret_cast<uint2*>(p.codes + (tile * p.blocks + block) * kBlockBytes + lane * 16 +
-                            half * 8) = out;
+  *reinterpret_cast<uint2*>(p.codes + (tile * p.chunks + blockIdx.x) * kTileBytes +
+                            (part >> 3) * 512 + lane * 16 + half * 8) = out;
 }
 
 template <typename T>
@@ -101,11 +103,12 @@ dequantize_kernel(const Packed p, T* w) {
   const int row = (int)(tile * kTileRows) + r;
   const int k = (int)blockIdx.x * 128 + part * 8;
   if (row >= p.N || k >= p.K) return;
-  const int block = (int)blockIdx.x * 2 + (part >> 3);
   const int lane = ((r & 7) << 2) | (part & 3), half = (part >> 2) & 1;
   const uint2 v = __ldg(reinterpret_cast<const uint2*>(
-      p.codes + (tile * p.blocks + block) * kBlockBytes + lane * 16 + half * 8));
-  const float s = __bfloat162float(p.scales[(tile * p.groups + k / p.group) * kTileRows + r]);
+      p.codes + (tile * p.chunks + blockIdx.x) * kTileBytes + (part >> 3) * 512 + lane * 16 +
+      half * 8));
+  const float s =
+      __bfloat162float(p.scales[(tile * p.groups + k / p.group) * kTileRows + scale_place(r)]);
   const uint32_t words[2] = {v.x >> (r >= 8 ? 4 : 0), v.y >> (r >= 8 ? 4 : 0)};
   float f[8];
 #pragma unroll
@@ -149,7 +152,8 @@ __device__ __forceinline__ void expand(uint32_t w, uint32_t (&a)[4]) {
   constexpr uint32_t kOne = kHalf ? 0x64006400u : 0x43004300u;       // 1024 or 128, twice
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const uint32_t v = ((w >> (4 * j)) & 0x000f000fu) | kOne;
+    uint32_t v;      // (w >> 4 j) & 0x000f000f | kOne: written out, else it is two instructions
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(v) : "r"(w >> (4 * j)), "n"(0x000f000f), "r"(kOne));
     if constexpr (kHalf) {
       const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&v), __float2half2_rn(1032.f));
       a[j] = *reinterpret_cast<const uint32_t*>(&d);
@@ -161,35 +165,32 @@ __device__ __forceinline__ void expand(uint32_t w, uint32_t (&a)[4]) {
   }
 }
 
-// Eight inputs of one column as four B words: x itself, or part `part` of the
-// float32 values cut into pieces of 8 significant bits.  (An infinity is all in
-// the first part.)
+// Part `part` of eight float32 values cut into pieces of 8 significant bits.  (An
+// infinity is all in the first part.)
+__device__ __forceinline__ uint4 cut8(const uint4& lo, const uint4& hi, int part) {
+  const uint32_t u[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+  uint32_t b[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    b[e] = u[e];
+    if (part > 0) {
+      float r = __uint_as_float(u[e]) - __uint_as_float(u[e] & 0xffff0000u);
+      if (part > 1) r -= __uint_as_float(__float_as_uint(r) & 0xffff0000u);
+      b[e] = (u[e] & 0x7f800000u) != 0x7f800000u ? __float_as_uint(r) : 0u;
+    }
+  }
+  return make_uint4(__byte_perm(b[0], b[1], 0x7632), __byte_perm(b[2], b[3], 0x7632),
+                    __byte_perm(b[4], b[5], 0x7632), __byte_perm(b[6], b[7], 0x7632));
+}
+
+// Eight inputs k .. k + 7 of one column as four B words (zeros past K).
 template <typename T>
 __device__ __forceinline__ uint4 column8(const T* x, int k, int K, bool in, int part) {
+  const uint4 none = make_uint4(0, 0, 0, 0);
   if constexpr (sizeof(T) == 2) {
-    return in && k < K ? ldg16(x + k) : make_uint4(0, 0, 0, 0);
+    return in && k < K ? ldg16(x + k) : none;
   } else {
-    uint32_t w[4];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint4 v = in && k + 4 * h < K ? ldg16(x + k + 4 * h) : make_uint4(0, 0, 0, 0);
-      const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-      uint32_t b[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float r = __uint_as_float(u[e]);
-        const bool finite = (u[e] & 0x7f800000u) != 0x7f800000u;
-        b[e] = u[e];
-        if (part > 0) {
-          r -= __uint_as_float(u[e] & 0xffff0000u);
-          if (part > 1) r -= __uint_as_float(__float_as_uint(r) & 0xffff0000u);
-          b[e] = finite ? __float_as_uint(r) : 0u;
-        }
-      }
-      w[2 * h] = __byte_perm(b[0], b[1], 0x7632);
-      w[2 * h + 1] = __byte_perm(b[2], b[3], 0x7632);
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
+    return cut8(in && k < K ? ldg16(x + k) : none, in && k + 4 < K ? ldg16(x + k + 4) : none, part);
   }
 }
 
@@ -198,135 +199,246 @@ template <typename T> struct LinearParams {
   T* y;
   const uint8_t* codes;
   const __nv_bfloat16* scales;
-  int M, N, K, group;
-  int tiles, blocks, groups;
+  int M, N, K;
+  int tiles, chunks;
 };
 
-constexpr int kWarps = 8;
+// The codes of a tile of 16 x 128 and the scales of its groups, as one lane holds them.
+template <int G> struct Tile {
+  uint4 c[2];
+  uint32_t s[kTileK / G];      // rows g and g + 8
+  __device__ __forceinline__ void load(const uint8_t* codes, const __nv_bfloat16* scales,
+                                       int64_t tile, int lane) {
+    c[0] = ldg16_stream(codes + tile * kTileBytes + lane * 16);
+    c[1] = ldg16_stream(codes + tile * kTileBytes + 512 + lane * 16);
+#pragma unroll
+    for (int i = 0; i < kTileK / G; ++i)
+      s[i] = __ldg(reinterpret_cast<const uint32_t*>(scales) + (tile * (kTileK / G) + i) * 8 + (lane >> 2));
+  }
+  __device__ __forceinline__ uint32_t word(int i) const {      // i = quarter of 32 inputs, s
+    const uint4& v = c[i >> 2];
+    return (i & 3) == 0 ? v.x : (i & 3) == 1 ? v.y : (i & 3) == 2 ? v.z : v.w;
+  }
+};
 
-// CTA = RT * WR tiles of weight rows x NT * 8 columns; its 8 warps are WR groups
-// of rows times WK = 8 / WR parts of K.  A cluster of CTAs along x splits K
-// further; the sums are joined in a fixed order.
-template <typename T, int NT, int RT, int WR>
-__global__ void __launch_bounds__(kWarps * 32)
-linear_kernel(const LinearParams<T> p) {
-  namespace cg = cooperative_groups;
+// acc += tile times 128 inputs of NT * 8 columns; B of quarter q in xb(q, n).
+template <typename H, int G, int NT, typename B>
+__device__ __forceinline__ void multiply(const Tile<G>& w, float (&acc)[NT][4], B&& xb) {
+  float sum[NT][4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    uint32_t a0[4], a1[4];
+    expand<H>(w.word(2 * q), a0);
+    expand<H>(w.word(2 * q + 1), a1);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      if ((q * 32) % G == 0)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[n][i] = 0.f;
+      const uint4 b = xb(q, n);
+      mma<H>(sum[n], a0, b.x, b.y);
+      mma<H>(sum[n], a1, b.z, b.w);
+    }
+    if ((q * 32 + 32) % G == 0) {
+      const uint32_t s = w.s[q * 32 / G];
+      const float lo = __uint_as_float(s << 16), hi = __uint_as_float(s & 0xffff0000u);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        acc[n][0] = fmaf(lo, sum[n][0], acc[n][0]);
+        acc[n][1] = fmaf(lo, sum[n][1], acc[n][1]);
+        acc[n][2] = fmaf(hi, sum[n][2], acc[n][2]);
+        acc[n][3] = fmaf(hi, sum[n][3], acc[n][3]);
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Up to 8 columns: bound by the stream of codes.  CTA = one tile of 16 weight rows,
+// its WK warps share K and join in shared memory; the codes that a warp begins with
+// are on their way before the kernel waits for the one before it (which made x).
+// ---------------------------------------------------------------------------
+template <typename T, int G, int WK>
+__global__ void __launch_bounds__(WK * 32)
+vector_kernel(const LinearParams<T> p) {
   using H = typename Operand<T>::Half;
   constexpr int P = Operand<T>::kParts;
-  constexpr int WK = kWarps / WR;
-  constexpr int kTokens = NT * 8 / P;                  // rows of x per CTA
-  constexpr int kRows = RT * WR * kTileRows, kCols = NT * 8;
-  __shared__ float s_part[WK][kRows][kCols + 1];
+  constexpr int U = 2;                                 // tiles in flight
+  __shared__ float s_part[WK][8][kTileRows];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const int c0 = (int)((int64_t)p.chunks * warp / WK), c1 = (int)((int64_t)p.chunks * (warp + 1) / WK);
+  const int64_t base = (int64_t)blockIdx.x * p.chunks;
+  Tile<G> w[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (c0 + u < c1) w[u].load(p.codes, p.scales, base + c0 + u, lane);
+  cudaTriggerProgrammaticLaunchCompletion();           // the next kernel may begin like this
+  cudaGridDependencySynchronize();
+  const int token = g / P, part = g % P;
+  const bool in = token < p.M && token < 8 / P;
+  const T* x = p.x + (int64_t)(in ? token : 0) * p.K;
+  float acc[1][4] = {{0.f, 0.f, 0.f, 0.f}};
+  for (int c = c0; c < c1; c += U) {
+    uint4 xb[U][4];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        xb[u][q] = column8(x, (c + u) * kTileK + q * 32 + t * 8, p.K, in && c + u < c1, part);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (c + u >= c1) break;
+      const Tile<G> now = w[u];
+      if (c + u + U < c1) w[u].load(p.codes, p.scales, base + c + u + U, lane);
+      multiply<H, G, 1>(now, acc, [&](int q, int) { return xb[u][q]; });
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) s_part[warp][2 * t + (i & 1)][g + (i >> 1) * 8] = acc[0][i];
+  __syncthreads();
+  const int row = threadIdx.x & 15;
+  for (int m = threadIdx.x >> 4; m < p.M; m += WK * 2) {
+    if ((int64_t)blockIdx.x * kTileRows + row >= p.N) break;
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < WK; ++k)
+#pragma unroll
+      for (int q = 0; q < P; ++q) sum += s_part[k][m * P + q][row];
+    p.y[(int64_t)m * p.N + (int64_t)blockIdx.x * kTileRows + row] = from_f32<T>(sum);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// More columns.  CTA = 8 warps on WR tiles of rows times NT * 8 columns, WK = 8 / WR
+// of them sharing K; a cluster of CTAs along x splits K further.  The columns'
+// inputs go through shared memory, kStageK at a time and the next stage while one
+// is used, as 16-bit rows 64 bytes (mod 128) apart, so that the lanes' 16-byte
+// reads meet no bank twice.
+// ---------------------------------------------------------------------------
+constexpr int kWarps = 8;
+
+template <typename T, int NT, int WR> struct Shape {
+  static constexpr int kParts = Operand<T>::kParts;
+  static constexpr int kTokens = NT * 8 / kParts;        // rows of x per CTA
+  static constexpr int kRows = WR * kTileRows, kCols = NT * 8;
+  static constexpr int kWK = kWarps / WR;
+  static constexpr int kStageK = NT == 8 ? 256 : 512;
+  static constexpr int kPitch = kStageK * 2 + 64;        // bytes of a column
+  static constexpr int kStageBytes = kCols * kPitch;
+  static constexpr int kSumBytes = kWK * kRows * (kCols + 1) * 4;
+  static constexpr int kShared = 2 * kStageBytes > kSumBytes ? 2 * kStageBytes : kSumBytes;
+};
+
+__device__ __forceinline__ void copy16_async(uint32_t to, const void* from, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(in ? 16 : 0)
+               : "memory");
+}
+
+template <typename T, int G, int NT, int WR>
+__global__ void __launch_bounds__(kWarps * 32, 2)
+rows_kernel(const LinearParams<T> p) {
+  namespace cg = cooperative_groups;
+  using S = Shape<T, NT, WR>;
+  using H = typename Operand<T>::Half;
+  constexpr int P = S::kParts, WK = S::kWK;
+  constexpr int kStage = S::kStageK / kTileK;            // chunks of a stage
+  extern __shared__ __align__(128) unsigned char s_mem[];
   const cg::cluster_group cluster = cg::this_cluster();
   const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int wr = warp % WR, wk = warp / WR;
   const int g = lane >> 2, t = lane & 3;
-  const int tile0 = (int)(blockIdx.x / ctas) * RT * WR + wr * RT;
-  const int m0 = (int)blockIdx.y * kTokens;
+  const int tile = (int)(blockIdx.x / ctas) * WR + wr;
+  const int m0 = (int)blockIdx.y * S::kTokens;
+  const int tokens = min(S::kTokens, p.M - m0);
+  const int c0 = (int)((int64_t)p.chunks * rank / ctas), c1 = (int)((int64_t)p.chunks * (rank + 1) / ctas);
+  // a tile past the last reads the last one again
+  const int64_t base = (int64_t)min(tile, p.tiles - 1) * p.chunks;
 
-  // this warp's blocks of K: an even split over the cluster's ctas * WK parts, in
-  // whole pairs so that a group of 128 has one owner
-  const int pairs = (p.blocks + 1) / 2, share = ctas * WK, me = rank * WK + wk;
-  const int b0 = 2 * (int)((int64_t)pairs * me / share);
-  const int b1 = min(p.blocks, 2 * (int)((int64_t)pairs * (me + 1) / share));
-
-  float acc[RT][NT][4];
+  float acc[NT][4];
 #pragma unroll
-  for (int r = 0; r < RT; ++r)
+  for (int i = 0; i < NT * 4; ++i) (&acc[0][0])[i] = 0.f;
+  // stage s: inputs of chunks c0 + s * kStage ..; 8 inputs of a row of x per thread
+  // and step, zeros where there is no row or no input
+  constexpr int kSteps = kStage * 16;
+  auto fill = [&](int s) {
+    unsigned char* buf = s_mem + (s & 1) * S::kStageBytes;
+    const int k8 = threadIdx.x % kSteps, k = (c0 + s * kStage) * kTileK + k8 * 8;
+    for (int token = threadIdx.x / kSteps; token < S::kTokens; token += kWarps * 32 / kSteps) {
+      const bool in = token < tokens;
+      const T* x = p.x + (int64_t)(m0 + (in ? token : 0)) * p.K;
+      if constexpr (P == 1) {
+        copy16_async((uint32_t)__cvta_generic_to_shared(buf + token * S::kPitch + k8 * 16),
+                     in && k < p.K ? x + k : x, in && k < p.K);
+      } else {
+        const uint4 none = make_uint4(0, 0, 0, 0);
+        const uint4 lo = in && k < p.K ? ldg16(x + k) : none;
+        const uint4 hi = in && k + 4 < p.K ? ldg16(x + k + 4) : none;
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[r][n][i] = 0.f;
-
-  const T* xc[NT];
-  bool in[NT];
-  int part[NT];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int c = n * 8 + g, token = c / P;
-    part[n] = c % P;
-    in[n] = token < kTokens && m0 + token < p.M;
-    xc[n] = p.x + (int64_t)(in[n] ? m0 + token : 0) * p.K;
-  }
-
-  constexpr int U = RT * NT >= 8 ? 2 : 4;              // blocks in flight
-  for (int b = b0; b < b1; b += U) {
-    uint4 codes[U][RT];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        const bool ok = b + u < b1 && tile0 + r < p.tiles;
-        codes[u][r] = ok ? ldg16_stream(p.codes + ((int64_t)(tile0 + r) * p.blocks + b + u) * kBlockBytes + lane * 16)
-                         : make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
-      }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (b + u >= b1) break;
-      float sum[RT][NT][4];
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int k = (b + u) * kBlockK + half * 32;
-        uint4 xb[NT];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) xb[n] = column8(xc[n], k + t * 8, p.K, in[n], part[n]);
-        const bool fresh = half == 0 || p.group == 32;
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          uint32_t a0[4], a1[4];
-          expand<H>(half ? codes[u][r].z : codes[u][r].x, a0);
-          expand<H>(half ? codes[u][r].w : codes[u][r].y, a1);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            if (fresh)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) sum[r][n][i] = 0.f;
-            mma<H>(sum[r][n], a0, xb[n].x, xb[n].y);
-            mma<H>(sum[r][n], a1, xb[n].z, xb[n].w);
-          }
-        }
-        if (half == 1 || p.group == 32) {
-          const int gi = k / p.group;
-#pragma unroll
-          for (int r = 0; r < RT; ++r) {
-            if (tile0 + r >= p.tiles || gi >= p.groups) break;
-            const __nv_bfloat16* s = p.scales + ((int64_t)(tile0 + r) * p.groups + gi) * kTileRows + g;
-            const float lo = __bfloat162float(s[0]), hi = __bfloat162float(s[8]);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              acc[r][n][0] = fmaf(lo, sum[r][n][0], acc[r][n][0]);
-              acc[r][n][1] = fmaf(lo, sum[r][n][1], acc[r][n][1]);
-              acc[r][n][2] = fmaf(hi, sum[r][n][2], acc[r][n][2]);
-              acc[r][n][3] = fmaf(hi, sum[r][n][3], acc[r][n][3]);
-            }
-          }
-        }
+        for (int q = 0; q < P; ++q)
+          *reinterpret_cast<uint4*>(buf + (token * P + q) * S::kPitch + k8 * 16) = cut8(lo, hi, q);
       }
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  if constexpr (S::kTokens * P < S::kCols) {             // columns without a row of x
+    for (int i = threadIdx.x; i < 2 * (S::kCols - S::kTokens * P) * (S::kPitch / 16); i += kWarps * 32) {
+      const int half = i / ((S::kCols - S::kTokens * P) * (S::kPitch / 16));
+      const int rest = i % ((S::kCols - S::kTokens * P) * (S::kPitch / 16));
+      *reinterpret_cast<uint4*>(s_mem + half * S::kStageBytes + S::kTokens * P * S::kPitch + rest * 16) =
+          make_uint4(0, 0, 0, 0);
+    }
   }
+  Tile<G> w;
+  if (c0 + wk < c1) w.load(p.codes, p.scales, base + c0 + wk, lane);
+  cudaTriggerProgrammaticLaunchCompletion();             // the next kernel may begin like this
+  cudaGridDependencySynchronize();
+  const int stages = (c1 - c0 + kStage - 1) / kStage;
+  if (stages > 0) fill(0);
+  for (int s = 0; s < stages; ++s) {
+    if (s + 1 < stages) {
+      fill(s + 1);
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+    } else {
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+    }
+    __syncthreads();
+    const unsigned char* buf = s_mem + (s & 1) * S::kStageBytes + g * S::kPitch + t * 16;
+    const int first = c0 + s * kStage, last = min(c1, first + kStage);
+#pragma unroll 1
+    for (int c = first + wk; c < last; c += WK) {
+      const Tile<G> now = w;
+      if (c + WK < c1) w.load(p.codes, p.scales, base + c + WK, lane);
+      const unsigned char* xs = buf + (c - first) * (kTileK * 2);
+      multiply<H, G, NT>(now, acc, [&](int q, int n) {
+        return *reinterpret_cast<const uint4*>(xs + n * 8 * S::kPitch + q * 64);
+      });
+    }
+    __syncthreads();                                     // the stage after next overwrites it
+  }
+  float* sums = reinterpret_cast<float*>(s_mem);         // [WK][rows][columns + 1]
 #pragma unroll
-  for (int r = 0; r < RT; ++r)
+  for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        s_part[wk][(wr * RT + r) * kTileRows + g + (i >> 1) * 8][n * 8 + 2 * t + (i & 1)] = acc[r][n][i];
+    for (int i = 0; i < 4; ++i)
+      sums[(wk * S::kRows + wr * kTileRows + g + (i >> 1) * 8) * (S::kCols + 1) + n * 8 + 2 * t +
+           (i & 1)] = acc[n][i];
   if (ctas > 1) cluster.sync(); else __syncthreads();
-  // outputs of the CTA group, split over the cluster; neighbouring threads write
-  // neighbouring weight rows of one row of y
-  const int row0 = (int)(blockIdx.x / ctas) * kRows;
-  const int tokens = min(kTokens, p.M - m0);
-  for (int i = rank * kWarps * 32 + threadIdx.x; i < tokens * kRows; i += ctas * kWarps * 32) {
-    const int token = i / kRows, row = i % kRows;
+  // the outputs are split over the cluster; neighbouring threads write neighbouring
+  // weight rows of one row of y
+  const int row0 = (int)(blockIdx.x / ctas) * S::kRows;
+  for (int i = rank * kWarps * 32 + threadIdx.x; i < tokens * S::kRows; i += ctas * kWarps * 32) {
+    const int token = i / S::kRows, row = i % S::kRows;
     if (row0 + row >= p.N) continue;
     float sum = 0.f;
     for (int c = 0; c < ctas; ++c) {
-      const float* base = ctas > 1 ? cluster.map_shared_rank(&s_part[0][0][0], c) : &s_part[0][0][0];
+      const float* from = ctas > 1 ? cluster.map_shared_rank(sums, c) : sums;
 #pragma unroll
-      for (int w = 0; w < WK; ++w)
+      for (int k = 0; k < WK; ++k)
 #pragma unroll
-        for (int q = 0; q < P; ++q) sum += base[(w * kRows + row) * (kCols + 1) + token * P + q];
+        for (int q = 0; q < P; ++q)
+          sum += from[(k * S::kRows + row) * (S::kCols + 1) + token * P + q];
     }
     p.y[(int64_t)(m0 + token) * p.N + row0 + row] = from_f32<T>(sum);
   }

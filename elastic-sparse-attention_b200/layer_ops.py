@@ -603,7 +603,7 @@ LINEAR4_ROWS = 64
 @dataclass(eq=False)
 class PackedWeight4:
     """A weight [n, k] in 4 bits: ``codes`` uint8 in the order of the product,
-    ``scales`` bfloat16 [ceil(n / 16), ceil(k / group), 16], ``shape`` (n, k) and
+    ``scales`` bfloat16 [ceil(n / 16), ceil(k / 128) * 128 / group, 16], ``shape`` (n, k) and
     ``dtype`` those of the weight it was made from."""
     codes: torch.Tensor
     scales: torch.Tensor
@@ -631,7 +631,7 @@ def quantize_weight4(weight: torch.Tensor, group: int = 128) -> PackedWeight4:
     code = _dtype_code(weight)
     lib = _lib.load()
     p = PackedWeight4(_empty((lib.esa_weight4_codes_size(n, k),), torch.uint8, dev),
-                      _empty((-(-n // 16), -(-k // group), 16), torch.bfloat16, dev), (n, k), group,
+                      _empty((-(-n // 16), -(-k // 128) * (128 // group), 16), torch.bfloat16, dev), (n, k), group,
                       weight.dtype)
     _lib.launch(lib.esa_quantize_weight4, dev, code, n, k, group, weight.data_ptr(),
                 p.codes.data_ptr(), p.scales.data_ptr())
@@ -641,9 +641,9 @@ def quantize_weight4(weight: torch.Tensor, group: int = 128) -> PackedWeight4:
 def _check_weight4(p: PackedWeight4) -> tuple:
     n, k = p.shape
     if (p.group not in WEIGHT4_GROUPS or p.codes.dtype != torch.uint8
-            or p.codes.numel() != -(-n // 16) * -(-k // 64) * 512
+            or p.codes.numel() != -(-n // 16) * -(-k // 128) * 1024
             or p.scales.dtype != torch.bfloat16
-            or p.scales.shape != (-(-n // 16), -(-k // p.group), 16)):
+            or p.scales.shape != (-(-n // 16), -(-k // 128) * (128 // p.group), 16)):
         raise ValueError("PackedWeight4: codes, scales, shape and group do not fit together")
     if not p.codes.is_contiguous() or not p.scales.is_contiguous():
         raise ValueError("PackedWeight4: codes and scales must be contiguous")

@@ -262,7 +262,7 @@ int esa_token_logprobs_backward(int32_t dtype, int32_t id_bytes, int64_t n_rows,
  * w / s (ties to even, the quotient taken exactly) and stands for code * s.  A
  * group with an infinity or a NaN decodes to NaN.  codes: esa_weight4_codes_size(
  * n, k) bytes in the order the product reads them; scales: bfloat16 [ceil(n / 16),
- * ceil(k / group), 16].  k * element size is a multiple of 16 bytes.
+ * ceil(k / 128) * 128 / group, 16].  k * element size is a multiple of 16 bytes.
  */
 size_t esa_weight4_codes_size(int64_t n, int64_t k);
 int esa_quantize_weight4(int32_t dtype, int64_t n, int64_t k, int32_t group, const void* weight,
