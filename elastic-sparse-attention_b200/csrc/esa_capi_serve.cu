@@ -102,14 +102,27 @@ w4::Packed packed(int64_t n, int64_t k, int32_t group, const void* codes, const 
   return p;
 }
 
+template <typename K>
+int reserve_shared(const char* what, K* kernel, int bytes) {
+  if (bytes > 48 * 1024 &&
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
+    cudaGetLastError();
+    return fail(ESA_ERR_CUDA, "%s: cannot reserve %d bytes of shared memory", what, bytes);
+  }
+  return ESA_OK;
+}
+
 // Up to 8 columns: as many warps on a tile of rows as leave all of them resident
-// (32 per SM), with two tiles of K per warp at least.
+// (some 24 per SM), with two tiles of K per warp at least.
 template <typename T, int G>
 int linear_vector(const w4::LinearParams<T>& p, cudaStream_t s) {
   auto go = [&](auto wk) {
     constexpr int WK = decltype(wk)::value;
-    return launch_after("esa_linear4", w4::vector_kernel<T, G, WK>, dim3((unsigned)p.tiles),
-                        dim3(WK * 32), s, p);
+    constexpr int kShared = WK * w4::kDepth * w4::Tile<G>::kBytes;
+    auto* kernel = w4::vector_kernel<T, G, WK>;
+    if (int rc = reserve_shared("esa_linear4", kernel, kShared)) return rc;
+    return launch_clusters("esa_linear4", kernel, dim3((unsigned)p.tiles), dim3(WK * 32), 1, s, p,
+                           kShared);
   };
   int wk = 2;
   while (wk < 16 && p.tiles * wk * 2 <= kSms * 32 && p.chunks >= wk * 4) wk *= 2;
@@ -122,21 +135,17 @@ int linear_vector(const w4::LinearParams<T>& p, cudaStream_t s) {
 }
 
 // More columns: K is split over a cluster until there are two CTAs per SM, with two
-// tiles of K per warp at least.
-template <typename T, int G, int NT, int WR>
+// stages at least.
+template <typename T, int G, int NT>
 int linear_rows(const w4::LinearParams<T>& p, cudaStream_t s) {
-  using S = w4::Shape<T, NT, WR>;
-  const int64_t row_ctas = ceil_div(p.tiles, WR), col_ctas = ceil_div(p.M, S::kTokens);
+  using S = w4::Shape<T, G, NT>;
+  const int64_t row_ctas = ceil_div(p.tiles, w4::kWarps), col_ctas = ceil_div(p.M, S::kTokens);
   if (col_ctas > 65535) return fail(ESA_ERR_UNSUPPORTED, "esa_linear4: too many rows");
   int ctas = 1;
-  while (ctas < 8 && row_ctas * col_ctas * ctas * 2 <= kSms * 2 && p.chunks >= ctas * 2 * S::kWK * 2)
+  while (ctas < 8 && row_ctas * col_ctas * ctas * 2 <= kSms * 2 && p.chunks >= ctas * 2 * 2 * S::kStage)
     ctas *= 2;
-  auto* kernel = w4::rows_kernel<T, G, NT, WR>;
-  if (S::kShared > 48 * 1024 &&
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kShared) != cudaSuccess) {
-    cudaGetLastError();
-    return fail(ESA_ERR_CUDA, "esa_linear4: cannot reserve %d bytes of shared memory", S::kShared);
-  }
+  auto* kernel = w4::rows_kernel<T, G, NT>;
+  if (int rc = reserve_shared("esa_linear4", kernel, S::kShared)) return rc;
   return launch_clusters("esa_linear4", kernel, dim3((unsigned)(row_ctas * ctas), (unsigned)col_ctas),
                          dim3(w4::kWarps * 32), ctas, s, p, S::kShared);
 }
@@ -145,9 +154,9 @@ template <typename T, int G>
 int linear(const w4::LinearParams<T>& p, cudaStream_t s) {
   const int64_t cols = (int64_t)p.M * w4::Operand<T>::kParts;
   if (cols <= 8) return linear_vector<T, G>(p, s);
-  if (cols <= 16) return linear_rows<T, G, 2, 4>(p, s);
-  if (cols <= 32) return linear_rows<T, G, 4, 4>(p, s);
-  return linear_rows<T, G, 8, 4>(p, s);
+  if (cols <= 16) return linear_rows<T, G, 2>(p, s);
+  if (cols <= 32) return linear_rows<T, G, 4>(p, s);
+  return linear_rows<T, G, 8>(p, s);
 }
 
 // ---------------------------------------------------------------------------

@@ -203,17 +203,39 @@ template <typename T> struct LinearParams {
   int tiles, chunks;
 };
 
-// The codes of a tile of 16 x 128 and the scales of its groups, as one lane holds them.
+__device__ __forceinline__ void copy16_async(uint32_t to, const void* from, bool in = true) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(in ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void wait_copies() {     // all but the last N groups
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// A tile of 16 x 128 codes and the scales of its groups, as one lane holds them.
+// They come through shared memory, each lane copying what it reads itself: many
+// tiles can be on their way without registers, and no barrier is needed.
 template <int G> struct Tile {
+  static constexpr int kGroups = kTileK / G;
+  static constexpr int kBytes = kTileBytes + kGroups * 128;           // in shared memory
   uint4 c[2];
-  uint32_t s[kTileK / G];      // rows g and g + 8
-  __device__ __forceinline__ void load(const uint8_t* codes, const __nv_bfloat16* scales,
-                                       int64_t tile, int lane) {
-    c[0] = ldg16_stream(codes + tile * kTileBytes + lane * 16);
-    c[1] = ldg16_stream(codes + tile * kTileBytes + 512 + lane * 16);
+  uint32_t s[kGroups];         // rows g and g + 8
+  __device__ __forceinline__ static void fetch(uint32_t to, const uint8_t* codes,
+                                               const __nv_bfloat16* scales, int64_t tile, int lane) {
+    copy16_async(to + lane * 16, codes + tile * kTileBytes + lane * 16);
+    copy16_async(to + 512 + lane * 16, codes + tile * kTileBytes + 512 + lane * 16);
 #pragma unroll
-    for (int i = 0; i < kTileK / G; ++i)
-      s[i] = __ldg(reinterpret_cast<const uint32_t*>(scales) + (tile * (kTileK / G) + i) * 8 + (lane >> 2));
+    for (int i = 0; i < kGroups; ++i)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + kTileBytes + i * 128 + lane * 4),
+                   "l"(reinterpret_cast<const uint32_t*>(scales) + (tile * kGroups + i) * 8 + (lane >> 2))
+                   : "memory");
+  }
+  __device__ __forceinline__ void take(const unsigned char* from, int lane) {
+    c[0] = *reinterpret_cast<const uint4*>(from + lane * 16);
+    c[1] = *reinterpret_cast<const uint4*>(from + 512 + lane * 16);
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i)
+      s[i] = *reinterpret_cast<const uint32_t*>(from + kTileBytes + i * 128 + lane * 4);
   }
   __device__ __forceinline__ uint32_t word(int i) const {      // i = quarter of 32 inputs, s
     const uint4& v = c[i >> 2];
@@ -225,20 +247,27 @@ template <int G> struct Tile {
 template <typename H, int G, int NT, typename B>
 __device__ __forceinline__ void multiply(const Tile<G>& w, float (&acc)[NT][4], B&& xb) {
   float sum[NT][4];
+  uint4 b[2][NT];                                      // the next quarter's B loads run ahead
+#pragma unroll
+  for (int n = 0; n < NT; ++n) b[0][n] = xb(0, n);
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
+    if (q < 3)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) b[(q + 1) & 1][n] = xb(q + 1, n);
     uint32_t a0[4], a1[4];
     expand<H>(w.word(2 * q), a0);
     expand<H>(w.word(2 * q + 1), a1);
+    if ((q * 32) % G == 0)
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      if ((q * 32) % G == 0)
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i) sum[n][i] = 0.f;
-      const uint4 b = xb(q, n);
-      mma<H>(sum[n], a0, b.x, b.y);
-      mma<H>(sum[n], a1, b.z, b.w);
-    }
+    // products of the same sum apart from each other
+#pragma unroll
+    for (int n = 0; n < NT; ++n) mma<H>(sum[n], a0, b[q & 1][n].x, b[q & 1][n].y);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) mma<H>(sum[n], a1, b[q & 1][n].z, b[q & 1][n].w);
     if ((q * 32 + 32) % G == 0) {
       const uint32_t s = w.s[q * 32 / G];
       const float lo = __uint_as_float(s << 16), hi = __uint_as_float(s & 0xffff0000u);
@@ -255,47 +284,59 @@ __device__ __forceinline__ void multiply(const Tile<G>& w, float (&acc)[NT][4], 
 
 // ---------------------------------------------------------------------------
 // Up to 8 columns: bound by the stream of codes.  CTA = one tile of 16 weight rows,
-// its WK warps share K and join in shared memory; the codes that a warp begins with
-// are on their way before the kernel waits for the one before it (which made x).
+// its WK warps share K and join in shared memory.  A warp has kDepth tiles on their
+// way, and begins with that before it waits for the kernel before it (which made x).
 // ---------------------------------------------------------------------------
+constexpr int kDepth = 8;
+
 template <typename T, int G, int WK>
 __global__ void __launch_bounds__(WK * 32)
 vector_kernel(const LinearParams<T> p) {
   using H = typename Operand<T>::Half;
   constexpr int P = Operand<T>::kParts;
-  constexpr int U = 2;                                 // tiles in flight
-  __shared__ float s_part[WK][8][kTileRows];
+  extern __shared__ __align__(128) unsigned char s_mem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const int c0 = (int)((int64_t)p.chunks * warp / WK), c1 = (int)((int64_t)p.chunks * (warp + 1) / WK);
   const int64_t base = (int64_t)blockIdx.x * p.chunks;
-  Tile<G> w[U];
+  unsigned char* ring = s_mem + warp * (kDepth * Tile<G>::kBytes);
+  const uint32_t to = (uint32_t)__cvta_generic_to_shared(ring);
 #pragma unroll
-  for (int u = 0; u < U; ++u)
-    if (c0 + u < c1) w[u].load(p.codes, p.scales, base + c0 + u, lane);
+  for (int i = 0; i < kDepth; ++i) {
+    if (c0 + i < c1) Tile<G>::fetch(to + i * Tile<G>::kBytes, p.codes, p.scales, base + c0 + i, lane);
+    commit_copies();
+  }
   cudaTriggerProgrammaticLaunchCompletion();           // the next kernel may begin like this
   cudaGridDependencySynchronize();
   const int token = g / P, part = g % P;
   const bool in = token < p.M && token < 8 / P;
-  const T* x = p.x + (int64_t)(in ? token : 0) * p.K;
+  const T* x = p.x + (int64_t)(in ? token : 0) * p.K + t * 8;
+  const int left = p.K - t * 8;
   float acc[1][4] = {{0.f, 0.f, 0.f, 0.f}};
-  for (int c = c0; c < c1; c += U) {
-    uint4 xb[U][4];
+  uint4 xb[4];
+  auto inputs = [&](int c) {
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        xb[u][q] = column8(x, (c + u) * kTileK + q * 32 + t * 8, p.K, in && c + u < c1, part);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (c + u >= c1) break;
-      const Tile<G> now = w[u];
-      if (c + u + U < c1) w[u].load(p.codes, p.scales, base + c + u + U, lane);
-      multiply<H, G, 1>(now, acc, [&](int q, int) { return xb[u][q]; });
-    }
+    for (int q = 0; q < 4; ++q) xb[q] = column8(x, c * kTileK + q * 32, left, in, part);
+  };
+  if (c0 < c1) inputs(c0);
+#pragma unroll 2
+  for (int c = c0; c < c1; ++c) {
+    wait_copies<kDepth - 1>();
+    const int slot = (c - c0) % kDepth;
+    Tile<G> w;
+    w.take(ring + slot * Tile<G>::kBytes, lane);
+    const uint4 now[4] = {xb[0], xb[1], xb[2], xb[3]};
+    if (c + 1 < c1) inputs(c + 1);
+    // the slot's next tile: this lane has read what it overwrites
+    if (c + kDepth < c1)
+      Tile<G>::fetch(to + slot * Tile<G>::kBytes, p.codes, p.scales, base + c + kDepth, lane);
+    commit_copies();
+    multiply<H, G, 1>(w, acc, [&](int q, int) { return now[q]; });
   }
+  __syncthreads();                                     // the ring holds the sums now
+  float(*part_sums)[8][kTileRows] = reinterpret_cast<float(*)[8][kTileRows]>(s_mem);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) s_part[warp][2 * t + (i & 1)][g + (i >> 1) * 8] = acc[0][i];
+  for (int i = 0; i < 4; ++i) part_sums[warp][2 * t + (i & 1)][g + (i >> 1) * 8] = acc[0][i];
   __syncthreads();
   const int row = threadIdx.x & 15;
   for (int m = threadIdx.x >> 4; m < p.M; m += WK * 2) {
@@ -304,126 +345,137 @@ vector_kernel(const LinearParams<T> p) {
 #pragma unroll
     for (int k = 0; k < WK; ++k)
 #pragma unroll
-      for (int q = 0; q < P; ++q) sum += s_part[k][m * P + q][row];
+      for (int q = 0; q < P; ++q) sum += part_sums[k][m * P + q][row];
     p.y[(int64_t)m * p.N + (int64_t)blockIdx.x * kTileRows + row] = from_f32<T>(sum);
   }
 }
 
 // ---------------------------------------------------------------------------
-// More columns.  CTA = 8 warps on WR tiles of rows times NT * 8 columns, WK = 8 / WR
-// of them sharing K; a cluster of CTAs along x splits K further.  The columns'
-// inputs go through shared memory, kStageK at a time and the next stage while one
-// is used, as 16-bit rows 64 bytes (mod 128) apart, so that the lanes' 16-byte
-// reads meet no bank twice.
+// More columns.  CTA = 8 warps, a tile of 16 weight rows each, times NT * 8 columns;
+// a cluster of CTAs along x splits K.  The columns' inputs go through shared memory
+// for all warps, the codes for the warp that uses them, kStages stages of kStage
+// tiles of K in a ring; a column's inputs lie 64 bytes (mod 128) after those of the
+// one before, so that the lanes' 16-byte reads meet no bank twice.
 // ---------------------------------------------------------------------------
 constexpr int kWarps = 8;
 
-template <typename T, int NT, int WR> struct Shape {
+template <typename T, int G, int NT> struct Shape {
   static constexpr int kParts = Operand<T>::kParts;
   static constexpr int kTokens = NT * 8 / kParts;        // rows of x per CTA
-  static constexpr int kRows = WR * kTileRows, kCols = NT * 8;
-  static constexpr int kWK = kWarps / WR;
-  static constexpr int kStageK = NT == 8 ? 256 : 512;
-  static constexpr int kPitch = kStageK * 2 + 64;        // bytes of a column
-  static constexpr int kStageBytes = kCols * kPitch;
-  static constexpr int kSumBytes = kWK * kRows * (kCols + 1) * 4;
-  static constexpr int kShared = 2 * kStageBytes > kSumBytes ? 2 * kStageBytes : kSumBytes;
+  static constexpr int kRows = kWarps * kTileRows, kCols = NT * 8;
+  static constexpr int kStage = NT == 8 ? 1 : 2;         // tiles of K in a stage
+  static constexpr int kStages = 3;
+  static constexpr int kPitch = kStage * kTileK * 2 + 64;              // bytes of a column
+  static constexpr int kInputBytes = kCols * kPitch;
+  static constexpr int kStageBytes = kInputBytes + kWarps * kStage * Tile<G>::kBytes;
+  static constexpr int kSumPitch = kRows + 4;            // floats of a column's sums
+  static constexpr int kSumBytes = kCols * kSumPitch * 4;
+  static constexpr int kShared = kStages * kStageBytes > kSumBytes ? kStages * kStageBytes : kSumBytes;
 };
 
-__device__ __forceinline__ void copy16_async(uint32_t to, const void* from, bool in) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(in ? 16 : 0)
-               : "memory");
-}
-
-template <typename T, int G, int NT, int WR>
+template <typename T, int G, int NT>
 __global__ void __launch_bounds__(kWarps * 32, 2)
 rows_kernel(const LinearParams<T> p) {
   namespace cg = cooperative_groups;
-  using S = Shape<T, NT, WR>;
+  using S = Shape<T, G, NT>;
   using H = typename Operand<T>::Half;
-  constexpr int P = S::kParts, WK = S::kWK;
-  constexpr int kStage = S::kStageK / kTileK;            // chunks of a stage
+  constexpr int P = S::kParts;
   extern __shared__ __align__(128) unsigned char s_mem[];
   const cg::cluster_group cluster = cg::this_cluster();
   const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int wr = warp % WR, wk = warp / WR;
   const int g = lane >> 2, t = lane & 3;
-  const int tile = (int)(blockIdx.x / ctas) * WR + wr;
+  const int tile = (int)(blockIdx.x / ctas) * kWarps + warp;
   const int m0 = (int)blockIdx.y * S::kTokens;
   const int tokens = min(S::kTokens, p.M - m0);
   const int c0 = (int)((int64_t)p.chunks * rank / ctas), c1 = (int)((int64_t)p.chunks * (rank + 1) / ctas);
-  // a tile past the last reads the last one again
+  // a warp past the last tile computes that one again
   const int64_t base = (int64_t)min(tile, p.tiles - 1) * p.chunks;
+  const uint32_t shared = (uint32_t)__cvta_generic_to_shared(s_mem);
 
   float acc[NT][4];
 #pragma unroll
   for (int i = 0; i < NT * 4; ++i) (&acc[0][0])[i] = 0.f;
-  // stage s: inputs of chunks c0 + s * kStage ..; 8 inputs of a row of x per thread
-  // and step, zeros where there is no row or no input
-  constexpr int kSteps = kStage * 16;
-  auto fill = [&](int s) {
-    unsigned char* buf = s_mem + (s & 1) * S::kStageBytes;
-    const int k8 = threadIdx.x % kSteps, k = (c0 + s * kStage) * kTileK + k8 * 8;
+  auto fetch_codes = [&](int s, int slot) {              // of stage s: chunks c0 + s * kStage ..
+#pragma unroll
+    for (int i = 0; i < S::kStage; ++i)
+      if (c0 + s * S::kStage + i < c1)
+        Tile<G>::fetch(shared + slot * S::kStageBytes + S::kInputBytes + (warp * S::kStage + i) * Tile<G>::kBytes,
+                       p.codes, p.scales, base + c0 + s * S::kStage + i, lane);
+  };
+  // 8 inputs of a row of x per thread and step, zeros where there is no row or input
+  constexpr int kSteps = S::kStage * 16;
+  const int k8 = threadIdx.x % kSteps;
+  auto fetch_inputs = [&](int s, int slot) {
+    unsigned char* buf = s_mem + slot * S::kStageBytes + k8 * 16;
+    const uint32_t to = shared + slot * S::kStageBytes + k8 * 16;
+    const int k = (c0 + s * S::kStage) * kTileK + k8 * 8;
     for (int token = threadIdx.x / kSteps; token < S::kTokens; token += kWarps * 32 / kSteps) {
       const bool in = token < tokens;
       const T* x = p.x + (int64_t)(m0 + (in ? token : 0)) * p.K;
       if constexpr (P == 1) {
-        copy16_async((uint32_t)__cvta_generic_to_shared(buf + token * S::kPitch + k8 * 16),
-                     in && k < p.K ? x + k : x, in && k < p.K);
+        copy16_async(to + token * S::kPitch, in && k < p.K ? x + k : x, in && k < p.K);
       } else {
         const uint4 none = make_uint4(0, 0, 0, 0);
         const uint4 lo = in && k < p.K ? ldg16(x + k) : none;
         const uint4 hi = in && k + 4 < p.K ? ldg16(x + k + 4) : none;
 #pragma unroll
         for (int q = 0; q < P; ++q)
-          *reinterpret_cast<uint4*>(buf + (token * P + q) * S::kPitch + k8 * 16) = cut8(lo, hi, q);
+          *reinterpret_cast<uint4*>(buf + (token * P + q) * S::kPitch) = cut8(lo, hi, q);
       }
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
   };
   if constexpr (S::kTokens * P < S::kCols) {             // columns without a row of x
-    for (int i = threadIdx.x; i < 2 * (S::kCols - S::kTokens * P) * (S::kPitch / 16); i += kWarps * 32) {
-      const int half = i / ((S::kCols - S::kTokens * P) * (S::kPitch / 16));
-      const int rest = i % ((S::kCols - S::kTokens * P) * (S::kPitch / 16));
-      *reinterpret_cast<uint4*>(s_mem + half * S::kStageBytes + S::kTokens * P * S::kPitch + rest * 16) =
-          make_uint4(0, 0, 0, 0);
-    }
+    constexpr int kSpare = (S::kCols - S::kTokens * P) * (S::kPitch / 16);
+    for (int i = threadIdx.x; i < S::kStages * kSpare; i += kWarps * 32)
+      *reinterpret_cast<uint4*>(s_mem + i / kSpare * S::kStageBytes + S::kTokens * P * S::kPitch +
+                                i % kSpare * 16) = make_uint4(0, 0, 0, 0);
   }
-  Tile<G> w;
-  if (c0 + wk < c1) w.load(p.codes, p.scales, base + c0 + wk, lane);
+  const int stages = (c1 - c0 + S::kStage - 1) / S::kStage;
+  // the codes of the first stages are on their way before x is waited for
+#pragma unroll
+  for (int s = 0; s < S::kStages - 1; ++s) fetch_codes(s, s);
   cudaTriggerProgrammaticLaunchCompletion();             // the next kernel may begin like this
   cudaGridDependencySynchronize();
-  const int stages = (c1 - c0 + kStage - 1) / kStage;
-  if (stages > 0) fill(0);
-  for (int s = 0; s < stages; ++s) {
-    if (s + 1 < stages) {
-      fill(s + 1);
-      asm volatile("cp.async.wait_group 1;" ::: "memory");
-    } else {
-      asm volatile("cp.async.wait_group 0;" ::: "memory");
-    }
-    __syncthreads();
-    const unsigned char* buf = s_mem + (s & 1) * S::kStageBytes + g * S::kPitch + t * 16;
-    const int first = c0 + s * kStage, last = min(c1, first + kStage);
+#pragma unroll
+  for (int s = 0; s < S::kStages - 1; ++s) {
+    if (s < stages) fetch_inputs(s, s);
+    commit_copies();                                     // the first group holds all codes so far
+  }
+  int slot = 0;
 #pragma unroll 1
-    for (int c = first + wk; c < last; c += WK) {
-      const Tile<G> now = w;
-      if (c + WK < c1) w.load(p.codes, p.scales, base + c + WK, lane);
-      const unsigned char* xs = buf + (c - first) * (kTileK * 2);
-      multiply<H, G, NT>(now, acc, [&](int q, int n) {
+  for (int s = 0; s < stages; ++s) {
+    wait_copies<S::kStages - 2>();
+    __syncthreads();               // stage s has come; the one before it is no longer read
+    const int next = slot == 0 ? S::kStages - 1 : slot - 1;
+    if (s + S::kStages - 1 < stages) {
+      fetch_codes(s + S::kStages - 1, next);
+      fetch_inputs(s + S::kStages - 1, next);
+    }
+    commit_copies();
+    const unsigned char* buf = s_mem + slot * S::kStageBytes;
+#pragma unroll
+    for (int i = 0; i < S::kStage; ++i) {
+      if (c0 + s * S::kStage + i >= c1) break;
+      Tile<G> w;
+      w.take(buf + S::kInputBytes + (warp * S::kStage + i) * Tile<G>::kBytes, lane);
+      const unsigned char* xs = buf + g * S::kPitch + i * (kTileK * 2) + t * 16;
+      multiply<H, G, NT>(w, acc, [&](int q, int n) {
         return *reinterpret_cast<const uint4*>(xs + n * 8 * S::kPitch + q * 64);
       });
     }
-    __syncthreads();                                     // the stage after next overwrites it
+    slot = slot == S::kStages - 1 ? 0 : slot + 1;
   }
-  float* sums = reinterpret_cast<float*>(s_mem);         // [WK][rows][columns + 1]
+  wait_copies<0>();
+  __syncthreads();
+  // [columns][rows]: neighbouring lanes read neighbouring words of another CTA's sums
+  // (one by one they cost the SM-to-SM network a packet each)
+  float* sums = reinterpret_cast<float*>(s_mem);
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      sums[(wk * S::kRows + wr * kTileRows + g + (i >> 1) * 8) * (S::kCols + 1) + n * 8 + 2 * t +
-           (i & 1)] = acc[n][i];
+      sums[(n * 8 + 2 * t + (i & 1)) * S::kSumPitch + warp * kTileRows + g + (i >> 1) * 8] = acc[n][i];
   if (ctas > 1) cluster.sync(); else __syncthreads();
   // the outputs are split over the cluster; neighbouring threads write neighbouring
   // weight rows of one row of y
@@ -431,15 +483,20 @@ rows_kernel(const LinearParams<T> p) {
   for (int i = rank * kWarps * 32 + threadIdx.x; i < tokens * S::kRows; i += ctas * kWarps * 32) {
     const int token = i / S::kRows, row = i % S::kRows;
     if (row0 + row >= p.N) continue;
-    float sum = 0.f;
-    for (int c = 0; c < ctas; ++c) {
-      const float* from = ctas > 1 ? cluster.map_shared_rank(sums, c) : sums;
+    float v[8][P], sum = 0.f;                            // all loads, then the sum in order
 #pragma unroll
-      for (int k = 0; k < WK; ++k)
+    for (int c = 0; c < 8; ++c) {
+      if (c < ctas) {
+        const float* from = ctas > 1 ? cluster.map_shared_rank(sums, c) : sums;
 #pragma unroll
-        for (int q = 0; q < P; ++q)
-          sum += from[(k * S::kRows + row) * (S::kCols + 1) + token * P + q];
+        for (int q = 0; q < P; ++q) v[c][q] = from[(token * P + q) * S::kSumPitch + row];
+      }
     }
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+      if (c < ctas)
+#pragma unroll
+        for (int q = 0; q < P; ++q) sum += v[c][q];
     p.y[(int64_t)(m0 + token) * p.N + row0 + row] = from_f32<T>(sum);
   }
   if (ctas > 1) cluster.sync();      // this CTA's sums are read by the others
