@@ -131,35 +131,50 @@ dequantize_kernel(const Packed p, T* w) {
 template <typename T> struct Operand { using Half = T; static constexpr int kParts = 1; };
 template <> struct Operand<float> { using Half = __nv_bfloat16; static constexpr int kParts = 3; };
 
-template <typename H>
+// c = A B + (FRESH ? 0 : c).  Volatile: all lanes of a warp execute it together.
+template <typename H, bool FRESH>
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (std::is_same<H, __half>::value)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-        "{%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-        "{%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+#define ESA_MMA(T)                                                                               \
+  if constexpr (FRESH)                                                                           \
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32." T "." T ".f32 {%0,%1,%2,%3}, "         \
+                 "{%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"                                    \
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])                                \
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));      \
+  else                                                                                           \
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32." T "." T ".f32 {%0,%1,%2,%3}, "         \
+                 "{%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"                                        \
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])                                \
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1))
+  if constexpr (std::is_same<H, __half>::value) {
+    ESA_MMA("f16");
+  } else {
+    ESA_MMA("bf16");
+  }
+#undef ESA_MMA
 }
 
-// The four A registers of a word of codes.
+// The four A registers of a word of codes.  bf16 has room for a nibble at the low end
+// of its 7 bits only: 128 + n, less 136.  fp16 takes nibbles 0 and 1 of its 10 bits
+// where they lie: 1024 + n less 1032, (1024 + 16 n) / 16 less 72.
+__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t bits) {
+  uint32_t v;          // (w & mask) | bits: written out, else it is two instructions
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(v) : "r"(w), "r"(mask), "r"(bits));
+  return v;
+}
 template <typename H>
 __device__ __forceinline__ void expand(uint32_t w, uint32_t (&a)[4]) {
-  constexpr bool kHalf = std::is_same<H, __half>::value;
-  constexpr uint32_t kOne = kHalf ? 0x64006400u : 0x43004300u;       // 1024 or 128, twice
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    uint32_t v;      // (w >> 4 j) & 0x000f000f | kOne: written out, else it is two instructions
-    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(v) : "r"(w >> (4 * j)), "n"(0x000f000f), "r"(kOne));
-    if constexpr (kHalf) {
-      const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&v), __float2half2_rn(1032.f));
+    if constexpr (std::is_same<H, __half>::value) {
+      const uint32_t v = and_or(j < 2 ? w : w >> 8, j & 1 ? 0x00f000f0u : 0x000f000fu, 0x64006400u);
+      const __half2 h = *reinterpret_cast<const __half2*>(&v);
+      const __half2 d = j & 1 ? __hfma2(h, __float2half2_rn(0.0625f), __float2half2_rn(-72.f))
+                              : __hadd2(h, __float2half2_rn(-1032.f));
       a[j] = *reinterpret_cast<const uint32_t*>(&d);
     } else {
+      const uint32_t v = and_or(w >> (4 * j), 0x000f000fu, 0x43004300u);
       const __nv_bfloat162 d =
-          __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), __float2bfloat162_rn(136.f));
+          __hadd2(*reinterpret_cast<const __nv_bfloat162*>(&v), __float2bfloat162_rn(-136.f));
       a[j] = *reinterpret_cast<const uint32_t*>(&d);
     }
   }
@@ -258,16 +273,14 @@ __device__ __forceinline__ void multiply(const Tile<G>& w, float (&acc)[NT][4], 
     uint32_t a0[4], a1[4];
     expand<H>(w.word(2 * q), a0);
     expand<H>(w.word(2 * q + 1), a1);
-    if ((q * 32) % G == 0)
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sum[n][i] = 0.f;
     // products of the same sum apart from each other
 #pragma unroll
-    for (int n = 0; n < NT; ++n) mma<H>(sum[n], a0, b[q & 1][n].x, b[q & 1][n].y);
+    for (int n = 0; n < NT; ++n) {
+      if ((q * 32) % G == 0) mma<H, true>(sum[n], a0, b[q & 1][n].x, b[q & 1][n].y);
+      else mma<H, false>(sum[n], a0, b[q & 1][n].x, b[q & 1][n].y);
+    }
 #pragma unroll
-    for (int n = 0; n < NT; ++n) mma<H>(sum[n], a1, b[q & 1][n].z, b[q & 1][n].w);
+    for (int n = 0; n < NT; ++n) mma<H, false>(sum[n], a1, b[q & 1][n].z, b[q & 1][n].w);
     if ((q * 32 + 32) % G == 0) {
       const uint32_t s = w.s[q * 32 / G];
       const float lo = __uint_as_float(s << 16), hi = __uint_as_float(s & 0xffff0000u);
@@ -405,24 +418,30 @@ rows_kernel(const LinearParams<T> p) {
   };
   // 8 inputs of a row of x per thread and step, zeros where there is no row or input
   constexpr int kSteps = S::kStage * 16;
-  const int k8 = threadIdx.x % kSteps;
+  constexpr int kTokenStep = kWarps * 32 / kSteps;
+  const int k8 = threadIdx.x % kSteps, token0 = threadIdx.x / kSteps;
+  const T* const x0 = p.x + (int64_t)(m0 + min(token0, tokens - 1)) * p.K + (int64_t)c0 * kTileK + k8 * 8;
+  const int left = p.K - c0 * kTileK - k8 * 8;           // inputs of the row from there
   auto fetch_inputs = [&](int s, int slot) {
-    unsigned char* buf = s_mem + slot * S::kStageBytes + k8 * 16;
-    const uint32_t to = shared + slot * S::kStageBytes + k8 * 16;
-    const int k = (c0 + s * S::kStage) * kTileK + k8 * 8;
-    for (int token = threadIdx.x / kSteps; token < S::kTokens; token += kWarps * 32 / kSteps) {
-      const bool in = token < tokens;
-      const T* x = p.x + (int64_t)(m0 + (in ? token : 0)) * p.K;
+    unsigned char* buf = s_mem + slot * S::kStageBytes + k8 * 16 + token0 * P * S::kPitch;
+    const uint32_t to = shared + slot * S::kStageBytes + k8 * 16 + token0 * S::kPitch;
+    const int k = s * S::kStage * kTileK;
+    const T* x = x0 + k;
+#pragma unroll
+    for (int j = 0; j < (S::kTokens + kTokenStep - 1) / kTokenStep; ++j) {
+      const bool row = token0 + j * kTokenStep < tokens;
       if constexpr (P == 1) {
-        copy16_async(to + token * S::kPitch, in && k < p.K ? x + k : x, in && k < p.K);
-      } else {
+        const bool in = row && k < left;
+        copy16_async(to + j * kTokenStep * S::kPitch, in ? x : p.x, in);
+      } else if (token0 + j * kTokenStep < S::kTokens) {
         const uint4 none = make_uint4(0, 0, 0, 0);
-        const uint4 lo = in && k < p.K ? ldg16(x + k) : none;
-        const uint4 hi = in && k + 4 < p.K ? ldg16(x + k + 4) : none;
+        const uint4 lo = row && k < left ? ldg16(x) : none;
+        const uint4 hi = row && k + 4 < left ? ldg16(x + 4) : none;
 #pragma unroll
         for (int q = 0; q < P; ++q)
-          *reinterpret_cast<uint4*>(buf + (token * P + q) * S::kPitch) = cut8(lo, hi, q);
+          *reinterpret_cast<uint4*>(buf + (j * kTokenStep * P + q) * S::kPitch) = cut8(lo, hi, q);
       }
+      if (token0 + (j + 1) * kTokenStep < tokens) x += (int64_t)kTokenStep * p.K;
     }
   };
   if constexpr (S::kTokens * P < S::kCols) {             // columns without a row of x
