@@ -85,53 +85,67 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t w, int j) {
 }
 
 // ---------------------------------------------------------------------------
-// Rows into the cache and out of it.  A thread owns 8 elements of a head row (of
-// k and of v); D / 8 neighbouring threads a row; rows in the order [B, L, H], as a
-// projection leaves them.
+// Rows into the cache and out of it.  A thread owns 8 elements of a head row of k and
+// of v; D / 8 neighbouring threads a row; rows in the order [L, H], as a projection
+// leaves them, two per thread so that twice the loads are on their way.
 // ---------------------------------------------------------------------------
 struct Heads { const void* data; int64_t sb, sh, ss; };
 
-constexpr int kRowThreads = 256;
+constexpr int kRowThreads = 256, kRowsPerThread = 2;
 
 template <typename T> struct RowParams {
   Cache c;
   Span span;
   Heads k, v;
-  int64_t units;              // B * L * Hkv * D / 8
+  unsigned rows;              // L * Hkv, of one sequence (blockIdx.y)
   int* err;
 };
 
 template <int D> struct Unit {          // which 8 elements a thread owns
-  int64_t l;
-  int b, h, part;
+  static constexpr int kPer = D / 8, kRows = kRowThreads / kPer;       // rows of a CTA at a time
+  int64_t l, pos;
+  int h, part;
+  bool in;
   template <typename T>
-  __device__ __forceinline__ Unit(const RowParams<T>& p, int64_t u) {
-    constexpr int PER = D / 8;
-    part = (int)(u % PER);
-    const int64_t r = u / PER, bl = r / p.c.Hkv;
-    h = (int)(r % p.c.Hkv);
-    b = (int)(bl / p.span.L);
-    l = bl % p.span.L;
+  __device__ __forceinline__ Unit(const RowParams<T>& p, int i) {
+    part = threadIdx.x % kPer;
+    const unsigned r = (blockIdx.x * kRowsPerThread + i) * kRows + threadIdx.x / kPer;
+    in = r < p.rows;
+    const unsigned q = in ? r : p.rows - 1;
+    l = q / (unsigned)p.c.Hkv;
+    h = (int)(q % (unsigned)p.c.Hkv);
+    pos = p.span.position(blockIdx.y, l, p.c.S);
+    if (pos == -2 && in && p.err) atomicOr(p.err, kErrKvRange);
   }
+  __device__ __forceinline__ bool go() const { return in && pos >= 0; }
   // The words of keys hold 4 elements of this thread and 4 of the thread with the
   // next group: two words, shared by two threads.
-  __device__ __forceinline__ int key_word() const { return (part & 3) * (D / 32) + (part >> 3) * 2; }
-  __device__ __forceinline__ int value_word() const { return (part & 7) * (D / 64) + (part >> 3); }
+  __device__ __forceinline__ int key_word() const {
+    return ((part & 3) * (D / 32) + (part >> 3) * 2 + (part >> 2 & 1)) ^ turn();
+  }
+  __device__ __forceinline__ int value_word() const {
+    return (D / 8 + (part & 7) * (D / 64) + (part >> 3)) ^ turn();
+  }
+  __device__ __forceinline__ int turn() const { return (int)turn_of<D>((uint32_t)pos) / 4; }
+  __device__ __forceinline__ int64_t row(const Cache& c) const {
+    return ((int64_t)blockIdx.y * c.Hkv + h) * c.S + pos;
+  }
 };
 
 // Codes (one nibble each) and scale of 8 elements whose group is 4 neighbouring lanes.
-__device__ __forceinline__ uint32_t encode8(const float (&f)[8], float& s) {
+template <typename T>
+__device__ __forceinline__ uint32_t encode8(const uint4 (&v)[sizeof(T) / 2], float& s) {
+  float f[8];
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) Vec<T>::to_float(v[i], f + i * Vec<T>::kElems);
   uint32_t top = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) top = max(top, int4::abs_bits(f[e]));
   top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
   top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-  s = int4::group_scale(top);
-  const float inv = 1.f / s;
-  uint32_t w = 0;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) w |= int4::code_of(f[e], s, inv) << (4 * e);
-  return w;
+  float inv;
+  s = int4::group_scale(top, inv);
+  return int4::codes_of<T>(f, s, inv);
 }
 
 // Two threads, four lanes apart, with the nibbles of their 8 elements <-> the first
@@ -160,82 +174,83 @@ __device__ __forceinline__ uint32_t unmix_keys(uint32_t w, int part) {
 }
 
 template <typename T>
-__device__ __forceinline__ void load8(const Heads& h, int b, int head, int64_t l, int part, bool in,
-                                      float (&f)[8]) {
-  const T* p = static_cast<const T*>(h.data) + b * h.sb + head * h.sh + l * h.ss + part * 8;
-#pragma unroll
-  for (int i = 0; i < 8 / Vec<T>::kElems; ++i) {
-    const uint4 v = in ? ldg16_stream(p + i * Vec<T>::kElems) : make_uint4(0, 0, 0, 0);
-    Vec<T>::to_float(v, f + i * Vec<T>::kElems);
-  }
+__device__ __forceinline__ T* unit_address(const Heads& h, int head, int64_t l, int part) {
+  return static_cast<T*>(const_cast<void*>(h.data)) + blockIdx.y * h.sb + head * h.sh + l * h.ss + part * 8;
 }
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kRowThreads)
 write_kernel(const RowParams<T> p) {
-  const int64_t u = (int64_t)blockIdx.x * kRowThreads + threadIdx.x;
-  const bool in = u < p.units;
-  const Unit<D> e(p, in ? u : p.units - 1);
-  int64_t pos = p.span.position(e.b, e.l, p.c.S);
-  if (pos == -2 && in && p.err) atomicOr(p.err, kErrKvRange);
-  const bool go = in && pos >= 0;
-  float f[8], sk, sv;
-  load8<T>(p.k, e.b, e.h, e.l, e.part, go, f);
-  const uint32_t kw = mix_keys(encode8(f, sk), e.part) ^ 0x88888888u;
-  load8<T>(p.v, e.b, e.h, e.l, e.part, go, f);
-  const uint32_t vw = transpose8(encode8(f, sv), e.part & 7);
-  if (!go) return;
-  const int64_t row = ((int64_t)e.b * p.c.Hkv + e.h) * p.c.S + pos;
-  uint32_t* codes = reinterpret_cast<uint32_t*>(p.c.codes + row * D);
-  const int turn = (int)turn_of<D>((uint32_t)pos) / 4;
-  codes[(e.key_word() + (e.part >> 2 & 1)) ^ turn] = kw;
-  codes[(D / 8 + e.value_word()) ^ turn] = vw;
-  if ((e.part & 3) == 0) {
-    __nv_bfloat16* s = p.c.scales + row * (2 * D / kGroup) + (e.part >> 2);
-    s[0] = __float2bfloat16_rn(sk);
-    s[D / kGroup] = __float2bfloat16_rn(sv);
+  constexpr int N = sizeof(T) / 2;                     // 16-byte vectors of 8 elements
+  uint4 x[kRowsPerThread][2][N];
+#pragma unroll
+  for (int i = 0; i < kRowsPerThread; ++i) {
+    const Unit<D> u(p, i);
+    const T* k = unit_address<T>(p.k, u.h, u.l, u.part);
+    const T* v = unit_address<T>(p.v, u.h, u.l, u.part);
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      x[i][0][n] = u.go() ? ldg16_stream(k + n * Vec<T>::kElems) : make_uint4(0, 0, 0, 0);
+      x[i][1][n] = u.go() ? ldg16_stream(v + n * Vec<T>::kElems) : make_uint4(0, 0, 0, 0);
+    }
   }
-}
-
-template <typename T>
-__device__ __forceinline__ void store8(const Heads& h, int b, int head, int64_t l, int part,
-                                       uint32_t w, float s) {
-  T* p = static_cast<T*>(const_cast<void*>(h.data)) + b * h.sb + head * h.sh + l * h.ss + part * 8;
-  float f[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) f[e] = int4::decode(w >> (4 * e), s);
-#pragma unroll
-  for (int i = 0; i < 8 / Vec<T>::kElems; ++i)
-    stg16(p + i * Vec<T>::kElems, Vec<T>::from_float(f + i * Vec<T>::kElems));
+  for (int i = 0; i < kRowsPerThread; ++i) {
+    const Unit<D> u(p, i);
+    float sk, sv;
+    const uint32_t kw = mix_keys(encode8<T>(x[i][0], sk), u.part) ^ 0x88888888u;
+    const uint32_t vw = transpose8(encode8<T>(x[i][1], sv), u.part & 7);
+    if (!u.go()) continue;
+    const int64_t row = u.row(p.c);
+    uint32_t* codes = reinterpret_cast<uint32_t*>(p.c.codes + row * D);
+    codes[u.key_word()] = kw;
+    codes[u.value_word()] = vw;
+    if ((u.part & 3) == 0) {
+      __nv_bfloat16* s = p.c.scales + row * (2 * D / kGroup) + (u.part >> 2);
+      s[0] = __float2bfloat16_rn(sk);
+      s[D / kGroup] = __float2bfloat16_rn(sv);
+    }
+  }
 }
 
 // Rows outside the cache come out as zeros.
 template <typename T, int D>
 __global__ void __launch_bounds__(kRowThreads)
 read_kernel(const RowParams<T> p) {
-  const int64_t u = (int64_t)blockIdx.x * kRowThreads + threadIdx.x;
-  const bool in = u < p.units;
-  const Unit<D> e(p, in ? u : p.units - 1);
-  const int64_t pos = p.span.position(e.b, e.l, p.c.S);
-  const bool go = in && pos >= 0;
-  if (pos == -2 && in && p.err) atomicOr(p.err, kErrKvRange);
-  uint32_t kw = 0u, vw = 0x88888888u;
-  float sk = 0.f, sv = 0.f;
-  if (go) {
-    const int64_t row = ((int64_t)e.b * p.c.Hkv + e.h) * p.c.S + pos;
-    const uint32_t* codes = reinterpret_cast<const uint32_t*>(p.c.codes + row * D);
-    const int turn = (int)turn_of<D>((uint32_t)pos) / 4;
-    kw = __ldg(codes + ((e.key_word() + (e.part >> 2 & 1)) ^ turn));
-    vw = __ldg(codes + ((D / 8 + e.value_word()) ^ turn));
-    const __nv_bfloat16* s = p.c.scales + row * (2 * D / kGroup) + (e.part >> 2);
-    sk = __bfloat162float(s[0]);
-    sv = __bfloat162float(s[D / kGroup]);
+  constexpr int N = sizeof(T) / 2;
+  uint32_t w[kRowsPerThread][2];
+  float s[kRowsPerThread][2];
+#pragma unroll
+  for (int i = 0; i < kRowsPerThread; ++i) {
+    const Unit<D> u(p, i);
+    w[i][0] = 0u;
+    w[i][1] = 0x88888888u;
+    s[i][0] = s[i][1] = 0.f;
+    if (u.go()) {
+      const int64_t row = u.row(p.c);
+      const uint32_t* codes = reinterpret_cast<const uint32_t*>(p.c.codes + row * D);
+      w[i][0] = __ldg(codes + u.key_word());
+      w[i][1] = __ldg(codes + u.value_word());
+      const __nv_bfloat16* f = p.c.scales + row * (2 * D / kGroup) + (u.part >> 2);
+      s[i][0] = __bfloat162float(f[0]);
+      s[i][1] = __bfloat162float(f[D / kGroup]);
+    }
   }
-  kw = unmix_keys(kw, e.part) ^ 0x88888888u;
-  vw = transpose8(vw, e.part & 7);
-  if (!in) return;
-  store8<T>(p.k, e.b, e.h, e.l, e.part, kw, sk);
-  store8<T>(p.v, e.b, e.h, e.l, e.part, vw, sv);
+#pragma unroll
+  for (int i = 0; i < kRowsPerThread; ++i) {
+    const Unit<D> u(p, i);
+    const uint32_t kv[2] = {unmix_keys(w[i][0], u.part) ^ 0x88888888u, transpose8(w[i][1], u.part & 7)};
+    if (!u.in) continue;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      T* to = unit_address<T>(j ? p.v : p.k, u.h, u.l, u.part);
+      uint32_t out[4 * N];
+      int4::decode8<T>(kv[j], s[i][j], out);
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+        stg16(to + n * Vec<T>::kElems, make_uint4(out[4 * n], out[4 * n + 1], out[4 * n + 2], out[4 * n + 3]));
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------

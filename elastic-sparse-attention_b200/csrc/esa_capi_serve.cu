@@ -220,16 +220,19 @@ int cache_rows(const char* what, bool write, int32_t dtype, const esa_cache4_t* 
     p.span = {start, counts, start0, seq_len};
     p.k = heads_of(k);
     p.v = heads_of(v);
-    p.units = (int64_t)cache->batch * seq_len * cache->num_kv_heads * (cache->head_dim / 8);
+    const int64_t rows = seq_len * cache->num_kv_heads;
+    if (rows > kMaxGrid || cache->batch > 65535)
+      return fail(ESA_ERR_UNSUPPORTED, "%s: more than 2^31 rows of a sequence, or 65535 sequences", what);
+    p.rows = (unsigned)rows;
     p.err = err;
-    const int64_t grid = ceil_div(p.units, c4::kRowThreads);
-    if (grid > kMaxGrid) return fail(ESA_ERR_UNSUPPORTED, "%s: too many rows", what);
     return by_head_dim(cache->head_dim, [&](auto d) {
       constexpr int D = decltype(d)::value;
+      const dim3 grid((unsigned)ceil_div(rows, c4::Unit<D>::kRows * c4::kRowsPerThread),
+                      (unsigned)cache->batch);
       if (write)
-        c4::write_kernel<T, D><<<(unsigned)grid, c4::kRowThreads, 0, (cudaStream_t)stream>>>(p);
+        c4::write_kernel<T, D><<<grid, c4::kRowThreads, 0, (cudaStream_t)stream>>>(p);
       else
-        c4::read_kernel<T, D><<<(unsigned)grid, c4::kRowThreads, 0, (cudaStream_t)stream>>>(p);
+        c4::read_kernel<T, D><<<grid, c4::kRowThreads, 0, (cudaStream_t)stream>>>(p);
       return check_launch(what);
     });
   });

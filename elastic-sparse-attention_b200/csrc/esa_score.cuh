@@ -12,12 +12,11 @@
 //
 // Top alternatives: order by value (NaN above all), then by the lower index; as
 // one 64-bit key per element no two are equal.  The pass leaves each thread with
-// the maximum of its own elements.  The k-th largest of those 32 NW maxima is a
-// lower bound of the k-th largest element, so only the threads at or above it
-// hold candidates: their warps read those few threads' elements again (from L1 /
-// L2, some k / (32 NW) of the row) and keep a sorted list of 32, one key per
-// lane.  The lists of the warps, then of the CTAs of a row, are merged two by
-// two.
+// the maximum of its own elements.  The k-th largest of the maxima of at least 2 k
+// groups of threads is a lower bound of the k-th largest element, so only the
+// threads at or above it hold candidates: their warps read those few threads'
+// elements again (from L1 / L2) and keep a sorted list of 32, one key per lane.
+// The lists of the warps, then of the CTAs of a row, are merged two by two.
 //
 // A row belongs to a cluster of 1, 2, 4 or 8 CTAs (few rows: more CTAs per row),
 // joined through distributed shared memory in the same launch.
@@ -81,6 +80,13 @@ template <typename K> __device__ __forceinline__ K merge32(K mine, K other_rever
 
 struct Stats { float m, s0, s1; };
 
+// Largest of the warp's values, none a NaN: their bits in the order of signed integers.
+__device__ __forceinline__ float max_of_warp(float x) {
+  const int b = __float_as_int(x);
+  const int m = __reduce_max_sync(0xffffffffu, b ^ ((b >> 31) & 0x7fffffff));
+  return __int_as_float(m ^ ((m >> 31) & 0x7fffffff));
+}
+
 // The step of m when it grows; its exponential is 0 long before the bound, which
 // keeps its product with a sum finite.
 __device__ __forceinline__ float rescale(float from, float to) { return fmaxf(from - to, -1e25f); }
@@ -95,30 +101,64 @@ __device__ __forceinline__ Stats join(const Stats& a, const Stats& b) {
   return r;
 }
 
-// Largest of the elements of a 16-byte vector and m; NaNs are passed over.
+// Two 16-bit elements: the larger ones (NaNs passed over, or kept), x - m in float32.
+template <typename T> struct Pair;
+// kFloor: elements below it count as it, which keeps -infinity out of the products;
+// next to a maximum of kSafe or more their exponential is 0 either way.
+#define ESA_PAIR(T, PTXTYPE, ONE, FLOOR2, NONE, FLOOR, SAFE)                                 \
+  template <> struct Pair<T> {                                                               \
+    static constexpr uint32_t kFloor2 = FLOOR2, kNone = NONE;                                \
+    static constexpr float kFloor = FLOOR, kSafe = SAFE;                                     \
+    __device__ __forceinline__ static uint32_t larger(uint32_t a, uint32_t b) {              \
+      uint32_t r;                                                                            \
+      asm("max." PTXTYPE "x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));                       \
+      return r;                                                                              \
+    }                                                                                        \
+    __device__ __forceinline__ static uint32_t larger_nan(uint32_t a, uint32_t b) {          \
+      uint32_t r;                                                                            \
+      asm("max.NaN." PTXTYPE "x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));                   \
+      return r;                                                                              \
+    }                                                                                        \
+    /* the products with one are exact: two conversions and two sums in two instructions */  \
+    __device__ __forceinline__ static void minus(uint32_t x, float neg_m, float& a, float& b) { \
+      asm("{\n\t.reg .b16 l, h, one;\n\tmov.b32 {l, h}, %2;\n\tmov.b16 one, " ONE ";\n\t"     \
+          "fma.rn.f32." PTXTYPE " %0, l, one, %3;\n\tfma.rn.f32." PTXTYPE " %1, h, one, %3;\n\t}" \
+          : "=f"(a), "=f"(b)                                                                 \
+          : "r"(x), "f"(neg_m));                                                             \
+    }                                                                                        \
+  };
+ESA_PAIR(__nv_bfloat16, "bf16", "0x3F80", 0xfe80fe80u, 0xff80ff80u, -0x1p126f, -0x1p125f)
+ESA_PAIR(__half, "f16", "0x3C00", 0xfbfffbffu, 0xfc00fc00u, -65504.f, -65000.f)
+#undef ESA_PAIR
+template <> struct Pair<float> {
+  static constexpr uint32_t kNone = 0xff800000u;
+  static constexpr float kFloor = kLowest, kSafe = -INFINITY;      // nothing is raised
+};
+
+__device__ __forceinline__ uint32_t word_of(const uint4& v, int i) {
+  return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+}
+
+// Largest of the elements of the vectors; NaNs are passed over.
 template <typename T> __device__ __forceinline__ float vec_max(const uint4 (&x)[kUnroll]) {
   if constexpr (std::is_same<T, float>::value) {
-    float m = kLowest;
+    float m = -INFINITY;
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
       m = fmaxf(fmaxf(fmaxf(m, __uint_as_float(x[u].x)), fmaxf(__uint_as_float(x[u].y), __uint_as_float(x[u].z))),
                 __uint_as_float(x[u].w));
     return m;
   } else {
-    using H2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
-    auto h2 = [](const uint32_t& w) { return *reinterpret_cast<const H2*>(&w); };
-    H2 m = __hmax2(__hmax2(h2(x[0].x), h2(x[0].y)), __hmax2(h2(x[0].z), h2(x[0].w)));
+    uint32_t m = Pair<T>::kNone;
 #pragma unroll
-    for (int u = 1; u < kUnroll; ++u)
-      m = __hmax2(m, __hmax2(__hmax2(h2(x[u].x), h2(x[u].y)), __hmax2(h2(x[u].z), h2(x[u].w))));
-    return fmaxf(fmaxf(kLowest, (float)m.x), (float)m.y);
+    for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m = Pair<T>::larger(m, word_of(x[u], i));
+    float a, b;
+    Pair<T>::minus(m, -0.f, a, b);
+    return fmaxf(a, b);
   }
 }
-
-template <typename T> __device__ __forceinline__ uint32_t lowest_bits();   // two (one) of -infinity
-template <> __device__ __forceinline__ uint32_t lowest_bits<float>() { return 0xff800000u; }
-template <> __device__ __forceinline__ uint32_t lowest_bits<__nv_bfloat16>() { return 0xff80ff80u; }
-template <> __device__ __forceinline__ uint32_t lowest_bits<__half>() { return 0xfc00fc00u; }
 
 __device__ __forceinline__ void grow(Stats& s, float m) {
   if (m > s.m) {
@@ -176,7 +216,8 @@ fwd_kernel(const FwdParams<T> p) {
   constexpr int E = Vec<T>::kElems;
   __shared__ __align__(16) Stats s_stats[NW];
   __shared__ Stats s_cta;                       // read by the other CTAs of the row
-  __shared__ float s_max[TOP ? NW : 1][32];
+  __shared__ float s_max[64];
+  __shared__ float s_bound;
   __shared__ uint64_t s_list[TOP ? NW : 1][32];
   cudaGridDependencySynchronize();
   const cg::cluster_group cluster = cg::this_cluster();
@@ -185,77 +226,98 @@ fwd_kernel(const FwdParams<T> p) {
   const int64_t row = blockIdx.x / ctas;
   const T* x = p.logits + row * p.stride;
   const RowParts<T> parts(x, p.V);
-  const int64_t step = (int64_t)ctas * NW * 32;
-  const int64_t first = (int64_t)rank * NW * 32 + threadIdx.x;
+  const int nvec = (int)parts.nvec;                  // < 2^29
+  const int step = ctas * NW * 32, first = rank * NW * 32 + threadIdx.x;
 
-  Stats s = {kLowest, 0.f, 0.f};
-  for (int64_t i = first; i < parts.nvec; i += kUnroll * step) {
+  Stats s = {Pair<T>::kFloor, 0.f, 0.f};
+  float own_max = -INFINITY;
+  for (int i = first; i < nvec; i += kUnroll * step) {
     uint4 v[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      const uint32_t none = lowest_bits<T>();
+      const uint32_t none = Pair<T>::kNone;
       v[u] = make_uint4(none, none, none, none);
-      if (i + u * step < parts.nvec) v[u] = ldg16(parts.body + i + u * step);
+      if (i + u * step < nvec) v[u] = ldg16(parts.body + i + u * step);
     }
-    grow(s, vec_max<T>(v));
-    const F2 neg_m = f2(-s.m, -s.m), l2e = f2(kLog2e, kLog2e);
+    own_max = fmaxf(own_max, vec_max<T>(v));
+    grow(s, own_max);
     F2 s0 = f2(0.f, 0.f), s1 = f2(0.f, 0.f);
+    const F2 l2e = f2(kLog2e, kLog2e);
+    auto add = [&](float za, float zb) {
+      float a, b;
+      split(mul2(f2(za, zb), l2e), a, b);
+      const F2 pe = f2(ex2(a), ex2(b));
+      s0 = add2(s0, pe);
+      return pe;
+    };
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      float f[E];
-      Vec<T>::to_float(v[u], f);
+    for (int u = 0; u < kUnroll; ++u)
 #pragma unroll
-      for (int e = 0; e < E; e += 2) {
-        const F2 z = add2(f2(f[e], f[e + 1]), neg_m);
-        float a, b, za, zb;
-        split(mul2(z, l2e), a, b);
-        split(z, za, zb);
-        const F2 pe = f2(ex2(a), ex2(b));
-        s0 = add2(s0, pe);
-        s1 = fma2(pe, f2(fmaxf(za, kLowest), fmaxf(zb, kLowest)), s1);   // 0 * -inf is 0 here
+      for (int e = 0; e < 4; e += sizeof(T) == 4 ? 2 : 1) {
+        float za, zb;
+        if constexpr (sizeof(T) == 4) {
+          za = __uint_as_float(word_of(v[u], e)) - s.m;
+          zb = __uint_as_float(word_of(v[u], e + 1)) - s.m;
+          const F2 pe = add(za, zb);
+          s1 = fma2(pe, f2(fmaxf(za, kLowest), fmaxf(zb, kLowest)), s1);   // 0 * -inf is 0 here
+        } else {
+          Pair<T>::minus(Pair<T>::larger_nan(word_of(v[u], e), Pair<T>::kFloor2), -s.m, za, zb);
+          s1 = fma2(add(za, zb), f2(za, zb), s1);
+        }
       }
-    }
     float a, b;
     split(s0, a, b);
     s.s0 += a + b;
     split(s1, a, b);
     s.s1 += a + b;
   }
-  const float own_max = s.m;
+  const float warp_max = max_of_warp(own_max);
+  if (warp_max == -INFINITY) {         // nothing, or -infinity (and NaNs) alone
+    if (s.s0 == s.s0) s = {kLowest, 0.f, 0.f};
+  } else if (warp_max < Pair<T>::kSafe) {
+    // what was raised to the floor does count here: element by element
+    s = {kLowest, 0.f, 0.f};
+    for (int i = first; i < nvec; i += step)
+      for (int e = 0; e < E; ++e) add_one(s, (float)x[parts.head + (int64_t)i * E + e]);
+  }
   // the ragged ends: at most 2 (E - 1) < 32 elements, one per lane of one warp
   int64_t edge = -1;
   if (rank == 0 && warp == 0) {
     if (lane < parts.head) edge = lane;
-    else if (lane < parts.head + parts.tail) edge = parts.head + parts.nvec * E + lane - parts.head;
+    else if (lane < parts.head + parts.tail) edge = (int64_t)nvec * E + lane;
     if (edge >= 0) add_one(s, (float)x[edge]);
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    Stats t;
-    t.m = __shfl_xor_sync(0xffffffffu, s.m, o);
-    t.s0 = __shfl_xor_sync(0xffffffffu, s.s0, o);
-    t.s1 = __shfl_xor_sync(0xffffffffu, s.s1, o);
-    s = join(s, t);
+  {
+    const float m = max_of_warp(s.m), d = rescale(s.m, m), e = ex2(d * kLog2e), s0 = s.s0;
+    s = {m, warp_sum(s0 * e), warp_sum(e * (s.s1 + d * s0))};
   }
   if (lane == 0) s_stats[warp] = s;
-  if constexpr (TOP) s_max[warp][lane] = sort32(own_max, lane);
+  bool nans = false;
+  float bound = -INFINITY;
+  if constexpr (TOP) {
+    // maxima of groups of `span` lanes, at least 2 k of them where there are as many
+    int span = 32;
+    while (span > 1 && NW * 32 / span < 2 * p.top) span >>= 1;
+    float gm = own_max;
+    for (int o = span >> 1; o > 0; o >>= 1) gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, o));
+    if (threadIdx.x < 64) s_max[threadIdx.x] = -INFINITY;
+    __syncthreads();
+    if (lane % span == 0) s_max[threadIdx.x / span] = gm;
+    nans = __syncthreads_or(s.s0 != s.s0);
+    if (warp == 0) {
+      const float a = sort32(s_max[lane], lane);
+      const float b = sort32(s_max[32 + lane], lane);
+      const float top = merge32(a, __shfl_xor_sync(0xffffffffu, b, 31), lane);
+      if (lane == p.top - 1) s_bound = top;
+    }
+  }
   __syncthreads();
-  s = s_stats[0];
-#pragma unroll
-  for (int w = 1; w < NW; ++w) s = join(s, s_stats[w]);
 
   uint64_t list = 0;           // below every real key
   if constexpr (TOP) {
-    // the k-th largest of the threads' maxima
-#pragma unroll
-    for (int n = NW / 2; n >= 1; n >>= 1) {
-      if (warp < n)
-        s_max[warp][lane] = merge32(s_max[warp][lane], s_max[warp + n][31 - lane], lane);
-      __syncthreads();
-    }
-    float bound = s_max[0][p.top - 1];
-    const bool all = s.s0 != s.s0 || bound == kLowest;   // NaNs are above every bound
-    if (all) bound = -INFINITY;
+    // NaNs are above every bound, and what is masked below those there are
+    const bool all = nans || s_bound == -INFINITY;
+    if (!all) bound = s_bound;
     uint64_t worst = 0;
     auto offer = [&](bool candidate, float v, int64_t idx) {
       const uint64_t key = candidate ? key_of(v, (uint32_t)idx) : 0;
@@ -274,10 +336,9 @@ fwd_kernel(const FwdParams<T> p) {
     while (owners) {
       const int o = __ffs(owners) - 1;
       owners &= owners - 1;
-      const int64_t base = (int64_t)rank * NW * 32 + warp * 32 + o;
-      for (int64_t j = base; j < parts.nvec; j += 32 * step) {   // the same on every lane
-        const int64_t i = j + lane * step;
-        const bool in = i < parts.nvec;
+      for (int64_t j = rank * NW * 32 + warp * 32 + o; j < nvec; j += 32 * (int64_t)step) {   // the same on every lane
+        const int64_t i = j + lane * (int64_t)step;
+        const bool in = i < nvec;
         uint4 v = make_uint4(0, 0, 0, 0);
         if (in) v = ldg16(parts.body + i);
         float f[E];
@@ -299,6 +360,20 @@ fwd_kernel(const FwdParams<T> p) {
         s_list[warp][lane] = merge32(s_list[warp][lane], s_list[warp + n][31 - lane], lane);
       __syncthreads();
     }
+  }
+  if (warp == 0) {
+    s = s_stats[lane < NW ? lane : 0];
+#pragma unroll
+    for (int o = NW / 2; o > 0; o >>= 1) {
+      Stats t;
+      t.m = __shfl_xor_sync(0xffffffffu, s.m, o);
+      t.s0 = __shfl_xor_sync(0xffffffffu, s.s0, o);
+      t.s1 = __shfl_xor_sync(0xffffffffu, s.s1, o);
+      s = join(s, t);
+    }
+    s.m = __shfl_sync(0xffffffffu, s.m, 0);
+    s.s0 = __shfl_sync(0xffffffffu, s.s0, 0);
+    s.s1 = __shfl_sync(0xffffffffu, s.s1, 0);
   }
   if (ctas > 1) {
     if (threadIdx.x == 0) s_cta = s;

@@ -73,17 +73,18 @@ quantize_kernel(const Packed p, const T* w) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) top = max(top, int4::abs_bits(f[e]));
   for (int o = 1; o < p.group / 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-  const float s = int4::group_scale(top), inv = 1.f / s;
+  float inv;
+  const float s = int4::group_scale(top, inv);
+  const uint32_t w8 = int4::codes_of<T>(f, s, inv);
   const int g = k / p.group;
   if (part % (p.group / 8) == 0)
     p.scales[(tile * p.groups + g) * kTileRows + scale_place(r)] = __float2bfloat16_rn(s);
   const int shift = r >= 8 ? 4 : 0;                  // registers 1 and 3 hold rows 8 .. 15
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    uint32_t c[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) c[e] = int4::code_of(f[4 * i + e], s, inv);
-    s_words[threadIdx.x][i] = (c[0] | c[1] << 16 | c[2] << 8 | c[3] << 24) << shift;
+    const uint32_t c = w8 >> (16 * i);
+    s_words[threadIdx.x][i] =
+        ((c & 15u) | (c >> 4 & 15u) << 16 | (c >> 8 & 15u) << 8 | (c >> 12 & 15u) << 24) << shift;
   }
   __syncthreads();
   if (r >= 8) return;
@@ -300,7 +301,7 @@ __device__ __forceinline__ void multiply(const Tile<G>& w, float (&acc)[NT][4], 
 // its WK warps share K and join in shared memory.  A warp has kDepth tiles on their
 // way, and begins with that before it waits for the kernel before it (which made x).
 // ---------------------------------------------------------------------------
-constexpr int kDepth = 8;
+constexpr int kDepth = 4;
 
 template <typename T, int G, int WK>
 __global__ void __launch_bounds__(WK * 32)
