@@ -61,12 +61,6 @@ struct Span {
     const int64_t c = counts[b];
     return c < 0 ? 0 : c < L ? c : L;
   }
-  // Position of row l of sequence b; -1 padding, -2 outside the cache.
-  __device__ __forceinline__ int64_t position(int b, int64_t l, int64_t S) const {
-    if (l >= count(b)) return -1;
-    const int64_t s = begin(b);
-    return s < 0 || s >= S - l ? -2 : s + l;
-  }
 };
 
 // What the byte offsets within a row of 128-byte lines are combined with by XOR.
@@ -103,32 +97,53 @@ template <typename T> struct RowParams {
 
 template <int D> struct Unit {          // which 8 elements a thread owns
   static constexpr int kPer = D / 8, kRows = kRowThreads / kPer;       // rows of a CTA at a time
-  int64_t l, pos;
-  int h, part;
-  bool in;
-  template <typename T>
-  __device__ __forceinline__ Unit(const RowParams<T>& p, int i) {
-    part = threadIdx.x % kPer;
-    const unsigned r = (blockIdx.x * kRowsPerThread + i) * kRows + threadIdx.x / kPer;
-    in = r < p.rows;
-    const unsigned q = in ? r : p.rows - 1;
-    l = q / (unsigned)p.c.Hkv;
-    h = (int)(q % (unsigned)p.c.Hkv);
-    pos = p.span.position(blockIdx.y, l, p.c.S);
-    if (pos == -2 && in && p.err) atomicOr(p.err, kErrKvRange);
+  int l, pos, h;
+  bool in, go;                          // a row of the call; one that lies in the cache
+  // Rows [lo, hi) of the sequence have positions begin + l in the cache.
+  __device__ __forceinline__ void set(unsigned r, unsigned rows, unsigned heads, int begin, int lo,
+                                      int hi) {
+    in = r < rows;
+    const unsigned q = in ? r : rows - 1;
+    l = (int)(q / heads);
+    h = (int)(q - (unsigned)l * heads);
+    pos = begin + l;
+    go = in && l >= lo && l < hi;
   }
-  __device__ __forceinline__ bool go() const { return in && pos >= 0; }
+};
+
+// The units of a thread, and the part of the rows that it owns.
+template <int D> struct Units {
+  Unit<D> u[kRowsPerThread];
+  int part;
+  template <typename T>
+  __device__ __forceinline__ explicit Units(const RowParams<T>& p) {
+    part = threadIdx.x % Unit<D>::kPer;
+    const int64_t begin = p.span.begin(blockIdx.y), count = p.span.count(blockIdx.y);
+    // begin is clamped to a place outside the cache, so that 32 bits hold it
+    const int first = (int)(begin < -p.c.S ? -p.c.S : begin > p.c.S ? p.c.S : begin);
+    const int n = (int)count, lo = first < 0 ? min(-first, n) : 0;
+    const int hi = max(min(n, (int)p.c.S - first), lo);
+    if ((lo > 0 || hi < n) && threadIdx.x == 0 && blockIdx.x == 0 && p.err) atomicOr(p.err, kErrKvRange);
+#pragma unroll
+    for (int i = 0; i < kRowsPerThread; ++i)
+      u[i].set((blockIdx.x * kRowsPerThread + i) * Unit<D>::kRows + threadIdx.x / Unit<D>::kPer, p.rows,
+               (unsigned)p.c.Hkv, first, lo, hi);
+  }
   // The words of keys hold 4 elements of this thread and 4 of the thread with the
   // next group: two words, shared by two threads.
-  __device__ __forceinline__ int key_word() const {
-    return ((part & 3) * (D / 32) + (part >> 3) * 2 + (part >> 2 & 1)) ^ turn();
+  __device__ __forceinline__ int key_word(int i) const {
+    return ((part & 3) * (D / 32) + (part >> 3) * 2 + (part >> 2 & 1)) ^ turn(i);
   }
-  __device__ __forceinline__ int value_word() const {
-    return (D / 8 + (part & 7) * (D / 64) + (part >> 3)) ^ turn();
+  __device__ __forceinline__ int value_word(int i) const {
+    return (D / 8 + (part & 7) * (D / 64) + (part >> 3)) ^ turn(i);
   }
-  __device__ __forceinline__ int turn() const { return (int)turn_of<D>((uint32_t)pos) / 4; }
-  __device__ __forceinline__ int64_t row(const Cache& c) const {
-    return ((int64_t)blockIdx.y * c.Hkv + h) * c.S + pos;
+  __device__ __forceinline__ int turn(int i) const { return (int)turn_of<D>((uint32_t)u[i].pos) / 4; }
+  __device__ __forceinline__ int64_t row(const Cache& c, int i) const {
+    return (int64_t)(blockIdx.y * (unsigned)c.Hkv + (unsigned)u[i].h) * c.S + u[i].pos;
+  }
+  template <typename T> __device__ __forceinline__ T* address(const Heads& x, int i) const {
+    return static_cast<T*>(const_cast<void*>(x.data)) + blockIdx.y * x.sb + u[i].h * x.sh +
+           u[i].l * x.ss + part * 8;
   }
 };
 
@@ -173,38 +188,35 @@ __device__ __forceinline__ uint32_t unmix_keys(uint32_t w, int part) {
   return gather(a >> s) | gather(b >> s) << 16;
 }
 
-template <typename T>
-__device__ __forceinline__ T* unit_address(const Heads& h, int head, int64_t l, int part) {
-  return static_cast<T*>(const_cast<void*>(h.data)) + blockIdx.y * h.sb + head * h.sh + l * h.ss + part * 8;
-}
-
 template <typename T, int D>
 __global__ void __launch_bounds__(kRowThreads)
 write_kernel(const RowParams<T> p) {
   constexpr int N = sizeof(T) / 2;                     // 16-byte vectors of 8 elements
+  const Units<D> u(p);
   uint4 x[kRowsPerThread][2][N];
 #pragma unroll
   for (int i = 0; i < kRowsPerThread; ++i) {
-    const Unit<D> u(p, i);
-    const T* k = unit_address<T>(p.k, u.h, u.l, u.part);
-    const T* v = unit_address<T>(p.v, u.h, u.l, u.part);
+    const T* k = u.template address<T>(p.k, i);
+    const T* v = u.template address<T>(p.v, i);
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      x[i][0][n] = u.go() ? ldg16_stream(k + n * Vec<T>::kElems) : make_uint4(0, 0, 0, 0);
-      x[i][1][n] = u.go() ? ldg16_stream(v + n * Vec<T>::kElems) : make_uint4(0, 0, 0, 0);
+      x[i][0][n] = x[i][1][n] = make_uint4(0, 0, 0, 0);
+      if (u.u[i].go) {
+        x[i][0][n] = ldg16_stream(k + n * Vec<T>::kElems);
+        x[i][1][n] = ldg16_stream(v + n * Vec<T>::kElems);
+      }
     }
   }
 #pragma unroll
   for (int i = 0; i < kRowsPerThread; ++i) {
-    const Unit<D> u(p, i);
     float sk, sv;
     const uint32_t kw = mix_keys(encode8<T>(x[i][0], sk), u.part) ^ 0x88888888u;
     const uint32_t vw = transpose8(encode8<T>(x[i][1], sv), u.part & 7);
-    if (!u.go()) continue;
-    const int64_t row = u.row(p.c);
+    if (!u.u[i].go) continue;
+    const int64_t row = u.row(p.c, i);
     uint32_t* codes = reinterpret_cast<uint32_t*>(p.c.codes + row * D);
-    codes[u.key_word()] = kw;
-    codes[u.value_word()] = vw;
+    codes[u.key_word(i)] = kw;
+    codes[u.value_word(i)] = vw;
     if ((u.part & 3) == 0) {
       __nv_bfloat16* s = p.c.scales + row * (2 * D / kGroup) + (u.part >> 2);
       s[0] = __float2bfloat16_rn(sk);
@@ -218,19 +230,19 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kRowThreads)
 read_kernel(const RowParams<T> p) {
   constexpr int N = sizeof(T) / 2;
+  const Units<D> u(p);
   uint32_t w[kRowsPerThread][2];
   float s[kRowsPerThread][2];
 #pragma unroll
   for (int i = 0; i < kRowsPerThread; ++i) {
-    const Unit<D> u(p, i);
     w[i][0] = 0u;
     w[i][1] = 0x88888888u;
     s[i][0] = s[i][1] = 0.f;
-    if (u.go()) {
-      const int64_t row = u.row(p.c);
+    if (u.u[i].go) {
+      const int64_t row = u.row(p.c, i);
       const uint32_t* codes = reinterpret_cast<const uint32_t*>(p.c.codes + row * D);
-      w[i][0] = __ldg(codes + u.key_word());
-      w[i][1] = __ldg(codes + u.value_word());
+      w[i][0] = __ldg(codes + u.key_word(i));
+      w[i][1] = __ldg(codes + u.value_word(i));
       const __nv_bfloat16* f = p.c.scales + row * (2 * D / kGroup) + (u.part >> 2);
       s[i][0] = __bfloat162float(f[0]);
       s[i][1] = __bfloat162float(f[D / kGroup]);
@@ -238,12 +250,11 @@ read_kernel(const RowParams<T> p) {
   }
 #pragma unroll
   for (int i = 0; i < kRowsPerThread; ++i) {
-    const Unit<D> u(p, i);
     const uint32_t kv[2] = {unmix_keys(w[i][0], u.part) ^ 0x88888888u, transpose8(w[i][1], u.part & 7)};
-    if (!u.in) continue;
+    if (!u.u[i].in) continue;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      T* to = unit_address<T>(j ? p.v : p.k, u.h, u.l, u.part);
+      T* to = u.template address<T>(j ? p.v : p.k, i);
       uint32_t out[4 * N];
       int4::decode8<T>(kv[j], s[i][j], out);
 #pragma unroll

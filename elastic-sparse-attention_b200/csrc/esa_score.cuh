@@ -218,7 +218,8 @@ fwd_kernel(const FwdParams<T> p) {
   __shared__ Stats s_cta;                       // read by the other CTAs of the row
   __shared__ float s_max[64];
   __shared__ float s_bound;
-  __shared__ uint64_t s_list[TOP ? NW : 1][32];
+  __shared__ int s_count;
+  __shared__ uint64_t s_list[TOP ? NW : 1][32];  // also the elements found
   cudaGridDependencySynchronize();
   const cg::cluster_group cluster = cg::this_cluster();
   const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
@@ -305,10 +306,13 @@ fwd_kernel(const FwdParams<T> p) {
     if (lane % span == 0) s_max[threadIdx.x / span] = gm;
     nans = __syncthreads_or(s.s0 != s.s0);
     if (warp == 0) {
-      const float a = sort32(s_max[lane], lane);
-      const float b = sort32(s_max[32 + lane], lane);
-      const float top = merge32(a, __shfl_xor_sync(0xffffffffu, b, 31), lane);
+      float top = sort32(s_max[lane], lane);
+      if (NW * 32 / span > 32) {
+        const float b = sort32(s_max[32 + lane], lane);
+        top = merge32(top, __shfl_xor_sync(0xffffffffu, b, 31), lane);
+      }
       if (lane == p.top - 1) s_bound = top;
+      if (lane == 0) s_count = 0;
     }
   }
   __syncthreads();
@@ -318,47 +322,89 @@ fwd_kernel(const FwdParams<T> p) {
     // NaNs are above every bound, and what is masked below those there are
     const bool all = nans || s_bound == -INFINITY;
     if (!all) bound = s_bound;
-    uint64_t worst = 0;
-    auto offer = [&](bool candidate, float v, int64_t idx) {
-      const uint64_t key = candidate ? key_of(v, (uint32_t)idx) : 0;
-      uint32_t mask = __ballot_sync(0xffffffffu, key > worst);
-      while (mask) {
-        const uint64_t c = __shfl_sync(0xffffffffu, key, __ffs(mask) - 1);
-        mask &= mask - 1;
-        const int at = __popc(__ballot_sync(0xffffffffu, list > c));
-        const uint64_t up = __shfl_up_sync(0xffffffffu, list, 1);
-        if (at < 32) list = lane < at ? list : lane == at ? c : up;
-        worst = __shfl_sync(0xffffffffu, list, 31);
+    // Few elements reach the bound as a rule: a list of all of them, sorted by one
+    // warp (whose order does not depend on that of the list).
+    constexpr int kMost = 64;
+    uint64_t* const found = &s_list[0][0];
+    bool listed = !all;
+    if (listed) {
+      auto add = [&](float v, int64_t idx) {
+        const int at = atomicAdd(&s_count, 1);
+        if (at < kMost) found[at] = key_of(v, (uint32_t)idx);
+      };
+      if (edge >= 0 && (float)x[edge] >= bound) add((float)x[edge], edge);
+      uint32_t owners = __ballot_sync(0xffffffffu, own_max >= bound);
+      while (owners) {
+        const int o = __ffs(owners) - 1;
+        owners &= owners - 1;
+        for (int64_t i = rank * NW * 32 + warp * 32 + o + lane * (int64_t)step; i < nvec;
+             i += 32 * (int64_t)step) {
+          const uint4 v = ldg16(parts.body + i);
+          float f[E];
+          Vec<T>::to_float(v, f);
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            if (f[e] >= bound) add(f[e], parts.head + i * E + e);
+        }
       }
-    };
-    if (rank == 0 && warp == 0) offer(edge >= 0, edge >= 0 ? (float)x[edge] : 0.f, edge);
-    uint32_t owners = __ballot_sync(0xffffffffu, all || own_max >= bound);
-    while (owners) {
-      const int o = __ffs(owners) - 1;
-      owners &= owners - 1;
-      for (int64_t j = rank * NW * 32 + warp * 32 + o; j < nvec; j += 32 * (int64_t)step) {   // the same on every lane
-        const int64_t i = j + lane * (int64_t)step;
-        const bool in = i < nvec;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (in) v = ldg16(parts.body + i);
-        float f[E];
-        Vec<T>::to_float(v, f);
-        bool some = all;
-#pragma unroll
-        for (int e = 0; e < E; ++e) some = some || f[e] >= bound;
-        if (!__any_sync(0xffffffffu, in && some)) continue;
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-          offer(in && (all || f[e] >= bound), f[e], parts.head + i * E + e);
-      }
-    }
-    s_list[warp][lane] = list;
-    __syncthreads();
-#pragma unroll
-    for (int n = NW / 2; n >= 1; n >>= 1) {
-      if (warp < n)
-        s_list[warp][lane] = merge32(s_list[warp][lane], s_list[warp + n][31 - lane], lane);
       __syncthreads();
+      listed = s_count <= kMost;
+    }
+    if (listed) {
+      if (warp == 0) {
+        list = sort32(lane < s_count ? found[lane] : 0, lane);
+        if (s_count > 32) {
+          const uint64_t b = sort32(lane + 32 < s_count ? found[lane + 32] : 0, lane);
+          list = merge32(list, __shfl_xor_sync(0xffffffffu, b, 31), lane);
+        }
+        __syncwarp();
+        s_list[0][lane] = list;
+      }
+    } else {
+      // Many (equal values, or NaNs): each warp keeps the 32 largest of its elements.
+      __syncthreads();
+      uint64_t worst = 0;
+      auto offer = [&](bool candidate, float v, int64_t idx) {
+        const uint64_t key = candidate ? key_of(v, (uint32_t)idx) : 0;
+        uint32_t mask = __ballot_sync(0xffffffffu, key > worst);
+        while (mask) {
+          const uint64_t c = __shfl_sync(0xffffffffu, key, __ffs(mask) - 1);
+          mask &= mask - 1;
+          const int at = __popc(__ballot_sync(0xffffffffu, list > c));
+          const uint64_t up = __shfl_up_sync(0xffffffffu, list, 1);
+          if (at < 32) list = lane < at ? list : lane == at ? c : up;
+          worst = __shfl_sync(0xffffffffu, list, 31);
+        }
+      };
+      if (rank == 0 && warp == 0) offer(edge >= 0, edge >= 0 ? (float)x[edge] : 0.f, edge);
+      uint32_t owners = __ballot_sync(0xffffffffu, all || own_max >= bound);
+      while (owners) {
+        const int o = __ffs(owners) - 1;
+        owners &= owners - 1;
+        for (int64_t j = rank * NW * 32 + warp * 32 + o; j < nvec; j += 32 * (int64_t)step) {   // the same on every lane
+          const int64_t i = j + lane * (int64_t)step;
+          const bool in = i < nvec;
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (in) v = ldg16(parts.body + i);
+          float f[E];
+          Vec<T>::to_float(v, f);
+          bool some = all;
+#pragma unroll
+          for (int e = 0; e < E; ++e) some = some || f[e] >= bound;
+          if (!__any_sync(0xffffffffu, in && some)) continue;
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            offer(in && (all || f[e] >= bound), f[e], parts.head + i * E + e);
+        }
+      }
+      s_list[warp][lane] = list;
+      __syncthreads();
+#pragma unroll
+      for (int n = NW / 2; n >= 1; n >>= 1) {
+        if (warp < n)
+          s_list[warp][lane] = merge32(s_list[warp][lane], s_list[warp + n][31 - lane], lane);
+        __syncthreads();
+      }
     }
   }
   if (warp == 0) {
