@@ -11,9 +11,10 @@ from .cache import PackedKVCache
 from .decoder import ElasticDecoderStack
 from .head_split import HeadShardedElasticSparseAttention, head_share
 from .ops import PatternSpec
+from .serving import PackedDecoder
 from .sharded import SequenceShardedElasticSparseAttention
 
 __all__ = ["ElasticSparseAttention", "ElasticSparseAttentionFunction", "ElasticDecoderStack",
-           "HeadShardedElasticSparseAttention", "KeyPlanCache", "PackedKVCache", "PatternSpec",
+           "HeadShardedElasticSparseAttention", "KeyPlanCache", "PackedDecoder", "PackedKVCache", "PatternSpec",
            "SequenceShardedElasticSparseAttention", "head_share", "layer_ops", "ops", "_lib"]
-__version__ = "0.1.4"
+__version__ = "0.1.5"

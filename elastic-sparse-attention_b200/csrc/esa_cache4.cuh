@@ -598,7 +598,7 @@ attend_kernel(const AttendParams<T> p) {
       up *= 0.9999847412109375f;    // 1 - 2^-16
       down *= 1.00001525902189f;
     }
-    uint8_t* digits = reinterpret_cast<uint8_t*>(s_buf[warp]);
+    unsigned char* digits = reinterpret_cast<unsigned char*>(s_buf[warp]);
 #pragma unroll
     for (int c = 0; c < NG; ++c) {
       uint32_t d;
@@ -606,7 +606,7 @@ attend_kernel(const AttendParams<T> p) {
       if constexpr (VC == 2) d = __float_as_uint(fmaf(vs[c], up, 8388608.f));
       else d = __float2uint_rn(vs[c] * up);
 #pragma unroll
-      for (int i = 0; i < VC; ++i) digits[(c * VC + i) * 32 + t * 8 + g] = (uint8_t)(d >> (8 * i));
+      for (int i = 0; i < VC; ++i) digits[(c * VC + i) * 32 + t * 8 + g] = (unsigned char)(d >> (8 * i));
     }
     __syncwarp();
     int acc[MT][4], eights[NV][4];

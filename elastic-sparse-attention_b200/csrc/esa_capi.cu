@@ -780,7 +780,7 @@ void set_plan(esa::AttnParams& p, const void* plan, const PlanGeom& g) {
 
 extern "C" {
 
-int esa_version(void) { return 140; }
+int esa_version(void) { return 150; }
 
 const char* esa_last_error(void) { return g_last_error.c_str(); }
 

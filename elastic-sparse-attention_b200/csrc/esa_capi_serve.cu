@@ -211,6 +211,9 @@ int cache_rows(const char* what, bool write, int32_t dtype, const esa_cache4_t* 
   if (seq_len == 0 || cache->batch == 0) return ESA_OK;
   if (int rc = check_tensor("k", k, elem_size(dtype))) return rc;
   if (int rc = check_tensor("v", v, elem_size(dtype))) return rc;
+  const int64_t rows = seq_len * cache->num_kv_heads;
+  if (rows > kMaxGrid || cache->batch > 65535)
+    return fail(ESA_ERR_UNSUPPORTED, "%s: more than 2^31 rows of a sequence, or 65535 sequences", what);
   int* err = nullptr;
   if (int rc = device_error_word(&err)) return rc;
   return by_dtype(dtype, [&](auto tag) {
@@ -220,9 +223,6 @@ int cache_rows(const char* what, bool write, int32_t dtype, const esa_cache4_t* 
     p.span = {start, counts, start0, seq_len};
     p.k = heads_of(k);
     p.v = heads_of(v);
-    const int64_t rows = seq_len * cache->num_kv_heads;
-    if (rows > kMaxGrid || cache->batch > 65535)
-      return fail(ESA_ERR_UNSUPPORTED, "%s: more than 2^31 rows of a sequence, or 65535 sequences", what);
     p.rows = (unsigned)rows;
     p.err = err;
     return by_head_dim(cache->head_dim, [&](auto d) {
@@ -432,6 +432,11 @@ int esa_cache4_forward(int32_t dtype, const esa_cache4_t* cache, int32_t num_hea
   if (int rc = check_tensor("q", q, elem_size(dtype))) return rc;
   if (int rc = check_tensor("o", o, elem_size(dtype))) return rc;
   if (!lse) return fail(ESA_ERR_INVALID, "%s: null lse", what);
+  const int64_t pairs = (int64_t)cache->batch * num_heads * q_len;
+  const int64_t rows = num_heads / cache->num_kv_heads * q_len;
+  const int64_t kv = (int64_t)cache->batch * cache->num_kv_heads;
+  if (rows > kMaxGrid || kv > 65535)
+    return fail(ESA_ERR_UNSUPPORTED, "%s: more than 2^31 rows per K/V head, or 65535 K/V heads", what);
   int* err = nullptr;
   if (int rc = device_error_word(&err)) return rc;
   return by_dtype(dtype, [&](auto tag) {
@@ -443,11 +448,6 @@ int esa_cache4_forward(int32_t dtype, const esa_cache4_t* cache, int32_t num_hea
     p.o = heads_of(o);
     p.Hq = num_heads;
     p.G = num_heads / cache->num_kv_heads;
-    const int64_t pairs = (int64_t)cache->batch * num_heads * q_len;
-    const int64_t rows = p.G * q_len, kv = (int64_t)cache->batch * cache->num_kv_heads;
-    if (rows > kMaxGrid || kv > 65535)
-      return fail(ESA_ERR_UNSUPPORTED, "%s: more than 2^31 rows per K/V head, or 65535 K/V heads",
-                  what);
     p.rows = (unsigned)rows;
     p.pat = esa::make_pattern(heads, attn_length, layer_idx, num_hidden_layers, head_offset);
     p.scale_log2 = scale * esa::kLog2e;

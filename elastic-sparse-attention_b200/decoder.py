@@ -408,6 +408,45 @@ class _LMHeadCrossEntropy(torch.autograd.Function):
         return (dy * s.to(dy.dtype)).view(ctx.shape), (dw * s).to(ctx.w_dtype), None, None
 
 
+class _LMHeadLogProbs(torch.autograd.Function):
+    """(log probabilities of ``tokens`` (-100: 0), entropies) of softmax(y W^T), over
+    row chunks; the backward forms each chunk's logits again."""
+
+    @staticmethod
+    def forward(ctx, y, w, tokens, chunk: int):
+        ctx.set_materialize_grads(False)
+        y2, t = y.reshape(-1, y.shape[-1]), tokens.reshape(-1)
+        parts = [layer_ops.token_logprobs(torch.matmul(y2[s:s + chunk], w.t()), t[s:s + chunk])
+                 for s in range(0, y2.shape[0], chunk)]
+        logprobs, entropy, stats = (
+            torch.cat([getattr(p, name) for p in parts]) if parts
+            else torch.empty((0,) + tail, device=y.device)
+            for name, tail in (("logprobs", ()), ("entropy", ()), ("stats", (2,))))
+        ctx.save_for_backward(y, w, tokens, entropy, stats)
+        ctx.chunk = chunk
+        # entropy is saved: what is returned is another tensor, so that writing to it
+        # does not reach the backward
+        return logprobs.view(tokens.shape), entropy.clone().view(tokens.shape)
+
+    @staticmethod
+    @_first_derivative_only
+    def backward(ctx, dlogprobs, dentropy):
+        y, w, tokens, entropy, stats = ctx.saved_tensors
+        y2, t, chunk = y.reshape(-1, y.shape[-1]), tokens.reshape(-1), ctx.chunk
+        rows = [None if g is None else g.reshape(-1).float() for g in (dlogprobs, dentropy)]
+        dy = torch.empty_like(y2)
+        dw = torch.zeros(w.shape, dtype=torch.float32, device=w.device)
+        for s in range(0, y2.shape[0], chunk):
+            part = slice(s, s + chunk)
+            logits = torch.matmul(y2[part], w.t())
+            scores = layer_ops.TokenLogProbs(None, entropy[part], stats[part], None, None)
+            g = layer_ops.token_logprobs_backward(
+                logits, t[part], scores, *(None if r is None else r[part] for r in rows), out=logits)
+            dy[part] = torch.matmul(g, w)
+            dw += torch.matmul(g.t(), y2[part]).float()
+        return dy.view(y.shape), dw.to(w.dtype), None, None
+
+
 class ElasticDecoderLayerWeights(nn.Module):
     """The parameters of one decoder layer (pre-norm, fused QKV and gate/up)."""
 
@@ -558,6 +597,20 @@ class ElasticDecoderStack(nn.Module):
         targets = torch.full_like(labels, -100)
         targets[:, :-1] = labels[:, 1:]
         return _LMHeadCrossEntropy.apply(y, self.lm_head, targets, self.loss_chunk_rows)
+
+    def token_logprobs(self, input_ids: torch.Tensor, labels: torch.Tensor | None = None,
+                       positions: torch.Tensor | None = None):
+        """(log probabilities, entropies), float32 [B, L]: of each row's next token in
+        ``labels`` (shifted by one as in :meth:`forward`, -100 ignored: 0; default:
+        ``input_ids``), and of the row's distribution over the vocabulary.  The last
+        row of a sequence has no next token: 0 and its entropy.  Both are
+        differentiable (policy gradients, distillation); the [L, vocab] logits exist
+        ``loss_chunk_rows`` rows at a time, in the backward again."""
+        labels = input_ids if labels is None else labels
+        targets = torch.full_like(labels, layer_ops.IGNORED_TOKEN)
+        targets[:, :-1] = labels[:, 1:]
+        return _LMHeadLogProbs.apply(self(input_ids, positions=positions), self.lm_head, targets,
+                                     self.loss_chunk_rows)
 
     def flops_per_token(self, seq_len: int) -> float:
         """Dense GEMM FLOPs per token of one forward + backward (3 x 2 x
