@@ -13,6 +13,7 @@ import ctypes
 import torch
 
 from . import _lib
+from .layer_ops import _empty
 from .ops import MAX_POSITION, _check_device, _span_args
 
 CACHE_GROUP = 32
@@ -113,7 +114,7 @@ class PackedKVCache:
         out = []
         for name, t in (("k_out", k_out), ("v_out", v_out)):
             if t is None:
-                t = torch.empty(shape, dtype=dtype, device=dev)
+                t = _empty(shape, dtype, dev)
             elif tuple(t.shape) != shape or t.dtype != dtype or t.device != dev:
                 raise ValueError(f"{name} must be {list(shape)} in {dtype} on {dev}")
             out.append(t)

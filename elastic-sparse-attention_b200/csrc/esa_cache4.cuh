@@ -36,6 +36,7 @@
 // warps of a CTA and joined in shared memory.
 #pragma once
 #include "esa_int4.cuh"
+#include "esa_pack8.cuh"
 
 namespace esa {
 namespace cache4 {
@@ -147,18 +148,42 @@ template <int D> struct Units {
   }
 };
 
-// Codes (one nibble each) and scale of 8 elements whose group is 4 neighbouring lanes.
+// Largest magnitudes (float bits, NaN above infinity above finite) of the groups of
+// two times 8 elements, a group being 4 neighbouring lanes.  16-bit types compare two
+// elements per instruction and carry both groups through one chain of shuffles.
 template <typename T>
-__device__ __forceinline__ uint32_t encode8(const uint4 (&v)[sizeof(T) / 2], float& s) {
-  float f[8];
+__device__ __forceinline__ void group_max(const uint4 (&x)[2][sizeof(T) / 2], uint32_t (&top)[2]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+        m = max(max(m, max(x[j][n].x & 0x7fffffffu, x[j][n].y & 0x7fffffffu)),
+                max(x[j][n].z & 0x7fffffffu, x[j][n].w & 0x7fffffffu));
+      m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      top[j] = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    }
+  } else {
+    using M = pack8::Max2<T>;
+    uint32_t m[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      m[j] = M::abs_max(M::abs_max(x[j][0].x, x[j][0].y), M::abs_max(x[j][0].z, x[j][0].w));
+    uint32_t r = M::abs_max(__byte_perm(m[0], m[1], 0x5410), __byte_perm(m[0], m[1], 0x7632));
+    r = M::abs_max(r, __shfl_xor_sync(0xffffffffu, r, 1));
+    r = M::abs_max(r, __shfl_xor_sync(0xffffffffu, r, 2));
+    top[0] = pack8::magnitude_bits<T>(r);
+    top[1] = pack8::magnitude_bits<T>(r >> 16);
+  }
+}
+
+// Codes (one nibble each) of 8 elements, and their group's scale.
+template <typename T>
+__device__ __forceinline__ uint32_t encode8(const uint4 (&v)[sizeof(T) / 2], uint32_t top, float& s) {
+  float f[8], inv;
 #pragma unroll
   for (int i = 0; i < (int)sizeof(T) / 2; ++i) Vec<T>::to_float(v[i], f + i * Vec<T>::kElems);
-  uint32_t top = 0;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) top = max(top, int4::abs_bits(f[e]));
-  top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-  top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-  float inv;
   s = int4::group_scale(top, inv);
   return int4::codes_of<T>(f, s, inv);
 }
@@ -210,8 +235,10 @@ write_kernel(const RowParams<T> p) {
 #pragma unroll
   for (int i = 0; i < kRowsPerThread; ++i) {
     float sk, sv;
-    const uint32_t kw = mix_keys(encode8<T>(x[i][0], sk), u.part) ^ 0x88888888u;
-    const uint32_t vw = transpose8(encode8<T>(x[i][1], sv), u.part & 7);
+    uint32_t top[2];
+    group_max<T>(x[i], top);
+    const uint32_t kw = mix_keys(encode8<T>(x[i][0], top[0], sk), u.part) ^ 0x88888888u;
+    const uint32_t vw = transpose8(encode8<T>(x[i][1], top[1], sv), u.part & 7);
     if (!u.u[i].go) continue;
     const int64_t row = u.row(p.c, i);
     uint32_t* codes = reinterpret_cast<uint32_t*>(p.c.codes + row * D);

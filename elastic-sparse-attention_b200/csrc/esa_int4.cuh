@@ -60,6 +60,12 @@ __device__ __forceinline__ float decode(uint32_t nibble, float s) {
   return (float)((int)(nibble & 15u) - 8) * s;
 }
 
+__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t bits) {
+  uint32_t v;          // (w & mask) | bits: written out, else it is two instructions
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(v) : "r"(w), "r"(mask), "r"(bits));
+  return v;
+}
+
 // The values of the 8 nibbles of w (code + 8) in T, two (one) per word.  For bf16 the
 // product of the code and the scale in bf16 is the rounding of their exact product;
 // so for fp16 where the scale is one of its normal numbers.
@@ -78,7 +84,7 @@ __device__ __forceinline__ void decode8(uint32_t w, float s, uint32_t (&out)[2 *
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         // 1024 + n (fp16) or 128 + n (bf16)
-        const uint32_t v = ((w >> (4 * j)) & 0x000f000fu) | (kHalf ? 0x64006400u : 0x43004300u);
+        const uint32_t v = and_or(w >> (4 * j), 0x000f000fu, kHalf ? 0x64006400u : 0x43004300u);
         if constexpr (kHalf) {
           const __half2 d = __hmul2(__hadd2(*reinterpret_cast<const __half2*>(&v), __float2half2_rn(-1032.f)),
                                     __float2half2_rn(s));

@@ -157,23 +157,18 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
 // The four A registers of a word of codes.  bf16 has room for a nibble at the low end
 // of its 7 bits only: 128 + n, less 136.  fp16 takes nibbles 0 and 1 of its 10 bits
 // where they lie: 1024 + n less 1032, (1024 + 16 n) / 16 less 72.
-__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t bits) {
-  uint32_t v;          // (w & mask) | bits: written out, else it is two instructions
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(v) : "r"(w), "r"(mask), "r"(bits));
-  return v;
-}
 template <typename H>
 __device__ __forceinline__ void expand(uint32_t w, uint32_t (&a)[4]) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     if constexpr (std::is_same<H, __half>::value) {
-      const uint32_t v = and_or(j < 2 ? w : w >> 8, j & 1 ? 0x00f000f0u : 0x000f000fu, 0x64006400u);
+      const uint32_t v = int4::and_or(j < 2 ? w : w >> 8, j & 1 ? 0x00f000f0u : 0x000f000fu, 0x64006400u);
       const __half2 h = *reinterpret_cast<const __half2*>(&v);
       const __half2 d = j & 1 ? __hfma2(h, __float2half2_rn(0.0625f), __float2half2_rn(-72.f))
                               : __hadd2(h, __float2half2_rn(-1032.f));
       a[j] = *reinterpret_cast<const uint32_t*>(&d);
     } else {
-      const uint32_t v = and_or(w >> (4 * j), 0x000f000fu, 0x43004300u);
+      const uint32_t v = int4::and_or(w >> (4 * j), 0x000f000fu, 0x43004300u);
       const __nv_bfloat162 d =
           __hadd2(*reinterpret_cast<const __nv_bfloat162*>(&v), __float2bfloat162_rn(-136.f));
       a[j] = *reinterpret_cast<const uint32_t*>(&d);

@@ -318,7 +318,7 @@ def forward_packed(q: torch.Tensor, cache, spec: PatternSpec, scale: float, star
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev:
         raise ValueError("out must match q")
     start, start0, counts = _span_args(B, start, counts, dev)
-    lse = torch.empty((B, Hq, L), dtype=torch.float32, device=dev)
+    lse = torch.empty_strided((B, Hq, L), (Hq * L, L, 1), dtype=torch.float32, device=dev)
     _lib.launch(_lib.load().esa_cache4_forward, dev, _lib.DTYPES[q.dtype],
                 ctypes.byref(cache.struct()), Hq, L, spec.attention_length, spec.layer_idx,
                 spec.num_hidden_layers, spec.pattern_heads, spec.head_offset, scale,
