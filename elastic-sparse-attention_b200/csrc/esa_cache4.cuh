@@ -658,8 +658,10 @@ attend_kernel(const AttendParams<T> p) {
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        mma<false>(acc[4 * c + j], x[0][j] & kLow, x[0][j] & kHigh, x[1][j] & kLow,
-                          x[1][j] & kHigh, vb[(2 * c + j / 2) / GT]);
+        // whole bytes for the high nibbles: 16 times them and the low ones, whose sum is
+        // there too
+        mma<false>(acc[4 * c + j], x[0][j] & kLow, x[0][j], x[1][j] & kLow, x[1][j],
+                   vb[(2 * c + j / 2) / GT]);
     }
     // the columns of this lane belong to one group of each set
 #pragma unroll
@@ -678,7 +680,7 @@ attend_kernel(const AttendParams<T> p) {
           }
         }
         total[nv][j][0] = fmaf((float)(lo - off), down, total[nv][j][0] * corr);
-        total[nv][j][1] = fmaf((float)(hi - off16), down * 0.0625f, total[nv][j][1] * corr);
+        total[nv][j][1] = fmaf((float)(hi - lo - off16), down * 0.0625f, total[nv][j][1] * corr);
       }
     }
   }
@@ -686,7 +688,9 @@ attend_kernel(const AttendParams<T> p) {
   // ---- the warps of a pair ----
 #pragma unroll
   for (int nv = 0; nv < NV; ++nv) {
-    const bool bad = (nans >> (nv * GT + owner)) & 1u;
+    if (nans && ((nans >> (nv * GT + owner)) & 1u))
+#pragma unroll
+      for (int j = 0; j < 4; ++j) (&total[nv][0][0])[j] = __uint_as_float(0x7fffffffu);
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -694,7 +698,6 @@ attend_kernel(const AttendParams<T> p) {
         float v = total[nv][j][r];
         if constexpr (VC == 4)                        // digits 2 and 3 are with the odd lanes
           v = fmaf(__shfl_xor_sync(0xffffffffu, v, 1), 65536.f, v);
-        if (bad) v = __uint_as_float(0x7fffffffu);
         const int gr = nv * GT + owner;
         if (gr < NG && (VC == 2 || (t & 1) == 0))
           s_buf[warp][gr * kGroup + j * 16 + r * 8 + g] = __float_as_uint(v);

@@ -459,7 +459,7 @@ int esa_cache4_forward(int32_t dtype, const esa_cache4_t* cache, int32_t num_hea
     p.warps_per_pair = wpp;
     // many pairs: several per warp, as long as every SM has its CTAs
     int ppw = 1;
-    while (wpp == 1 && ppw < 16 && pairs >= (int64_t)kSms * 20 * ppw * 4) ppw *= 2;
+    while (wpp == 1 && ppw < 4 && pairs >= (int64_t)kSms * 20 * ppw * 4) ppw *= 2;
     p.pairs_per_warp = ppw;
     const dim3 grid((unsigned)ceil_div(rows, c4::kAttendWarps / wpp * ppw), (unsigned)kv);
     return by_head_dim(cache->head_dim, [&](auto d) {
