@@ -2,6 +2,7 @@
 // their gradient, products with weights in 4 bits, the key / value cache in 4 bits
 // and the attention over it.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include "esa_layer.h"
@@ -39,7 +40,7 @@ int launch_clusters(const char* what, void (*kernel)(const Q), dim3 grid, dim3 b
   a[1].val.clusterDim.y = 1;
   a[1].val.clusterDim.z = 1;
   c.attrs = a;
-  c.numAttrs = 2;
+  c.numAttrs = ctas > 1 ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&c, kernel, params);
   if (e != cudaSuccess) {
     cudaGetLastError();
@@ -102,13 +103,20 @@ w4::Packed packed(int64_t n, int64_t k, int32_t group, const void* codes, const 
   return p;
 }
 
+// Allows `kernel` its shared memory on the current device, once per device (the call
+// takes a good part of a launch's time on the host).  `done` is the kernel's own.
 template <typename K>
-int reserve_shared(const char* what, K* kernel, int bytes) {
-  if (bytes > 48 * 1024 &&
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
+int reserve_shared(const char* what, K* kernel, int bytes, std::atomic<uint64_t>& done) {
+  if (bytes <= 48 * 1024) return ESA_OK;
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) device = 64;
+  const uint64_t bit = device < 64 ? uint64_t(1) << device : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return ESA_OK;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
     cudaGetLastError();
     return fail(ESA_ERR_CUDA, "%s: cannot reserve %d bytes of shared memory", what, bytes);
   }
+  done.fetch_or(bit, std::memory_order_relaxed);
   return ESA_OK;
 }
 
@@ -120,7 +128,8 @@ int linear_vector(const w4::LinearParams<T>& p, cudaStream_t s) {
     constexpr int WK = decltype(wk)::value;
     constexpr int kShared = WK * w4::kDepth * w4::Tile<G>::kBytes;
     auto* kernel = w4::vector_kernel<T, G, WK>;
-    if (int rc = reserve_shared("esa_linear4", kernel, kShared)) return rc;
+    static std::atomic<uint64_t> done{0};
+    if (int rc = reserve_shared("esa_linear4", kernel, kShared, done)) return rc;
     return launch_clusters("esa_linear4", kernel, dim3((unsigned)p.tiles), dim3(WK * 32), 1, s, p,
                            kShared);
   };
@@ -134,18 +143,20 @@ int linear_vector(const w4::LinearParams<T>& p, cudaStream_t s) {
   }
 }
 
-// More columns: K is split over a cluster until there are two CTAs per SM, with two
-// stages at least.
+// More columns: K is split over a cluster until there are up to three CTAs per SM
+// (two are resident: 32 x 4096 x 12288 takes 18 us with 384 CTAs, 21 with 192), with
+// two stages at least.
 template <typename T, int G, int NT>
 int linear_rows(const w4::LinearParams<T>& p, cudaStream_t s) {
   using S = w4::Shape<T, G, NT>;
   const int64_t row_ctas = ceil_div(p.tiles, w4::kWarps), col_ctas = ceil_div(p.M, S::kTokens);
   if (col_ctas > 65535) return fail(ESA_ERR_UNSUPPORTED, "esa_linear4: too many rows");
   int ctas = 1;
-  while (ctas < 8 && row_ctas * col_ctas * ctas * 2 <= kSms * 2 && p.chunks >= ctas * 2 * 2 * S::kStage)
+  while (ctas < 8 && row_ctas * col_ctas * ctas * 2 <= kSms * 3 && p.chunks >= ctas * 2 * 2 * S::kStage)
     ctas *= 2;
   auto* kernel = w4::rows_kernel<T, G, NT>;
-  if (int rc = reserve_shared("esa_linear4", kernel, S::kShared)) return rc;
+  static std::atomic<uint64_t> done{0};
+  if (int rc = reserve_shared("esa_linear4", kernel, S::kShared, done)) return rc;
   return launch_clusters("esa_linear4", kernel, dim3((unsigned)(row_ctas * ctas), (unsigned)col_ctas),
                          dim3(w4::kWarps * 32), ctas, s, p, S::kShared);
 }
@@ -153,7 +164,10 @@ int linear_rows(const w4::LinearParams<T>& p, cudaStream_t s) {
 template <typename T, int G>
 int linear(const w4::LinearParams<T>& p, cudaStream_t s) {
   const int64_t cols = (int64_t)p.M * w4::Operand<T>::kParts;
-  if (cols <= 8) return linear_vector<T, G>(p, s);
+  // float32 rows are cut in three parts, which a CTA of 128 weight rows does once where
+  // eight of 16 do it each (2 x 4096 x 4096: 12 -> 6 us)
+  if constexpr (w4::Operand<T>::kParts == 1)
+    if (cols <= 8) return linear_vector<T, G>(p, s);
   if (cols <= 16) return linear_rows<T, G, 2>(p, s);
   if (cols <= 32) return linear_rows<T, G, 4>(p, s);
   return linear_rows<T, G, 8>(p, s);

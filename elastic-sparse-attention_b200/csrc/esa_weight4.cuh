@@ -372,14 +372,17 @@ template <typename T, int G, int NT> struct Shape {
   static constexpr int kParts = Operand<T>::kParts;
   static constexpr int kTokens = NT * 8 / kParts;        // rows of x per CTA
   static constexpr int kRows = kWarps * kTileRows, kCols = NT * 8;
-  static constexpr int kStage = NT == 8 ? 1 : 2;         // tiles of K in a stage
-  static constexpr int kStages = 3;
+  // Tiles of K in a stage and stages in the ring, so that two CTAs fit an SM (a third
+  // of the speed is lost where one does).
+  static constexpr int kStage = NT == 2 ? 2 : 1;
+  static constexpr int kStages = NT == 4 ? 5 : 3;
   static constexpr int kPitch = kStage * kTileK * 2 + 64;              // bytes of a column
   static constexpr int kInputBytes = kCols * kPitch;
   static constexpr int kStageBytes = kInputBytes + kWarps * kStage * Tile<G>::kBytes;
   static constexpr int kSumPitch = kRows + 4;            // floats of a column's sums
   static constexpr int kSumBytes = kCols * kSumPitch * 4;
   static constexpr int kShared = kStages * kStageBytes > kSumBytes ? kStages * kStageBytes : kSumBytes;
+  static_assert(kShared <= 112 * 1024, "two CTAs per SM");
 };
 
 template <typename T, int G, int NT>

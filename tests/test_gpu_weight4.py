@@ -69,7 +69,7 @@ def test_codes_are_exact(lops, dtype, group, kind, n, k):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_extreme_groups(lops, dtype):
-    w = torch.randn(20, 256, device=DEV).to(dtype)
+    w = torch.randn(20, 256, generator=torch.Generator().manual_seed(1)).to(DEV, dtype)
     w[1, 3] = math.nan
     w[2, 200] = math.inf
     w[3, 40] = -math.inf
@@ -137,13 +137,18 @@ def test_linear_large(lops, dtype):
 
 def test_float32_rows_keep_their_bits(lops):
     """x with 24 significant bits and a wide range, against a weight of one code per
-    row: the three 8-bit parts of x lose nothing."""
+    row: the three 8-bit parts of x lose nothing.  What is left are the two float32
+    additions that put 7 times them together: two halves of a unit."""
     k = 256
     w = torch.zeros(16, k, device=DEV)
     w[torch.arange(16), torch.arange(16) * 16] = 7.0
     p = lops.quantize_weight4(w, 128)
-    x = torch.randn(3, k, device=DEV) * 2.0 ** torch.randint(-60, 60, (3, k), device=DEV).float()
-    assert torch.equal(lops.linear4(x, p), 7.0 * x[:, ::16])
+    g = torch.Generator().manual_seed(19)
+    for m in (2, 3, 40):
+        x = (torch.randn(m, k, generator=g) * 2.0 ** torch.randint(-60, 60, (m, k), generator=g).float())
+        x = x.to(DEV)
+        want = 7.0 * x[:, ::16].double()
+        assert ((lops.linear4(x, p).double() - want).abs() <= 2 * U * (1 + 2.0 ** -7) * want.abs()).all()
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
