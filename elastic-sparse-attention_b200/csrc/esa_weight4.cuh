@@ -336,11 +336,12 @@ vector_kernel(const LinearParams<T> p) {
     w.take(ring + slot * Tile<G>::kBytes, lane);
     const uint4 now[4] = {xb[0], xb[1], xb[2], xb[3]};
     if (c + 1 < c1) inputs(c + 1);
-    // the slot's next tile: this lane has read what it overwrites
+    multiply<H, G, 1>(w, acc, [&](int q, int) { return now[q]; });
+    // the slot's next tile: the products have waited for what this lane read, and
+    // nobody else reads it
     if (c + kDepth < c1)
       Tile<G>::fetch(to + slot * Tile<G>::kBytes, p.codes, p.scales, base + c + kDepth, lane);
     commit_copies();
-    multiply<H, G, 1>(w, acc, [&](int q, int) { return now[q]; });
   }
   __syncthreads();                                     // the ring holds the sums now
   float(*part_sums)[8][kTileRows] = reinterpret_cast<float(*)[8][kTileRows]>(s_mem);
