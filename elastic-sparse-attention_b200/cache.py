@@ -46,35 +46,29 @@ class PackedKVCache:
         if device.type == "cuda" and device.index is None:
             device = torch.device("cuda", torch.cuda.current_device())
         shape = (batch, num_kv_heads, max_len, 2)
-        self.codes = torch.zeros(shape + (head_dim // 2,), dtype=torch.uint8, device=device)
-        self.scales = torch.zeros(shape + (head_dim // CACHE_GROUP,), dtype=torch.bfloat16,
-                                  device=device)
+        self._codes = torch.zeros(shape + (head_dim // 2,), dtype=torch.uint8, device=device)
+        self._scales = torch.zeros(shape + (head_dim // CACHE_GROUP,), dtype=torch.bfloat16,
+                                   device=device)
+        self.batch, self.num_kv_heads, self.max_len = batch, num_kv_heads, max_len
         self.head_dim = head_dim
+        # the C ABI's view of the cache, whose tensors stay where they are
+        self.struct = _lib.EsaCache4(self._codes.data_ptr(), self._scales.data_ptr(), batch,
+                                     num_kv_heads, head_dim, 0, max_len)
 
     @property
-    def batch(self) -> int:
-        return self.codes.shape[0]
+    def codes(self) -> torch.Tensor:
+        return self._codes
 
     @property
-    def num_kv_heads(self) -> int:
-        return self.codes.shape[1]
-
-    @property
-    def max_len(self) -> int:
-        return self.codes.shape[2]
+    def scales(self) -> torch.Tensor:
+        return self._scales
 
     @property
     def device(self) -> torch.device:
-        return self.codes.device
+        return self._codes.device
 
     def nbytes(self) -> int:
         return self.codes.numel() + 2 * self.scales.numel()
-
-    def struct(self) -> _lib.EsaCache4:
-        """The C ABI's view of the cache."""
-        B, H, S = self.codes.shape[:3]
-        return _lib.EsaCache4(self.codes.data_ptr(), self.scales.data_ptr(), B, H, self.head_dim, 0,
-                              S)
 
     def _check_rows(self, name: str, x: torch.Tensor, length: int) -> None:
         want = (self.batch, self.num_kv_heads, length, self.head_dim)
@@ -96,7 +90,7 @@ class PackedKVCache:
             raise TypeError(f"k and v must share one of {sorted(map(str, _lib.DTYPES))}")
         start, start0, counts = _span_args(self.batch, start, counts, dev)
         _lib.launch(_lib.load().esa_cache4_write, dev, _lib.DTYPES[k.dtype],
-                    ctypes.byref(self.struct()), L, _lib.tensor4(k), _lib.tensor4(v),
+                    ctypes.byref(self.struct), L, _lib.tensor4(k), _lib.tensor4(v),
                     _lib.ptr(start), start0, _lib.ptr(counts))
 
     def read(self, start, length: int, dtype: torch.dtype = torch.bfloat16,
@@ -120,6 +114,6 @@ class PackedKVCache:
             out.append(t)
         start, start0, _ = _span_args(self.batch, start, None, dev)
         _lib.launch(_lib.load().esa_cache4_read, dev, _lib.DTYPES[dtype],
-                    ctypes.byref(self.struct()), length, _lib.tensor4(out[0]),
+                    ctypes.byref(self.struct), length, _lib.tensor4(out[0]),
                     _lib.tensor4(out[1]), _lib.ptr(start), start0)
         return tuple(out)

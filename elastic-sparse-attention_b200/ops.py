@@ -320,7 +320,7 @@ def forward_packed(q: torch.Tensor, cache, spec: PatternSpec, scale: float, star
     start, start0, counts = _span_args(B, start, counts, dev)
     lse = torch.empty_strided((B, Hq, L), (Hq * L, L, 1), dtype=torch.float32, device=dev)
     _lib.launch(_lib.load().esa_cache4_forward, dev, _lib.DTYPES[q.dtype],
-                ctypes.byref(cache.struct()), Hq, L, spec.attention_length, spec.layer_idx,
+                ctypes.byref(cache.struct), Hq, L, spec.attention_length, spec.layer_idx,
                 spec.num_hidden_layers, spec.pattern_heads, spec.head_offset, scale,
                 _lib.tensor4(q), _lib.ptr(start), start0, _lib.ptr(counts), _lib.tensor4(out),
                 lse.data_ptr())
