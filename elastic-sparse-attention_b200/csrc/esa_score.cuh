@@ -333,18 +333,26 @@ fwd_kernel(const FwdParams<T> p) {
         if (at < kMost) found[at] = key_of(v, (uint32_t)idx);
       };
       if (edge >= 0 && (float)x[edge] >= bound) add((float)x[edge], edge);
-      uint32_t owners = __ballot_sync(0xffffffffu, own_max >= bound);
-      while (owners) {
-        const int o = __ffs(owners) - 1;
-        owners &= owners - 1;
-        for (int64_t i = rank * NW * 32 + warp * 32 + o + lane * (int64_t)step; i < nvec;
-             i += 32 * (int64_t)step) {
-          const uint4 v = ldg16(parts.body + i);
-          float f[E];
-          Vec<T>::to_float(v, f);
+      auto look = [&](int64_t i) {
+        const uint4 v = ldg16(parts.body + i);
+        float f[E];
+        Vec<T>::to_float(v, f);
 #pragma unroll
-          for (int e = 0; e < E; ++e)
-            if (f[e] >= bound) add(f[e], parts.head + i * E + e);
+        for (int e = 0; e < E; ++e)
+          if (f[e] >= bound) add(f[e], parts.head + i * E + e);
+      };
+      if (nvec <= 4 * step) {
+        // few vectors each: every owner looks through its own
+        if (own_max >= bound)
+          for (int64_t i = first; i < nvec; i += step) look(i);
+      } else {
+        uint32_t owners = __ballot_sync(0xffffffffu, own_max >= bound);
+        while (owners) {
+          const int o = __ffs(owners) - 1;
+          owners &= owners - 1;
+          for (int64_t i = rank * NW * 32 + warp * 32 + o + lane * (int64_t)step; i < nvec;
+               i += 32 * (int64_t)step)
+            look(i);
         }
       }
       __syncthreads();
@@ -424,12 +432,35 @@ fwd_kernel(const FwdParams<T> p) {
   if (ctas > 1) {
     if (threadIdx.x == 0) s_cta = s;
     cluster.sync();
-    if (rank == 0 && warp == 0) {
-      if constexpr (TOP) list = s_list[0][lane];
-      for (int r = 1; r < ctas; ++r) {
-        s = join(s, *cluster.map_shared_rank(&s_cta, r));
-        if constexpr (TOP)
-          list = merge32(list, *cluster.map_shared_rank(&s_list[0][31 - lane], r), lane);
+    if (rank == 0) {
+      if constexpr (TOP && NW >= 8) {
+        // a warp fetches the list of each CTA; they are merged two by two
+        if (warp > 0 && warp < ctas) s_list[warp][lane] = *cluster.map_shared_rank(&s_list[0][lane], warp);
+        __syncthreads();
+        for (int n = ctas / 2; n >= 1; n >>= 1) {
+          if (warp < n)
+            s_list[warp][lane] = merge32(s_list[warp][lane], s_list[warp + n][31 - lane], lane);
+          __syncthreads();
+        }
+      }
+      if (warp == 0) {
+        if constexpr (TOP) {
+          list = s_list[0][lane];
+          if constexpr (NW < 8)
+            for (int r = 1; r < ctas; ++r)
+              list = merge32(list, *cluster.map_shared_rank(&s_list[0][31 - lane], r), lane);
+        }
+        s = *cluster.map_shared_rank(&s_cta, lane & (ctas - 1));
+        for (int o = ctas / 2; o > 0; o >>= 1) {
+          Stats t;
+          t.m = __shfl_xor_sync(0xffffffffu, s.m, o);
+          t.s0 = __shfl_xor_sync(0xffffffffu, s.s0, o);
+          t.s1 = __shfl_xor_sync(0xffffffffu, s.s1, o);
+          s = join(s, t);
+        }
+        s.m = __shfl_sync(0xffffffffu, s.m, 0);
+        s.s0 = __shfl_sync(0xffffffffu, s.s0, 0);
+        s.s1 = __shfl_sync(0xffffffffu, s.s1, 0);
       }
     }
     cluster.sync();        // the other CTAs' shared memory lives until it is read
