@@ -31,6 +31,12 @@
 // (f16 products with the nibbles as denormals need as little decoding, but lose
 // 9 bits when the tensor core aligns them: the output was 2^-11 off.)
 //
+// Measured: 4096 rows x 32 heads of 128, w = 64, at the end of 131072 positions:
+// 206 us (the 16-bit attention's rate on that many pairs is 218); some 1200
+// instructions a pair fill 70 % of the issue slots, the integer pipe two thirds.  8
+// single rows: 3.6 us.  Rows in: 82 us, out: 64 us for 3 x 20011 x 8 rows of 128 fp16
+// (48 and 48 at the measured copy), bound by instructions (5 per element in, 2 out).
+//
 // A warp takes 32 slots of a pair at a time, all their loads in flight, with an
 // online softmax in float32; with few pairs a pair's slots are split over the
 // warps of a CTA and joined in shared memory.

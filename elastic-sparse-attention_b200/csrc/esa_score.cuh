@@ -20,6 +20,13 @@
 //
 // A row belongs to a cluster of 1, 2, 4 or 8 CTAs (few rows: more CTAs per row),
 // joined through distributed shared memory in the same launch.
+//
+// What bounds it: the forward pass makes an exponential per element, and those alone
+// take 71 us of the 80 that HBM needs for 8192 x 32000 bf16; the rest is kept to four
+// instructions per element by packed maxima, mixed-precision differences and packed
+// float32 sums.  That case takes 93 us (86 % of the measured copy), 103 with five
+// alternatives; the gradient 170 us (94 %).  8 rows, 20 alternatives: 6.6 us, 3.5
+// without: a chain of short sorts.
 #pragma once
 #include <cooperative_groups.h>
 

@@ -11,6 +11,14 @@
 // as 8 columns.)  float32 rows of x are split into three bf16 parts (8 bits
 // each, exact), three columns whose sums are added at the end.
 //
+// Measured (1 x B200, weights from HBM, launches one after the other): 1 x 4096 x
+// 12288 in 8.5 us (its bytes alone: 4.0; the stream without arithmetic and without x
+// 5.9, with x 6.8), 32 x 11008 x 4096 in 15.3 (3.7), where the matrix instructions
+// alone take 5.2 and a CTA has only some six stages of K.  Not taken up: x in fixed
+// point against 8-bit integer products, which needs a third of the instructions for
+// one row but took as long (the chain of loads bounds it), and loses bits of float32
+// rows with a wide range.
+//
 // Layout, made once by quantize_kernel: 16 weight rows x 128 inputs in 1024 bytes
 // (the tiles of a row side by side, padded with zeros to whole tiles), twice 16
 // bytes per lane.  Lane 4 g + t holds rows g and g + 8, inputs t * 8 .. + 8 of each
