@@ -32,10 +32,10 @@
 // 9 bits when the tensor core aligns them: the output was 2^-11 off.)
 //
 // Measured: 4096 rows x 32 heads of 128, w = 64, at the end of 131072 positions:
-// 206 us (the 16-bit attention's rate on that many pairs is 218); some 1200
-// instructions a pair fill 70 % of the issue slots, the integer pipe two thirds.  8
-// single rows: 3.6 us.  Rows in: 82 us, out: 64 us for 3 x 20011 x 8 rows of 128 fp16
-// (48 and 48 at the measured copy), bound by instructions (5 per element in, 2 out).
+// 206 us (esa_forward on a 16-bit cache of that shape: 444); some 1230 instructions a
+// pair fill 71 % of the issue slots, the integer pipe 63 %.  8 single rows: 3.6 us.
+// Rows in: 79 us, out: 62 us for 3 x 20011 x 8 rows of 128 fp16 (profiled; together 138
+// without), bound by instructions: 78 and 74 % of the issue slots, DRAM at 25 and 50 %.
 //
 // A warp takes 32 slots of a pair at a time, all their loads in flight, with an
 // online softmax in float32; with few pairs a pair's slots are split over the

@@ -21,12 +21,12 @@
 // A row belongs to a cluster of 1, 2, 4 or 8 CTAs (few rows: more CTAs per row),
 // joined through distributed shared memory in the same launch.
 //
-// What bounds it: the forward pass makes an exponential per element, and those alone
-// take 71 us of the 80 that HBM needs for 8192 x 32000 bf16; the rest is kept to four
-// instructions per element by packed maxima, mixed-precision differences and packed
-// float32 sums.  That case takes 93 us (86 % of the measured copy), 103 with five
-// alternatives; the gradient 170 us (94 %).  8 rows, 20 alternatives: 6.6 us, 3.5
-// without: a chain of short sorts.
+// What bounds it: the forward pass makes an exponential per element.  8192 x 32000 bf16
+// takes 84 us (95 % of the measured copy rate), 105 with five alternatives; the
+// special-function pipe is busy for three quarters of it, and some 7.5 instructions per
+// element, few by packed maxima, mixed-precision differences and packed float32 sums,
+// fill 64 % of the issue slots.  The gradient takes 176 us (91 %).  8 rows of 32000, 20
+// alternatives: 6.6 us, 3.4 without: a chain of short sorts.
 #pragma once
 #include <cooperative_groups.h>
 

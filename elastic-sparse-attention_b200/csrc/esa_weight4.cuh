@@ -12,9 +12,10 @@
 // each, exact), three columns whose sums are added at the end.
 //
 // Measured (1 x B200, weights from HBM, launches one after the other): 1 x 4096 x
-// 12288 in 8.5 us (its bytes alone: 4.0; the stream without arithmetic and without x
-// 5.9, with x 6.8), 32 x 11008 x 4096 in 15.3 (3.7), where the matrix instructions
-// alone take 5.2 and a CTA has only some six stages of K.  Not taken up: x in fixed
+// 12288 in 8.5 us (its bytes alone: 4.0; a copy of an earlier state of the kernel with
+// the arithmetic taken out needed 6.8, without x as well 5.8), 32 x 11008 x 4096 in 15.4
+// (3.7), where the matrix instructions alone take 5.2 at their measured rate and a CTA
+// has only some six stages of K.  Not taken up: x in fixed
 // point against 8-bit integer products, which needs a third of the instructions for
 // one row but took as long (the chain of loads bounds it), and loses bits of float32
 // rows with a wide range.

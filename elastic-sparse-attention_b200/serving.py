@@ -55,9 +55,9 @@ class PackedDecoder:
 
     @staticmethod
     def _project(x: torch.Tensor, weight: layer_ops.PackedWeight4) -> torch.Tensor:
-        """x W^T: from the codes for few rows, else with the weight decoded for the
-        call."""
-        if x.numel() // x.shape[-1] <= layer_ops.LINEAR4_ROWS:
+        """x W^T: from the codes for float32 and for few rows of a 16-bit type, else
+        with the weight decoded for the call."""
+        if x.dtype == torch.float32 or x.numel() // x.shape[-1] <= layer_ops.LINEAR4_ROWS:
             return layer_ops.linear4(x, weight)
         return torch.matmul(x, layer_ops.dequantize_weight4(weight, x.dtype).t())
 
