@@ -12,8 +12,8 @@
 // each, exact), three columns whose sums are added at the end.
 //
 // Measured (1 x B200, weights from HBM, launches one after the other): 1 x 4096 x
-// 12288 in 8.5 us (its bytes alone: 4.0; a copy of an earlier state of the kernel with
-// the arithmetic taken out needed 6.8, without x as well 5.8), 32 x 11008 x 4096 in 15.4
+// 12288 in 9.1 us (its bytes alone: 4.0; a copy of an earlier state of the kernel with
+// the arithmetic taken out needed 6.8, without x as well 5.8), 32 x 11008 x 4096 in 15.7
 // (3.7), where the matrix instructions alone take 5.2 at their measured rate and a CTA
 // has only some six stages of K.  Not taken up: x in fixed
 // point against 8-bit integer products, which needs a third of the instructions for
@@ -240,6 +240,16 @@ template <int G> struct Tile {
   static constexpr int kBytes = kTileBytes + kGroups * 128;           // in shared memory
   uint4 c[2];
   uint32_t s[kGroups];         // rows g and g + 8
+  // Asks for `count` tiles from `tile` on in L2, where a later write of them is seen:
+  // this alone may be done before the kernel before has been waited for, which may
+  // have made the codes.
+  __device__ __forceinline__ static void prefetch(const uint8_t* codes, const __nv_bfloat16* scales,
+                                                  int64_t tile, int count) {
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(codes + tile * kTileBytes),
+                 "r"(count * kTileBytes) : "memory");
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(scales + tile * (kGroups * 16)),
+                 "r"(count * kGroups * 32) : "memory");
+  }
   __device__ __forceinline__ static void fetch(uint32_t to, const uint8_t* codes,
                                                const __nv_bfloat16* scales, int64_t tile, int lane) {
     copy16_async(to + lane * 16, codes + tile * kTileBytes + lane * 16);
@@ -303,7 +313,8 @@ __device__ __forceinline__ void multiply(const Tile<G>& w, float (&acc)[NT][4], 
 // ---------------------------------------------------------------------------
 // Up to 8 columns: bound by the stream of codes.  CTA = one tile of 16 weight rows,
 // its WK warps share K and join in shared memory.  A warp has kDepth tiles on their
-// way, and begins with that before it waits for the kernel before it (which made x).
+// way.  Before it waits for the kernel before it (which made x, or the codes) it only
+// has the first of them brought into L2.
 // ---------------------------------------------------------------------------
 constexpr int kDepth = 4;
 
@@ -319,13 +330,14 @@ vector_kernel(const LinearParams<T> p) {
   const int64_t base = (int64_t)blockIdx.x * p.chunks;
   unsigned char* ring = s_mem + warp * (kDepth * Tile<G>::kBytes);
   const uint32_t to = (uint32_t)__cvta_generic_to_shared(ring);
+  if (lane == 0 && c0 < c1) Tile<G>::prefetch(p.codes, p.scales, base + c0, min(kDepth, c1 - c0));
+  cudaTriggerProgrammaticLaunchCompletion();           // the next kernel may begin like this
+  cudaGridDependencySynchronize();
 #pragma unroll
   for (int i = 0; i < kDepth; ++i) {
     if (c0 + i < c1) Tile<G>::fetch(to + i * Tile<G>::kBytes, p.codes, p.scales, base + c0 + i, lane);
     commit_copies();
   }
-  cudaTriggerProgrammaticLaunchCompletion();           // the next kernel may begin like this
-  cudaGridDependencySynchronize();
   const int token = g / P, part = g % P;
   const bool in = token < p.M && token < 8 / P;
   const T* x = p.x + (int64_t)(in ? token : 0) * p.K + t * 8;
@@ -460,15 +472,16 @@ rows_kernel(const LinearParams<T> p) {
                                 i % kSpare * 16) = make_uint4(0, 0, 0, 0);
   }
   const int stages = (c1 - c0 + S::kStage - 1) / S::kStage;
-  // the codes of the first stages are on their way before x is waited for
-#pragma unroll
-  for (int s = 0; s < S::kStages - 1; ++s) fetch_codes(s, s);
+  // the codes of the first stages are on their way to L2 before x is waited for
+  if (lane == 0 && c0 < c1)
+    Tile<G>::prefetch(p.codes, p.scales, base + c0, min((S::kStages - 1) * S::kStage, c1 - c0));
   cudaTriggerProgrammaticLaunchCompletion();             // the next kernel may begin like this
   cudaGridDependencySynchronize();
 #pragma unroll
   for (int s = 0; s < S::kStages - 1; ++s) {
+    fetch_codes(s, s);
     if (s < stages) fetch_inputs(s, s);
-    commit_copies();                                     // the first group holds all codes so far
+    commit_copies();
   }
   int slot = 0;
 #pragma unroll 1

@@ -227,3 +227,33 @@ def test_captured_beside_other_kernels(lops):
         xx = torch.randn(2, 1024, generator=g).to(DEV, torch.bfloat16)
         y1 = lops.linear4(xx, lops.quantize_weight4(w, 128))
         check(y1, xx, decoded(w, 128), 128, "fresh")
+
+
+@pytest.mark.parametrize("rows", [1, 24])
+@pytest.mark.parametrize("how", ["quantize", "copy"])
+def test_codes_made_by_the_kernel_before(lops, rows, how):
+    """The product reads what the kernel right before it wrote: codes and scales of
+    other weights put into the same memory, nothing waited for in between."""
+    from elastic_sparse_attention_b200 import _lib
+    g = torch.Generator(device=DEV).manual_seed(11)
+    n, k = 4096, 1024
+    x = torch.randn(rows, k, device=DEV, generator=g).bfloat16()
+    weights = [torch.randn(n, k, device=DEV, generator=g).bfloat16() for _ in range(2)]
+    packed = [lops.quantize_weight4(w) for w in weights]
+    torch.cuda.synchronize()
+    want = [lops.linear4(x, p) for p in packed]
+    torch.cuda.synchronize()
+    shared = lops.quantize_weight4(weights[0])
+    lib = _lib.load()
+    got = []
+    for i in range(24):
+        if how == "copy":
+            shared.scales.copy_(packed[i % 2].scales)
+            shared.codes.copy_(packed[i % 2].codes)
+        else:
+            _lib.launch(lib.esa_quantize_weight4, x.device, _lib.DTYPES[x.dtype], n, k,
+                        shared.group, weights[i % 2].data_ptr(), shared.codes.data_ptr(),
+                        shared.scales.data_ptr())
+        got.append(lops.linear4(x, shared))
+    for i, y in enumerate(got):
+        assert torch.equal(y, want[i % 2]), i
