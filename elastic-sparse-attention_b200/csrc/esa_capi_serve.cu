@@ -355,7 +355,7 @@ int esa_quantize_weight4(int32_t dtype, int64_t n, int64_t k, int32_t group, con
   if (int rc = check_weight4(what, dtype, n, k, group, codes, scales)) return rc;
   if (!weight || !aligned16(weight)) return fail(ESA_ERR_INVALID, "%s: null or misaligned weight", what);
   const w4::Packed p = packed(n, k, group, codes, scales);
-  const dim3 grid((unsigned)ceil_div(k, 128), (unsigned)p.tiles);
+  const dim3 grid((unsigned)p.chunks * (unsigned)p.tiles);       // up to 2^29
   return by_dtype(dtype, [&](auto tag) {
     using T = decltype(tag);
     w4::quantize_kernel<T><<<grid, w4::kPackThreads, 0, (cudaStream_t)stream>>>(
@@ -370,7 +370,7 @@ int esa_dequantize_weight4(int32_t dtype, int64_t n, int64_t k, int32_t group, c
   if (int rc = check_weight4(what, dtype, n, k, group, codes, scales)) return rc;
   if (!weight || !aligned16(weight)) return fail(ESA_ERR_INVALID, "%s: null or misaligned weight", what);
   const w4::Packed p = packed(n, k, group, codes, scales);
-  const dim3 grid((unsigned)ceil_div(k, 128), (unsigned)p.tiles);
+  const dim3 grid((unsigned)p.chunks * (unsigned)p.tiles);       // up to 2^29
   return by_dtype(dtype, [&](auto tag) {
     using T = decltype(tag);
     w4::dequantize_kernel<T><<<grid, w4::kPackThreads, 0, (cudaStream_t)stream>>>(

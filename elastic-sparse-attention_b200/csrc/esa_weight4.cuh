@@ -73,9 +73,10 @@ __global__ void __launch_bounds__(kPackThreads)
 quantize_kernel(const Packed p, const T* w) {
   __shared__ uint32_t s_words[kPackThreads][2];
   const int r = threadIdx.x >> 4, part = threadIdx.x & 15;
-  const int64_t tile = blockIdx.y;
+  const int64_t tile = blockIdx.x / (unsigned)p.chunks;
+  const int chunk = (int)(blockIdx.x % (unsigned)p.chunks);
   const int row = (int)(tile * kTileRows) + r;
-  const int k = (int)blockIdx.x * 128 + part * 8;
+  const int k = chunk * 128 + part * 8;
   float f[8];
   load8(w + (int64_t)row * p.K + k, row < p.N, k, p.K, f);
   uint32_t top = 0;
@@ -101,7 +102,7 @@ quantize_kernel(const Packed p, const T* w) {
   uint2 out;
   out.x = s_words[threadIdx.x][0] | s_words[threadIdx.x + 128][0];
   out.y = s_words[threadIdx.x][1] | s_words[threadIdx.x + 128][1];
-  *reinterpret_cast<uint2*>(p.codes + (tile * p.chunks + blockIdx.x) * kTileBytes +
+  *reinterpret_cast<uint2*>(p.codes + (tile * p.chunks + chunk) * kTileBytes +
                             (part >> 3) * 512 + lane * 16 + half * 8) = out;
 }
 
@@ -109,13 +110,14 @@ template <typename T>
 __global__ void __launch_bounds__(kPackThreads)
 dequantize_kernel(const Packed p, T* w) {
   const int r = threadIdx.x >> 4, part = threadIdx.x & 15;
-  const int64_t tile = blockIdx.y;
+  const int64_t tile = blockIdx.x / (unsigned)p.chunks;
+  const int chunk = (int)(blockIdx.x % (unsigned)p.chunks);
   const int row = (int)(tile * kTileRows) + r;
-  const int k = (int)blockIdx.x * 128 + part * 8;
+  const int k = chunk * 128 + part * 8;
   if (row >= p.N || k >= p.K) return;
   const int lane = ((r & 7) << 2) | (part & 3), half = (part >> 2) & 1;
   const uint2 v = __ldg(reinterpret_cast<const uint2*>(
-      p.codes + (tile * p.chunks + blockIdx.x) * kTileBytes + (part >> 3) * 512 + lane * 16 +
+      p.codes + (tile * p.chunks + chunk) * kTileBytes + (part >> 3) * 512 + lane * 16 +
       half * 8));
   const float s =
       __bfloat162float(p.scales[(tile * p.groups + k / p.group) * kTileRows + scale_place(r)]);

@@ -257,3 +257,15 @@ def test_codes_made_by_the_kernel_before(lops, rows, how):
         got.append(lops.linear4(x, shared))
     for i, y in enumerate(got):
         assert torch.equal(y, want[i % 2]), i
+
+
+def test_the_most_weight_rows(lops):
+    """2^20 rows, 65536 tiles of 16: the last ones as if they were alone."""
+    g = torch.Generator(device=DEV).manual_seed(12)
+    w = torch.randn(1 << 20, 32, device=DEV, generator=g).bfloat16()
+    x = torch.randn(2, 32, device=DEV, generator=g).bfloat16()
+    p, last = lops.quantize_weight4(w, 32), lops.quantize_weight4(w[-32:].contiguous(), 32)
+    assert torch.equal(p.codes[-2048:], last.codes)
+    assert torch.equal(p.scales[-2:, :1], last.scales[:, :1])
+    assert torch.equal(lops.dequantize_weight4(p)[-32:], lops.dequantize_weight4(last))
+    assert torch.equal(lops.linear4(x, p)[:, -32:], lops.linear4(x, last))
