@@ -599,8 +599,9 @@ WEIGHT4_GROUPS = (32, 64, 128)
 # with the weight decoded for it.  12288 x 4096 bf16, us: 64 rows 30 (decoded 53),
 # 128 rows 55 (51), 256 rows 102 (58); 4096 x 4096 in groups of 32: 64 rows 15 (20),
 # 96 rows 23 (20).  float32 rows have no such number: 4096 x 4096, 64 rows 40 (104),
-# 512 rows 217 (327).
+# 512 rows 217 (327), 8192 rows 3041 (4226).
 LINEAR4_ROWS = 64
+LINEAR4_MAX_ROWS = 1 << 20     # of one call
 
 
 @dataclass(eq=False)
@@ -667,7 +668,8 @@ def dequantize_weight4(packed: PackedWeight4, dtype: torch.dtype | None = None) 
 def linear4(x: torch.Tensor, packed: PackedWeight4) -> torch.Tensor:
     """x [..., k] times the transposed weight: [..., n].  Exact products of x and
     the codes, float32 sums, rounded once.  Made for few rows (decoding:
-    16-bit types up to ``LINEAR4_ROWS``); it takes any number."""
+    16-bit types up to ``LINEAR4_ROWS``); it takes
+    ``LINEAR4_MAX_ROWS``."""
     n, k = _check_weight4(packed)
     dev = _check_device(x, packed.codes, packed.scales)
     shape = _shape(x)

@@ -57,7 +57,9 @@ class PackedDecoder:
     def _project(x: torch.Tensor, weight: layer_ops.PackedWeight4) -> torch.Tensor:
         """x W^T: from the codes for float32 and for few rows of a 16-bit type, else
         with the weight decoded for the call."""
-        if x.dtype == torch.float32 or x.numel() // x.shape[-1] <= layer_ops.LINEAR4_ROWS:
+        most = (layer_ops.LINEAR4_MAX_ROWS if x.dtype == torch.float32 else
+                layer_ops.LINEAR4_ROWS)
+        if x.numel() // x.shape[-1] <= most:
             return layer_ops.linear4(x, weight)
         return torch.matmul(x, layer_ops.dequantize_weight4(weight, x.dtype).t())
 

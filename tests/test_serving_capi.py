@@ -175,3 +175,16 @@ def test_python_callers_refuse_host_tensors_and_bad_shapes(esa):
         cache.write(torch.zeros(2, 3, 1, 128), torch.zeros(2, 3, 1, 128), 0)
     with pytest.raises(RuntimeError, match="CUDA"):
         esa.ops.forward_packed(torch.zeros(2, 3, 1, 128), cache, esa.PatternSpec(0, 1, 4), 1.0, 0)
+
+
+@pytest.mark.parametrize("dtype,rows,way", [
+    (torch.bfloat16, 64, "codes"), (torch.bfloat16, 65, "decoded"), (torch.float32, 65, "codes"),
+    (torch.float32, 1 << 20, "codes"), (torch.float32, (1 << 20) + 1, "decoded")])
+def test_how_the_packed_decoder_multiplies(esa, monkeypatch, dtype, rows, way):
+    """The way that was measured to be faster, where the product takes so many rows."""
+    taken = []
+    monkeypatch.setattr(esa.layer_ops, "linear4", lambda x, w: taken.append("codes"))
+    monkeypatch.setattr(esa.layer_ops, "dequantize_weight4",
+                        lambda w, d: taken.append("decoded") or torch.zeros(1, 8, dtype=d))
+    esa.PackedDecoder._project(torch.zeros(1, 8, dtype=dtype).expand(rows, 8), None)
+    assert taken == [way]
