@@ -289,8 +289,8 @@ def _span_args(batch: int, start, counts, dev: torch.device) -> tuple:
         counts = per_sequence("counts", counts)
     if isinstance(start, torch.Tensor):
         return per_sequence("start", start), 0, counts
-    if start < 0:
-        raise ValueError(f"start {start} is negative")
+    if not 0 <= start < 1 << 63:
+        raise ValueError(f"start {start} is negative or above 63 bits")
     return None, int(start), counts
 
 

@@ -188,3 +188,11 @@ def test_how_the_packed_decoder_multiplies(esa, monkeypatch, dtype, rows, way):
                         lambda w, d: taken.append("decoded") or torch.zeros(1, 8, dtype=d))
     esa.PackedDecoder._project(torch.zeros(1, 8, dtype=dtype).expand(rows, 8), None)
     assert taken == [way]
+
+
+@pytest.mark.parametrize("start", [-1, 1 << 63, 1 << 64, (1 << 64) + 3])
+def test_a_start_beyond_64_bits_is_refused(esa, start):
+    """It must not come out as another position."""
+    with pytest.raises(ValueError, match="start"):
+        esa.ops._span_args(2, start, None, torch.device("cpu"))
+    assert esa.ops._span_args(2, (1 << 63) - 1, None, torch.device("cpu"))[1] == (1 << 63) - 1
