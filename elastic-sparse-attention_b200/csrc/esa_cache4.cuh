@@ -126,8 +126,9 @@ template <int D> struct Units {
   __device__ __forceinline__ explicit Units(const RowParams<T>& p) {
     part = threadIdx.x % Unit<D>::kPer;
     const int64_t begin = p.span.begin(blockIdx.y), count = p.span.count(blockIdx.y);
-    // begin is clamped to a place outside the cache, so that 32 bits hold it
-    const int first = (int)(begin < -p.c.S ? -p.c.S : begin > p.c.S ? p.c.S : begin);
+    // begin is clamped to a place from which no row lies in the cache, so that 32 bits hold
+    // it: the cache's end, or as many positions before its begin as the call has rows
+    const int first = (int)(begin < -p.span.L ? -p.span.L : begin > p.c.S ? p.c.S : begin);
     const int n = (int)count, lo = first < 0 ? min(-first, n) : 0;
     const int hi = max(min(n, (int)p.c.S - first), lo);
     if ((lo > 0 || hi < n) && threadIdx.x == 0 && blockIdx.x == 0 && p.err) atomicOr(p.err, kErrKvRange);
