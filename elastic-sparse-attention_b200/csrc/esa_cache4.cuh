@@ -24,8 +24,8 @@
 //           group times its scale in float32
 //   output: A = 16 elements x 32 keys, B column = (group, digit) of the weight
 //           times that group's scale, two digits (16 bits below the largest of
-//           the 32 keys) for 16-bit types and four for float32; an output element
-//           reads the columns of its group
+//           the 32 keys in that group) for 16-bit types and four for float32; an
+//           output element reads the columns of its group
 // Keys are signed bytes, 16 times the code; what the stored + 8 of the values adds
 // is taken out exactly by one product with a matrix of eights.
 // (f16 products with the nibbles as denormals need as little decoding, but lose
@@ -333,11 +333,14 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 // 2^e with x 2^e in [2^TOP, 2^(TOP + 1)) for the float bits of x >= 0 (2^126 where x
-// is 0 or too small for that), and its inverse.
-template <int TOP> __device__ __forceinline__ float lift(uint32_t bits, float& inverse) {
-  const int field = min(253, TOP + 254 - (int)(bits >> 23));
-  inverse = __uint_as_float((uint32_t)(254 - field) << 23);
-  return __uint_as_float((uint32_t)field << 23);
+// is 0 or too small for that), and its inverse.  (Of an infinity or a NaN: some finite
+// power.)  SHRINK: the power is 1 - 2^-16 times that, 256 units of its last place less.
+template <int TOP, bool SHRINK = false>
+__device__ __forceinline__ float lift(uint32_t bits, float& inverse) {
+  constexpr uint32_t kLess = SHRINK ? 256u : 0u;
+  const uint32_t up = min((253u << 23) - kLess, ((TOP + 254u) << 23) - kLess - (bits & 0x7f800000u));
+  inverse = __uint_as_float((254u << 23) - kLess - up);
+  return __uint_as_float(up);
 }
 
 // Byte j of four words, in x[j].
@@ -407,6 +410,8 @@ template <int N> __device__ __forceinline__ float scale_at(const uint32_t (&w)[N
 // a value's code is then.
 constexpr uint32_t kLow = 0x0f0f0f0fu, kHigh = 0xf0f0f0f0u;
 constexpr uint32_t kEight = 0x08080808u, kEightHigh = 0x80808080u;     // 8, 128
+// 1 / (1 - 2^-16), which two digits' weights are short of: taken once per output.
+constexpr float kGrow = 1.00001525902189f;
 
 // SPLIT: the warps of a CTA share pairs, one pair at a time; else each warp has
 // pairs of its own, one after the other.
@@ -603,45 +608,35 @@ attend_kernel(const AttendParams<T> p) {
     const float e = ex2(s - ref);
     l_lane = fmaf(l_lane, corr, e);
     m_run = mn;
-    // ---- weight times the scales of the own key's value, in fixed point ----
-    float vs[NG];
-    uint32_t top = 0;
-#pragma unroll
-    for (int c = 0; c < NG; ++c) {
-      const uint32_t w = sw[(NG + c) / 2];
-      vs[c] = e * __uint_as_float(c & 1 ? w & 0xffff0000u : w << 16);
-      // a masked slot's scale is one that is in use, so 0 times it is 0 or a NaN that
-      // the key in use brings anyway
-      top = max(top, __float_as_uint(vs[c]));         // none is negative
-    }
-    top = __reduce_max_sync(0xffffffffu, top);
-    if (top >= 0x7f800000u) {       // a group with a NaN: its elements come out as NaN
-      top = 0;
-#pragma unroll
-      for (int c = 0; c < NG; ++c) {
-        const bool bad = vs[c] != vs[c];
-        if (bad) vs[c] = 0.f;
-        top = max(top, __float_as_uint(vs[c]));
-        if (__any_sync(0xffffffffu, bad)) nans |= 1u << c;
-      }
-      top = __reduce_max_sync(0xffffffffu, top);
-    }
-    float down;
-    float up = lift<VC == 4 ? 31 : 15>(top, down);
-    if constexpr (VC == 2) {        // below 65535 after the rounding, so two digits hold it
-      up *= 0.9999847412109375f;    // 1 - 2^-16
-      down *= 1.00001525902189f;
-    }
+    // ---- weight times the scales of the own key's value, in fixed point: each group
+    // on a grid of its own, since its outputs are no other group's ----
+    float down[NV];                                  // of the groups this lane's columns hold
+    uint32_t top[NG];
     unsigned char* digits = reinterpret_cast<unsigned char*>(s_buf[warp]);
 #pragma unroll
     for (int c = 0; c < NG; ++c) {
+      const uint32_t w = sw[(NG + c) / 2];
+      // a masked slot's scale is one that is in use, so 0 times it is 0 or a NaN that
+      // the key in use brings anyway
+      const float vs = e * __uint_as_float(c & 1 ? w & 0xffff0000u : w << 16);
+      top[c] = __reduce_max_sync(0xffffffffu, __float_as_uint(vs));   // none is negative
+      // two digits: at most 65535 after the rounding
+      float inverse;
+      const float up = lift<VC == 4 ? 31 : 15, VC == 2>(top[c], inverse);
+      if (c % GT == 0 || owner == c % GT) down[c / GT] = inverse;
       uint32_t d;
       // the product plus 2^23 has the rounded product as its low bits
-      if constexpr (VC == 2) d = __float_as_uint(fmaf(vs[c], up, 8388608.f));
-      else d = __float2uint_rn(vs[c] * up);
+      if constexpr (VC == 2) d = __float_as_uint(fmaf(vs, up, 8388608.f));
+      else d = __float2uint_rn(vs * up);
 #pragma unroll
       for (int i = 0; i < VC; ++i) digits[(c * VC + i) * 32 + t * 8 + g] = (unsigned char)(d >> (8 * i));
     }
+    uint32_t highest = 0;
+#pragma unroll
+    for (int c = 0; c < NG; ++c) highest = max(highest, top[c]);
+    if (highest >= 0x7f800000u)     // groups with a NaN: their elements come out as NaN
+#pragma unroll
+      for (int c = 0; c < NG; ++c) nans |= top[c] >= 0x7f800000u ? 1u << c : 0u;
     __syncwarp();
     int acc[MT][4], eights[NV][4];
     uint32_t vb[NV][2];
@@ -686,8 +681,8 @@ attend_kernel(const AttendParams<T> p) {
             hi = owner == o ? a[2] + a[3] * 256 : hi;
           }
         }
-        total[nv][j][0] = fmaf((float)(lo - off), down, total[nv][j][0] * corr);
-        total[nv][j][1] = fmaf((float)(hi - lo - off16), down * 0.0625f, total[nv][j][1] * corr);
+        total[nv][j][0] = fmaf((float)(lo - off), down[nv], total[nv][j][0] * corr);
+        total[nv][j][1] = fmaf((float)(hi - lo - off16), down[nv] * 0.0625f, total[nv][j][1] * corr);
       }
     }
   }
@@ -741,6 +736,7 @@ attend_kernel(const AttendParams<T> p) {
   float inv;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(sum));
   if (sum == 0.f) inv = 0.f;
+  if constexpr (VC == 2) inv *= kGrow;
   T* o = static_cast<T*>(const_cast<void*>(p.o.data)) + b * p.o.sb + my_h * p.o.sh +
          (int64_t)my_l * p.o.ss + lane * PL;
   struct alignas(PL * sizeof(T) < 16 ? PL * sizeof(T) : 16) Pack { T v[PL]; } pack;
