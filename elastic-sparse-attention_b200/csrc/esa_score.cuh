@@ -111,7 +111,9 @@ __device__ __forceinline__ Stats join(const Stats& a, const Stats& b) {
 // Two 16-bit elements: the larger ones (NaNs passed over, or kept), x - m in float32.
 template <typename T> struct Pair;
 // kFloor: elements below it count as it, which keeps -infinity out of the products;
-// next to a maximum of kSafe or more their exponential is 0 either way.
+// next to a maximum of kSafe or more their exponential is 0 either way.  No difference
+// from a maximum of the type may reach -infinity: -2^100 less bfloat16's largest value,
+// (2 - 2^-7) 2^127, is within float32, -2^126 less it would not be.
 #define ESA_PAIR(T, PTXTYPE, ONE, FLOOR2, NONE, FLOOR, SAFE)                                 \
   template <> struct Pair<T> {                                                               \
     static constexpr uint32_t kFloor2 = FLOOR2, kNone = NONE;                                \
@@ -134,7 +136,7 @@ template <typename T> struct Pair;
           : "r"(x), "f"(neg_m));                                                             \
     }                                                                                        \
   };
-ESA_PAIR(__nv_bfloat16, "bf16", "0x3F80", 0xfe80fe80u, 0xff80ff80u, -0x1p126f, -0x1p125f)
+ESA_PAIR(__nv_bfloat16, "bf16", "0x3F80", 0xf180f180u, 0xff80ff80u, -0x1p100f, -0x1p99f)
 ESA_PAIR(__half, "f16", "0x3C00", 0xfbfffbffu, 0xfc00fc00u, -65504.f, -65000.f)
 #undef ESA_PAIR
 template <> struct Pair<float> {
