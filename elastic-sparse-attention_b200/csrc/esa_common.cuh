@@ -316,6 +316,11 @@ __device__ __forceinline__ uint4 ldg16(const void* p) {
   return __ldg(reinterpret_cast<const uint4*>(p));
 }
 
+// The same with an ordinary load: for memory that the kernel before may still be writing
+// when this one starts (one that waits for it with cudaGridDependencySynchronize); the
+// read-only path wants memory that does not change while a kernel runs.
+__device__ __forceinline__ uint4 ld16(const void* p) { return *reinterpret_cast<const uint4*>(p); }
+
 // Read-only load that is not kept in L1 (streamed operands such as Q rows of
 // the query being processed, or the output/gradient rows).
 __device__ __forceinline__ uint4 ldg16_stream(const void* p) {

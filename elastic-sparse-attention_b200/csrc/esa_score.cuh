@@ -247,7 +247,7 @@ fwd_kernel(const FwdParams<T> p) {
     for (int u = 0; u < kUnroll; ++u) {
       const uint32_t none = Pair<T>::kNone;
       v[u] = make_uint4(none, none, none, none);
-      if (i + u * step < nvec) v[u] = ldg16(parts.body + i + u * step);
+      if (i + u * step < nvec) v[u] = ld16(parts.body + i + u * step);
     }
     own_max = fmaxf(own_max, vec_max<T>(v));
     grow(s, own_max);
@@ -343,7 +343,7 @@ fwd_kernel(const FwdParams<T> p) {
       };
       if (edge >= 0 && (float)x[edge] >= bound) add((float)x[edge], edge);
       auto look = [&](int64_t i) {
-        const uint4 v = ldg16(parts.body + i);
+        const uint4 v = ld16(parts.body + i);
         float f[E];
         Vec<T>::to_float(v, f);
 #pragma unroll
@@ -402,7 +402,7 @@ fwd_kernel(const FwdParams<T> p) {
           const int64_t i = j + lane * (int64_t)step;
           const bool in = i < nvec;
           uint4 v = make_uint4(0, 0, 0, 0);
-          if (in) v = ldg16(parts.body + i);
+          if (in) v = ld16(parts.body + i);
           float f[E];
           Vec<T>::to_float(v, f);
           bool some = all;

@@ -210,9 +210,9 @@ template <typename T>
 __device__ __forceinline__ uint4 column8(const T* x, int k, int K, bool in, int part) {
   const uint4 none = make_uint4(0, 0, 0, 0);
   if constexpr (sizeof(T) == 2) {
-    return in && k < K ? ldg16(x + k) : none;
+    return in && k < K ? ld16(x + k) : none;
   } else {
-    return cut8(in && k < K ? ldg16(x + k) : none, in && k + 4 < K ? ldg16(x + k + 4) : none, part);
+    return cut8(in && k < K ? ld16(x + k) : none, in && k + 4 < K ? ld16(x + k + 4) : none, part);
   }
 }
 
@@ -458,8 +458,8 @@ rows_kernel(const LinearParams<T> p) {
         copy16_async(to + j * kTokenStep * S::kPitch, in ? x : p.x, in);
       } else if (token0 + j * kTokenStep < S::kTokens) {
         const uint4 none = make_uint4(0, 0, 0, 0);
-        const uint4 lo = row && k < left ? ldg16(x) : none;
-        const uint4 hi = row && k + 4 < left ? ldg16(x + 4) : none;
+        const uint4 lo = row && k < left ? ld16(x) : none;
+        const uint4 hi = row && k + 4 < left ? ld16(x + 4) : none;
 #pragma unroll
         for (int q = 0; q < P; ++q)
           *reinterpret_cast<uint4*>(buf + (j * kTokenStep * P + q) * S::kPitch) = cut8(lo, hi, q);

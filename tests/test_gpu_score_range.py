@@ -81,3 +81,26 @@ def test_the_largest_logits(esa, dtype, kind, rows, V):
              + U * hot * a.abs() + 2.0 ** -126)
     half_step = torch.finfo(dtype).eps / 2
     close(got, want, half_step * (want.abs() + slack) + slack + TINY[dtype], "dlogits")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows", [2, 30])
+def test_logits_of_the_product_right_before(esa, dtype, rows):
+    """The 4-bit LM head and the scores of its logits, issued back to back into the same
+    memory: each call scores the logits of the product right before it."""
+    lops = esa.layer_ops
+    g = torch.Generator().manual_seed(rows)
+    head = lops.quantize_weight4((0.2 * torch.randn(20000, 512, generator=g)).to(DEV, dtype))
+    xs = [torch.randn(rows, 512, generator=g).to(DEV, dtype) for _ in range(12)]
+    tokens = torch.randint(0, 20000, (rows,), generator=g).to(DEV)
+    want = []
+    for x in xs:
+        y = lops.linear4(x, head)
+        torch.cuda.synchronize()
+        want.append(lops.token_logprobs(y, tokens, top_k=5))
+        torch.cuda.synchronize()
+        del y                                  # its memory serves the next product
+    got = [lops.token_logprobs(lops.linear4(x, head), tokens, top_k=5) for x in xs]
+    for a, b in zip(got, want):
+        assert torch.equal(a.logprobs, b.logprobs) and torch.equal(a.entropy, b.entropy)
+        assert torch.equal(a.top_ids, b.top_ids) and torch.equal(a.top_logprobs, b.top_logprobs)

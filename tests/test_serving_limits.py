@@ -1,0 +1,74 @@
+"""CPU: calls of the serving side at their limits, through the C ABI with addresses
+that are never read or with the GPU's part replaced, and what its kernels' sources
+have to keep to."""
+import os
+import re
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+CSRC = os.path.join(ROOT, "elastic-sparse-attention_b200", "csrc")
+
+
+# ---------------------------------------------------------------------------
+# A kernel that may start while the kernel before it still writes reads what that one
+# wrote with ordinary loads: those of the read-only path want memory that does not
+# change while the kernel runs.
+# ---------------------------------------------------------------------------
+READ_ONLY = re.compile(r"__ldg\b|\bldg16\b|\bldg16_stream\b|\.nc\b")
+
+
+def functions(source):
+    """{name: text} of the functions of a source file; a function's text begins at its
+    name (its declaration's templates and qualifiers are not looked at)."""
+    source = re.sub(r"//[^\n]*", "", source)
+    found = {}
+    for m in re.finditer(r"\b(\w+)\s*\((?:[^()]|\([^()]*\))*\)\s*(?:const\s*)?\{", source):
+        if m[1] in ("if", "for", "while", "switch", "constexpr"):
+            continue
+        depth, i = 0, m.end() - 1
+        while True:
+            depth += {"{": 1, "}": -1}.get(source[i], 0)
+            i += 1
+            if depth == 0:
+                break
+        found.setdefault(m[1], "")
+        found[m[1]] += source[m.start():i]
+    return found
+
+
+def early_read_only_loads(source):
+    """(kernel, function) of read-only loads in the kernels that wait for the one before
+    them, and in the functions of the file that they call."""
+    all_ = functions(source)
+    bad = []
+    for name, text in all_.items():
+        if "cudaGridDependencySynchronize" not in text:
+            continue
+        todo, seen = [name], set()
+        while todo:
+            f = todo.pop()
+            if f in seen:
+                continue
+            seen.add(f)
+            if READ_ONLY.search(all_[f]):
+                bad.append((name, f))
+            todo += [w for w in set(re.findall(r"\b(\w+)\s*(?:<[\w, ]*>)?\(", all_[f])) if w in all_]
+    return bad
+
+
+def test_the_check_sees_read_only_loads():
+    text = ("int help(const int* p) {{ return {}(p); }}\n"
+            "__global__ void k(const int* p) {{\n  cudaGridDependencySynchronize();\n  help(p);\n}}\n"
+            "__global__ void other(const int* p) {{ __ldg(p); }}\n")
+    assert early_read_only_loads(text.format("__ldg")) == [("k", "help")]
+    assert early_read_only_loads(text.format("load")) == []
+
+
+@pytest.mark.parametrize("name", ["esa_score.cuh", "esa_weight4.cuh"])
+def test_kernels_that_start_early_read_with_ordinary_loads(name):
+    with open(os.path.join(CSRC, name)) as f:
+        source = f.read()
+    waiting = [k for k, t in functions(source).items() if "cudaGridDependencySynchronize" in t]
+    assert waiting
+    assert early_read_only_loads(source) == []
