@@ -23,7 +23,8 @@ class PackedDecoder:
 
     :meth:`step` and :meth:`score` take each sequence's next tokens ``input_ids``
     [batch, L] (a prompt, a part of one, or single tokens), ``counts`` [batch] of
-    them (default: all; the rest is padding), and extend the caches.  ``lengths``
+    them (default: all; the rest is padding, whose ids are not looked at), and extend
+    the caches.  ``lengths``
     (int64 [batch], on the device) holds what has been fed so far.  Nothing is read
     back to the host: a call can be captured into a CUDA graph, whose replays read
     the ids and extend the caches.  Tokens beyond ``max_len`` are left out and set
@@ -83,6 +84,10 @@ class PackedDecoder:
         Hq, Hkv, D = s.Hq, s.Hkv, s.D
         if B == 0 or L == 0:
             return s.embed.new_empty(B, L, s.hidden)
+        if counts is not None:
+            # padding may hold any id: the lookup gets one of the vocabulary
+            padding = torch.arange(L, device=counts.device) >= counts[:, None]
+            input_ids = input_ids.masked_fill(padding, 0)
         # all tokens of the batch in one row of positions
         positions = (self.lengths[:, None] + torch.arange(L, device=self.lengths.device)).view(-1)
         h = s._embed(input_ids)

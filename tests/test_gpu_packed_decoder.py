@@ -203,3 +203,25 @@ def test_limits_and_refusals(esa):
 
 def t_first(esa, stack, ids):
     return esa.PackedDecoder(stack, 2, 10).step(ids[:, :10])
+
+
+@pytest.mark.parametrize("pad", [-100, 1 << 40])
+@torch.no_grad()
+def test_padding_with_any_id(esa, pad):
+    """The rows of tokens are as with padding of an id of the vocabulary, with the
+    library's lookup and with torch's."""
+    torch.manual_seed(3)
+    for kw in (dict(), dict(embed_scale=2.0)):
+        stack = make_stack(esa, **kw)
+        ids = torch.randint(0, 301, (3, 20), device=DEV)
+        counts = torch.tensor([20, 7, 0], device=DEV)
+        esa.ops.device_errors()
+        a, b = (esa.PackedDecoder(stack, 3, 40) for _ in range(2))
+        want = a.score(ids, counts, top_k=3)
+        padded = ids.masked_fill(torch.arange(20, device=DEV) >= counts[:, None], pad)
+        got = b.score(padded, counts, top_k=3)
+        for i, n in enumerate(counts.tolist()):
+            assert torch.equal(got.logprobs[i, :n], want.logprobs[i, :n])
+            assert torch.equal(got.top_ids[i, :n], want.top_ids[i, :n])
+        assert all(torch.equal(x.codes, y.codes) for x, y in zip(a.caches, b.caches))
+        assert esa.ops.device_errors() == 0

@@ -5,6 +5,7 @@ import os
 import re
 
 import pytest
+import torch
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(ROOT, "elastic-sparse-attention_b200", "csrc")
@@ -72,3 +73,37 @@ def test_kernels_that_start_early_read_with_ordinary_loads(name):
     waiting = [k for k, t in functions(source).items() if "cudaGridDependencySynchronize" in t]
     assert waiting
     assert early_read_only_loads(source) == []
+
+
+def session_without_a_gpu(esa, batch, vocab=50):
+    s = object.__new__(esa.PackedDecoder)
+    s.lengths = torch.zeros(batch, dtype=torch.int64)
+    s.lm_head = esa.layer_ops.PackedWeight4(None, None, (vocab, 64), 32, torch.bfloat16)
+    return s
+
+
+@pytest.mark.parametrize("pad", [-1, -100, 50, 1 << 40])
+def test_ids_of_padding_are_not_looked_up(esa, pad):
+    """Whatever a padded place holds, the embedding sees an id of the vocabulary there
+    (its lookup on the GPU does not survive another one)."""
+    class Seen(Exception):
+        pass
+
+    class Stack:
+        Hq, Hkv, D, hidden, eps = 1, 1, 64, 64, 1e-6
+
+        def _embed(self, ids):
+            raise Seen(ids)
+
+    s = session_without_a_gpu(esa, 3)
+    s.stack = Stack()
+    ids = torch.tensor([[1, 2, 3], [4, pad, pad], [pad, pad, pad]])
+    given = ids.clone()
+    for call in (s.step, s.score):
+        with pytest.raises(Seen) as e:
+            call(ids, torch.tensor([3, 1, 0]))
+        assert e.value.args[0].tolist() == [[1, 2, 3], [4, 0, 0], [0, 0, 0]]
+        assert torch.equal(ids, given)
+        with pytest.raises(Seen) as e:
+            call(ids, None)
+        assert torch.equal(e.value.args[0], ids)                  # without counts all are tokens
