@@ -539,6 +539,11 @@ def _score_args(logits: torch.Tensor, tokens: torch.Tensor):
     return dev, code, n, vocab, stride, _ids(tokens)
 
 
+def check_top_k(top_k: int, vocab: int) -> None:
+    if not 0 <= top_k <= min(MAX_TOP, vocab):
+        raise ValueError(f"top_k {top_k} outside [0, {min(MAX_TOP, vocab)}]")
+
+
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0) -> TokenLogProbs:
     """Log probability of one token per row of ``logits`` [..., vocab], the
     entropy of the row and, with ``top_k`` (up to 32), its most likely tokens
@@ -548,8 +553,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0) -
     (a row to ignore) gives 0; another one outside [0, vocab) gives NaN and sets
     ``_lib.DEVERR_TOKEN_RANGE`` (``ops.device_errors``)."""
     dev, code, n, vocab, stride, tokens = _score_args(logits, tokens)
-    if not 0 <= top_k <= min(MAX_TOP, vocab):
-        raise ValueError(f"top_k {top_k} outside [0, {min(MAX_TOP, vocab)}]")
+    check_top_k(top_k, vocab)
     shape = tuple(tokens.shape)
     r = TokenLogProbs(_empty(shape, torch.float32, dev), _empty(shape, torch.float32, dev),
                       _empty(shape + (2,), torch.float32, dev), None, None)

@@ -126,6 +126,7 @@ class PackedDecoder:
         likely next tokens.  The last token of a sequence has no token after it (log
         probability 0): its alternatives are the next token's."""
         counts = self._check(input_ids, counts)
+        layer_ops.check_top_k(top_k, self.lm_head.shape[0])     # before the tokens are fed
         B, L = input_ids.shape
         nxt = F.pad(input_ids[:, 1:], (0, 1), value=layer_ops.IGNORED_TOKEN) if L else input_ids
         if counts is not None:

@@ -107,3 +107,14 @@ def test_ids_of_padding_are_not_looked_up(esa, pad):
         with pytest.raises(Seen) as e:
             call(ids, None)
         assert torch.equal(e.value.args[0], ids)                  # without counts all are tokens
+
+
+@pytest.mark.parametrize("top_k,vocab", [(33, 50), (-1, 50), (8, 7)])
+def test_scores_refuse_top_k_before_the_tokens_are_fed(esa, monkeypatch, top_k, vocab):
+    """A refused call leaves the sequences as they were."""
+    s = session_without_a_gpu(esa, 2, vocab)
+    fed = []
+    monkeypatch.setattr(esa.PackedDecoder, "step", lambda *a: fed.append(a))
+    with pytest.raises(ValueError, match="top_k"):
+        s.score(torch.zeros(2, 3, dtype=torch.int64), top_k=top_k)
+    assert not fed and not s.lengths.any()
