@@ -192,6 +192,7 @@ int check_cache(const char* what, int32_t dtype, const esa_cache4_t* c, int64_t 
   if (!start && start0 < 0) return fail(ESA_ERR_INVALID, "%s: negative start", what);
   if (reinterpret_cast<uintptr_t>(start) % 8 || reinterpret_cast<uintptr_t>(counts) % 8)
     return fail(ESA_ERR_INVALID, "%s: misaligned start or counts", what);
+  if (c->batch == 0) return ESA_OK;            // no memory: there is nothing to read or write
   if (!c->codes || !c->scales || !aligned16(c->codes) || !aligned16(c->scales))
     return fail(ESA_ERR_INVALID, "%s: null or misaligned codes or scales", what);
   return ESA_OK;

@@ -141,3 +141,15 @@ def test_a_group_does_not_touch_the_others(esa, dtype, D, L):
         o, lse = esa.ops.forward_packed(q, cache, spec, 0.1, S - L)
         assert torch.equal(o[..., keep], clean[..., keep]) and torch.equal(lse, cl)
     assert o[..., 32:64].isnan().all()
+
+
+def test_a_batch_of_no_sequences(esa):
+    cache = esa.PackedKVCache(0, 2, 10, 64, device=DEV)
+    x = torch.zeros(0, 2, 3, 64, device=DEV)
+    for start in (0, torch.zeros(0, dtype=torch.int64, device=DEV)):
+        cache.write(x, x, start)
+        assert [t.shape for t in cache.read(start, 3)] == [(0, 2, 3, 64)] * 2
+        o, lse = esa.ops.forward_packed(torch.zeros(0, 4, 3, 64, device=DEV), cache,
+                                        esa.PatternSpec(1, 2, 8), 0.1, start)
+        assert o.shape == (0, 4, 3, 64) and lse.shape == (0, 4, 3)
+    assert esa.ops.device_errors() == 0

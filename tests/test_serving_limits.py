@@ -1,6 +1,7 @@
 """CPU: calls of the serving side at their limits, through the C ABI with addresses
 that are never read or with the GPU's part replaced, and what its kernels' sources
 have to keep to."""
+import ctypes
 import os
 import re
 
@@ -118,3 +119,23 @@ def test_scores_refuse_top_k_before_the_tokens_are_fed(esa, monkeypatch, top_k, 
     with pytest.raises(ValueError, match="top_k"):
         s.score(torch.zeros(2, 3, dtype=torch.int64), top_k=top_k)
     assert not fed and not s.lengths.any()
+
+
+# ---------------------------------------------------------------------------
+# empty and refused calls
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("name", ["write", "read", "forward"])
+def test_a_cache_of_no_sequences(esa, name):
+    """Its tensors have no memory; there is nothing to do."""
+    lib = esa._lib.load()
+    none = esa._lib.EsaTensor(None, 0, 64, 64)
+    c = esa._lib.EsaCache4(None, None, 0, 2, 64, 0, 100)
+    c = ctypes.byref(c)
+    if name == "write":
+        rc = lib.esa_cache4_write(1, c, 4, none, none, None, 0, None, None)
+    elif name == "read":
+        rc = lib.esa_cache4_read(1, c, 4, none, none, None, 0, None)
+    else:
+        rc = lib.esa_cache4_forward(1, c, 4, 4, 16, 1, 4, 0, 0, 0.1, none, None, 0, None, none, None,
+                                    None)
+    assert rc == 0, lib.esa_last_error()
