@@ -188,13 +188,14 @@ __device__ __forceinline__ void expand(uint32_t w, uint32_t (&a)[4]) {
 }
 
 // Part `part` of eight float32 values cut into pieces of 8 significant bits.  (An
-// infinity is all in the first part.)
+// infinity or a NaN is all in the first part; a NaN's set bits may all be among those
+// that are cut off, so it gets one that is not.)
 __device__ __forceinline__ uint4 cut8(const uint4& lo, const uint4& hi, int part) {
   const uint32_t u[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
   uint32_t b[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    b[e] = u[e];
+    b[e] = (u[e] & 0x7fffffffu) > 0x7f800000u ? u[e] | 0x00400000u : u[e];
     if (part > 0) {
       float r = __uint_as_float(u[e]) - __uint_as_float(u[e] & 0xffff0000u);
       if (part > 1) r -= __uint_as_float(__float_as_uint(r) & 0xffff0000u);
