@@ -607,6 +607,9 @@ class ElasticDecoderStack(nn.Module):
         differentiable (policy gradients, distillation); the [L, vocab] logits exist
         ``loss_chunk_rows`` rows at a time, in the backward again."""
         labels = input_ids if labels is None else labels
+        if labels.shape != input_ids.shape:
+            raise ValueError(f"labels {list(labels.shape)} must be shaped like input_ids "
+                             f"{list(input_ids.shape)}")
         targets = torch.full_like(labels, layer_ops.IGNORED_TOKEN)
         targets[:, :-1] = labels[:, 1:]
         return _LMHeadLogProbs.apply(self(input_ids, positions=positions), self.lm_head, targets,

@@ -139,3 +139,12 @@ def test_a_cache_of_no_sequences(esa, name):
         rc = lib.esa_cache4_forward(1, c, 4, 4, 16, 1, 4, 0, 0, 0.1, none, None, 0, None, none, None,
                                     None)
     assert rc == 0, lib.esa_last_error()
+
+
+@pytest.mark.parametrize("shape", [(1, 12), (3, 4), (12,), (2, 7)])
+def test_scores_refuse_labels_of_another_shape(esa, shape):
+    """As many labels in another shape would be paired with other rows."""
+    stack = object.__new__(esa.ElasticDecoderStack)
+    with pytest.raises(ValueError, match="labels"):
+        esa.ElasticDecoderStack.token_logprobs(stack, torch.zeros(2, 6, dtype=torch.int64),
+                                               torch.zeros(shape, dtype=torch.int64))
