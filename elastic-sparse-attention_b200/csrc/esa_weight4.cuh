@@ -206,17 +206,6 @@ __device__ __forceinline__ uint4 cut8(const uint4& lo, const uint4& hi, int part
                     __byte_perm(b[4], b[5], 0x7632), __byte_perm(b[6], b[7], 0x7632));
 }
 
-// Eight inputs k .. k + 7 of one column as four B words (zeros past K).
-template <typename T>
-__device__ __forceinline__ uint4 column8(const T* x, int k, int K, bool in, int part) {
-  const uint4 none = make_uint4(0, 0, 0, 0);
-  if constexpr (sizeof(T) == 2) {
-    return in && k < K ? ld16(x + k) : none;
-  } else {
-    return cut8(in && k < K ? ld16(x + k) : none, in && k + 4 < K ? ld16(x + k + 4) : none, part);
-  }
-}
-
 template <typename T> struct LinearParams {
   const T* x;
   T* y;
@@ -314,7 +303,7 @@ __device__ __forceinline__ void multiply(const Tile<G>& w, float (&acc)[NT][4], 
 }
 
 // ---------------------------------------------------------------------------
-// Up to 8 columns: bound by the stream of codes.  CTA = one tile of 16 weight rows,
+// Up to 8 rows of a 16-bit type: bound by the stream of codes.  CTA = one tile of 16 weight rows,
 // its WK warps share K and join in shared memory.  A warp has kDepth tiles on their
 // way.  Before it waits for the kernel before it (which made x, or the codes) it only
 // has the first of them brought into L2.
@@ -324,8 +313,7 @@ constexpr int kDepth = 4;
 template <typename T, int G, int WK>
 __global__ void __launch_bounds__(WK * 32)
 vector_kernel(const LinearParams<T> p) {
-  using H = typename Operand<T>::Half;
-  constexpr int P = Operand<T>::kParts;
+  static_assert(Operand<T>::kParts == 1, "a column per row of x");
   extern __shared__ __align__(128) unsigned char s_mem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
@@ -341,15 +329,17 @@ vector_kernel(const LinearParams<T> p) {
     if (c0 + i < c1) Tile<G>::fetch(to + i * Tile<G>::kBytes, p.codes, p.scales, base + c0 + i, lane);
     commit_copies();
   }
-  const int token = g / P, part = g % P;
-  const bool in = token < p.M && token < 8 / P;
-  const T* x = p.x + (int64_t)(in ? token : 0) * p.K + t * 8;
+  const bool in = g < p.M;                             // column g: row g of x
+  const T* x = p.x + (int64_t)(in ? g : 0) * p.K + t * 8;
   const int left = p.K - t * 8;
   float acc[1][4] = {{0.f, 0.f, 0.f, 0.f}};
   uint4 xb[4];
-  auto inputs = [&](int c) {
+  auto inputs = [&](int c) {                           // zeros past K
 #pragma unroll
-    for (int q = 0; q < 4; ++q) xb[q] = column8(x, c * kTileK + q * 32, left, in, part);
+    for (int q = 0; q < 4; ++q) {
+      const int k = c * kTileK + q * 32;
+      xb[q] = in && k < left ? ld16(x + k) : make_uint4(0, 0, 0, 0);
+    }
   };
   if (c0 < c1) inputs(c0);
 #pragma unroll 2
@@ -360,7 +350,7 @@ vector_kernel(const LinearParams<T> p) {
     w.take(ring + slot * Tile<G>::kBytes, lane);
     const uint4 now[4] = {xb[0], xb[1], xb[2], xb[3]};
     if (c + 1 < c1) inputs(c + 1);
-    multiply<H, G, 1>(w, acc, [&](int q, int) { return now[q]; });
+    multiply<T, G, 1>(w, acc, [&](int q, int) { return now[q]; });
     // the slot's next tile: the products have waited for what this lane read, and
     // nobody else reads it
     if (c + kDepth < c1)
@@ -377,9 +367,7 @@ vector_kernel(const LinearParams<T> p) {
     if ((int64_t)blockIdx.x * kTileRows + row >= p.N) break;
     float sum = 0.f;
 #pragma unroll
-    for (int k = 0; k < WK; ++k)
-#pragma unroll
-      for (int q = 0; q < P; ++q) sum += part_sums[k][m * P + q][row];
+    for (int k = 0; k < WK; ++k) sum += part_sums[k][m][row];
     p.y[(int64_t)m * p.N + (int64_t)blockIdx.x * kTileRows + row] = from_f32<T>(sum);
   }
 }
