@@ -5,7 +5,9 @@
 // exactly), -7 .. 7, stored as code + 8, and stands for code * s (exact in
 // float32: 4 bits times 8).  The codes are formed with the rounded scale, so its
 // rounding costs no accuracy.  A group with an infinity or a NaN gets s = NaN
-// and codes 0 and decodes to NaN.
+// and codes 0 and decodes to NaN.  One finite value decodes to infinity, and in
+// bfloat16 alone: its largest, 255 * 2^120, has s = 146 * 2^118 and stands for
+// 1022 * 2^118, which lies halfway to 2^128 and rounds to that.
 #pragma once
 #include "esa_common.cuh"
 

@@ -626,7 +626,8 @@ class PackedWeight4:
 def quantize_weight4(weight: torch.Tensor, group: int = 128) -> PackedWeight4:
     """``weight`` [n, k] (a projection's, rows of outputs) in 4 bits: even steps
     of max|w| / 7 within ``group`` (32, 64 or 128) consecutive inputs of a row,
-    the step a bfloat16.  A group with an infinity or a NaN decodes to NaN."""
+    the step a bfloat16.  A group with an infinity or a NaN decodes to NaN; the
+    largest bfloat16 decodes to 1022 * 2^118, an infinity in bfloat16."""
     dev = _check_device(weight)
     if weight.dim() != 2:
         raise ValueError("weight must be [n, k]")
@@ -671,9 +672,9 @@ def dequantize_weight4(packed: PackedWeight4, dtype: torch.dtype | None = None) 
 
 def linear4(x: torch.Tensor, packed: PackedWeight4) -> torch.Tensor:
     """x [..., k] times the transposed weight: [..., n].  Exact products of x and
-    the codes, float32 sums, rounded once.  Made for few rows (decoding:
-    16-bit types up to ``LINEAR4_ROWS``); it takes
-    ``LINEAR4_MAX_ROWS``."""
+    the codes, float32 sums (of a group before its scale is taken: |x| up to 2^118),
+    rounded once.  Made for few rows (decoding: 16-bit types up to
+    ``LINEAR4_ROWS``); it takes ``LINEAR4_MAX_ROWS``."""
     n, k = _check_weight4(packed)
     dev = _check_device(x, packed.codes, packed.scales)
     shape = _shape(x)

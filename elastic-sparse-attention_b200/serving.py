@@ -57,7 +57,7 @@ class PackedDecoder:
     @staticmethod
     def _project(x: torch.Tensor, weight: layer_ops.PackedWeight4) -> torch.Tensor:
         """x W^T: from the codes for float32 and for few rows of a 16-bit type, else
-        with the weight decoded for the call."""
+        with the weight decoded, and rounded to the type, for the call."""
         most = (layer_ops.LINEAR4_MAX_ROWS if x.dtype == torch.float32 else
                 layer_ops.LINEAR4_ROWS)
         if x.numel() // x.shape[-1] <= most:

@@ -260,7 +260,8 @@ int esa_token_logprobs_backward(int32_t dtype, int32_t id_bytes, int64_t n_rows,
  * a row of weight [n, k] (the last may be shorter) has the scale s = the bfloat16
  * nearest to f32(max|w| / 7), at least 2^-126; a code is the integer nearest to
  * w / s (ties to even, the quotient taken exactly) and stands for code * s.  A
- * group with an infinity or a NaN decodes to NaN.  codes: esa_weight4_codes_size(
+ * group with an infinity or a NaN decodes to NaN; bfloat16's largest value decodes
+ * to 1022 * 2^118, which rounds to infinity in that type.  codes: esa_weight4_codes_size(
  * n, k) bytes in the order the product reads them; scales: bfloat16 [ceil(n / 16),
  * ceil(k / 128) * 128 / group, 16].  k * element size is a multiple of 16 bytes.
  */
@@ -271,8 +272,10 @@ int esa_quantize_weight4(int32_t dtype, int64_t n, int64_t k, int32_t group, con
 int esa_dequantize_weight4(int32_t dtype, int64_t n, int64_t k, int32_t group, const void* codes,
                            const void* scales, void* weight, void* stream);
 /* y [n_rows, n] = x [n_rows, k] times the transposed weight: exact products of x
- * and the codes, float32 sums, one rounding to dtype.  Made for few rows (up to
- * some 64); it takes any number. */
+ * and the codes, float32 sums, one rounding to dtype.  A group's sum is formed before
+ * its scale is taken: |x| up to 2^118 (128 codes of 7 stay within float32); parts of
+ * float32 x below 2^-133 are left out.  Made for few rows (up to some 64); it takes
+ * 2^20. */
 int esa_linear4(int32_t dtype, int64_t n_rows, int64_t n, int64_t k, int32_t group, const void* x,
                 const void* codes, const void* scales, void* y, void* stream);
 

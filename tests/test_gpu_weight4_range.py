@@ -1,8 +1,10 @@
 """GPU: weights in 4 bits and products with them at the ends of their types' range."""
+import math
+
 import pytest
 import torch
 
-from test_gpu_weight4 import DEV
+from test_gpu_weight4 import DEV, decoded
 
 pytestmark = pytest.mark.gpu
 
@@ -25,3 +27,28 @@ def test_every_nan_of_float32_rows(lops, rows, bits):
     assert x[0, 150].isnan()
     y = lops.linear4(x, p)
     assert y[0].isnan().all() and torch.isfinite(y[1:]).all()
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_the_largest_weights(lops, group):
+    """7 steps of a group whose largest magnitude is bfloat16's largest value are
+    1022 * 2^118, halfway between that value and 2^128: its rounding is infinity.  So
+    in bfloat16 alone: no other value, and not in float32, where a product takes it as
+    it is."""
+    big = torch.finfo(torch.bfloat16).max
+    w = torch.zeros(4, 128, device=DEV, dtype=torch.bfloat16)
+    w[0, 3], w[1, 3] = big, -big
+    w[2, 3] = torch.nextafter(torch.tensor(big, dtype=torch.bfloat16), torch.tensor(0.0, dtype=torch.bfloat16))
+    w[3, 3] = 1.0
+    p = lops.quantize_weight4(w, group)
+    v = lops.dequantize_weight4(p, torch.float32)
+    assert torch.equal(v.double(), decoded(w, group)) and torch.isfinite(v).all()
+    assert float(v[0, 3]) == 1022 * 2.0 ** 118
+    h = lops.dequantize_weight4(p)
+    assert h[0, 3] == math.inf and h[1, 3] == -math.inf and torch.isfinite(h[2:]).all()
+    x = torch.zeros(1, 128, device=DEV, dtype=torch.bfloat16)
+    x[0, 3] = 0.25
+    assert lops.linear4(x, p)[0, :2].tolist() == [2.0 ** 126, -2.0 ** 126]
+    for dtype in (torch.float16, torch.float32):      # the largest values there stay finite
+        w = torch.full((1, 128), torch.finfo(dtype).max, device=DEV, dtype=dtype)
+        assert torch.isfinite(lops.dequantize_weight4(lops.quantize_weight4(w, group))).all()
