@@ -153,3 +153,32 @@ def test_a_batch_of_no_sequences(esa):
                                         esa.PatternSpec(1, 2, 8), 0.1, start)
         assert o.shape == (0, 4, 3, 64) and lse.shape == (0, 4, 3)
     assert esa.ops.device_errors() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("layer,layers,w", [(1, 4, 64), (5, 8, 100), (3, 4, 33), (0, 4, 64)])
+def test_positions_next_to_2_24(esa, dtype, layer, layers, w):
+    """Strided and window layers at the end of the longest cache: only the rows of the
+    definition's pattern hold anything, so that another row would show."""
+    S, D, L, Hq = 1 << 24, 64, 4, 2
+    g = torch.Generator().manual_seed(w)
+    cache = esa.PackedKVCache(1, 1, S, D, device=DEV)
+    idx, mask = pattern.elastic_indices(range(S - L, S), Hq, w, layer, layers)
+    mask = mask.astype(bool)
+    places = sorted(set(idx[mask].tolist()))
+    assert places[-1] < S and places[0] >= 0
+    k, v = (head_rows((1, 1, len(places), D), g, dtype) for _ in range(2))
+    for i, p in enumerate(places):
+        cache.write(k[:, :, i:i + 1], v[:, :, i:i + 1], p)
+    q = head_rows((1, L, Hq, D), g, dtype).transpose(1, 2)
+    o, lse = esa.ops.forward_packed(q, cache, esa.PatternSpec(layer, layers, w), D ** -0.5, S - L)
+    dk, dv, sv = decoded(k)[0, 0], decoded(v)[0, 0], scales_of(v)[0, 0]
+    which = {p: i for i, p in enumerate(places)}
+    for h in range(Hq):
+        for r in range(L):
+            at = torch.tensor([which[p] for p in idx[h, r][mask[h, r]].tolist()], device=DEV)
+            keep = torch.ones(len(at), dtype=torch.bool, device=DEV)
+            wo, wl, so, sl = row64(q[0, h, r].double(), dk[at], dv[at], sv[at], keep, D ** -0.5,
+                                   fixed_point(dtype) * w / len(at))
+            check_row(o[0, h, r], lse[0, h, r], (wo, wl, so, sl))
+    assert esa.ops.device_errors() == 0
