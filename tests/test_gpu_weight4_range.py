@@ -52,3 +52,47 @@ def test_the_largest_weights(lops, group):
     for dtype in (torch.float16, torch.float32):      # the largest values there stay finite
         w = torch.full((1, 128), torch.finfo(dtype).max, device=DEV, dtype=dtype)
         assert torch.isfinite(lops.dequantize_weight4(lops.quantize_weight4(w, group))).all()
+
+
+def test_captured_on_two_streams_that_join(lops):
+    """Products and scores of two branches of one graph, then a product that needs both,
+    with copies in between: kernels that may start early have several predecessors, not
+    all of them kernels."""
+    g = torch.Generator().manual_seed(21)
+    ps = [lops.quantize_weight4((0.05 * torch.randn(512, 512, generator=g)).to(DEV, torch.bfloat16), 64)
+          for _ in range(4)]
+    xs = [torch.randn(m, 512, generator=g).to(DEV, torch.bfloat16) for m in (3, 20)]
+    tokens = torch.randint(0, 512, (20,), generator=g).to(DEV)
+    side = torch.cuda.Stream()
+
+    def run(two):
+        main = torch.cuda.current_stream()
+        a = lops.linear4(xs[0], ps[0])
+        if two:
+            side.wait_stream(main)
+        with torch.cuda.stream(side if two else main):
+            b = lops.linear4(lops.linear4(xs[1], ps[1]), ps[2])
+            scores = lops.token_logprobs(b, tokens, top_k=4)
+        a = lops.linear4(a, ps[3])
+        if two:
+            main.wait_stream(side)
+        both = torch.cat([a, b])
+        y = lops.linear4(both, ps[0])
+        both.copy_(y)
+        return lops.linear4(both, ps[1]), scores.logprobs, scores.top_ids
+
+    warm = torch.cuda.Stream()
+    warm.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(warm):
+        run(True)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run(True)
+    for seed in range(4):
+        for x in xs:
+            x.copy_(torch.randn(x.shape, generator=torch.Generator().manual_seed(seed)))
+        graph.replay()
+        torch.cuda.synchronize()
+        for t, want in zip(got, run(False)):
+            assert torch.equal(t, want)
