@@ -32,8 +32,10 @@
 // 9 bits when the tensor core aligns them: the output was 2^-11 off.)
 //
 // Measured: 4096 rows x 32 heads of 128, w = 64, at the end of 131072 positions:
-// 206 us (esa_forward on a 16-bit cache of that shape: 444); some 1230 instructions a
-// pair fill 71 % of the issue slots, the integer pipe 63 %.  8 single rows: 3.6 us.
+// 212 us (esa_forward on a 16-bit cache of that shape: 444; 206 with one grid of weights
+// for all groups of a head, on which a group 4096 times smaller than the largest was
+// a tenth off); some 1290 instructions a pair fill 73 % of the issue slots, the integer
+// pipe 67 %.  8 single rows: 3.6 us.
 // Rows in: 79 us, out: 62 us for 3 x 20011 x 8 rows of 128 fp16 (profiled; together 138
 // without), bound by instructions: 78 and 74 % of the issue slots, DRAM at 25 and 50 %.
 //

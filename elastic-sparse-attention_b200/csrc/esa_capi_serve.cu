@@ -289,8 +289,9 @@ int esa_token_logprobs_forward(int32_t dtype, int32_t id_bytes, int64_t n_rows, 
     const int64_t vecs = vocab / esa::Vec<T>::kElems;
     auto go = [&](auto nw) {
       constexpr int NW = decltype(nw)::value;
-      // few rows: a row over up to 8 CTAs, with a vector per thread at least (beyond a
-      // CTA per SM it does not pay: 333 x 50021 float32 takes 20 us, split in four 24)
+      // few rows: a row over up to 8 CTAs, with a vector per thread at least, until there
+      // is a CTA per SM (333 x 50021 float32, beyond that, takes 20 us, split in four 24;
+      // in two was not tried)
       int ctas = 1;
       while (ctas < 8 && n_rows * ctas < kSms && vecs >= (int64_t)ctas * 2 * NW * 32) ctas *= 2;
       const dim3 grid((unsigned)(n_rows * ctas)), block(NW * 32);

@@ -6,16 +6,18 @@
 // instructions.  The arithmetic is mma.sync m16n8k16: 16 weight rows as A, 8
 // columns (rows of x) as B, float32 sums.  Codes are integers of 4 bits and
 // exact in bf16 and fp16, so every product is exact; the sum of a group is
-// multiplied by its scale in float32.  (A tcgen05 product would need the codes
-// expanded through shared memory first, for tiles of 128 weight rows by as few
-// as 8 columns.)  float32 rows of x are split into three bf16 parts (8 bits
-// each, exact), three columns whose sums are added at the end.
+// multiplied by its scale in float32.  (A tcgen05 product takes tiles of 128 weight
+// rows, whose decoded codes could go from registers to tensor memory, and its
+// accumulator would be read once per group for the scale; it was not built.)  float32
+// rows of x are split into three bf16 parts (8 bits each, exact down to 2^-133), three
+// columns whose sums are added at the end.
 //
 // Measured (1 x B200, weights from HBM, launches one after the other): 1 x 4096 x
 // 12288 in 9.1 us (its bytes alone: 4.0; a copy of an earlier state of the kernel with
 // the arithmetic taken out needed 6.8, without x as well 5.8), 32 x 11008 x 4096 in 15.7
-// (3.7), where the matrix instructions alone take 5.2 at their measured rate and a CTA
-// has only some six stages of K.  Not taken up: x in fixed
+// (3.7), where the matrix instructions alone take 5.2 at their measured rate, the reads
+// of x from shared memory by every warp for its 16 weight rows 5.0, and a CTA has only
+// some six stages of K.  Not taken up: x in fixed
 // point against 8-bit integer products, which needs a third of the instructions for
 // one row but took as long (the chain of loads bounds it), and loses bits of float32
 // rows with a wide range.
