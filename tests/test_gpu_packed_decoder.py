@@ -225,3 +225,46 @@ def test_padding_with_any_id(esa, pad):
             assert torch.equal(got.top_ids[i, :n], want.top_ids[i, :n])
         assert all(torch.equal(x.codes, y.codes) for x, y in zip(a.caches, b.caches))
         assert esa.ops.device_errors() == 0
+
+
+@torch.no_grad()
+def test_no_sequences_narrow_ids_and_small_chunks(esa):
+    torch.manual_seed(4)
+    stack = make_stack(esa)
+    none = esa.PackedDecoder(stack, 0, 10)
+    ids = torch.randint(0, 301, (2, 30), device=DEV)
+    assert none.step(ids[:0]).shape == (0, 30, 256)
+    r = none.score(ids[:0], top_k=2)
+    assert r.logprobs.shape == (0, 30) and r.top_ids.shape == (0, 30, 2) and none.nbytes() > 0
+    a, b, c = (esa.PackedDecoder(stack, 2, 40) for _ in range(3))
+    counts = torch.tensor([30, 11], dtype=torch.int32)
+    want = a.score(ids, counts.to(DEV).long(), top_k=3)
+    got = b.score(ids.int(), counts, top_k=3)
+    # (float32 products of few rows and of many sum in other orders)
+    stack.loss_chunk_rows = 7
+    parts = c.score(ids, counts, top_k=3)
+    for i, n in enumerate(counts.tolist()):
+        assert torch.equal(got.logprobs[i, :n], want.logprobs[i, :n])
+        assert torch.equal(got.top_ids[i, :n], want.top_ids[i, :n])
+        assert (parts.logprobs[i, :n] - want.logprobs[i, :n]).abs().max() <= 1e-3
+        assert (parts.entropy[i, :n] - want.entropy[i, :n]).abs().max() <= 1e-3
+    assert a.lengths.tolist() == b.lengths.tolist() == c.lengths.tolist() == [30, 11]
+
+
+@torch.no_grad()
+def test_half_precision_session(esa):
+    """float16, prompts above and below the rows that are multiplied by codes: as far from
+    the float32 run of the same weights as each other (twice the root mean square)."""
+    torch.manual_seed(5)
+    stack = make_stack(esa, torch.float16)
+    exact = make_stack(esa)
+    for p, q in zip(exact.parameters(), stack.parameters()):
+        p.copy_(q)
+    ids = torch.randint(0, 301, (1, 90), device=DEV)
+    e = esa.PackedDecoder(exact, 1, 90).score(ids)
+    whole = esa.PackedDecoder(stack, 1, 90).score(ids)
+    s = esa.PackedDecoder(stack, 1, 90)
+    parts = [s.score(ids[:, i:i + 30]).entropy for i in (0, 30, 60)]
+    rms = lambda x, y: (x - y).square().mean().sqrt()
+    assert rms(torch.cat(parts, 1), e.entropy) <= 2 * rms(whole.entropy, e.entropy)
+    assert esa.ops.device_errors() == 0
