@@ -460,7 +460,8 @@ attend_kernel(const AttendParams<T> p) {
       const int set = i * 32 + lane;
       qv[i] = QV{};
       if (in && (NG * 8 % 32 == 0 || set < NG * 8))
-        qv[i] = __ldg(reinterpret_cast<const QV*>(q + h * p.q.sh + (int64_t)l * p.q.ss + set * 4));
+        // o may be q: a pair's query is read before its output is written, and by an ordinary load
+        qv[i] = *reinterpret_cast<const QV*>(q + h * p.q.sh + (int64_t)l * p.q.ss + set * 4);
     }
   };
   load_query(pair < p.rows);

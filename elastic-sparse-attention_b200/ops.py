@@ -302,7 +302,7 @@ def forward_packed(q: torch.Tensor, cache, spec: PatternSpec, scale: float, star
     [B, Hq, L, D] as a view of a [B, L, Hq, D] buffer, lse float32 [B, Hq, L] base
     2).  Rows l >= counts[b] are padding: zeros and -infinity; so is a row whose
     position is beyond the cache, which also sets
-    ``_lib.DEVERR_QUERY_RANGE``."""
+    ``_lib.DEVERR_QUERY_RANGE``.  ``out`` receives o (``q`` itself for in place)."""
     dev = _check_device(q, cache.codes)
     if q.dim() != 4:
         raise ValueError("q must be [batch, num_heads, L, head_dim]")

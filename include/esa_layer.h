@@ -313,12 +313,13 @@ int esa_cache4_read(int32_t dtype, const esa_cache4_t* cache, int64_t seq_len, e
 /*
  * Elastic attention of q [batch, num_heads, q_len, head_dim] over the cache: row l
  * of sequence b attends, as position start[b] + l, to the cached rows of its
- * pattern (as esa_forward's query at that position).  o like q, lse float32
- * [batch, num_heads, q_len] (base 2).  Scores, softmax and sums are float32; an
+ * pattern (as esa_forward's query at that position).  o like q (or q itself), lse
+ * float32 [batch, num_heads, q_len] (base 2).  Scores, softmax and sums are float32; an
  * element of the query is kept to 2^-30 of the query's largest.  For 16-bit dtypes a
  * softmax weight times the scale of a group of values is kept to 2^-16 of the largest
- * of 32 slots in that group, for float32 to 2^-31.  A padding row, and one whose position is outside the cache (which sets
- * ESA_DEVERR_QUERY_RANGE), gets zeros and -infinity.
+ * of 32 slots in that group, for float32 to 2^-31.  A padding row, and one whose
+ * position is outside the cache (which sets ESA_DEVERR_QUERY_RANGE), gets zeros and
+ * -infinity.
  */
 int esa_cache4_forward(int32_t dtype, const esa_cache4_t* cache, int32_t num_heads, int64_t q_len,
                        int32_t attn_length, int32_t layer_idx, int32_t num_hidden_layers,

@@ -182,3 +182,22 @@ def test_positions_next_to_2_24(esa, dtype, layer, layers, w):
                                    fixed_point(dtype) * w / len(at))
             check_row(o[0, h, r], lse[0, h, r], (wo, wl, so, sl))
     assert esa.ops.device_errors() == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("L", [1, 600])
+def test_outputs_in_place_of_the_queries(esa, dtype, L):
+    """`out` may be q itself, or rows of another layout."""
+    g = torch.Generator().manual_seed(L)
+    k, v = (head_rows((2, 2, 900, 128), g, dtype) for _ in range(2))
+    cache = esa.PackedKVCache(2, 2, 900, 128, device=DEV)
+    cache.write(k, v, 0)
+    q = head_rows((2, L, 8, 128), g, dtype).transpose(1, 2)
+    spec = esa.PatternSpec(2, 4, 64)
+    want, wl = esa.ops.forward_packed(q, cache, spec, 0.1, 300)
+    rows = torch.full((2, 8, L, 256), 3.0, device=DEV, dtype=dtype)
+    o, lse = esa.ops.forward_packed(q, cache, spec, 0.1, 300, out=rows[..., 64:192])
+    assert torch.equal(o, want) and torch.equal(lse, wl)
+    assert (rows[..., :64] == 3).all() and (rows[..., 192:] == 3).all()
+    o, lse = esa.ops.forward_packed(q, cache, spec, 0.1, 300, out=q)
+    assert torch.equal(q, want) and torch.equal(lse, wl)
